@@ -26,8 +26,10 @@ LIB = os.path.join(HERE, "libattn_b200.so")
 
 NVCC_FLAGS = ["-gencode", "arch=compute_100a,code=sm_100a", "-lineinfo", "-O3", "-std=c++17",
               "-Xcompiler", "-fPIC", "-I" + INCLUDE, "-I" + CSRC]
-CU_SOURCES = ["attn_capi.cu", "attn_prep.cu", "attn_simt.cu", "attn_tc.cu", "attn_tc_fb.cu", "attn_tc_fwd.cu", "attn_tc_hvp_row.cu", "attn_tc_hvp_col.cu"]
-HEADERS = ["attn_common.cuh", "attn_launch.h", "simt_split.h", "tc_primitives.cuh", "tc_common.cuh", os.path.join(INCLUDE, "attn_b200.h")]
+CU_SOURCES = ["attn_capi.cu", "attn_prep.cu", "attn_simt.cu", "attn_tc.cu", "attn_tc_fb.cu", "attn_tc_fwd.cu", "attn_tc_hvp_row.cu", "attn_tc_hvp_col.cu",
+              "packed_capi.cu", "packed_plan.cu"]
+EXT_SOURCES = ["attention_ext.cpp", "packed_ext.cpp"]
+HEADERS = ["attn_common.cuh", "attn_launch.h", "capi_common.h", "packed_geometry.cuh", "packed_launch.h", "simt_split.h", "tc_primitives.cuh", "tc_common.cuh", os.path.join(INCLUDE, "attn_b200.h")]
 
 
 def _nvcc() -> str:
@@ -97,23 +99,31 @@ def build_extension(force: bool = False, verbose: bool = False) -> str:
 
     build_library(force, verbose)
     target = ext_path()
-    src = os.path.join(CSRC, "attention_ext.cpp")
-    digest = _digest([src, os.path.join(INCLUDE, "attn_b200.h"), __file__]) + torch.__version__
+    srcs = [os.path.join(CSRC, s) for s in EXT_SOURCES]
+    digest = _digest(srcs + [os.path.join(CSRC, "ext_common.h"), os.path.join(INCLUDE, "attn_b200.h"), __file__]) + torch.__version__
     if not force and not _stale(target, "ext.stamp", digest):
         return target
     inc = []
     for p in ce.include_paths("cuda") if "device_type" in ce.include_paths.__code__.co_varnames else ce.include_paths(True):
         inc += ["-isystem", p]
-    inc += ["-isystem", sysconfig.get_paths()["include"], "-I" + INCLUDE]
+    inc += ["-isystem", sysconfig.get_paths()["include"], "-I" + INCLUDE, "-I" + CSRC]
     torch_lib = os.path.join(os.path.dirname(torch.__file__), "lib")
     cuda_home = ce.CUDA_HOME or "/usr/local/cuda"
-    cmd = ["g++", "-O2", "-std=c++17", "-fPIC", "-shared", "-DTORCH_EXTENSION_NAME=attention_cuda",
-           "-DTORCH_API_INCLUDE_EXTENSION_H", "-D_GLIBCXX_USE_CXX11_ABI=%d" % int(torch._C._GLIBCXX_USE_CXX11_ABI),
-           src, "-o", target] + inc + [
-           "-L" + torch_lib, "-L" + HERE, "-L" + os.path.join(cuda_home, "lib64"),
-           "-lattn_b200", "-lc10", "-lc10_cuda", "-ltorch_cpu", "-ltorch_cuda", "-ltorch", "-ltorch_python",
-           "-lcudart", "-Wl,-rpath,$ORIGIN", "-Wl,-rpath," + torch_lib]
-    _run(cmd, verbose)
+    procs, objs = [], []
+    for s in srcs:
+        o = os.path.join(BUILD, os.path.basename(s)[:-4] + ".o")
+        objs.append(o)
+        cmd = ["g++", "-O2", "-std=c++17", "-fPIC", "-DTORCH_EXTENSION_NAME=attention_cuda", "-DTORCH_API_INCLUDE_EXTENSION_H",
+               "-D_GLIBCXX_USE_CXX11_ABI=%d" % int(torch._C._GLIBCXX_USE_CXX11_ABI), "-c", s, "-o", o] + inc
+        if verbose:
+            print(" ".join(cmd), flush=True)
+        procs.append(subprocess.Popen(cmd))
+    if any([p.wait() != 0 for p in procs]):
+        raise RuntimeError("g++ failed")
+    _run(["g++", "-shared", "-o", target] + objs + [
+         "-L" + torch_lib, "-L" + HERE, "-L" + os.path.join(cuda_home, "lib64"),
+         "-lattn_b200", "-lc10", "-lc10_cuda", "-ltorch_cpu", "-ltorch_cuda", "-ltorch", "-ltorch_python",
+         "-lcudart", "-Wl,-rpath,$ORIGIN", "-Wl,-rpath," + torch_lib], verbose)
     _write_stamp("ext.stamp", digest)
     return target
 

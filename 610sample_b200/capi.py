@@ -26,12 +26,19 @@ EXPORTS = (
     "attn_b200_last_launch_count", "attn_b200_device_status", "attn_b200_last_error",
     "attn_b200_version", "attn_b200_selftest_gemm", "attn_b200_set_status_mirror", "attn_b200_qk_norm_rope",
     "attn_b200_qk_norm_rope_backward", "attn_b200_qk_norm_rope_backward_scratch_bytes",
+    "attn_b200_packed_plan_ints", "attn_b200_packed_plan", "attn_b200_packed_forward", "attn_b200_packed_backward",
+    "attn_b200_packed_backward_scratch_bytes",
 )
 
 
 class Shape(C.Structure):
     _fields_ = [(n, C.c_int32) for n in
                 ("B", "H", "N_q", "N_kv", "D", "window_size", "chunk_id", "mask_mode", "dtype", "impl")]
+
+
+class PackedShape(C.Structure):
+    _fields_ = [(n, C.c_int32) for n in ("n_tok", "n_seq", "q_heads", "kv_heads", "D", "window_size", "dtype", "reserved")] + [
+        ("row_stride", C.c_int64 * 4), ("head_stride", C.c_int64 * 4)]
 
 
 _lib = None
@@ -62,6 +69,13 @@ def lib() -> C.CDLL:
         L.attn_b200_last_error.restype = C.c_char_p
         L.attn_b200_version.restype = C.c_char_p
         L.attn_b200_selftest_gemm.argtypes = [vp, vp, fp, C.c_int32, C.c_int32, C.c_int32, C.c_int32, vp]
+        L.attn_b200_packed_plan_ints.argtypes = [C.c_int32] * 2
+        L.attn_b200_packed_plan_ints.restype = C.c_size_t
+        L.attn_b200_packed_plan.argtypes = [vp, C.c_int32, C.c_int32, vp, vp]
+        L.attn_b200_packed_forward.argtypes = [C.POINTER(PackedShape)] + [vp] * 7
+        L.attn_b200_packed_backward.argtypes = [C.POINTER(PackedShape)] + [vp] * 12
+        L.attn_b200_packed_backward_scratch_bytes.argtypes = [C.POINTER(PackedShape)]
+        L.attn_b200_packed_backward_scratch_bytes.restype = C.c_size_t
         for name in EXPORTS:
             getattr(L, name)
         _lib = L

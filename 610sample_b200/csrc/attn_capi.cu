@@ -2,6 +2,7 @@
 // kernel-family dispatch, per-thread error text and the device status word.
 #include "attn_b200.h"
 #include "attn_launch.h"
+#include "capi_common.h"
 #include "tc_primitives.cuh"
 
 #include <atomic>
@@ -155,6 +156,41 @@ int run(int op, const attn_shape_t* s, attn::Tensors& t, void* stream, int phase
   tl_error[0] = 0;
   return ATTN_OK;
 }
+
+}  // namespace
+
+// ---- for the other files of the C ABI (capi_common.h)
+namespace attn {
+namespace capi {
+
+int fail(int code, const char* fmt, ...) {
+  va_list ap;
+  va_start(ap, fmt);
+  vsnprintf(tl_error, sizeof(tl_error), fmt, ap);
+  va_end(ap);
+  return code;
+}
+
+int begin(unsigned int** status) {
+  tl_launches = 0;
+  int dev = 0;
+  cudaError_t e = cudaGetDevice(&dev);
+  if (e == cudaSuccess) e = cudaSetDevice(dev);      // as in run(): binds the primary context to this thread
+  if (e != cudaSuccess) return ::fail(ATTN_ECUDA, "binding the device context: %s", cudaGetErrorString(e));
+  return status_pointer(dev, status);
+}
+
+int done(cudaError_t e, const char* what, const char* why, int launches) {
+  if (e != cudaSuccess) return ::fail(ATTN_ECUDA, "%s: %s%s%s", what, cudaGetErrorString(e), why ? ": " : "", why ? why : "");
+  tl_launches = launches;
+  tl_error[0] = 0;
+  return ATTN_OK;
+}
+
+}  // namespace capi
+}  // namespace attn
+
+namespace {
 
 // A tensor without elements (B, H, N or the other side's N is 0) may be passed as null.
 #define REQUIRE_PTR(p)                                                                        \

@@ -25,6 +25,7 @@ constexpr float kLn2 = 0.6931471805599453f;
 
 // Everything a kernel needs to know about the problem besides its pointers.
 struct Geometry {
+  static constexpr bool kPacked = false;
   int BH;        // batch * heads
   int N_q, N_kv, D;
   int qi_base;   // absolute index of query row 0  (= chunk_id * N_q)

@@ -37,6 +37,7 @@
 // bitwise reproducible either way.
 #include "attn_common.cuh"
 #include "attn_launch.h"
+#include "packed_launch.h"
 #include "simt_split.h"
 #include "tc_common.cuh"
 
@@ -86,16 +87,16 @@ template <typename T> __device__ __forceinline__ float4 widen4(const T* p) {
   return make_float4(a.x, a.y, b.x, b.y);
 }
 
-// Stage `rows` rows from row0 of a [n_rows, D] matrix as fp32, zero beyond n_rows.  DC * 16 of the NT threads
+// Stage `rows` rows from row0 of a [n_rows, D] matrix (`pitch` elements from row to row) as fp32, zero beyond n_rows.  DC * 16 of the NT threads
 // share a row.  float goes by cp.async (complete after cp_async_wait_all and a barrier).
 template <int DC, int NT, typename T>
-__device__ __forceinline__ void stage_tile(float* dst, const Layout& lay, const T* src, int row0, int rows, int n_rows, int D) {
+__device__ __forceinline__ void stage_tile(float* dst, const Layout& lay, const T* src, int row0, int rows, int n_rows, int D, size_t pitch) {
   constexpr int kLanes = 16 * DC;
   const int chunk = threadIdx.x % kLanes;
   if (chunk * 4 >= D) return;
   for (int r = threadIdx.x / kLanes; r < rows; r += NT / kLanes) {
     const bool in = row0 + r < n_rows;
-    const T* p = src + (size_t)(in ? row0 + r : 0) * D + chunk * 4;
+    const T* p = src + (size_t)(in ? row0 + r : 0) * pitch + chunk * 4;
     float* q = dst + lay.at(r, chunk);
     if constexpr (sizeof(T) == 4) cp_async16(q, p, in);
     else *reinterpret_cast<float4*>(q) = in ? widen4<T>(p) : make_float4(0.f, 0.f, 0.f, 0.f);
@@ -211,9 +212,10 @@ __host__ __device__ constexpr int smem_floats(int D) {
 
 // DC: 1 for D <= 64, 2 up to 128.
 // The work of CTA `block` of a kind's grid.
-template <int KIND, int DC, typename T>
-__device__ __forceinline__ void simt_tile(const Geometry& g, const Tensors& t, const int split, const int block) {
+template <int KIND, int DC, typename T, typename Geo>
+__device__ __forceinline__ void simt_tile(const Geo& g, const Tensors& t, const int split, const int block) {
   using SP = Spec<KIND>;
+  constexpr bool kPacked = Geo::kPacked;
   constexpr int RA = rows_of(KIND, DC), NT = threads_of(KIND, DC);
   // g_dO = P g_dV + (P o gdS) V - dot2 o (P V).  In fp32 P V is the O of the call; an O of half precision has
   // been rounded, so there the kernel sums its own (bf16, g_dK offset by one: relative error 1.66e-3
@@ -223,12 +225,37 @@ __device__ __forceinline__ void simt_tile(const Geometry& g, const Tensors& t, c
   extern __shared__ __align__(16) float smem[];
   const int D = g.D;
   const Layout lay(D);
-  const int n_stat = SP::kCol ? g.N_kv : g.N_q, n_strm = SP::kCol ? g.N_q : g.N_kv;
+  int n_stat = SP::kCol ? g.N_kv : g.N_q, n_strm = SP::kCol ? g.N_q : g.N_kv;      // rows of either axis that may be read
   const int tiles = (n_stat + TS - 1) / TS;
   const int unit = block / split, part = block - unit * split;
   const int bh = unit % g.BH, rank = unit / g.BH;
   const int tile = (SP::kCol || g.mask_mode != 0) ? rank : tiles - 1 - rank;     // heavy tiles first
-  const int r0 = tile * TS;
+  int r0 = tile * TS, lo, hi;
+  // a packed batch's entry holds kPlanRows / TS tiles; the keys of one meet the queries of all heads of their group
+  [[maybe_unused]] PackedWork work = {};
+  int heads = 1;
+  if constexpr (kPacked) {
+    constexpr int kParts = kPlanRows / TS;
+    tc::pdl_begin(g);
+    if (!packed_work(g, SP::kCol, rank / kParts, work) || (r0 = work.r0 + rank % kParts * TS) >= work.row_end) {
+      tc::pdl_trigger();
+      tc::pdl_end(g);
+      return;
+    }
+    n_stat = work.row_end;
+    lo = hi = r0;
+    if (work.lo < work.hi) {      // what these TS rows see, or are seen by
+      const int last = min(r0 + TS, n_stat) - 1;
+      if constexpr (SP::kCol) hi = (int)min((long long)work.end, (long long)last + g.window);
+      else { lo = max(work.begin, r0 - g.window + 1); hi = last + 1; }
+      if (hi < lo) hi = lo;
+    }
+    n_strm = hi;
+    if (SP::kCol) heads = g.group;
+  } else {
+    if constexpr (SP::kCol) query_range_for_keys(g, r0, r0 + TS, lo, hi);
+    else key_range_for_queries(g, r0, r0 + TS, lo, hi);
+  }
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int ty = (lane & 1) | ((lane >> 4) << 1), tx = (lane >> 1) & 7, wcol = warp & 1;      // 2 x 2 in every quad of lanes
   const int row0 = (warp >> 1) * 4 * RA + ty;         // this thread's rows: row0 + 4 a
@@ -245,7 +272,17 @@ __device__ __forceinline__ void simt_tile(const Geometry& g, const Tensors& t, c
   for (int i = 0; i < 3; ++i) { op[i] = p; if (i < SP::kNOp) p += TS * TT; }
   float* const aux = p;                               // [4][64]: scalars of the streamed queries, or row exchange
 
-  const size_t q_off = (size_t)bh * g.N_q * D, kv_off = (size_t)bh * g.N_kv * D, row_off = (size_t)bh * g.N_q;
+  // packed tensors are [rows, heads, D]; bh is a query head, in the column kinds a key head whose queries' first head is q_head
+  const int q_head = kPacked && SP::kCol ? bh * heads : bh;
+  size_t q_pitch = D, kv_pitch = D, q_off = (size_t)bh * g.N_q * D, kv_off = (size_t)bh * g.N_kv * D, row_off = (size_t)bh * g.N_q;
+  if constexpr (kPacked) {
+    q_pitch = (size_t)g.q_heads * D;
+    kv_pitch = (size_t)g.kv_heads * D;
+    q_off = (size_t)q_head * D;
+    kv_off = (size_t)(SP::kCol ? bh : bh / g.group) * D;
+    row_off = (size_t)q_head * g.N_q;
+  }
+  const size_t stat_pitch = SP::kCol ? kv_pitch : q_pitch, strm_pitch = SP::kCol ? q_pitch : kv_pitch;
   const T* const Q = (const T*)t.Q + q_off;
   const T* const K = (const T*)t.K + kv_off;
   const T* const V = (const T*)t.V + kv_off;
@@ -257,17 +294,16 @@ __device__ __forceinline__ void simt_tile(const Geometry& g, const Tensors& t, c
   const T* const stat_src[4] = {SP::kCol ? K : Q, SP::kCol ? V : dO, SP::kCol ? gK : gQ, gV};
   const T* const strm_src[4] = {SP::kCol ? Q : K, SP::kCol ? dO : V, SP::kCol ? gQ : gK, gV};
 
-  int lo, hi;
-  if constexpr (SP::kCol) query_range_for_keys(g, r0, r0 + TS, lo, hi);
-  else key_range_for_queries(g, r0, r0 + TS, lo, hi);
-  const int t_end = hi > lo ? (hi + TT - 1) / TT : 0;
-  const int t_first = lo / TT + part;
+  // streamed tiles t_first, t_first + split, ...; a packed batch's start at lo, head by head
+  const int head_tiles = kPacked ? (hi - lo + TT - 1) / TT : 0;
+  const int t_end = kPacked ? heads * head_tiles : hi > lo ? (hi + TT - 1) / TT : 0;
+  const int t_first = kPacked ? 0 : lo / TT + part;
 
   tc::pdl_begin(g);
   tc::pdl_trigger();
 
 #pragma unroll
-  for (int i = 0; i < SP::kNStat; ++i) stage_tile<DC, NT, T>(stat[i], lay, stat_src[i], r0, TS, n_stat, D);
+  for (int i = 0; i < SP::kNStat; ++i) stage_tile<DC, NT, T>(stat[i], lay, stat_src[i], r0, TS, n_stat, D, stat_pitch);
 
   // ---- scalars of this thread's rows (row kinds)
   float L2[RA] = {}, Dv[RA] = {}, d2[RA] = {}, d3[RA] = {};
@@ -275,7 +311,7 @@ __device__ __forceinline__ void simt_tile(const Geometry& g, const Tensors& t, c
 #pragma unroll
     for (int a = 0; a < RA; ++a) {
       const int r = r0 + row0 + 4 * a;
-      const bool in = r < g.N_q;
+      const bool in = r < (kPacked ? n_stat : g.N_q);
       L2[a] = in ? tc::from_l2(t.L + row_off + r) * kLog2e : INFINITY;
       if constexpr (KIND == K_HVP_ROW) {
         if (in) { Dv[a] = tc::from_l2(t.Dv + row_off + r); d2[a] = tc::from_l2(t.dot2 + row_off + r); d3[a] = tc::from_l2(t.dot3 + row_off + r); }
@@ -284,7 +320,7 @@ __device__ __forceinline__ void simt_tile(const Geometry& g, const Tensors& t, c
         float s = 0.f;
         if (in)
           for (int c = tx; c < chunks; c += 8) {
-            const float4 x = load4(dO + (size_t)r * D + 4 * c), y = load4(O + (size_t)r * D + 4 * c);
+            const float4 x = load4(dO + (size_t)r * q_pitch + 4 * c), y = load4(O + (size_t)r * q_pitch + 4 * c);
             s += x.x * y.x + x.y * y.y + x.z * y.z + x.w * y.w;
           }
         Dv[a] = row_sum(s);
@@ -304,10 +340,12 @@ __device__ __forceinline__ void simt_tile(const Geometry& g, const Tensors& t, c
       for (int c = 0; c < DC; ++c) out[o][a][c][0] = out[o][a][c][1] = make_float2(0.f, 0.f);
 
   for (int tt = t_first; tt < t_end; tt += split) {
-    const int s0 = tt * TT;
+    const int head = kPacked ? tt / head_tiles : 0;
+    const int s0 = kPacked ? lo + (tt - head * head_tiles) * TT : tt * TT;
+    const size_t head_off = kPacked ? (size_t)head * D : 0, head_rows = kPacked ? (size_t)head * g.N_q : 0;
     __syncthreads();                                  // the previous tile has been used
 #pragma unroll
-    for (int i = 0; i < SP::kNStream; ++i) stage_tile<DC, NT, T>(strm[i], lay, strm_src[i], s0, TT, n_strm, D);
+    for (int i = 0; i < SP::kNStream; ++i) stage_tile<DC, NT, T>(strm[i], lay, strm_src[i] + head_off, s0, TT, n_strm, D, strm_pitch);
     if constexpr (SP::kCol) {                         // [L2 | Dv | dot2 | dot3] of the streamed queries
       if constexpr (SP::kHvp) {
 #pragma unroll
@@ -320,16 +358,17 @@ __device__ __forceinline__ void simt_tile(const Geometry& g, const Tensors& t, c
       } else {
         constexpr int TQ = NT / TT;                   // threads per query
         const int r = s0 + tid / TQ;
+        const bool in = r < (kPacked ? n_strm : g.N_q);
         float s = 0.f;
-        if (r < g.N_q)
+        if (in)
           for (int c = tid % TQ; c < chunks; c += TQ) {
-            const float4 x = load4(dO + (size_t)r * D + 4 * c), y = load4(O + (size_t)r * D + 4 * c);
+            const float4 x = load4(dO + head_off + (size_t)r * q_pitch + 4 * c), y = load4(O + head_off + (size_t)r * q_pitch + 4 * c);
             s += x.x * y.x + x.y * y.y + x.z * y.z + x.w * y.w;
           }
 #pragma unroll
         for (int o = TQ / 2; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
         if (tid % TQ == 0) {
-          aux[tid / TQ] = r < g.N_q ? tc::from_l2(t.L + row_off + r) * kLog2e : INFINITY;
+          aux[tid / TQ] = in ? tc::from_l2(t.L + row_off + head_rows + r) * kLog2e : INFINITY;
           aux[TT + tid / TQ] = s;
         }
       }
@@ -338,9 +377,13 @@ __device__ __forceinline__ void simt_tile(const Geometry& g, const Tensors& t, c
     __syncthreads();
     float s[SP::kNAcc][RA][CB];
     scores<KIND, RA>(stat, strm, lay, D, row0, col0, s);
-    const bool full = SP::kCol ? tile_fully_visible(g, s0, s0 + TT, r0, r0 + TS) : tile_fully_visible(g, r0, r0 + TS, s0, s0 + TT);
+    const bool full = kPacked ? false : SP::kCol ? tile_fully_visible(g, s0, s0 + TT, r0, r0 + TS) : tile_fully_visible(g, r0, r0 + TS, s0, s0 + TT);
     auto sees = [&](int a, int b) {
       const int i = r0 + row0 + 4 * a, j = s0 + col0 + 8 * b;
+      if constexpr (kPacked) {
+        const int q = SP::kCol ? j : i, k = SP::kCol ? i : j;      // rows behind either range are not in this sequence
+        return i < n_stat && j < n_strm && q >= k && q < k + g.window;
+      }
       return full || (SP::kCol ? visible(g, j, i) : visible(g, i, j));
     };
 
@@ -472,12 +515,12 @@ __device__ __forceinline__ void simt_tile(const Geometry& g, const Tensors& t, c
     for (int q = 0; q < split; ++q) v += row_part(q, which, 0, r) + row_part(q, which, 1, r);
     return v;
   };
-  if (tid < TS && part == 0 && r0 + tid < g.N_q) {
+  if (tid < TS && part == 0 && r0 + tid < (kPacked ? n_stat : g.N_q)) {
     if constexpr (KIND == K_FWD) {
       const float m = fwd_max(tid);
       float l = 0.f;
       for (int q = 0; q < split; ++q) l += (row_part(q, 1, 0, tid) + row_part(q, 1, 1, tid)) * factor(q, tid, m);
-      t.out_L[row_off + r0 + tid] = l > 0.f ? (m + log2f(l)) * kLn2 : -INFINITY;
+      t.out_L[row_off + r0 + tid] = l > 0.f ? (m + log2f(l)) * kLn2 : kPacked && l != l ? l : -INFINITY;
     } else if constexpr (KIND == K_HVP_PRE) {
       const float D_ = row_total(0, tid), d2_ = row_total(1, tid), A = row_total(2, tid), E = row_total(3, tid);
       t.Dv[row_off + r0 + tid] = D_;
@@ -488,7 +531,7 @@ __device__ __forceinline__ void simt_tile(const Geometry& g, const Tensors& t, c
   // one float4 of output o, row r (within the tile), given its sum over the parts (and that of P V)
   auto finish = [&](int o, int r, int chunk, float4 v, float4 pv) {
     if (r0 + r >= n_stat) return;
-    const size_t at = (size_t)(r0 + r) * D + 4 * chunk;
+    const size_t at = (size_t)(r0 + r) * stat_pitch + 4 * chunk;
     float mul = 1.f;
     if constexpr (KIND == K_BWD_ROW || KIND == K_HVP_ROW) mul = g.scale;
     if constexpr (KIND == K_BWD_COL) mul = o == 1 ? g.scale : 1.f;
@@ -497,7 +540,7 @@ __device__ __forceinline__ void simt_tile(const Geometry& g, const Tensors& t, c
       const float m = fwd_max(r);
       float l = 0.f;
       for (int q = 0; q < split; ++q) l += (row_part(q, 1, 0, r) + row_part(q, 1, 1, r)) * factor(q, r, m);
-      mul = l > 0.f ? 1.f / l : 0.f;
+      mul = l > 0.f ? 1.f / l : kPacked && l != l ? l : 0.f;
     }
     v = make_float4(v.x * mul, v.y * mul, v.z * mul, v.w * mul);
     if constexpr (KIND == K_HVP_PRE) {
@@ -549,9 +592,9 @@ __device__ __forceinline__ void simt_tile(const Geometry& g, const Tensors& t, c
   tc::pdl_end(g);
 }
 
-template <int KIND, int DC, typename T>
-__global__ void __launch_bounds__(threads_of(KIND, DC), DC == 1 ? 2 : 1) attn_simt_kernel(const Geometry g, const Tensors t, const int split) {
-  simt_tile<KIND, DC, T>(g, t, split, blockIdx.x);
+template <int KIND, int DC, typename T, typename Geo = Geometry>
+__global__ void __launch_bounds__(threads_of(KIND, DC), DC == 1 ? 2 : 1) attn_simt_kernel(const Geo g, const Tensors t, const int split) {
+  simt_tile<KIND, DC, T, Geo>(g, t, split, blockIdx.x);
 }
 
 // Two kinds of one operation that do not depend on each other in one grid, the CTAs of FIRST in front: one
@@ -560,8 +603,8 @@ template <int FIRST, int SECOND, int DC, typename T>
 __global__ void __launch_bounds__(threads_of(FIRST, DC), DC == 1 ? 2 : 1)
 attn_simt_pair_kernel(const Geometry g, const Tensors t, const int split, const int first_ctas) {
   static_assert(threads_of(FIRST, DC) == threads_of(SECOND, DC), "one launch configuration");
-  if ((int)blockIdx.x < first_ctas) simt_tile<FIRST, DC, T>(g, t, split, blockIdx.x);
-  else simt_tile<SECOND, DC, T>(g, t, split, blockIdx.x - first_ctas);
+  if ((int)blockIdx.x < first_ctas) simt_tile<FIRST, DC, T, Geometry>(g, t, split, blockIdx.x);
+  else simt_tile<SECOND, DC, T, Geometry>(g, t, split, blockIdx.x - first_ctas);
 }
 
 template <int KIND>
@@ -646,6 +689,29 @@ static cudaError_t launch_two(const Geometry& g, const Tensors& t, cudaStream_t 
   return g.D <= 64 ? launch_two_dc<FIRST, SECOND, 1, T>(g, t, stream, n, which) : launch_two_dc<FIRST, SECOND, 2, T>(g, t, stream, n, which);
 }
 
+// packed batches: one CTA per tile
+template <int KIND, int DC>
+static cudaError_t launch_packed_kind(PackedGeometry g, const Tensors& t, cudaStream_t stream) {
+  g.BH = Spec<KIND>::kCol ? g.kv_heads : g.q_heads;
+  const long long ctas = (long long)g.BH * g.cap * (kPlanRows / TS);
+  if (ctas > 0x7fffffffLL) return cudaErrorInvalidValue;
+  auto kern = attn_simt_kernel<KIND, DC, float, PackedGeometry>;
+  static std::atomic<unsigned long long> smem_set{0};
+  const cudaError_t e = tc::set_smem_once(kern, kVariantSmem<KIND, DC>, smem_set);
+  return e != cudaSuccess ? e : tc::launch_pdl(kern, (unsigned)ctas, threads_of(KIND, DC), sizeof(float) * smem_floats<KIND>(g.D), stream, g, t, 1);
+}
+
+template <int DC>
+static cudaError_t dispatch_packed(int op, const PackedGeometry& g, const Tensors& t, cudaStream_t s, int* n) {
+  *n = 1;
+  if (op == OP_FORWARD) return launch_packed_kind<K_FWD, DC>(g, t, s);
+  *n = 2;
+  const cudaError_t e = launch_packed_kind<K_BWD_COL, DC>(g, t, s);
+  PackedGeometry second = g;
+  second.beside = 1;
+  return e != cudaSuccess ? e : launch_packed_kind<K_BWD_ROW, DC>(second, t, s);
+}
+
 template <typename T>
 static cudaError_t dispatch(int op, const Geometry& g, const Tensors& t, cudaStream_t s, int* n, int phases) {
   cudaError_t e = cudaSuccess;
@@ -669,6 +735,10 @@ static cudaError_t dispatch(int op, const Geometry& g, const Tensors& t, cudaStr
 }
 
 }  // namespace simt
+
+cudaError_t launch_packed_simt(int op, const PackedGeometry& g, const Tensors& t, cudaStream_t s, int* launches) {
+  return g.D <= 64 ? simt::dispatch_packed<1>(op, g, t, s, launches) : simt::dispatch_packed<2>(op, g, t, s, launches);
+}
 
 cudaError_t launch_simt(int op, int dtype, const Geometry& g, const Tensors& t, cudaStream_t s,
                         int* launches, int phases) {

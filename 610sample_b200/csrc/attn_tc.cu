@@ -4,6 +4,7 @@
 // the first backward and the tcgen05 primitive self-test.
 #include "attn_common.cuh"
 #include "attn_launch.h"
+#include "packed_launch.h"
 #include "tc_common.cuh"
 
 #include <cstdio>
@@ -217,15 +218,15 @@ static EncodeTiledFn get_encode_fn() {
 // [planes][rows][cols] half-precision tensor, box = 64 cols x 64 rows x 1 plane, 128-byte swizzle.
 static thread_local char tl_encode_error[160] = "";
 
-static bool encode_map(CUtensorMap* map, const void* ptr, int is_bf16, long long planes, long long rows,
-                       long long cols, int box_rows = 64) {
+static bool encode_strided(CUtensorMap* map, const void* ptr, int is_bf16, long long planes, long long rows, long long cols,
+                           long long row_stride, long long plane_stride, int box_rows) {
   EncodeTiledFn fn = get_encode_fn();
   if (!fn) {
     snprintf(tl_encode_error, sizeof(tl_encode_error), "driver entry point cuTensorMapEncodeTiled not found");
     return false;
   }
   cuuint64_t dims[3] = {(cuuint64_t)cols, (cuuint64_t)rows, (cuuint64_t)planes};
-  cuuint64_t strides[2] = {(cuuint64_t)cols * 2, (cuuint64_t)rows * (cuuint64_t)cols * 2};
+  cuuint64_t strides[2] = {(cuuint64_t)row_stride * 2, (cuuint64_t)plane_stride * 2};
   cuuint32_t box[3] = {64, (cuuint32_t)box_rows, 1};
   cuuint32_t estr[3] = {1, 1, 1};
   CUresult r = fn(map, is_bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 3,
@@ -236,6 +237,11 @@ static bool encode_map(CUtensorMap* map, const void* ptr, int is_bf16, long long
     snprintf(tl_encode_error, sizeof(tl_encode_error),
              "cuTensorMapEncodeTiled returned %d for ptr=%p dims=[%lld,%lld,%lld]", (int)r, ptr, planes, rows, cols);
   return r == CUDA_SUCCESS;
+}
+
+static bool encode_map(CUtensorMap* map, const void* ptr, int is_bf16, long long planes, long long rows,
+                       long long cols, int box_rows = 64) {
+  return encode_strided(map, ptr, is_bf16, planes, rows, cols, cols, rows * cols, box_rows);
 }
 
 // The maps an operation uses; the others are left alone.
@@ -315,6 +321,84 @@ cudaError_t launch_tc(int op, int dtype, const Geometry& g, const Tensors& t, cu
   if (!encode_maps(&maps, op, g, t, bf, err)) return cudaErrorInvalidValue;
   return bf ? launch_op<__nv_bfloat16>(op, maps, g, t, s, launches, phases)
             : launch_op<__half>(op, maps, g, t, s, launches, phases);
+}
+
+namespace tc {
+
+cudaError_t launch_packed_fwd(int is_bf16, const TmaMaps& maps, const PackedGeometry& g, const Tensors& t, cudaStream_t s);
+cudaError_t launch_packed_bwd(int is_bf16, const TmaMaps& maps, const PackedGeometry& g, const Tensors& t, cudaStream_t s, int* launches);
+
+// D_i of a packed batch: dO [n_tok, heads, D] in strides, O dense, out [heads, n_tok].  Eight or sixteen lanes own a row,
+// 16 bytes each; consecutive lane groups take consecutive heads, which lie side by side in memory.  Bound by one read of dO and O.
+template <typename T, int G>
+__global__ void __launch_bounds__(256)
+packed_rowdot_kernel(const T* dO, const T* O, float* out, int n_tok, int heads, int D, long long row_stride, long long head_stride) {
+  pdl_wait();
+  pdl_trigger();
+  const int sub = threadIdx.x % G;
+  const long long r = (long long)blockIdx.x * (256 / G) + threadIdx.x / G, rows = (long long)n_tok * heads;
+  const bool in = r < rows;
+  const int tok = in ? (int)(r / heads) : 0, h = in ? (int)(r - (long long)tok * heads) : 0;
+  float acc = 0.f;
+  if (in && sub * 8 < D) {
+    const uint4 a = from_l2(reinterpret_cast<const uint4*>(dO + tok * row_stride + h * head_stride + sub * 8));
+    const uint4 b = from_l2(reinterpret_cast<const uint4*>(O + r * D + sub * 8));
+    const uint32_t wa[4] = {a.x, a.y, a.z, a.w}, wb[4] = {b.x, b.y, b.z, b.w};
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {
+      const float2 x = widen_pair<T>(wa[q]), y = widen_pair<T>(wb[q]);
+      acc = fmaf(x.x, y.x, acc);
+      acc = fmaf(x.y, y.y, acc);
+    }
+  }
+#pragma unroll
+  for (int o = G / 2; o > 0; o >>= 1) acc += __shfl_xor_sync(0xffffffffu, acc, o);
+  if (in && sub == 0) out[(long long)h * n_tok + tok] = acc;
+}
+
+template <typename T>
+static cudaError_t launch_packed_rowdot(const Tensors& t, const PackedGeometry& g, const PackedStrides& st, cudaStream_t s) {
+  const int G = g.D <= 64 ? 8 : 16;
+  const long long ctas = ((long long)g.N_q * g.q_heads + 256 / G - 1) / (256 / G);
+  if (ctas > 0x7fffffffLL) return cudaErrorInvalidValue;
+  auto kern = G == 8 ? packed_rowdot_kernel<T, 8> : packed_rowdot_kernel<T, 16>;
+  return launch_pdl(kern, (unsigned)ctas, 256, 0, s, (const T*)t.dO, (const T*)t.O, t.Dv, g.N_q, g.q_heads, g.D, st.row, st.head);
+}
+
+}  // namespace tc
+
+cudaError_t launch_packed_tc(int op, int dtype, const PackedGeometry& g, const Tensors& t, const PackedLayout& lay, cudaStream_t s,
+                             int* launches, const char** err) {
+  using namespace tc;
+  *err = nullptr;
+  TmaMaps maps;
+  const int bf = dtype == 1, n_in = op == OP_FORWARD ? 3 : 4;
+  const TensorId ids[PI_COUNT] = {T_Q, T_K, T_V, T_dO};
+  const void* ins[PI_COUNT] = {t.Q, t.K, t.V, t.dO};
+  bool ok = true;
+  for (int i = 0; i < n_in && ok; ++i)
+    ok = encode_strided(&maps.m[ids[i]], ins[i], bf, i == PI_K || i == PI_V ? g.kv_heads : g.q_heads, g.N_q, g.D, lay.of[i].row, lay.of[i].head, 64);
+  auto out = [&](int id, void* p, int heads) {
+    ok = ok && encode_strided(&maps.out[id], p, bf, heads, g.N_q, g.D, (long long)heads * g.D, g.D, 128);
+  };
+  if (op == OP_FORWARD) {
+    out(TO_O, t.out_O, g.q_heads);
+  } else {
+    out(TO_dQ, t.out_dQ, g.q_heads);
+    out(TO_dK, t.out_dK, g.kv_heads);
+    out(TO_dV, t.out_dV, g.kv_heads);
+  }
+  if (!ok) {
+    *err = tl_encode_error;
+    return cudaErrorInvalidValue;
+  }
+  if (op == OP_FORWARD) {
+    *launches = 1;
+    return launch_packed_fwd(bf, maps, g, t, s);
+  }
+  *launches = 1;
+  const cudaError_t e = bf ? launch_packed_rowdot<__nv_bfloat16>(t, g, lay.of[PI_dO], s) : launch_packed_rowdot<__half>(t, g, lay.of[PI_dO], s);
+  return e != cudaSuccess ? e : launch_packed_bwd(bf, maps, g, t, s, launches);
 }
 
 cudaError_t launch_tc_selftest(const void* A, const void* B, float* C, int N, int K, int dtype, int flags,

@@ -50,6 +50,7 @@ struct FbControl {
   uint64_t ra_free[2];       // the scores of a tile are in the math warps' registers
   uint64_t acc_done;
   uint64_t stats_ready[2];
+  uint64_t ragged_full;      // packed batches: a tile whose last rows are to be cleared
   uint32_t tmem_base;
   volatile uint32_t abort_flag;
 };
@@ -96,16 +97,18 @@ struct FbCfg {
   __host__ __device__ static constexpr int stream_tensor(int s) { return kCol ? (s == 0 ? T_Q : T_dO) : (s == 0 ? T_K : T_V); }
 };
 
-template <int KIND, int D, typename T, bool SPLIT, bool DUAL>
+template <int KIND, int D, typename T, bool SPLIT, bool DUAL, typename Geo = Geometry>
 struct fb_kernel {
   using CF = FbCfg<KIND, D, DUAL>;
   static constexpr int kThreads = CF::kThreads, kPerSm = DUAL ? 2 : 1;
-  static __device__ __forceinline__ void run(const TmaMaps& maps, const Geometry& g, const Tensors& t, unsigned block);
+  static __device__ __forceinline__ void run(const TmaMaps& maps, const Geo& g, const Tensors& t, unsigned block);
 };
 
-template <int KIND, int D, typename T, bool SPLIT, bool DUAL>
-__device__ __forceinline__ void fb_kernel<KIND, D, T, SPLIT, DUAL>::run(const TmaMaps& maps, const Geometry& g, const Tensors& t,
-                                                                        const unsigned block) {
+template <int KIND, int D, typename T, bool SPLIT, bool DUAL, typename Geo>
+__device__ __forceinline__ void fb_kernel<KIND, D, T, SPLIT, DUAL, Geo>::run(const TmaMaps& maps, const Geo& g, const Tensors& t,
+                                                                             const unsigned block) {
+  constexpr bool kPacked = Geo::kPacked;
+  static_assert(!(kPacked && SPLIT), "packed batches are not split");
   constexpr int kAtoms = CF::kAtoms, kHalves = CF::kHalves;
   constexpr int kMathWarps = CF::kMathWarps, kMathThreads = CF::kMathThreads, kProducerWarp = CF::kProducerWarp;
   constexpr int kFbMmaWarp = CF::kMmaWarp, kTmemCols = CF::kTmemCols;
@@ -133,23 +136,41 @@ __device__ __forceinline__ void fb_kernel<KIND, D, T, SPLIT, DUAL>::run(const Tm
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int n_stat = CF::kCol ? g.N_kv : g.N_q;
-  const int tiles = (n_stat + BM - 1) / BM;
+  const int tiles = kPacked ? packed_cap(g) : (n_stat + BM - 1) / BM;
   const unsigned split = SPLIT ? (unsigned)g.split : 1u;      // CTAs that share this tile: a cluster (tc_common.cuh)
   const int part = SPLIT ? (int)(block % split) : 0;
   int bh, rank;
   tile_to_head_and_rank(g, block / split, tiles, bh, rank);
-  const int tile = (CF::kCol || g.mask_mode != 0) ? rank : (tiles - 1 - rank);   // heavy tiles first
-  const int r0 = tile * BM;
-
-  int lo, hi;
-  if (CF::kCol) query_range_for_keys(g, r0, r0 + BM, lo, hi);
-  else key_range_for_queries(g, r0, r0 + BM, lo, hi);
-  int t_begin = lo / BN;
-  int n_iter = (hi > lo) ? ((hi + BN - 1) / BN - t_begin) : 0;
+  [[maybe_unused]] PackedWork work = {};
+  int r0, lo, hi;
+  if constexpr (kPacked) {
+    pdl_begin(g);          // the plan may be the work of the kernel before
+    if (!packed_work(g, CF::kCol, rank, work)) {
+      pdl_trigger();
+      pdl_end(g);
+      return;
+    }
+    r0 = work.r0; lo = work.lo; hi = work.hi;
+  } else {
+    const int tile = (CF::kCol || g.mask_mode != 0) ? rank : (tiles - 1 - rank);   // heavy tiles first
+    r0 = tile * BM;
+    if (CF::kCol) query_range_for_keys(g, r0, r0 + BM, lo, hi);
+    else key_range_for_queries(g, r0, r0 + BM, lo, hi);
+  }
+  int t_begin = kPacked ? 0 : lo / BN;
+  int n_iter = (hi > lo) ? (kPacked ? (hi - lo + BN - 1) / BN : (hi + BN - 1) / BN - t_begin) : 0;
+  const int row_end = kPacked ? work.row_end : n_stat;
+  // keys of a packed batch meet the queries of all heads of their group, one head after the other
+  const int head_iter = n_iter;
+  if constexpr (kPacked && CF::kCol) n_iter *= g.group;
   if (n_iter == 0) {       // nothing to visit
     pdl_begin(g);
     pdl_trigger();
-    if (part == 0) {
+    if constexpr (kPacked) {
+      const int heads = CF::kCol ? g.kv_heads : g.q_heads;
+      store_packed_rows<true>(CF::kCol ? t.out_dK : t.out_dQ, 0u, r0, row_end, bh, heads, g.D, blockDim.x);
+      if constexpr (CF::kCol) store_packed_rows<true>(t.out_dV, 0u, r0, row_end, bh, heads, g.D, blockDim.x);
+    } else if (part == 0) {
       if constexpr (CF::kCol) {
         zero_rows(t.out_dK, bh, r0, g.N_kv, g.D, blockDim.x);
         zero_rows(t.out_dV, bh, r0, g.N_kv, g.D, blockDim.x);
@@ -194,21 +215,35 @@ __device__ __forceinline__ void fb_kernel<KIND, D, T, SPLIT, DUAL>::run(const Tm
       mbar_init(smem_u32(&ctl->stats_ready[b]), kMathWarps);
     }
     mbar_init(bar_acc_done, 1);
+    if constexpr (kPacked) mbar_init(smem_u32(&ctl->ragged_full), 1);
     ctl->abort_flag = 0u;
     fence_barrier_init();
     fence_proxy_async_smem();
   }
+  const int strm0 = kPacked ? lo : t_begin * BN;      // first streamed row
+  const int last_rows = kPacked ? (hi - lo) % BN : 0; // of a head's last tile, where they are not all of it
+  // tile `it` of the stream: its plane, its first row, whether its last rows are to be cleared
+  auto plane_of = [&](int it) {
+    if constexpr (kPacked) return CF::kCol ? bh * g.group + it / head_iter : kv_plane_of(g, bh);
+    else return bh;
+  };
+  auto row_of = [&](int it) {
+    if constexpr (kPacked && CF::kCol) return strm0 + (it % head_iter) * BN;
+    else return strm0 + it * BN;
+  };
+  auto is_ragged = [&](int it) { return kPacked && last_rows != 0 && (it + 1) % head_iter == 0; };
   // the streamed tile `it` into its stage
   auto request_tile = [&](int it) {
     const int st = it % CF::kStages;
-    mbar_arrive_expect_tx(bar_stream_full(st), CF::kStageBytes);
+    const uint32_t bar = is_ragged(it) ? smem_u32(&ctl->ragged_full) : bar_stream_full(st);
+    mbar_arrive_expect_tx(bar, CF::kStageBytes);
     const uint32_t stage = strm_base + st * CF::kStageBytes;
+    const int row = row_of(it), plane = plane_of(it);
 #pragma unroll
     for (int s = 0; s < CF::kNStream; ++s)
 #pragma unroll
       for (int a = 0; a < kAtoms; ++a)
-        tma_load_3d(stage + CF::stream_off(s, a), &maps.m[CF::stream_tensor(s)], a * 64, (t_begin + it) * BN, bh,
-                    bar_stream_full(st));
+        tma_load_3d(stage + CF::stream_off(s, a), &maps.m[CF::stream_tensor(s)], a * 64, row, plane, bar);
   };
   if (warp == kFbMmaWarp) tmem_alloc(smem_u32(&ctl->tmem_base), kTmemCols);
   pdl_begin(g);
@@ -237,7 +272,35 @@ __device__ __forceinline__ void fb_kernel<KIND, D, T, SPLIT, DUAL>::run(const Tm
   // TMA producer
   // =========================================================================
   if (warp == kProducerWarp) {
-    if (lane == 0 && n_iter > 0) {
+    if constexpr (kPacked) {
+      // The whole warp, to clear the rows of ragged tiles (clear_tile_rows).  One is cleared after the next tile has been
+      // requested: the wait for that one's stage never needs the ragged tile before it.
+      bool ok = true;
+      uint32_t cleared = 0;
+      auto clear = [&](int it) {
+        ok = __all_sync(0xffffffffu, mbar_wait(smem_u32(&ctl->ragged_full), cleared & 1, abort_flag, t.status, wait_code(KCODE, 11)));
+        ++cleared;
+        if (!ok) return;
+        const int st = it % CF::kStages;
+        clear_tile_rows(strm_base + st * CF::kStageBytes, CF::kNStream * kAtoms, last_rows);
+        if (lane == 0) mbar_arrive(bar_stream_full(st));
+      };
+      for (int it = 1; it <= n_iter && ok; ++it) {     // tile 0 was requested above
+        // two ragged tiles in a row (heads of one tile each) share a barrier: the first is cleared before the second is requested
+        const bool before = is_ragged(it - 1), early = before && it < n_iter && is_ragged(it);
+        if (early) clear(it - 1);
+        if (ok && it < n_iter) {
+          ok = __all_sync(0xffffffffu, mbar_wait(bar_stream_empty(it % CF::kStages), ((it / CF::kStages) & 1) ^ 1, abort_flag, t.status, wait_code(KCODE, 1)));
+          if (ok && lane == 0) request_tile(it);
+          __syncwarp();
+        }
+        if (ok && before && !early) clear(it - 1);
+      }
+      if (!ok) {   // give copies already in flight a bounded chance to land before the CTA exits
+        const long long t0 = clock64();
+        while (clock64() - t0 < 2000000LL) { }
+      }
+    } else if (lane == 0 && n_iter > 0) {
       bool ok = true;
       for (int it = 1; it < n_iter; ++it) {     // tile 0 was requested above
         ok = mbar_wait(bar_stream_empty(it % CF::kStages), ((it / CF::kStages) & 1) ^ 1, abort_flag, t.status, wait_code(KCODE, 1));
@@ -381,9 +444,13 @@ __device__ __forceinline__ void fb_kernel<KIND, D, T, SPLIT, DUAL>::run(const Tm
     const size_t row_off = (size_t)bh * g.N_q;
 
     int vlo, vhi;                                // streamed indices visible to this stationary row
-    if (CF::kCol) query_range_for_keys(g, gidx, gidx + 1, vlo, vhi);
-    else key_range_for_queries(g, gidx, gidx + 1, vlo, vhi);
-    if (gidx >= n_stat) { vlo = 0; vhi = 0; }
+    if constexpr (kPacked) {
+      packed_row_range(g, work, CF::kCol, gidx, vlo, vhi);
+    } else {
+      if (CF::kCol) query_range_for_keys(g, gidx, gidx + 1, vlo, vhi);
+      else key_range_for_queries(g, gidx, gidx + 1, vlo, vhi);
+      if (gidx >= n_stat) { vlo = 0; vhi = 0; }
+    }
     const uint32_t vspan = (uint32_t)(vhi - vlo);
 
     // ---- one-time copy of the stationary rows from the staging buffer to tensor memory.
@@ -423,7 +490,7 @@ __device__ __forceinline__ void fb_kernel<KIND, D, T, SPLIT, DUAL>::run(const Tm
     // per-row scalars (row kinds), negated so that every use is a packed add / fma
     float2 nL2 = make_float2(-INFINITY, -INFINITY), nDv = make_float2(0.f, 0.f);
     if constexpr (KIND == FB_BWD_ROW) {
-      if (gidx < g.N_q) {
+      if (gidx < row_end) {
         const float L2 = from_l2(t.L + row_off + gidx) * kLog2e, Dv = from_l2(t.Dv + row_off + gidx);
         nL2 = make_float2(-L2, -L2);
         nDv = make_float2(-Dv, -Dv);
@@ -438,10 +505,10 @@ __device__ __forceinline__ void fb_kernel<KIND, D, T, SPLIT, DUAL>::run(const Tm
     // its latency never stalls the warp.
     auto fetch_stat = [&](int tile_it) {
       const int which = (threadIdx.x >> 6) & 1, c = threadIdx.x & 63;
-      const int qi = (t_begin + tile_it) * BN + c;
+      const int qi = row_of(tile_it) + c;
       float raw = (which == 0) ? INFINITY : 0.f;      // beyond N_q: L = +inf (p = 0), Dv = 0
-      if (CF::kCol && threadIdx.x < 128 && tile_it < n_iter && qi < g.N_q)
-        raw = from_l2((which == 0 ? t.L : t.Dv) + row_off + qi);
+      if (CF::kCol && threadIdx.x < 128 && tile_it < n_iter && qi < (kPacked ? hi : g.N_q))
+        raw = from_l2((which == 0 ? t.L : t.Dv) + (kPacked ? (size_t)plane_of(tile_it) * g.N_q : row_off) + qi);
       return raw;
     };
     auto publish_stat = [&](int tile_it, float raw) {
@@ -470,7 +537,7 @@ __device__ __forceinline__ void fb_kernel<KIND, D, T, SPLIT, DUAL>::run(const Tm
           ok = __all_sync(0xffffffffu, ok);
           if (!ok) break;
         }
-        const int j0 = (t_begin + it) * BN;
+        const int j0 = row_of(it);
         const bool masked = !(j0 >= vlo && j0 + BN - 1 < vhi);
         const uint32_t ra = lane_addr + CF::kRA + 64 * b;
         const uint32_t rb = lane_addr + CF::kRB + 64 * b;
@@ -560,7 +627,7 @@ __device__ __forceinline__ void fb_kernel<KIND, D, T, SPLIT, DUAL>::run(const Tm
     } else
     for (int it = 0; it < n_iter && ok; ++it) {
       const int b = it % kBufs;
-      const int j0 = (t_begin + it) * BN;
+      const int j0 = row_of(it);
       const int first = j0 + half * 32;
       const bool masked = !(first >= vlo && first + 31 < vhi);
       const uint32_t ra = lane_addr + CF::kRA + 64 * b + half * 32;
@@ -700,7 +767,14 @@ __device__ __forceinline__ void fb_kernel<KIND, D, T, SPLIT, DUAL>::run(const Tm
       }
       fence_proxy_async_smem();
       named_barrier_sync(2, kMathThreads);
-      if (!SPLIT && threadIdx.x == 0) {
+      if (kPacked && row_end - r0 < BM) {      // uniform over the CTA
+        if constexpr (kPacked) {
+          const int heads = CF::kCol ? g.kv_heads : g.q_heads;
+          store_packed_rows<false>(CF::kCol ? t.out_dV : t.out_dQ, staging, r0, row_end, bh, heads, g.D, kMathThreads);
+          if constexpr (CF::kCol)
+            store_packed_rows<false>(t.out_dK, staging + kAtoms * kAtomBytesStat, r0, row_end, bh, heads, g.D, kMathThreads);
+        }
+      } else if (!SPLIT && threadIdx.x == 0) {
         for (int o = 0; o < CF::kNOut; ++o) {
           const int id = (KIND == FB_BWD_ROW) ? TO_dQ : (o == 0 ? TO_dV : TO_dK);
           for (int a = 0; a * 64 < g.D; ++a)
@@ -803,6 +877,42 @@ static cudaError_t launch_bwd_tiles(const TmaMaps& maps, const Geometry& g, cons
   *launches += 2;
   return side_by_side(g, [&](const Geometry& q) { return launch_fb<FB_BWD_ROW, D, T>(maps, q, t, s, row); },
                       [&](const Geometry& q) { return launch_fb<FB_BWD_COL, D, T>(maps, q, t, s, col); });
+}
+
+// Packed batches: dK/dV, whose tiles cost more, and dQ beside it.
+template <int KIND, int D, typename T, bool DUAL>
+static cudaError_t launch_packed_kind(const TmaMaps& maps, PackedGeometry g, const Tensors& t, cudaStream_t s) {
+  using Kernel = fb_kernel<KIND, D, T, false, DUAL, PackedGeometry>;
+  constexpr bool kCol = KIND == FB_BWD_COL;
+  g.BH = kCol ? g.kv_heads : g.q_heads;
+  const long long ctas = (long long)g.BH * g.cap;
+  if (ctas > 0x7fffffffLL) return cudaErrorInvalidValue;
+  g.head_group = pick_head_group(ctas, g.BH, 2ll * g.N_q * g.D * 2 * (kCol ? g.group : 1));
+  const size_t smem = DUAL ? half_sm_smem(Kernel::CF::kSmemBytes) : whole_sm_smem(Kernel::CF::kSmemBytes);
+  static std::atomic<unsigned long long> smem_set{0};
+  auto kern = tile_kernel<Kernel, PackedGeometry>;
+  const cudaError_t e = set_smem_once(kern, smem, smem_set);
+  return e != cudaSuccess ? e : launch_pdl(kern, (unsigned)ctas, Kernel::kThreads, smem, s, maps, g, t);
+}
+
+template <int D, typename T>
+static cudaError_t launch_packed_bwd_one(const TmaMaps& maps, const PackedGeometry& g, const Tensors& t, cudaStream_t s) {
+  PackedGeometry second = g;
+  second.beside = 1;
+  if constexpr (D == 64) {
+    if ((long long)g.cap * g.kv_heads >= kSms) {
+      const cudaError_t e = launch_packed_kind<FB_BWD_COL, D, T, true>(maps, g, t, s);
+      return e != cudaSuccess ? e : launch_packed_kind<FB_BWD_ROW, D, T, true>(maps, second, t, s);
+    }
+  }
+  const cudaError_t e = launch_packed_kind<FB_BWD_COL, D, T, false>(maps, g, t, s);
+  return e != cudaSuccess ? e : launch_packed_kind<FB_BWD_ROW, D, T, false>(maps, second, t, s);
+}
+
+cudaError_t launch_packed_bwd(int is_bf16, const TmaMaps& maps, const PackedGeometry& g, const Tensors& t, cudaStream_t s, int* launches) {
+  *launches += 2;
+  if (g.D <= 64) return is_bf16 ? launch_packed_bwd_one<64, __nv_bfloat16>(maps, g, t, s) : launch_packed_bwd_one<64, __half>(maps, g, t, s);
+  return is_bf16 ? launch_packed_bwd_one<128, __nv_bfloat16>(maps, g, t, s) : launch_packed_bwd_one<128, __half>(maps, g, t, s);
 }
 
 // dQ, dK and dV, given Dv

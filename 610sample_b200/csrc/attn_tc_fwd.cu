@@ -54,6 +54,7 @@ struct FwdControl {
   uint64_t p_full[kFwdMaxSBufs];       // P written by the owning math group
   uint64_t pv_done[kFwdMaxSBufs];      // the P V product that read the buffer has completed
   uint64_t acc_done;
+  uint64_t ragged_full[2];             // packed batches: the K and the V half of a tile whose last rows are to be cleared
   uint32_t tmem_base;
   volatile uint32_t abort_flag;
 };
@@ -94,10 +95,12 @@ struct FwdCfg {
   }
 };
 
-template <int D, typename T, bool SPLIT, int G>
+template <int D, typename T, bool SPLIT, int G, typename Geo = Geometry>
 __global__ void __launch_bounds__((FwdCfg<D, G>::kThreads), 3 - G)
-fwd_kernel(const __grid_constant__ TmaMaps maps, const Geometry g, const Tensors t) {
+fwd_kernel(const __grid_constant__ TmaMaps maps, const Geo g, const Tensors t) {
   using CF = FwdCfg<D, G>;
+  constexpr bool kPacked = Geo::kPacked;
+  static_assert(!(kPacked && SPLIT), "packed batches are not split");
   constexpr int kAtoms = CF::kAtoms, kFwdSBufs = CF::kSBufs;
   constexpr int kMathWarps = CF::kMathWarps, kMathThreads = CF::kMathThreads, kProducerWarp = CF::kProducerWarp;
   constexpr int kFwdSWarp = CF::kSWarp, kFwdPvWarp = CF::kPvWarp, kTmemCols = CF::kTmemCols;
@@ -126,24 +129,36 @@ fwd_kernel(const __grid_constant__ TmaMaps maps, const Geometry g, const Tensors
   float* part_f = part_ml + 2 * BM;                           // [parts][128]
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int tiles = (g.N_q + BM - 1) / BM;
+  const int tiles = kPacked ? packed_cap(g) : (g.N_q + BM - 1) / BM;
   const unsigned split = SPLIT ? (unsigned)g.split : 1u;      // CTAs that share this tile: a cluster (tc_common.cuh)
   const int part = SPLIT ? (int)(blockIdx.x % split) : 0;
   int bh, rank;
   tile_to_head_and_rank(g, blockIdx.x / split, tiles, bh, rank);
-  const int tile = (g.mask_mode != 0) ? rank : (tiles - 1 - rank);   // heavy tiles first
-  const int r0 = tile * BM;
-
-  int lo, hi;
-  key_range_for_queries(g, r0, r0 + BM, lo, hi);
-  int t_begin = lo / BN;
-  int n_iter = (hi > lo) ? ((hi + BN - 1) / BN - t_begin) : 0;
+  [[maybe_unused]] PackedWork work = {};
+  int r0, lo, hi;
+  if constexpr (kPacked) {
+    pdl_begin(g);          // the plan may be the work of the kernel before
+    if (!packed_work(g, false, rank, work)) {
+      pdl_trigger();
+      pdl_end(g);
+      return;
+    }
+    r0 = work.r0; lo = work.lo; hi = work.hi;
+  } else {
+    const int tile = (g.mask_mode != 0) ? rank : (tiles - 1 - rank);   // heavy tiles first
+    r0 = tile * BM;
+    key_range_for_queries(g, r0, r0 + BM, lo, hi);
+  }
+  int t_begin = kPacked ? 0 : lo / BN;
+  int n_iter = (hi > lo) ? (kPacked ? (hi - lo + BN - 1) / BN : (hi + BN - 1) / BN - t_begin) : 0;
+  const int row_end = kPacked ? work.row_end : g.N_q;
   if (n_iter == 0) {       // nothing to visit
     pdl_begin(g);
     pdl_trigger();
     if (part == 0) {
-      zero_rows(t.out_O, bh, r0, g.N_q, g.D, blockDim.x);
-      if (threadIdx.x < BM && r0 + threadIdx.x < g.N_q) t.out_L[(size_t)bh * g.N_q + r0 + threadIdx.x] = -INFINITY;
+      if constexpr (kPacked) store_packed_rows<true>(t.out_O, 0u, r0, row_end, bh, g.q_heads, g.D, blockDim.x);
+      else zero_rows(t.out_O, bh, r0, g.N_q, g.D, blockDim.x);
+      if (threadIdx.x < BM && r0 + threadIdx.x < row_end) t.out_L[(size_t)bh * g.N_q + r0 + threadIdx.x] = -INFINITY;
     }
     pdl_end(g);
     return;
@@ -178,20 +193,28 @@ fwd_kernel(const __grid_constant__ TmaMaps maps, const Geometry g, const Tensors
       mbar_init(bar_pv_done(b), 1);
     }
     mbar_init(bar_acc_done, 1);
+    if constexpr (kPacked)
+      for (int h = 0; h < 2; ++h) mbar_init(smem_u32(&ctl->ragged_full[h]), 1);
     ctl->abort_flag = 0u;
     fence_barrier_init();
     fence_proxy_async_smem();
   }
 
+  const int strm0 = kPacked ? lo : t_begin * BN;      // first streamed row
+  const int last_rows = kPacked ? (hi - lo) % BN : 0; // of the last tile, where they are not all of it
+  const int kv_plane = kv_plane_of(g, bh);
   // one half of the stage of tile `it`: K (h = 0) or V (h = 1)
   auto request_half = [&](int it, int h) {
     const int st = it % CF::kStages;
     const uint32_t stage = strm_base + st * CF::kStageBytes;
-    mbar_arrive_expect_tx(bar_stream_full(h, st), CF::kStageBytes / 2);
+    uint32_t bar = bar_stream_full(h, st);
+    if constexpr (kPacked) {
+      if (last_rows != 0 && it + 1 == n_iter) bar = smem_u32(&ctl->ragged_full[h]);
+    }
+    mbar_arrive_expect_tx(bar, CF::kStageBytes / 2);
 #pragma unroll
     for (int a = 0; a < kAtoms; ++a)
-      tma_load_3d(stage + CF::stream_off(h, a), &maps.m[h == 0 ? T_K : T_V], a * 64, (t_begin + it) * BN, bh,
-                  bar_stream_full(h, st));
+      tma_load_3d(stage + CF::stream_off(h, a), &maps.m[h == 0 ? T_K : T_V], a * 64, strm0 + it * BN, kv_plane, bar);
   };
   if (warp == kFwdSWarp) tmem_alloc(smem_u32(&ctl->tmem_base), kTmemCols);
   pdl_begin(g);
@@ -217,8 +240,8 @@ fwd_kernel(const __grid_constant__ TmaMaps maps, const Geometry g, const Tensors
   // TMA producer
   // =========================================================================
   if (warp == kProducerWarp) {
+    bool ok = true;
     if (lane == 0 && n_iter > 0) {
-      bool ok = true;
       auto wait_free = [&](int it, int h) {
         if (it < CF::kStages) return true;
         return mbar_wait(bar_stream_empty(h, it % CF::kStages), ((it / CF::kStages) & 1) ^ 1, abort_flag, t.status, wait_code(KFWD, 1));
@@ -235,6 +258,21 @@ fwd_kernel(const __grid_constant__ TmaMaps maps, const Geometry g, const Tensors
           request_half(u + kFwdSBufs, 0);
         }
       }
+    }
+    if constexpr (kPacked) {
+      // the last tile's rows behind the range; no tile before it waits for this
+      if (last_rows != 0) {
+        const int st = (n_iter - 1) % CF::kStages;
+        ok = __shfl_sync(0xffffffffu, (int)ok, 0) != 0;
+        for (int h = 0; h < 2 && ok; ++h) {
+          ok = __all_sync(0xffffffffu, mbar_wait(smem_u32(&ctl->ragged_full[h]), 0, abort_flag, t.status, wait_code(KFWD, 10)));
+          if (!ok) break;
+          clear_tile_rows(strm_base + st * CF::kStageBytes + CF::stream_off(h, 0), kAtoms, last_rows);
+          if (lane == 0) mbar_arrive(bar_stream_full(h, st));
+        }
+      }
+    }
+    if (lane == 0 && n_iter > 0) {
       if (!ok) {   // give copies already in flight a bounded chance to land before the CTA exits
         const long long t0 = clock64();
         while (clock64() - t0 < 2000000LL) { }
@@ -325,8 +363,12 @@ fwd_kernel(const __grid_constant__ TmaMaps maps, const Geometry g, const Tensors
     const size_t row_off = (size_t)bh * g.N_q;
 
     int vlo, vhi;
-    key_range_for_queries(g, gidx, gidx + 1, vlo, vhi);
-    if (gidx >= g.N_q) { vlo = 0; vhi = 0; }
+    if constexpr (kPacked) {
+      packed_row_range(g, work, false, gidx, vlo, vhi);
+    } else {
+      key_range_for_queries(g, gidx, gidx + 1, vlo, vhi);
+      if (gidx >= g.N_q) { vlo = 0; vhi = 0; }
+    }
     const uint32_t vspan = (uint32_t)(vhi - vlo);
 
     // ---- one-time copy of the Q rows from the staging buffer to tensor memory: the two groups
@@ -367,7 +409,7 @@ fwd_kernel(const __grid_constant__ TmaMaps maps, const Geometry g, const Tensors
     for (int it = grp; it < n_iter && ok; it += G) {
       const int b = it % kFwdSBufs;
       const uint32_t sbuf = lane_addr + CF::kS + 64u * (uint32_t)b;
-      const int j0 = (t_begin + it) * BN;
+      const int j0 = strm0 + it * BN;
       const bool masked = !(j0 >= vlo && j0 + BN - 1 < vhi);
 
       ok = mbar_wait(bar_s_full(b), (it / kFwdSBufs) & 1, abort_flag, t.status, wait_code(KFWD, 7));
@@ -491,10 +533,12 @@ fwd_kernel(const __grid_constant__ TmaMaps maps, const Geometry g, const Tensors
       l_all = l_sum * f_me + l_o * f_ot;
     }
     // a split tile is normalised where the parts meet
-    const float inv = l_all > 0.f ? (SPLIT ? 1.f : 1.f / l_all) : 0.f;
+    float inv = l_all > 0.f ? (SPLIT ? 1.f : 1.f / l_all) : 0.f;
+    const bool nan_row = kPacked && l_sum + l_o != l_sum + l_o;      // a visible score that is not a number goes on to the result
+    if (nan_row) inv = l_sum + l_o;
     if constexpr (SPLIT) {
       if (grp == 0) { part_ml[row] = m_all; part_ml[BM + row] = l_all; }
-    } else if (grp == 0 && gidx < g.N_q) t.out_L[row_off + gidx] = (l_all > 0.f) ? (m_all + log2f(l_all)) * kLn2 : -INFINITY;
+    } else if (grp == 0 && gidx < row_end) t.out_L[row_off + gidx] = nan_row ? inv : (l_all > 0.f) ? (m_all + log2f(l_all)) * kLn2 : -INFINITY;
 
     if (n_iter > 0 && ok) ok = mbar_wait(bar_acc_done, 0, abort_flag, t.status, wait_code(KFWD, 9));
     ok = __all_sync(0xffffffffu, ok);
@@ -522,16 +566,22 @@ fwd_kernel(const __grid_constant__ TmaMaps maps, const Geometry g, const Tensors
         if (n_iter > 0 && ok) {
           if (use0) { v0 = __uint_as_float(a_[2 * e]) * f0; v1 = __uint_as_float(a_[2 * e + 1]) * f0; }
           if (G == 2 && use1) { v0 = fmaf(__uint_as_float(b_[2 * e]), f1, v0); v1 = fmaf(__uint_as_float(b_[2 * e + 1]), f1, v1); }
+          if (nan_row) v0 = v1 = inv;
         }
         w[e] = Pack<T>::pack(v0, v1);
         f[2 * e] = v0; f[2 * e + 1] = v1;
       }
       if constexpr (SPLIT) store_partial16<D>(partial, row, col, f);
-      else if (gidx < g.N_q) store_op16(staging + (uint32_t)(col >> 6) * kAtomBytesStat, row, col & 63, w);
+      else if (gidx < row_end) store_op16(staging + (uint32_t)(col >> 6) * kAtomBytesStat, row, col & 63, w);
     }
     // The O tile leaves through the staging buffer: Q has been in tensor memory since the prologue, or, where it is
     // read from here, every score product was complete before its scores were read.
-    store_tile_tma(&maps.out[TO_O], staging, g.D, r0, bh, !SPLIT && threadIdx.x == 0, kMathThreads);
+    if (kPacked && row_end - r0 < BM) {      // uniform over the CTA
+      named_barrier_sync(2, (uint32_t)kMathThreads);
+      if constexpr (kPacked) store_packed_rows<false>(t.out_O, staging, r0, row_end, bh, g.q_heads, g.D, kMathThreads);
+    } else {
+      store_tile_tma(&maps.out[TO_O], staging, g.D, r0, bh, !SPLIT && threadIdx.x == 0, kMathThreads);
+    }
   }
 
   if constexpr (SPLIT) {
@@ -583,6 +633,34 @@ static cudaError_t launch_fwd_one(const TmaMaps& maps, const Geometry& g_in, con
   using CF = FwdCfg<D, 2>;
   static TileKernelState state;
   return launch_tiles(fwd_kernel<D, T, false, 2>, fwd_kernel<D, T, true, 2>, maps, g, t, s, false, CF::kThreads, CF::kSmemBytes, 850.f, 0.f, state);
+}
+
+// packed batches
+template <int D, typename T>
+static cudaError_t launch_packed_fwd_one(const TmaMaps& maps, const PackedGeometry& g_in, const Tensors& t, cudaStream_t s) {
+  PackedGeometry g = g_in;
+  g.BH = g.q_heads;
+  const long long ctas = (long long)g.BH * g.cap;
+  g.head_group = pick_head_group(ctas, g.BH, 2ll * g.N_kv * g.D * 2);
+  if (ctas > 0x7fffffffLL) return cudaErrorInvalidValue;
+  static std::atomic<unsigned long long> smem_set[2];
+  if (ctas >= 2 * kSms) {
+    using CF = FwdCfg<D, 1>;
+    auto kern = fwd_kernel<D, T, false, 1, PackedGeometry>;
+    const size_t smem = half_sm_smem(CF::kSmemBytes);
+    const cudaError_t e = set_smem_once(kern, smem, smem_set[0]);
+    return e != cudaSuccess ? e : launch_pdl(kern, (unsigned)ctas, CF::kThreads, smem, s, maps, g, t);
+  }
+  using CF = FwdCfg<D, 2>;
+  auto kern = fwd_kernel<D, T, false, 2, PackedGeometry>;
+  const size_t smem = whole_sm_smem(CF::kSmemBytes);
+  const cudaError_t e = set_smem_once(kern, smem, smem_set[1]);
+  return e != cudaSuccess ? e : launch_pdl(kern, (unsigned)ctas, CF::kThreads, smem, s, maps, g, t);
+}
+
+cudaError_t launch_packed_fwd(int is_bf16, const TmaMaps& maps, const PackedGeometry& g, const Tensors& t, cudaStream_t s) {
+  if (g.D <= 64) return is_bf16 ? launch_packed_fwd_one<64, __nv_bfloat16>(maps, g, t, s) : launch_packed_fwd_one<64, __half>(maps, g, t, s);
+  return is_bf16 ? launch_packed_fwd_one<128, __nv_bfloat16>(maps, g, t, s) : launch_packed_fwd_one<128, __half>(maps, g, t, s);
 }
 
 // forward: O and L in one launch

@@ -3,6 +3,7 @@
 #pragma once
 
 #include "attn_common.cuh"
+#include "packed_geometry.cuh"
 #include "tc_primitives.cuh"
 
 #include <atomic>
@@ -365,9 +366,9 @@ inline int longest_stream(const Geometry& g) {
 // keys, D64 7.0 -> 5.9 us; B2 H8, 200 of 500, D96 11.0 -> 9.7; B2 H12, 777 of 1301, D80 42.2 -> 40.6; B4 H16
 // N1024 D128 96.9 -> 94.7.  Kernels in clusters and kernels that take over CTAs of their grid keep a launch
 // of their own, and so do long streams.
-template <typename Tile>
+template <typename Tile, typename Geo = Geometry>
 __global__ void __launch_bounds__(Tile::kThreads, Tile::kPerSm)
-tile_kernel(const __grid_constant__ TmaMaps maps, const Geometry g, const Tensors t) {
+tile_kernel(const __grid_constant__ TmaMaps maps, const Geo g, const Tensors t) {
   Tile::run(maps, g, t, blockIdx.x);
 }
 
@@ -603,6 +604,36 @@ __device__ __forceinline__ void zero_rows(void* out, int plane, int row0, int n_
   const int rows = min(BM, n_rows - row0);
   uint4* p = reinterpret_cast<uint4*>(static_cast<uint16_t*>(out) + ((size_t)plane * n_rows + row0) * D);
   for (int i = threadIdx.x; i < rows * D / 8; i += threads) p[i] = make_uint4(0u, 0u, 0u, 0u);
+}
+
+// ---- Packed batches (packed_geometry.cuh) ------------------------------------------------------
+// The last streamed tile of a stationary tile usually reaches past the rows that any of its rows sees, into later
+// ones and other sequences.  Masked scores do not keep those out of the output products, where 0 * inf and
+// 0 * NaN are not 0, so the producer warp clears them in shared memory between their arrival and the first product.
+// A whole warp: rows [from, BN) of `atoms` [BN][64] atoms from `stage` on.
+__device__ __forceinline__ void clear_tile_rows(uint32_t stage, int atoms, int from) {
+  const int per_atom = (BN - from) * 8;      // 16-byte chunks
+  for (int a = 0; a < atoms; ++a)
+    for (int i = (int)(threadIdx.x & 31); i < per_atom; i += 32)
+      asm volatile("st.shared.v4.b32 [%0], {%1, %1, %1, %1};" ::"r"(stage + a * kAtomBytesStrm + from * 128 + i * 16), "r"(0u) : "memory");
+  fence_proxy_async_smem();
+  __syncwarp();
+}
+
+// Rows [r0, row_end) of head `head` of a dense [n_tok, heads, D] result: from a result tile in shared memory (store_op16), or zeros.
+// The math threads; those of a tile have all written.  A tile with fewer than 128 rows must not be stored as a whole: the
+// rows behind belong to another CTA.
+template <bool ZERO>
+__device__ __forceinline__ void store_packed_rows(void* out, uint32_t tile, int r0, int row_end, int head, int heads, int D, int threads) {
+  const int chunks = D >> 3;
+  for (int i = threadIdx.x; i < (row_end - r0) * chunks; i += threads) {
+    const int row = i / chunks, c = i - row * chunks;
+    uint4 v = make_uint4(0u, 0u, 0u, 0u);
+    if constexpr (!ZERO)
+      asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w)
+                   : "r"(tile + (uint32_t)(c >> 3) * kAtomBytesStat + sw128_offset(row, (c & 7) * 8)) : "memory");
+    *reinterpret_cast<uint4*>(static_cast<uint16_t*>(out) + ((size_t)(r0 + row) * heads + head) * D + c * 8) = v;
+  }
 }
 
 // Epilogue of the tensor-core kernels.  The 256 math threads have written a [128 rows][cols]

@@ -1,0 +1,54 @@
+"""Packed batches: sequences of different lengths laid end to end on one axis of rows, without padding.
+
+    plan = packed_plan(cu_seqlens, n_tok)                  # once per batch, shared by all layers
+    O = packed_attention(q, k, v, plan)                    # [n_tok, heads, D]
+
+Attention is causal within each sequence, optionally within a sliding window, with grouped heads: `q` has a
+multiple of the heads of `k` and `v`, head h of `q` reading head h // (heads of q / heads of k).  It is
+differentiable to second order, as `flash_attention_v7`; the second derivative runs on rows padded to the
+longest sequence.  There is no counterpart in the reference, whose batches are dense [B, H, N, D]
+(e2e/ttt_pytorch/model.py:174-191).  There is no fallback: importing this module fails if the compiled
+extension `attention_cuda` is missing.
+"""
+import torch
+
+try:  # used as part of the package
+    from . import attention_cuda as _attention_cuda
+except ImportError:  # used the reference's way: this directory on sys.path
+    import attention_cuda as _attention_cuda
+
+
+class PackedPlan:
+    """What the kernels need to know about a batch's sequences; made by `packed_plan`."""
+
+    __slots__ = ("tensor", "n_tok", "n_seq", "max_seqlen")
+
+    def __init__(self, tensor, n_tok, n_seq, max_seqlen):
+        self.tensor, self.n_tok, self.n_seq, self.max_seqlen = tensor, n_tok, n_seq, max_seqlen
+
+
+def packed_plan(cu_seqlens, n_tok, max_seqlen=None):
+    """The plan of a batch of `n_tok` rows whose sequence i is rows [cu_seqlens[i], cu_seqlens[i + 1]).
+
+    cu_seqlens: int32 or int64 CUDA tensor of n_seq + 1 offsets, from small to large; one outside [0, n_tok] or
+    below an earlier one is cut to it.  Sequences may be empty, and rows may belong to none.  The offsets are read
+    on the device, by one launch on the current stream: nothing waits for the host, and a plan made inside a
+    captured graph is made anew by each replay.  A later change of `cu_seqlens` does not change the plan.
+    max_seqlen: length of the longest sequence, or an upper bound, if the caller knows it; only the second
+    derivative uses it, which else reads it from the device.  Sequences longer than a given one are not
+    covered by the second derivative."""
+    if max_seqlen is not None and max_seqlen < 0:
+        raise ValueError("max_seqlen must be >= 0")
+    return PackedPlan(_attention_cuda.packed_plan(cu_seqlens, n_tok), n_tok, cu_seqlens.numel() - 1, max_seqlen)
+
+
+def packed_attention(q, k, v, plan, window_size=None):
+    """q: (n_tok, H, D); k, v: (n_tok, H_kv, D), H a multiple of H_kv; fp16, bf16 or fp32 CUDA tensors, D a
+    multiple of 16 up to 128; for fp16 and bf16 views such as slices of one projection's result are read in place.
+
+    Key j is visible to query i of the same sequence when j <= i and, with a `window_size`, i < j + window_size.
+    The softmax scale is 1 / sqrt(D).  Rows that see no key (of no sequence, or a window of 0) give 0.  What
+    rows of other sequences or of none hold, infinities and NaN too, has no influence on a sequence's result;
+    within a sequence, an infinite or NaN key or value may reach the queries of up to 127 rows before it as well.
+    Returns O: (n_tok, H, D), dense."""
+    return _attention_cuda.packed_attention(q, k, v, plan.tensor, plan.n_tok, plan.n_seq, window_size, plan.max_seqlen)

@@ -170,6 +170,40 @@ int attn_b200_qk_norm_rope_backward(const void* x, const void* weight, const flo
                                     void* gw, float* scratch, int32_t n_tok, int32_t H, int32_t d, int32_t pos0,
                                     int32_t norm_from, float eps, int32_t dtype, void* stream);
 
+/* ---- Packed batches ---------------------------------------------------------------------------
+ * Sequences of different lengths end to end on one axis of n_tok rows, without padding; causal
+ * attention within each sequence, q_heads / kv_heads query heads to a key/value head:
+ *     Q, dO : [n_tok, q_heads, D] in strides     K, V : [n_tok, kv_heads, D] in strides
+ *     O, dQ : dense [n_tok, q_heads, D]          dK, dV : dense [n_tok, kv_heads, D]
+ *     L : [q_heads, n_tok] float32
+ * Key j is visible to query i of the same sequence when j <= i and i < j + window_size.  Rows of no
+ * sequence give O = 0, L = -inf and zero gradients, and what they hold, inf and NaN too, reaches no other
+ * sequence's result; neither does one sequence's content another's.  The reference has no counterpart: its
+ * batches are dense [B, H, N, D] (e2e/ttt_pytorch/model.py:174-191).
+ *
+ * Strides are in elements, indexed Q, K, V, dO, the last axis dense.  f16 / bf16: multiples of 8, pointers
+ * 16-byte aligned; f32: dense inputs only. */
+typedef struct attn_packed_shape {
+  int32_t n_tok, n_seq, q_heads, kv_heads, D;
+  int32_t window_size;   /* 2^31 - 1: none */
+  int32_t dtype;         /* ATTN_F16 / ATTN_BF16 / ATTN_F32 */
+  int32_t reserved;
+  int64_t row_stride[4], head_stride[4];
+} attn_packed_shape_t;
+
+/* The plan of a batch, attn_b200_packed_plan_ints int32 on the device (16-byte aligned), from the offsets
+ * cu_seqlens[n_seq + 1] on the device: sequence i is rows [cu_seqlens[i], cu_seqlens[i + 1]).  Offsets
+ * outside [0, n_tok] or below an earlier one are cut to it.  A plan belongs to one n_tok and n_seq and serves any
+ * number of calls; it does not follow later changes of cu_seqlens. */
+size_t attn_b200_packed_plan_ints(int32_t n_tok, int32_t n_seq);
+int attn_b200_packed_plan(const int32_t* cu_seqlens, int32_t n_tok, int32_t n_seq, int32_t* plan, void* stream);
+
+int attn_b200_packed_forward(const attn_packed_shape_t* shape, const int32_t* plan, const void* Q, const void* K, const void* V,
+                             void* O, float* L, void* stream);
+size_t attn_b200_packed_backward_scratch_bytes(const attn_packed_shape_t* shape);
+int attn_b200_packed_backward(const attn_packed_shape_t* shape, const int32_t* plan, const void* dO, const void* Q, const void* K,
+                              const void* V, const void* O, const float* L, void* dQ, void* dK, void* dV, float* scratch, void* stream);
+
 /* Number of kernels the last successful call of the calling thread launched. */
 int attn_b200_last_launch_count(void);
 
