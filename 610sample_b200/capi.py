@@ -28,6 +28,8 @@ EXPORTS = (
     "attn_b200_qk_norm_rope_backward", "attn_b200_qk_norm_rope_backward_scratch_bytes",
     "attn_b200_packed_plan_ints", "attn_b200_packed_plan", "attn_b200_packed_forward", "attn_b200_packed_backward",
     "attn_b200_packed_backward_scratch_bytes",
+    "attn_b200_linear_ce_forward_scratch_bytes", "attn_b200_linear_ce_forward", "attn_b200_linear_ce_backward_scratch_bytes",
+    "attn_b200_linear_ce_backward",
 )
 
 
@@ -39,6 +41,10 @@ class Shape(C.Structure):
 class PackedShape(C.Structure):
     _fields_ = [(n, C.c_int32) for n in ("n_tok", "n_seq", "q_heads", "kv_heads", "D", "window_size", "dtype", "reserved")] + [
         ("row_stride", C.c_int64 * 4), ("head_stride", C.c_int64 * 4)]
+
+
+class LceShape(C.Structure):
+    _fields_ = [(n, C.c_int32) for n in ("n", "d", "V", "dtype", "reduction", "reserved")] + [("ignore_index", C.c_int64)]
 
 
 _lib = None
@@ -76,6 +82,12 @@ def lib() -> C.CDLL:
         L.attn_b200_packed_backward.argtypes = [C.POINTER(PackedShape)] + [vp] * 12
         L.attn_b200_packed_backward_scratch_bytes.argtypes = [C.POINTER(PackedShape)]
         L.attn_b200_packed_backward_scratch_bytes.restype = C.c_size_t
+        L.attn_b200_linear_ce_forward_scratch_bytes.argtypes = [C.POINTER(LceShape)]
+        L.attn_b200_linear_ce_forward_scratch_bytes.restype = C.c_size_t
+        L.attn_b200_linear_ce_forward.argtypes = [C.POINTER(LceShape)] + [vp] * 9
+        L.attn_b200_linear_ce_backward_scratch_bytes.argtypes = [C.POINTER(LceShape), C.c_int32, C.c_int32]
+        L.attn_b200_linear_ce_backward_scratch_bytes.restype = C.c_size_t
+        L.attn_b200_linear_ce_backward.argtypes = [C.POINTER(LceShape)] + [vp] * 10
         for name in EXPORTS:
             getattr(L, name)
         _lib = L

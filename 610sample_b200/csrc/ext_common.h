@@ -101,7 +101,22 @@ inline bool leave_to_python(std::initializer_list<const torch::Tensor*> inputs) 
   return torch::jit::tracer::isTracing() || has_tangent(inputs);
 }
 
+// For operators without a Python form: what a C++ autograd function cannot do is refused.
+inline void refuse_transforms(std::initializer_list<const torch::Tensor*> inputs, const char* what) {
+  if (const auto& functorch = at::functorch::functorchTLSAccessor()) functorch->checkSupportsCppAutogradFunction();
+  TORCH_CHECK(!torch::jit::tracer::isTracing(), what, " cannot be traced");
+  TORCH_CHECK(!has_tangent(inputs), what, " has no forward-mode derivative");
+}
+
+inline bool wants_graph(std::initializer_list<const torch::Tensor*> inputs) {
+  if (!at::GradMode::is_enabled()) return false;
+  for (const torch::Tensor* t : inputs)
+    if (t->defined() && t->requires_grad()) return true;
+  return false;
+}
+
 void register_packed(pybind11::module& m);
+void register_loss(pybind11::module& m);
 
 }  // namespace ext
 

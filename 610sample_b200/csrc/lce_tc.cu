@@ -1,0 +1,474 @@
+// The matrix products of the linear cross entropy on the tensor cores (f16/bf16, sm_100a): one persistent kernel, four uses.
+//
+//   use    A                      B                     result of a tile
+//   LSE    x [n, d]               W [V, d]              per row: maximum, sum of exponentials; the target's logit
+//   GRAD   x [n, d]               W [piece, d]          G = coef (exp(z - lse) - onehot), rounded to the input type
+//   DX     G [n, piece]           W [piece, d], read by columns    dx (float between pieces)
+//   DW     G [n, piece], by columns   x [n, d], by columns         dW rows of the piece
+//
+// A pair of CTAs (a cluster) owns a tile of 256 rows x up to 256 columns: either holds 128 rows of A and half of B's columns, one
+// tcgen05.mma.cta_group::2 reads both.  A single CTA's 128 x 256 tile would stream 96 bytes per clock from L2 and read 96 more from
+// shared memory for the product, above either's rate; the pair needs 64 of each.  Tiles are dealt to the pairs in turn; a warp
+// loads through a ring of six stages of 64 in k, one (in rank 0) issues the products, eight finish a tile from tensor memory while
+// the next one accumulates in the other half of it.  The order of the tiles runs along the axis of the smaller operand first, so
+// that the larger one is read from HBM once and the smaller one stays in L2.
+#include "lce_launch.h"
+#include "tc_common.cuh"
+
+#include <cstdio>
+#include <mutex>
+
+namespace attn {
+namespace lce {
+
+using namespace tc;
+
+enum Use { LSE = 0, GRAD = 1, DX = 2, DW = 3 };
+
+constexpr int kTileM = 256, kTileN = 256, kBlockK = 64;
+constexpr int kStages = 6;
+constexpr uint32_t kOperandBytes = 128 * 128;                  // 128 rows (or columns) of 64 in k, of A or of B, in one CTA
+constexpr uint32_t kStageBytes = 2 * kOperandBytes;
+constexpr uint32_t kStagingBytes = 128 * 128;                  // [128 rows][64 columns] of a result, for either half of the epilogue
+constexpr int kEpilogueWarps = 8, kLoadWarp = 8, kIssueWarp = 9, kThreads = 320;
+constexpr int KLCE = 32;                                       // kernel id inside device status codes: 32 + use
+
+struct Control {
+  uint64_t full[kStages], empty[kStages];      // full: rank 0's counts both CTAs' loads
+  uint64_t acc_full[2], acc_empty[2];          // acc_empty: rank 0's counts both CTAs' warps
+  uint32_t tmem_base;
+  volatile uint32_t abort_flag;
+};
+constexpr uint32_t kContentBytes = kStages * kStageBytes + 2 * kStagingBytes + sizeof(Control);
+constexpr uint32_t kSmemBytes = kContentBytes + 1024;
+static_assert(kSmemBytes <= 232448, "shared memory");
+
+struct GemmMaps { CUtensorMap a, b, out; };
+
+struct GemmArgs {
+  int m_tiles, n_tiles, k_blocks;
+  int splits, split_blocks;      // DX, DW: shares of the blocks in k, each with its own sum
+  int tile_n;                    // columns of a tile, a multiple of 32
+  int rows, cols;                // of the result
+  int m_fast;                    // tiles in sequence along the rows
+  // LSE, GRAD
+  const int64_t* targets;
+  int first_col;                 // vocabulary index of column 0
+  Partial* partial;
+  float* target_logit;
+  const float *lse, *coef;
+  // DX, DW
+  float* acc;                    // [splits][rows, cols], where there are several pieces or splits
+  int acc_in, acc_out;           // add it; leave the sum there instead of in the result
+  const float* scale;
+  unsigned int* status;
+};
+
+template <typename T, int USE>
+__global__ void __launch_bounds__(kThreads, 1)
+lce_gemm_kernel(const __grid_constant__ GemmMaps maps, const GemmArgs g) {
+  constexpr bool kByColumns = USE == DX || USE == DW;            // B, and in DW A, is read along its rows as k
+  constexpr int KCODE = KLCE + USE;
+  extern __shared__ __align__(1024) uint8_t smem_raw[];
+  const uint32_t smem_base = (smem_u32(smem_raw) + 1023u) & ~1023u;
+  const uint32_t staging = smem_base + kStages * kStageBytes;
+  Control* ctl = reinterpret_cast<Control*>(smem_raw + (smem_base - smem_u32(smem_raw)) + kStages * kStageBytes + 2 * kStagingBytes);
+  float2* halves = reinterpret_cast<float2*>(smem_raw + (staging - smem_u32(smem_raw)));      // LSE, [2][128]: the upper half's (m, l)
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const uint32_t rank = cluster_rank();
+  const int pair = blockIdx.x >> 1, pairs = gridDim.x >> 1;
+  const int plane = g.m_tiles * g.n_tiles, tiles = plane * g.splits;
+
+  auto bar_full = [&](int s) { return smem_u32(&ctl->full[s]); };
+  auto bar_empty = [&](int s) { return smem_u32(&ctl->empty[s]); };
+  auto bar_acc_full = [&](int b) { return smem_u32(&ctl->acc_full[b]); };
+  auto bar_acc_empty = [&](int b) { return smem_u32(&ctl->acc_empty[b]); };
+
+  if (warp == kLoadWarp && lane == 0) {
+    tma_prefetch_desc(&maps.a);
+    tma_prefetch_desc(&maps.b);
+    for (int s = 0; s < kStages; ++s) {
+      mbar_init(bar_full(s), 1);
+      mbar_init(bar_empty(s), 1);
+    }
+    for (int b = 0; b < 2; ++b) {
+      mbar_init(bar_acc_full(b), 1);
+      mbar_init(bar_acc_empty(b), 2 * kEpilogueWarps);
+    }
+    ctl->abort_flag = 0u;
+    fence_barrier_init();
+    fence_proxy_async_smem();
+  }
+  if (warp == kIssueWarp) tmem_alloc_pair(smem_u32(&ctl->tmem_base), 512);
+  tc_fence_before_sync();
+  cluster_barrier();
+  tc_fence_after_sync();
+  const uint32_t tmem_base = ctl->tmem_base;
+  volatile uint32_t* abort_flag = &ctl->abort_flag;
+  pdl_wait();
+  pdl_trigger();
+
+  auto tile_at = [&](int t, int& mt, int& nt, int& split) {
+    split = t / plane;
+    t -= split * plane;
+    if (g.m_fast) { nt = t / g.m_tiles; mt = t - nt * g.m_tiles; }
+    else { mt = t / g.n_tiles; nt = t - mt * g.n_tiles; }
+  };
+  const int half_n = g.tile_n >> 1;      // columns of B in this CTA
+
+  if (warp == kLoadWarp) {
+    if (lane == 0) {
+      const uint32_t stage_bytes = kOperandBytes + (kByColumns ? kOperandBytes : (uint32_t)half_n * 128u);
+      bool ok = true;
+      int it = 0;
+      for (int t = pair; t < tiles && ok; t += pairs) {
+        int mt, nt, split;
+        tile_at(t, mt, nt, split);
+        const int first_block = split * g.split_blocks, blocks = min(g.split_blocks, g.k_blocks - first_block);
+        const int m0 = mt * kTileM + (int)rank * 128, n0 = nt * g.tile_n + (int)rank * half_n;
+        for (int kb = 0; kb < blocks; ++kb, ++it) {
+          const int s = it % kStages;
+          if (it >= kStages) {
+            ok = mbar_wait(bar_empty(s), ((it / kStages) & 1) ^ 1, abort_flag, g.status, wait_code(KCODE, 1));
+            if (!ok) break;
+          }
+          if (rank == 0) mbar_arrive_expect_tx(bar_full(s), 2 * stage_bytes);
+          const uint32_t bar = map_rank(bar_full(s), 0), a = smem_base + s * kStageBytes, b = a + kOperandBytes;
+          const int k0 = (first_block + kb) * kBlockK;
+          if constexpr (USE == DW) {
+            for (int i = 0; i < 2; ++i) tma_load_2d_pair(a + i * 8192, &maps.a, m0 + 64 * i, k0, bar);
+          } else {
+            tma_load_2d_pair(a, &maps.a, k0, m0, bar);
+          }
+          if constexpr (kByColumns) {
+            for (int i = 0; i < 2; ++i) tma_load_2d_pair(b + i * 8192, &maps.b, n0 + 64 * i, k0, bar);
+          } else {
+            tma_load_2d_pair(b, &maps.b, k0, n0, bar);
+          }
+        }
+      }
+      // every product that reads this CTA's stages has completed, and told this CTA so, before it leaves
+      for (int j = it > kStages ? it - kStages : 0; j < it && ok; ++j)
+        ok = mbar_wait(bar_empty(j % kStages), (j / kStages) & 1, abort_flag, g.status, wait_code(KCODE, 5));
+      if (!ok) {   // give copies already in flight a bounded chance to land before the CTA exits
+        const long long t0 = clock64();
+        while (clock64() - t0 < 2000000LL) { }
+      }
+    }
+  } else if (warp == kIssueWarp) {
+    if (rank == 0) {
+      const uint32_t idesc = make_idesc(kTileM, g.tile_n, Pack<T>::kIsBf16, USE == DW ? 1 : 0, kByColumns ? 1 : 0);
+      bool ok = true;
+      int it = 0, i = 0;
+      for (int t = pair; t < tiles && ok; t += pairs, ++i) {
+        const int buf = i & 1;
+        if (i >= 2) {
+          ok = __all_sync(0xffffffffu, mbar_wait(bar_acc_empty(buf), ((i >> 1) & 1) ^ 1, abort_flag, g.status, wait_code(KCODE, 2)));
+          if (!ok) break;
+          tc_fence_after_sync();
+        }
+        const uint32_t acc = tmem_base + (uint32_t)buf * 256u;
+        const int first_block = t / plane * g.split_blocks, blocks = min(g.split_blocks, g.k_blocks - first_block);
+        for (int kb = 0; kb < blocks; ++kb, ++it) {
+          const int s = it % kStages;
+          ok = __all_sync(0xffffffffu, mbar_wait(bar_full(s), (it / kStages) & 1, abort_flag, g.status, wait_code(KCODE, 3)));
+          if (!ok) break;
+          tc_fence_after_sync();
+          const uint32_t a = smem_base + s * kStageBytes, b = a + kOperandBytes;
+          // rows along k: blocks of 64 rows (or columns) 8 KB apart, a step of 16 in k is 16 rows; else 32 bytes within a row
+          const uint64_t da = smem_desc_sw128(a, USE == DW ? 8192 : 16, 1024), db = smem_desc_sw128(b, kByColumns ? 8192 : 16, 1024);
+          constexpr uint64_t step_a = (USE == DW ? 2048 : 32) >> 4, step_b = (kByColumns ? 2048 : 32) >> 4;
+          if (elect_one()) {
+#pragma unroll
+            for (int ks = 0; ks < 4; ++ks) mma_ss_pair(acc, da + ks * step_a, db + ks * step_b, idesc, (kb | ks) != 0);
+            mma_commit_pair(bar_empty(s));
+            if (kb + 1 == blocks) mma_commit_pair(bar_acc_full(buf));
+          }
+          __syncwarp();
+        }
+      }
+    }
+  } else {
+    const int quarter = warp & 3, half = warp >> 2;
+    const int row = quarter * 32 + lane;
+    const uint32_t lane_addr = tmem_base + ((uint32_t)(quarter * 32) << 16);
+    const uint32_t tile_smem = staging + (uint32_t)half * kStagingBytes;
+    float scale = 1.f;
+    if constexpr (kByColumns) scale = from_l2(g.scale);
+    bool ok = true;
+    int i = 0;
+    for (int t = pair; t < tiles && ok; t += pairs, ++i) {
+      int mt, nt, split;
+      tile_at(t, mt, nt, split);
+      const int buf = i & 1, r0 = mt * kTileM + (int)rank * 128, r = r0 + row;
+      const int col0 = nt * g.tile_n + half * half_n;      // this half's first column
+      const uint32_t acc = lane_addr + (uint32_t)buf * 256u + (uint32_t)(half * half_n);
+      const bool in = r < g.rows;
+      int target = -1;                                     // column of this row's target, counted from col0
+      float lse2 = 0.f, coef = 0.f;
+      if constexpr (USE == LSE || USE == GRAD) {
+        if (in) {
+          const int64_t y = from_l2(reinterpret_cast<const long long*>(g.targets) + r) - g.first_col - col0;
+          if (y >= 0 && y < half_n) target = (int)y;
+          if constexpr (USE == GRAD) { lse2 = from_l2(g.lse + r) * kLog2e; coef = from_l2(g.coef + r); }
+        }
+      }
+      // the eight warps go on, or give up, together: the barriers below need all of them
+      ok = named_barrier_all(1, 32 * kEpilogueWarps, mbar_wait(bar_acc_full(buf), (i >> 1) & 1, abort_flag, g.status, wait_code(KCODE, 4)));
+      if (!ok) break;
+      tc_fence_after_sync();
+      auto release = [&]() {                               // the accumulator is in registers
+        tc_fence_before_sync();
+        __syncwarp();
+        if (lane == 0) mbar_arrive_cluster(map_rank(bar_acc_empty(buf), 0));
+      };
+
+      if constexpr (USE == LSE) {
+        float m = -INFINITY, l = 0.f;
+        const int left = g.cols - col0;                    // valid columns of this half, where less than half_n
+        for (int c = 0; c < half_n; c += 16) {
+          uint32_t v[16];
+          tmem_ld16(acc + c, v);
+          tmem_ld_wait(v);
+          if (c >= left) continue;                         // uniform
+          float z[16];
+#pragma unroll
+          for (int e = 0; e < 16; ++e) z[e] = c + e < left ? __uint_as_float(v[e]) : -INFINITY;
+          if (__any_sync(0xffffffffu, (uint32_t)(target - c) < 16u)) {
+#pragma unroll
+            for (int e = 0; e < 16; ++e)
+              if (target == c + e) g.target_logit[r] = z[e];
+          }
+          float mx = z[0];
+#pragma unroll
+          for (int e = 1; e < 16; ++e) mx = fmaxf(mx, z[e]);
+          const float m_new = fmaxf(m, mx * kLog2e);
+          float sum = 0.f;
+#pragma unroll
+          for (int e = 0; e < 16; ++e) sum += ex2(fmaf(z[e], kLog2e, -m_new));
+          l = fmaf(l, m == -INFINITY ? 0.f : ex2(m - m_new), sum);
+          m = m_new;
+        }
+        release();
+        if (half == 1) halves[buf * 128 + row] = make_float2(m, l);
+        named_barrier_sync(2, 32 * kEpilogueWarps);
+        if (half == 0 && in) {
+          const float2 o = halves[buf * 128 + row];
+          const float m_all = fmaxf(m, o.x);
+          const float l_all = fmaf(l, ex2(m - m_all), o.y * (o.x == -INFINITY ? 0.f : ex2(o.x - m_all)));
+          g.partial[(size_t)nt * g.rows + r] = Partial{m_all, l_all};
+        }
+      } else {
+        const bool to_acc = kByColumns && g.acc_out;
+#pragma unroll 1
+        for (int c = 0; c < 128; c += 64) {
+          uint32_t v[4][16];
+#pragma unroll
+          for (int q = 0; q < 4; ++q) tmem_ld16(acc + c + 16 * q, v[q]);
+#pragma unroll
+          for (int q = 0; q < 4; ++q) tmem_ld_wait(v[q]);
+          if (c == 64) release();
+          const int col = col0 + c;
+          if (col >= g.cols) continue;                     // uniform
+          float f[64];
+#pragma unroll
+          for (int e = 0; e < 64; ++e) f[e] = __uint_as_float(v[e >> 4][e & 15]);
+          if constexpr (USE == GRAD) {
+            // a row that does not count has a factor of 0 and G = 0, whatever its logits are
+#pragma unroll
+            for (int e = 0; e < 64; ++e) f[e] = coef == 0.f ? 0.f : ex2(fmaf(f[e], kLog2e, -lse2)) * coef;
+            if (__any_sync(0xffffffffu, (uint32_t)(target - c) < 64u)) {
+#pragma unroll
+              for (int e = 0; e < 64; ++e)
+                if (target == c + e) f[e] -= coef;
+            }
+          } else {
+            if ((g.acc_in || to_acc) && in) {
+              float4* at = reinterpret_cast<float4*>(g.acc + ((size_t)split * g.rows + r) * g.cols + col);
+#pragma unroll
+              for (int q = 0; q < 16; ++q)
+                if (col + 4 * q < g.cols) {                // cols is a multiple of 8
+                  if (g.acc_in) {
+                    const float4 x = __ldcg(at + q);
+                    f[4 * q] += x.x; f[4 * q + 1] += x.y; f[4 * q + 2] += x.z; f[4 * q + 3] += x.w;
+                  }
+                  if (to_acc) __stcg(at + q, make_float4(f[4 * q], f[4 * q + 1], f[4 * q + 2], f[4 * q + 3]));
+                }
+            }
+#pragma unroll
+            for (int e = 0; e < 64; ++e) f[e] *= scale;
+          }
+          if (!to_acc) {
+            // through shared memory; the store before must have read it
+            if (quarter == 0 && lane == 0) bulk_wait_group_read_all();
+            named_barrier_sync(3 + half, 128);
+#pragma unroll
+            for (int q = 0; q < 4; ++q) {
+              uint32_t w[8];
+#pragma unroll
+              for (int e = 0; e < 8; ++e) w[e] = Pack<T>::pack(f[16 * q + 2 * e], f[16 * q + 2 * e + 1]);
+              store_op16(tile_smem, row, 16 * q, w);
+            }
+            fence_proxy_async_smem();
+            named_barrier_sync(3 + half, 128);
+            if (quarter == 0 && lane == 0) {
+              tma_store_2d(&maps.out, tile_smem, col, r0);
+              bulk_commit_group();
+            }
+          }
+        }
+      }
+    }
+    if (quarter == 0 && lane == 0) bulk_wait_group_read_all();
+  }
+  tc_fence_before_sync();
+  cluster_barrier();      // no barrier or tensor memory of a CTA is used by the other one any more
+  if (warp == kIssueWarp) {
+    tc_fence_after_sync();
+    tmem_dealloc_pair(tmem_base, 512);
+  }
+}
+
+// ---- host ---------------------------------------------------------------------------------------
+typedef CUresult (*EncodeTiledFn)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*, const cuuint32_t*,
+                                  const cuuint32_t*, CUtensorMapInterleave, CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+static EncodeTiledFn encode_fn() {
+  static EncodeTiledFn fn = nullptr;
+  static std::once_flag once;
+  std::call_once(once, [] {
+    void* p = nullptr;
+    cudaDriverEntryPointQueryResult q;
+    if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &p, cudaEnableDefault, &q) == cudaSuccess && q == cudaDriverEntryPointSuccess)
+      fn = reinterpret_cast<EncodeTiledFn>(p);
+  });
+  return fn;
+}
+
+// [rows][cols] with `ld` elements from row to row, boxes of 64 columns x `box_rows`; outside of it loads give zeros and stores nothing
+static bool encode(CUtensorMap* map, const void* p, bool bf16, long long rows, long long cols, long long ld, int box_rows) {
+  const EncodeTiledFn fn = encode_fn();
+  if (fn == nullptr) return false;
+  cuuint64_t dims[2] = {(cuuint64_t)cols, (cuuint64_t)rows};
+  cuuint64_t strides[1] = {(cuuint64_t)ld * 2};
+  cuuint32_t box[2] = {64, (cuuint32_t)box_rows};
+  cuuint32_t estr[2] = {1, 1};
+  return fn(map, bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 2, const_cast<void*>(p), dims, strides, box, estr,
+            CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+template <int USE>
+static cudaError_t launch_use(const GemmMaps& maps, GemmArgs g, int dtype, long long k, cudaStream_t stream) {
+  g.m_tiles = (g.rows + kTileM - 1) / kTileM;
+  g.n_tiles = (g.cols + g.tile_n - 1) / g.tile_n;
+  g.k_blocks = (int)((k + kBlockK - 1) / kBlockK);
+  g.m_fast = g.rows < g.cols;      // A, of `rows` rows, is the smaller operand
+  if (g.splits < 1) g.splits = 1;
+  g.split_blocks = (g.k_blocks + g.splits - 1) / g.splits;
+  g.splits = (g.k_blocks + g.split_blocks - 1) / g.split_blocks;      // a share without blocks would never complete
+  const long long tiles = (long long)g.m_tiles * g.n_tiles * g.splits;
+  if (tiles > 0x7fffffffLL) return cudaErrorInvalidValue;
+  const int pairs = (int)(tiles < kSms / 2 ? tiles : kSms / 2);
+  static std::atomic<unsigned long long> smem_set[2];
+  auto kern = dtype == 1 ? lce_gemm_kernel<__nv_bfloat16, USE> : lce_gemm_kernel<__half, USE>;
+  const cudaError_t e = set_smem_once(kern, kSmemBytes, smem_set[dtype == 1]);
+  return e != cudaSuccess ? e : launch_pdl_cluster(kern, (unsigned)pairs * 2, kThreads, kSmemBytes, 2, stream, maps, g);
+}
+
+static const char* const kMapError = "cuTensorMapEncodeTiled refused a tensor";
+
+int tc_tiles(int V) { return (V + kTileN - 1) / kTileN; }
+
+// Where the tiles are too few for the pairs, k is shared out, down to 16 blocks (1024 in k) a share, and the shares' sums are added
+// by a kernel of their own.  No share is without blocks.
+int tc_splits(long long rows, long long cols, long long k) {
+  const long long tiles = ((rows + kTileM - 1) / kTileM) * ((cols + kTileN - 1) / kTileN), blocks = (k + kBlockK - 1) / kBlockK;
+  long long s = (kSms / 2) / tiles;
+  if (s > blocks / 16) s = blocks / 16;
+  if (s < 2) return 1;
+  const long long each = (blocks + s - 1) / s;
+  return (int)((blocks + each - 1) / each);
+}
+
+cudaError_t tc_scores(const Problem& p, const Scores& s, cudaStream_t stream, const char** err) {
+  GemmMaps maps;
+  GemmArgs g = {};
+  const bool bf = p.dtype == 1;
+  g.tile_n = kTileN;
+  if (!encode(&maps.a, p.x, bf, p.n, p.d, p.d, 128) || !encode(&maps.b, p.w, bf, p.V, p.d, p.d, g.tile_n / 2)) {
+    *err = kMapError;
+    return cudaErrorInvalidValue;
+  }
+  maps.out = maps.a;      // not used
+  g.rows = p.n; g.cols = p.V;
+  g.targets = p.targets;
+  g.partial = s.partial;
+  g.target_logit = s.target_logit;
+  g.status = p.status;
+  return launch_use<LSE>(maps, g, p.dtype, p.d, stream);
+}
+
+cudaError_t tc_piece_grad(const Problem& p, const Piece& piece, const float* lse, const Coefficients& c, void* G, cudaStream_t stream, const char** err) {
+  GemmMaps maps;
+  GemmArgs g = {};
+  const bool bf = p.dtype == 1;
+  g.tile_n = kTileN;
+  const void* w = static_cast<const uint16_t*>(p.w) + (size_t)piece.first * p.d;
+  if (!encode(&maps.a, p.x, bf, p.n, p.d, p.d, 128) || !encode(&maps.b, w, bf, piece.cols, p.d, p.d, 128) ||
+      !encode(&maps.out, G, bf, p.n, piece.cols, piece.ld, 128)) {
+    *err = kMapError;
+    return cudaErrorInvalidValue;
+  }
+  g.rows = p.n; g.cols = piece.cols;
+  g.targets = p.targets;
+  g.first_col = piece.first;
+  g.lse = lse;
+  g.coef = c.coef;
+  g.status = p.status;
+  return launch_use<GRAD>(maps, g, p.dtype, p.d, stream);
+}
+
+cudaError_t tc_piece_dx(const Problem& p, const Piece& piece, const Coefficients& c, const void* G, int splits, bool keep, float* acc, void* dx,
+                        cudaStream_t stream, const char** err) {
+  GemmMaps maps;
+  GemmArgs g = {};
+  const bool bf = p.dtype == 1;
+  g.tile_n = kTileN;
+  const void* w = static_cast<const uint16_t*>(p.w) + (size_t)piece.first * p.d;
+  if (!encode(&maps.a, G, bf, p.n, piece.cols, piece.ld, 128) || !encode(&maps.b, w, bf, piece.cols, p.d, p.d, 64) ||
+      !encode(&maps.out, dx, bf, p.n, p.d, p.d, 128)) {
+    *err = kMapError;
+    return cudaErrorInvalidValue;
+  }
+  g.rows = p.n; g.cols = p.d;
+  g.splits = splits;
+  g.acc = acc;
+  g.acc_in = !piece.is_first;
+  g.acc_out = !piece.is_last || keep;
+  g.scale = c.scale;
+  g.status = p.status;
+  return launch_use<DX>(maps, g, p.dtype, piece.cols, stream);
+}
+
+cudaError_t tc_piece_dw(const Problem& p, const Piece& piece, const Coefficients& c, const void* G, const void* x, int splits, float* acc,
+                        void* dw, cudaStream_t stream, const char** err) {
+  GemmMaps maps;
+  GemmArgs g = {};
+  const bool bf = p.dtype == 1;
+  g.tile_n = kTileN;
+  void* out = static_cast<uint16_t*>(dw) + (size_t)piece.first * p.d;
+  if (!encode(&maps.a, G, bf, p.n, piece.cols, piece.ld, 64) || !encode(&maps.b, x, bf, p.n, p.d, p.d, 64) ||
+      !encode(&maps.out, out, bf, piece.cols, p.d, p.d, 128)) {
+    *err = kMapError;
+    return cudaErrorInvalidValue;
+  }
+  g.rows = piece.cols; g.cols = p.d;
+  g.splits = splits;
+  g.acc = acc;
+  g.acc_out = splits > 1;
+  g.scale = c.scale;
+  g.status = p.status;
+  return launch_use<DW>(maps, g, p.dtype, p.n, stream);
+}
+
+}  // namespace lce
+}  // namespace attn

@@ -11,19 +11,6 @@ namespace ext {
 
 namespace {
 
-void refuse_transforms(std::initializer_list<const torch::Tensor*> inputs, const char* what) {
-  if (const auto& functorch = at::functorch::functorchTLSAccessor()) functorch->checkSupportsCppAutogradFunction();
-  TORCH_CHECK(!torch::jit::tracer::isTracing(), what, " cannot be traced");
-  TORCH_CHECK(!has_tangent(inputs), what, " has no forward-mode derivative");
-}
-
-bool wants_graph(std::initializer_list<const torch::Tensor*> inputs) {
-  if (!at::GradMode::is_enabled()) return false;
-  for (const torch::Tensor* t : inputs)
-    if (t->defined() && t->requires_grad()) return true;
-  return false;
-}
-
 int64_t window_of(const c10::optional<int64_t>& window_size) {
   if (!window_size.has_value()) return std::numeric_limits<int32_t>::max();
   TORCH_CHECK(*window_size >= 0, "window_size must be >= 0, or None");

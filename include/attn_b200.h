@@ -204,6 +204,34 @@ size_t attn_b200_packed_backward_scratch_bytes(const attn_packed_shape_t* shape)
 int attn_b200_packed_backward(const attn_packed_shape_t* shape, const int32_t* plan, const void* dO, const void* Q, const void* K,
                               const void* V, const void* O, const float* L, void* dQ, void* dK, void* dV, float* scratch, void* stream);
 
+/* ---- Cross entropy of a linear layer --------------------------------------------------------------
+ * z = x W^T, loss_i = log sum_j exp(z_ij) - z_i,targets[i], without z being kept: the forward reduces it tile by tile, the
+ * backward forms its gradient for a piece of the vocabulary at a time (at most 256 MB, or 1024 columns).  x: [n, d], w: [V, d]
+ * dense, of one type, 16-byte aligned; f16 / bf16 with d a multiple of 8 run on the tensor cores, all else on the CUDA cores in
+ * fp32.  A row whose target is ignore_index has loss 0 and gradients 0 and does not count in the mean, whatever x holds there; a
+ * target outside [0, V) otherwise gives NaN.  The reference takes the loss of whole logits
+ * (e2e/ttt_pytorch/model.py:540-671). */
+enum { ATTN_REDUCE_NONE = 0, ATTN_REDUCE_SUM = 1, ATTN_REDUCE_MEAN = 2 };
+typedef struct attn_lce_shape {
+  int32_t n, d, V;
+  int32_t dtype;         /* ATTN_F16 / ATTN_BF16 / ATTN_F32 */
+  int32_t reduction;     /* ATTN_REDUCE_* */
+  int32_t reserved;
+  int64_t ignore_index;
+} attn_lce_shape_t;
+
+/* loss, lse: [n] float32 (the losses of the rows, the log-sum-exps that the backward takes); value, counted (not for
+ * ATTN_REDUCE_NONE): one float32 each, the sum or mean and the number of rows that count. */
+size_t attn_b200_linear_ce_forward_scratch_bytes(const attn_lce_shape_t* shape);
+int attn_b200_linear_ce_forward(const attn_lce_shape_t* shape, const void* x, const void* w, const int64_t* targets, float* loss,
+                                float* lse, float* value, float* counted, void* scratch, void* stream);
+
+/* dx [n, d], dw [V, d] in the type of x, either null if not wanted.  grad: the gradient of the rows' losses, [n] float32
+ * (ATTN_REDUCE_NONE), or of the value, one float32; counted: the forward's (ATTN_REDUCE_MEAN). */
+size_t attn_b200_linear_ce_backward_scratch_bytes(const attn_lce_shape_t* shape, int32_t want_dx, int32_t want_dw);
+int attn_b200_linear_ce_backward(const attn_lce_shape_t* shape, const void* x, const void* w, const int64_t* targets, const float* lse,
+                                 const float* grad, const float* counted, void* dx, void* dw, void* scratch, void* stream);
+
 /* Number of kernels the last successful call of the calling thread launched. */
 int attn_b200_last_launch_count(void);
 
