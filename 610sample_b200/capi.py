@@ -29,7 +29,8 @@ EXPORTS = (
     "attn_b200_packed_plan_ints", "attn_b200_packed_plan", "attn_b200_packed_forward", "attn_b200_packed_backward",
     "attn_b200_packed_backward_scratch_bytes",
     "attn_b200_linear_ce_forward_scratch_bytes", "attn_b200_linear_ce_forward", "attn_b200_linear_ce_backward_scratch_bytes",
-    "attn_b200_linear_ce_backward",
+    "attn_b200_linear_ce_backward", "attn_b200_packed_qk_norm_rope", "attn_b200_packed_qk_norm_rope_backward_scratch_bytes",
+    "attn_b200_packed_qk_norm_rope_backward",
 )
 
 
@@ -45,6 +46,12 @@ class PackedShape(C.Structure):
 
 class LceShape(C.Structure):
     _fields_ = [(n, C.c_int32) for n in ("n", "d", "V", "dtype", "reduction", "reserved")] + [("ignore_index", C.c_int64)]
+
+
+class RopeShape(C.Structure):
+    _fields_ = [(n, C.c_int32) for n in ("n_tok", "q_heads", "k_heads", "D", "dtype", "table_rows", "axes", "positions64")] + [
+        ("section", C.c_int32 * 4), ("weight_float", C.c_int32 * 2), ("eps", C.c_float), ("reserved", C.c_int32), ("axis_stride", C.c_int64),
+        ("row_stride", C.c_int64 * 2), ("head_stride", C.c_int64 * 2), ("g_row_stride", C.c_int64 * 2), ("g_head_stride", C.c_int64 * 2)]
 
 
 _lib = None
@@ -88,6 +95,10 @@ def lib() -> C.CDLL:
         L.attn_b200_linear_ce_backward_scratch_bytes.argtypes = [C.POINTER(LceShape), C.c_int32, C.c_int32]
         L.attn_b200_linear_ce_backward_scratch_bytes.restype = C.c_size_t
         L.attn_b200_linear_ce_backward.argtypes = [C.POINTER(LceShape)] + [vp] * 10
+        L.attn_b200_packed_qk_norm_rope.argtypes = [C.POINTER(RopeShape)] + [vp] * 9
+        L.attn_b200_packed_qk_norm_rope_backward.argtypes = [C.POINTER(RopeShape)] + [vp] * 14
+        L.attn_b200_packed_qk_norm_rope_backward_scratch_bytes.argtypes = [C.POINTER(RopeShape)]
+        L.attn_b200_packed_qk_norm_rope_backward_scratch_bytes.restype = C.c_size_t
         for name in EXPORTS:
             getattr(L, name)
         _lib = L

@@ -220,6 +220,224 @@ torch::Tensor packed_attention(const torch::Tensor& q, const torch::Tensor& k, c
   return PackedAttention::apply(q, k, v, plan, n_seq, window, max_seqlen.value_or(-1));
 }
 
+// ---- norm and rotation of q and k ---------------------------------------------------------------
+
+struct RopeArgs { std::vector<int64_t> sections; double eps; };
+
+torch::Tensor or_none(const torch::Tensor& w) { return w.numel() > 0 ? w : torch::Tensor(); }
+
+void check_rope(const torch::Tensor& q, const torch::Tensor& k, const torch::Tensor& qw, const torch::Tensor& kw, const torch::Tensor& freqs,
+                const torch::Tensor& positions, const RopeArgs& a) {
+  TORCH_CHECK(q.is_cuda() && k.is_cuda() && freqs.is_cuda() && positions.is_cuda(), "q, k, freqs and positions must be CUDA tensors");
+  TORCH_CHECK(q.device() == k.device() && q.device() == freqs.device() && q.device() == positions.device(), "all tensors must be on one device");
+  TORCH_CHECK(q.dim() == 3 && k.dim() == 3, "q and k must be [n_tok, heads, D]");
+  TORCH_CHECK(q.size(0) == k.size(0) && q.size(2) == k.size(2), "q and k must agree in n_tok and D");
+  TORCH_CHECK(q.scalar_type() == k.scalar_type(), "q and k must have the same dtype");
+  TORCH_CHECK(q.size(0) <= (1 << 30) && q.size(1) <= (1 << 20) && k.size(1) <= (1 << 20), "q or k is too large");
+  for (const torch::Tensor* w : {&qw, &kw}) {
+    if (!w->defined()) continue;
+    TORCH_CHECK(w->is_cuda() && w->device() == q.device() && w->dim() == 1 && w->size(0) == q.size(2), "a weight must be a CUDA tensor [D]");
+    TORCH_CHECK(w->scalar_type() == q.scalar_type() || w->scalar_type() == at::kFloat, "a weight must have the dtype of q and k, or be float32");
+  }
+  TORCH_CHECK(freqs.scalar_type() == at::kFloat && freqs.dim() == 3 && freqs.size(2) == 2 && freqs.size(1) * 2 == q.size(2) && freqs.size(0) <= (1 << 30),
+              "freqs must be float32 [rows, D / 2, 2]");
+  TORCH_CHECK(positions.scalar_type() == at::kInt || positions.scalar_type() == at::kLong, "positions must be int32 or int64");
+  TORCH_CHECK((positions.dim() == 1 || positions.dim() == 2) && positions.size(-1) == q.size(0), "positions must be [n_tok] or [axes, n_tok]");
+  TORCH_CHECK((int64_t)a.sections.size() == (positions.dim() == 1 ? 1 : positions.size(0)) && a.sections.size() <= 4,
+              "sections must name the pairs of every axis of positions, at most 4");
+}
+
+// rows whose elements lie side by side
+torch::Tensor with_dense_rows(const torch::Tensor& t) { return t.stride(2) == 1 || t.size(2) == 1 ? t : t.contiguous(); }
+
+attn_rope_shape_t rope_shape(const torch::Tensor& q, const torch::Tensor& k, const torch::Tensor& qw, const torch::Tensor& kw, const torch::Tensor& freqs,
+                             const torch::Tensor& positions, const RopeArgs& a) {
+  attn_rope_shape_t s{};
+  s.n_tok = (int32_t)q.size(0);
+  s.q_heads = (int32_t)q.size(1);
+  s.k_heads = (int32_t)k.size(1);
+  s.D = (int32_t)q.size(2);
+  s.dtype = dtype_code(q);
+  s.table_rows = (int32_t)freqs.size(0);
+  s.axes = (int32_t)a.sections.size();
+  s.positions64 = positions.scalar_type() == at::kLong;
+  for (size_t i = 0; i < a.sections.size(); ++i) s.section[i] = (int32_t)std::min<int64_t>(a.sections[i], 1 << 20);
+  s.weight_float[0] = qw.defined() && qw.scalar_type() == at::kFloat;
+  s.weight_float[1] = kw.defined() && kw.scalar_type() == at::kFloat;
+  s.eps = (float)a.eps;
+  s.axis_stride = positions.dim() == 2 ? positions.stride(0) : 0;
+  s.row_stride[0] = q.stride(0); s.head_stride[0] = q.stride(1);
+  s.row_stride[1] = k.stride(0); s.head_stride[1] = k.stride(1);
+  return s;
+}
+
+void* ptr_or_null(const torch::Tensor& t) { return t.defined() ? t.data_ptr() : nullptr; }
+
+variable_list rope_forward(const torch::Tensor& q_in, const torch::Tensor& k_in, const torch::Tensor& qw_in, const torch::Tensor& kw_in,
+                           const torch::Tensor& freqs_in, const torch::Tensor& positions_in, const RopeArgs& a) {
+  check_rope(q_in, k_in, qw_in, kw_in, freqs_in, positions_in, a);
+  c10::cuda::CUDAGuard guard(q_in.device());
+  const torch::Tensor q = with_dense_rows(q_in), k = with_dense_rows(k_in), freqs = freqs_in.contiguous();
+  const torch::Tensor positions = positions_in.size(-1) > 1 && positions_in.stride(-1) != 1 ? positions_in.contiguous() : positions_in;
+  const torch::Tensor qw = qw_in.defined() ? qw_in.contiguous() : qw_in, kw = kw_in.defined() ? kw_in.contiguous() : kw_in;
+  const attn_rope_shape_t s = rope_shape(q, k, qw, kw, freqs, positions, a);
+  variable_list out{fresh(q.sizes(), q.scalar_type(), q), fresh(k.sizes(), k.scalar_type(), k)};
+  check_rc(attn_b200_packed_qk_norm_rope(&s, q.data_ptr(), k.data_ptr(), ptr_or_null(qw), ptr_or_null(kw), freqs.data_ptr<float>(), positions.data_ptr(),
+                                         out[0].data_ptr(), out[1].data_ptr(), at::cuda::getCurrentCUDAStream().stream()),
+           "packed_qk_norm_rope");
+  return out;
+}
+
+// {gq, gk, gq_weight, gk_weight}; a weight's is undefined without it or where it is not wanted
+variable_list rope_backward(const torch::Tensor& gq_in, const torch::Tensor& gk_in, const torch::Tensor& q_in, const torch::Tensor& k_in,
+                            const torch::Tensor& qw_in, const torch::Tensor& kw_in, const torch::Tensor& freqs_in, const torch::Tensor& positions_in,
+                            const RopeArgs& a, bool want_qw, bool want_kw) {
+  c10::cuda::CUDAGuard guard(q_in.device());
+  const torch::Tensor q = with_dense_rows(q_in), k = with_dense_rows(k_in), freqs = freqs_in.contiguous();
+  const torch::Tensor positions = positions_in.size(-1) > 1 && positions_in.stride(-1) != 1 ? positions_in.contiguous() : positions_in;
+  const torch::Tensor qw = qw_in.defined() ? qw_in.contiguous() : qw_in, kw = kw_in.defined() ? kw_in.contiguous() : kw_in;
+  auto gradient = [](const torch::Tensor& g, const torch::Tensor& like) {
+    TORCH_CHECK(!g.defined() || (g.sizes() == like.sizes() && g.scalar_type() == like.scalar_type() && g.device() == like.device()),
+                "the gradients of packed_qk_norm_rope's results must be like them");
+    return g.defined() ? with_dense_rows(g) : torch::zeros(like.sizes(), like.options());
+  };
+  const torch::Tensor gq = gradient(gq_in, q), gk = gradient(gk_in, k);
+  attn_rope_shape_t s = rope_shape(q, k, qw, kw, freqs, positions, a);
+  s.g_row_stride[0] = gq.stride(0); s.g_head_stride[0] = gq.stride(1);
+  s.g_row_stride[1] = gk.stride(0); s.g_head_stride[1] = gk.stride(1);
+  variable_list out{fresh(q.sizes(), q.scalar_type(), q), fresh(k.sizes(), k.scalar_type(), k), torch::Tensor(), torch::Tensor()};
+  if (want_qw && qw.defined()) out[2] = fresh(qw.sizes(), qw.scalar_type(), qw);
+  if (want_kw && kw.defined()) out[3] = fresh(kw.sizes(), kw.scalar_type(), kw);
+  torch::Tensor scratch;
+  if (out[2].defined() || out[3].defined())
+    scratch = fresh({(int64_t)(attn_b200_packed_qk_norm_rope_backward_scratch_bytes(&s) / sizeof(float)) + 4}, at::kFloat, q);
+  check_rc(attn_b200_packed_qk_norm_rope_backward(&s, q.data_ptr(), k.data_ptr(), ptr_or_null(qw), ptr_or_null(kw), freqs.data_ptr<float>(),
+                                                  positions.data_ptr(), gq.data_ptr(), gk.data_ptr(), out[0].data_ptr(), out[1].data_ptr(),
+                                                  ptr_or_null(out[2]), ptr_or_null(out[3]), static_cast<float*>(ptr_or_null(scratch)),
+                                                  at::cuda::getCurrentCUDAStream().stream()),
+           "packed_qk_norm_rope backward");
+  return out;
+}
+
+// The same out of ordinary operations, for the second backward.
+torch::Tensor rope_angles(const torch::Tensor& freqs, const torch::Tensor& positions, const RopeArgs& a) {
+  const torch::Tensor nan = torch::full({}, std::numeric_limits<float>::quiet_NaN(), freqs.options());
+  if (freqs.size(0) == 0) return nan.expand({positions.size(-1), 1, freqs.size(1), 2});
+  std::vector<torch::Tensor> parts;
+  int64_t first = 0;
+  for (size_t i = 0; i < a.sections.size(); ++i) {
+    const torch::Tensor p = (positions.dim() == 2 ? positions.select(0, (int64_t)i) : positions).to(at::kLong);
+    const torch::Tensor in = (p >= 0) & (p < freqs.size(0));
+    const torch::Tensor t = freqs.slice(1, first, first + a.sections[i]).index_select(0, torch::where(in, p, torch::zeros_like(p)));
+    parts.push_back(torch::where(in.view({-1, 1, 1}), t, nan));
+    first += a.sections[i];
+  }
+  return torch::cat(parts, 1).unsqueeze(1);      // [n_tok, 1, D / 2, 2]
+}
+
+torch::Tensor rope_formula(const torch::Tensor& x, const torch::Tensor& w, const torch::Tensor& angles, double eps) {
+  torch::Tensor y = x.to(at::kFloat);
+  if (w.defined()) y = y * torch::rsqrt(y.pow(2).mean({-1}, true) + eps) * w.to(at::kFloat);
+  const torch::Tensor pair = y.reshape({x.size(0), x.size(1), x.size(2) / 2, 2});
+  const torch::Tensor u = pair.select(-1, 0), v = pair.select(-1, 1), c = angles.select(-1, 0), s = angles.select(-1, 1);
+  return torch::stack({u * c - v * s, u * s + v * c}, -1).reshape(x.sizes()).to(x.scalar_type());
+}
+
+void save_rope(AutogradContext* ctx, const std::vector<int64_t>& sections, double eps) {
+  ctx->set_materialize_grads(false);
+  ctx->saved_data["sections"] = sections;
+  ctx->saved_data["eps"] = eps;
+}
+RopeArgs saved_rope(AutogradContext* ctx) { return {ctx->saved_data["sections"].toIntVector(), ctx->saved_data["eps"].toDouble()}; }
+
+struct PackedQKNormRopeBackward : public torch::autograd::Function<PackedQKNormRopeBackward> {
+  static variable_list forward(AutogradContext* ctx, const torch::Tensor& gq, const torch::Tensor& gk, const torch::Tensor& q, const torch::Tensor& k,
+                               const torch::Tensor& qw, const torch::Tensor& kw, const torch::Tensor& freqs, const torch::Tensor& positions,
+                               std::vector<int64_t> sections, double eps) {
+    save_rope(ctx, sections, eps);
+    ctx->save_for_backward({gq, gk, q, k, qw, kw, freqs, positions});
+    variable_list r = rope_backward(gq, gk, q, k, or_none(qw), or_none(kw), freqs, positions, {sections, eps}, true, true);
+    for (int i = 2; i < 4; ++i)
+      if (!r[i].defined()) r[i] = fresh({0}, at::kFloat, q);
+    return r;
+  }
+
+  static variable_list backward(AutogradContext* ctx, variable_list tangents) {
+    variable_list out(10);      // gq, gk, q, k, qw, kw, freqs, positions, sections, eps
+    const variable_list s = ctx->get_saved_variables();
+    const RopeArgs a = saved_rope(ctx);
+    const bool keep_graph = at::GradMode::is_enabled();
+    at::AutoGradMode on(true);
+    const torch::Tensor angles = rope_angles(s[6], s[7], a).detach();
+    // aliases of the inputs, so that the derivatives are partial ones even where the inputs depend on one another
+    auto alias = [&](const torch::Tensor& t) { return keep_graph && t.requires_grad() ? t.view_as(t) : t.detach().requires_grad_(true); };
+    for (int side = 0; side < 2; ++side) {
+      const torch::Tensor g = alias(s[side]), x = alias(s[2 + side]);
+      variable_list first_wrt{x}, wrt{g, x};
+      torch::Tensor w;
+      if (s[4 + side].numel() > 0) {
+        w = alias(s[4 + side]);
+        first_wrt.push_back(w);
+        wrt.push_back(w);
+      }
+      const variable_list first = torch::autograd::grad({rope_formula(x, w, angles, a.eps)}, first_wrt, {g}, true, true);
+      variable_list of, with;
+      for (size_t i = 0; i < first.size(); ++i) {
+        const torch::Tensor& t = tangents[i == 0 ? side : 2 + side];
+        if (t.defined()) { of.push_back(first[i]); with.push_back(t); }
+      }
+      if (of.empty()) continue;
+      const variable_list r = torch::autograd::grad(of, wrt, with, true, keep_graph, true);
+      out[side] = r[0];
+      out[2 + side] = r[1];
+      if (w.defined()) out[4 + side] = r[2];
+    }
+    return out;
+  }
+};
+
+struct PackedQKNormRope : public torch::autograd::Function<PackedQKNormRope> {
+  static variable_list forward(AutogradContext* ctx, const torch::Tensor& q, const torch::Tensor& k, const torch::Tensor& qw, const torch::Tensor& kw,
+                               const torch::Tensor& freqs, const torch::Tensor& positions, std::vector<int64_t> sections, double eps) {
+    variable_list r = rope_forward(q, k, or_none(qw), or_none(kw), freqs, positions, {sections, eps});
+    save_rope(ctx, sections, eps);
+    ctx->save_for_backward({q, k, qw, kw, freqs, positions});
+    return r;
+  }
+
+  static variable_list backward(AutogradContext* ctx, variable_list g) {
+    variable_list out(8);      // q, k, qw, kw, freqs, positions, sections, eps
+    if (!g[0].defined() && !g[1].defined()) return out;
+    const variable_list s = ctx->get_saved_variables();
+    const RopeArgs a = saved_rope(ctx);
+    TORCH_CHECK(!has_tangent({&g[0], &g[1], &s[0], &s[1], &s[2], &s[3]}), "packed_qk_norm_rope has no forward-mode derivative");
+    variable_list r;
+    if (at::GradMode::is_enabled()) {
+      auto whole = [](const torch::Tensor& t, const torch::Tensor& like) { return t.defined() ? t : torch::zeros(like.sizes(), like.options()); };
+      r = PackedQKNormRopeBackward::apply(whole(g[0], s[0]), whole(g[1], s[1]), s[0], s[1], s[2], s[3], s[4], s[5], a.sections, a.eps);
+      for (int i = 2; i < 4; ++i)
+        if (s[i].numel() == 0) r[i] = torch::Tensor();
+    } else {
+      r = rope_backward(g[0], g[1], s[0], s[1], or_none(s[2]), or_none(s[3]), s[4], s[5], a, ctx->needs_input_grad(2), ctx->needs_input_grad(3));
+    }
+    for (int i = 0; i < 4; ++i) out[i] = std::move(r[i]);
+    return out;
+  }
+};
+
+variable_list packed_qk_norm_rope(const torch::Tensor& q, const torch::Tensor& k, c10::optional<torch::Tensor> q_weight,
+                                  c10::optional<torch::Tensor> k_weight, const torch::Tensor& freqs, const torch::Tensor& positions,
+                                  std::vector<int64_t> sections, double eps) {
+  const torch::Tensor qw = q_weight.value_or(torch::Tensor()), kw = k_weight.value_or(torch::Tensor());
+  refuse_transforms({&q, &k, &qw, &kw, &freqs}, "packed_qk_norm_rope");
+  TORCH_CHECK(!freqs.requires_grad(), "packed_qk_norm_rope has no gradient of freqs");
+  TORCH_CHECK(q.dim() != 3 || q.size(2) > 0, "D must be positive");
+  if (!wants_graph({&q, &k, &qw, &kw})) return rope_forward(q, k, qw, kw, freqs, positions, {sections, eps});
+  check_rope(q, k, qw, kw, freqs, positions, {sections, eps});
+  const torch::Tensor none = qw.defined() && kw.defined() ? torch::Tensor() : fresh({0}, q.scalar_type(), q);
+  return PackedQKNormRope::apply(q, k, qw.defined() ? qw : none, kw.defined() ? kw : none, freqs, positions, sections, eps);
+}
+
 }  // namespace
 
 void register_packed(pybind11::module& m) {
@@ -228,6 +446,9 @@ void register_packed(pybind11::module& m) {
   m.def("packed_attention", &packed_attention, "causal attention within the sequences of a packed batch, grouped heads, twice differentiable -> O",
         py::arg("q"), py::arg("k"), py::arg("v"), py::arg("plan"), py::arg("n_tok"), py::arg("n_seq"), py::arg("window_size") = py::none(),
         py::arg("max_seqlen") = py::none(), py::call_guard<py::gil_scoped_release>());
+  m.def("packed_qk_norm_rope", &packed_qk_norm_rope, "RMS norm of q and k per head and rotation by per-token positions, twice differentiable -> [q, k]",
+        py::arg("q"), py::arg("k"), py::arg("q_weight"), py::arg("k_weight"), py::arg("freqs"), py::arg("positions"), py::arg("sections"),
+        py::arg("eps") = 1e-6, py::call_guard<py::gil_scoped_release>());
 }
 
 }  // namespace ext

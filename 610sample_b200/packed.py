@@ -1,13 +1,15 @@
 """Packed batches: sequences of different lengths laid end to end on one axis of rows, without padding.
 
     plan = packed_plan(cu_seqlens, n_tok)                  # once per batch, shared by all layers
+    q, k = packed_qk_norm_rope(q, k, q_weight, k_weight, freqs, positions)
     O = packed_attention(q, k, v, plan)                    # [n_tok, heads, D]
 
 Attention is causal within each sequence, optionally within a sliding window, with grouped heads: `q` has a
 multiple of the heads of `k` and `v`, head h of `q` reading head h // (heads of q / heads of k).  It is
 differentiable to second order, as `flash_attention_v7`; the second derivative runs on rows padded to the
 longest sequence.  There is no counterpart in the reference, whose batches are dense [B, H, N, D]
-(e2e/ttt_pytorch/model.py:174-191).  There is no fallback: importing this module fails if the compiled
+(e2e/ttt_pytorch/model.py:174-191).  `packed_qk_norm_rope` is the step in front of it, as `qk_norm_rope` is
+for dense batches, with positions given per token.  There is no fallback: importing this module fails if the compiled
 extension `attention_cuda` is missing.
 """
 import torch
@@ -52,3 +54,21 @@ def packed_attention(q, k, v, plan, window_size=None):
     within a sequence, an infinite or NaN key or value may reach the queries of up to 127 rows before it as well.
     Returns O: (n_tok, H, D), dense."""
     return _attention_cuda.packed_attention(q, k, v, plan.tensor, plan.n_tok, plan.n_seq, window_size, plan.max_seqlen)
+
+
+def packed_qk_norm_rope(q, k, q_weight, k_weight, freqs, positions, sections=None, eps=1e-6):
+    """RMS norm of every row of q: (n_tok, H, D) and k: (n_tok, H_kv, D) over D, times a weight, then rotation of its pairs
+    (elements 2i and 2i + 1) by the angle of the token's position; one pass over both.  Returns (q, k), dense.
+
+    q_weight, k_weight: (D,), of the type of q and k or float32; None: no norm, only the rotation.
+    freqs: `qk_prep.rope_table(...)`, float32 (rows, D / 2, 2); positions: (n_tok,) or (axes, n_tok), int32 or int64, rows of
+    freqs; one outside of it gives NaN.  sections: how many of the D / 2 pairs turn with each axis, in order (up to four
+    axes: time, height and width of a video's patches, say); None for positions of one axis.
+    q and k may be slices of one projection's result.  D even, up to 128; fp16, bf16 or fp32.  Computed in float32 and
+    rounded once (`qk_norm_rope` rounds where the reference's separate operations do).  Twice differentiable in q, k and the
+    weights; the second derivative is computed by PyTorch operations."""
+    if sections is None:
+        if positions.dim() != 1:
+            raise ValueError("positions of several axes need sections")
+        sections = (q.shape[-1] // 2,)
+    return tuple(_attention_cuda.packed_qk_norm_rope(q, k, q_weight, k_weight, freqs, positions, list(sections), eps))

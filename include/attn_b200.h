@@ -204,6 +204,37 @@ size_t attn_b200_packed_backward_scratch_bytes(const attn_packed_shape_t* shape)
 int attn_b200_packed_backward(const attn_packed_shape_t* shape, const int32_t* plan, const void* dO, const void* Q, const void* K,
                               const void* V, const void* O, const float* L, void* dQ, void* dK, void* dV, float* scratch, void* stream);
 
+/* The step in front of packed attention: per (token, head) RMS normalisation with a learned weight and rotation by positions
+ * that are given per token, on up to four axes, of Q and K in one pass.  Pair i of a row, elements 2i and 2i + 1, is turned by
+ * row positions[axis][token] of freqs, float32 [table_rows, D / 2, 2] = (cos, sin); axis 0 has the first section[0] pairs, axis 1
+ * the next section[1], and so on, D / 2 in all.  A position outside of the table gives NaN.  Arithmetic in fp32, rounded once
+ * (attn_b200_qk_norm_rope has the rounding points of the reference's separate operations instead).
+ * q: [n_tok, q_heads, D], k: [n_tok, k_heads, D] in strides of elements, results dense; weights [D], null for no norm, of the type of
+ * q and k or (weight_float) float32; positions [axes][n_tok], axis_stride elements apart, int32 or (positions64) int64.  D even, up to
+ * 128; multiples of 8 with 16-byte aligned rows are read 16 bytes at a time. */
+typedef struct attn_rope_shape {
+  int32_t n_tok, q_heads, k_heads, D;
+  int32_t dtype;
+  int32_t table_rows, axes, positions64;
+  int32_t section[4], weight_float[2];
+  float eps;
+  int32_t reserved;
+  int64_t axis_stride;
+  int64_t row_stride[2], head_stride[2];       /* q, k */
+  int64_t g_row_stride[2], g_head_stride[2];   /* the gradients of the results, in the backward */
+} attn_rope_shape_t;
+
+int attn_b200_packed_qk_norm_rope(const attn_rope_shape_t* shape, const void* q, const void* k, const void* q_weight,
+                                  const void* k_weight, const float* freqs, const void* positions, void* q_out, void* k_out, void* stream);
+
+/* gq, gk: dense, the gradients of q and k; gq_weight, gk_weight: [D] in the weights' types, null if not wanted (scratch is only
+ * used with one of them). */
+size_t attn_b200_packed_qk_norm_rope_backward_scratch_bytes(const attn_rope_shape_t* shape);
+int attn_b200_packed_qk_norm_rope_backward(const attn_rope_shape_t* shape, const void* q, const void* k, const void* q_weight,
+                                           const void* k_weight, const float* freqs, const void* positions, const void* gq_out,
+                                           const void* gk_out, void* gq, void* gk, void* gq_weight, void* gk_weight, float* scratch,
+                                           void* stream);
+
 /* ---- Cross entropy of a linear layer --------------------------------------------------------------
  * z = x W^T, loss_i = log sum_j exp(z_ij) - z_i,targets[i], without z being kept: the forward reduces it tile by tile, the
  * backward forms its gradient for a piece of the vocabulary at a time (at most 256 MB, or 1024 columns).  x: [n, d], w: [V, d]
