@@ -101,6 +101,7 @@ fwd_kernel(const __grid_constant__ TmaMaps maps, const Geo g, const Tensors t) {
   using CF = FwdCfg<D, G>;
   constexpr bool kPacked = Geo::kPacked;
   static_assert(!(kPacked && SPLIT), "packed batches are not split");
+  constexpr bool kTakeMax = CF::kTakeMax || kPacked;
   constexpr int kAtoms = CF::kAtoms, kFwdSBufs = CF::kSBufs;
   constexpr int kMathWarps = CF::kMathWarps, kMathThreads = CF::kMathThreads, kProducerWarp = CF::kProducerWarp;
   constexpr int kFwdSWarp = CF::kSWarp, kFwdPvWarp = CF::kPvWarp, kTmemCols = CF::kTmemCols;
@@ -453,13 +454,26 @@ fwd_kernel(const __grid_constant__ TmaMaps maps, const Geo g, const Tensors t) {
         tile_sum = (sum_a.x + sum_a.y) + (sum_b.x + sum_b.y);
       };
       // The reference is tried as it stands, unless the maximum is likely to be needed.
-      const bool attempt = !CF::kTakeMax && !exact && !need_max;
+      const bool attempt = !kTakeMax && !exact && !need_max;
       bool take_max = true;
       if (attempt) {
         exponentials(-m_ref);
         take_max = __any_sync(0xffffffffu, !(tile_sum <= CF::kMaxSum));
       }
       if (take_max) {
+        float mx;
+        if constexpr (kPacked) {
+          // three scores to an instruction, in four independent chains
+          float m4[4];
+#pragma unroll
+          for (int c = 0; c < 4; ++c) {
+            m4[c] = max3(__uint_as_float(s_[c][0]), __uint_as_float(s_[c][1]), __uint_as_float(s_[c][2]));
+#pragma unroll
+            for (int e = 3; e < 15; e += 2) m4[c] = max3(m4[c], __uint_as_float(s_[c][e]), __uint_as_float(s_[c][e + 1]));
+            m4[c] = fmaxf(m4[c], __uint_as_float(s_[c][15]));
+          }
+          mx = fmaxf(max3(m4[0], m4[1], m4[2]), m4[3]) * g.scale_log2e;
+        } else {
         // maximum of the raw scores (-inf where masked) in eight independent chains
         float mx8[8];
 #pragma unroll
@@ -468,8 +482,8 @@ fwd_kernel(const __grid_constant__ TmaMaps maps, const Geo g, const Tensors t) {
         for (int c = 1; c < 4; ++c)
 #pragma unroll
           for (int e = 0; e < 8; ++e) mx8[e] = fmaxf(mx8[e], fmaxf(__uint_as_float(s_[c][e]), __uint_as_float(s_[c][8 + e])));
-        const float mx = fmaxf(fmaxf(fmaxf(mx8[0], mx8[1]), fmaxf(mx8[2], mx8[3])), fmaxf(fmaxf(mx8[4], mx8[5]), fmaxf(mx8[6], mx8[7]))) *
-                         g.scale_log2e;
+        mx = fmaxf(fmaxf(fmaxf(mx8[0], mx8[1]), fmaxf(mx8[2], mx8[3])), fmaxf(fmaxf(mx8[4], mx8[5]), fmaxf(mx8[6], mx8[7]))) * g.scale_log2e;
+        }
         // a row's own scores alone decide whether its reference moves
         const bool grow = mx > m_ref + tau || (m_ref == -INFINITY && mx > -INFINITY);
         const bool any_grow = __any_sync(0xffffffffu, grow);

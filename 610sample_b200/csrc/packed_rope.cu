@@ -21,7 +21,8 @@ namespace rope {
 
 using tc::from_l2;
 
-constexpr int kThreads = 256, kHeads = 4, kMaxAxes = 4;
+constexpr int kThreads = 256, kMaxAxes = 4;
+constexpr int kForwardHeads = 4, kBackwardHeads = 2;      // of a batch
 
 struct Side {                    // q or k
   const void *x, *g, *w;         // w: null for no norm
@@ -98,18 +99,38 @@ template <typename T, bool WIDE> __device__ __forceinline__ void store8(T* p, co
     for (int i = 0; i < n; ++i) p[i] = Elem<T>::from_float(v[i]);
 }
 
-template <typename T>
+// this lane's eight weights; 1 where there is no norm
+template <typename T, bool WIDE>
 __device__ __forceinline__ void load_weight(const Side& s, int col, int n, float (&w)[8]) {
 #pragma unroll
-  for (int e = 0; e < 8; ++e) {
-    w[e] = 1.f;
-    if (s.w != nullptr && e < n)
-      w[e] = s.w_float ? static_cast<const float*>(s.w)[col + e] : Elem<T>::to_float(static_cast<const T*>(s.w)[col + e]);
+  for (int e = 0; e < 8; ++e) w[e] = 1.f;
+  if (s.w == nullptr || n <= 0) return;
+  if (s.w_float) {
+    const float* p = static_cast<const float*>(s.w) + col;
+#pragma unroll
+    for (int e = 0; e < 8; ++e)
+      if (e < n) w[e] = p[e];
+  } else if (WIDE) {
+    Eight<T> e;
+    e.load(static_cast<const T*>(s.w) + col);
+    e.get(w);
+  } else {
+#pragma unroll
+    for (int e = 0; e < 8; ++e)
+      if (e < n) w[e] = Elem<T>::to_float(static_cast<const T*>(s.w)[col + e]);
   }
 }
 
 // (cos, sin) of this lane's four pairs; not a number for a position outside of the table
 __device__ __forceinline__ void load_angles(const Args& a, int tok, int pair0, int pairs, float2 (&cs)[4]) {
+  if (a.axes == 1) {
+    const long long pos = a.positions64 ? from_l2(static_cast<const long long*>(a.positions) + tok) : from_l2(static_cast<const int*>(a.positions) + tok);
+    const bool in = pos >= 0 && pos < a.table_rows;
+    const float2* row = reinterpret_cast<const float2*>(a.table) + (in ? pos : 0) * pairs + pair0;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) cs[i] = in && pair0 + i < pairs ? from_l2(row + i) : make_float2(NAN, NAN);
+    return;
+  }
   int axis = 0, row = -1, row_axis = -1;
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
@@ -133,85 +154,132 @@ template <int G> __device__ __forceinline__ float group_sum(float v) {
   return v;
 }
 
+// Heads are taken a few at a time, those of q first: a batch's side, its first head and how many heads it has.
+struct Batch { int which, h0, heads; };
+template <int H>
+__device__ __forceinline__ Batch batch_at(const Args& a, int b) {
+  const int q_batches = (a.side[0].heads + H - 1) / H, which = b >= q_batches;
+  const int h0 = (which ? b - q_batches : b) * H;
+  return {which, h0, min(H, a.side[which].heads - h0)};
+}
+__host__ __device__ inline int batches_of(long long q_heads, long long k_heads, int H) { return (int)((q_heads + H - 1) / H + (k_heads + H - 1) / H); }
+
+// A group of G lanes owns a token and walks over its share of the batches, the next one on its way meanwhile; the angles are
+// fetched once.  `shares` CTAs have the same tokens.
 template <typename T, int G, bool WIDE>
 __global__ void __launch_bounds__(kThreads)
-forward_kernel(const Args a) {
+forward_kernel(const __grid_constant__ Args a, const int shares) {
   tc::pdl_wait();
   tc::pdl_trigger();
-  const int q_blocks = (a.side[0].heads + kHeads - 1) / kHeads, blocks = q_blocks + (a.side[1].heads + kHeads - 1) / kHeads;
-  const int hb = (int)(blockIdx.x % (unsigned)blocks), which = hb >= q_blocks;
-  const Side& s = a.side[which];
-  const int h0 = (which ? hb - q_blocks : hb) * kHeads, heads = min(kHeads, s.heads - h0);
+  const int share = (int)(blockIdx.x % (unsigned)shares), batches = batches_of(a.side[0].heads, a.side[1].heads, kForwardHeads);
+  const int first = (int)((long long)batches * share / shares), last = (int)((long long)batches * (share + 1) / shares);
   const int sub = threadIdx.x % G, col = sub * 8, n = min(8, a.D - col);
-  const int tok = (int)(blockIdx.x / (unsigned)blocks) * (kThreads / G) + threadIdx.x / G;
+  const int tok = (int)(blockIdx.x / (unsigned)shares) * (kThreads / G) + threadIdx.x / G;
   const bool on = tok < a.n_tok && n > 0;      // the shuffles need every lane of a warp
-  Eight<T> raw[kHeads];
+  const float inv_d = 1.f / (float)a.D;
+  auto load = [&](const Batch& b, Eight<T> (&raw)[kForwardHeads]) {
+    const Side& s = a.side[b.which];
+    const T* p = static_cast<const T*>(s.x) + tok * s.row + b.h0 * s.head + col;
 #pragma unroll
-  for (int i = 0; i < kHeads; ++i) {
-    raw[i].zero();
-    if (on && i < heads) load8<T, WIDE>(raw[i], static_cast<const T*>(s.x) + tok * s.row + (h0 + i) * s.head + col, n);
-  }
-  float2 cs[4] = {};
-  float w[8];
-  if (on) load_angles(a, tok, sub * 4, a.D >> 1, cs);
-  load_weight<T>(s, col, on ? n : 0, w);
-  const bool norm = s.w != nullptr;      // uniform over the CTA
-#pragma unroll
-  for (int i = 0; i < kHeads; ++i) {
-    float v[8];
-    raw[i].get(v);
-    if (norm) {
-      float ss = 0.f;
-#pragma unroll
-      for (int e = 0; e < 8; ++e) ss = fmaf(v[e], v[e], ss);
-      const float r = rsqrtf(group_sum<G>(ss) / (float)a.D + a.eps);
-#pragma unroll
-      for (int e = 0; e < 8; ++e) v[e] *= r * w[e];
+    for (int i = 0; i < kForwardHeads; ++i) {
+      raw[i].zero();
+      if (on && i < b.heads) load8<T, WIDE>(raw[i], p + i * s.head, n);
     }
-    if (on && i < heads) {
-      float o[8];
+  };
+  Batch cur = batch_at<kForwardHeads>(a, first);
+  Eight<T> raw[kForwardHeads], next[kForwardHeads];
+  load(cur, raw);
+  float2 cs[4] = {};
+  if (on) load_angles(a, tok, sub * 4, a.D >> 1, cs);
+  int side = -1;
+  float w[8];
+  for (int b = first; b < last; ++b) {
+    const Batch now = cur;
+    const bool more = b + 1 < last;
+    if (more) {
+      cur = batch_at<kForwardHeads>(a, b + 1);
+      load(cur, next);
+    }
+    const Side& s = a.side[now.which];
+    if (now.which != side) {
+      side = now.which;
+      load_weight<T, WIDE>(s, col, on ? n : 0, w);
+    }
+    const bool norm = s.w != nullptr;      // uniform over the CTA
+    T* out = static_cast<T*>(s.out) + ((size_t)tok * s.heads + now.h0) * a.D + col;
 #pragma unroll
-      for (int p = 0; p < 4; ++p) {
-        o[2 * p] = v[2 * p] * cs[p].x - v[2 * p + 1] * cs[p].y;
-        o[2 * p + 1] = v[2 * p] * cs[p].y + v[2 * p + 1] * cs[p].x;
+    for (int i = 0; i < kForwardHeads; ++i) {
+      float v[8];
+      raw[i].get(v);
+      if (norm) {
+        float ss = 0.f;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) ss = fmaf(v[e], v[e], ss);
+        const float r = rsqrtf(fmaf(group_sum<G>(ss), inv_d, a.eps));
+#pragma unroll
+        for (int e = 0; e < 8; ++e) v[e] *= r * w[e];
       }
-      store8<T, WIDE>(static_cast<T*>(s.out) + ((size_t)tok * s.heads + h0 + i) * a.D + col, o, n);
+      if (on && i < now.heads) {
+        float o[8];
+#pragma unroll
+        for (int p = 0; p < 4; ++p) {
+          o[2 * p] = v[2 * p] * cs[p].x - v[2 * p + 1] * cs[p].y;
+          o[2 * p + 1] = v[2 * p] * cs[p].y + v[2 * p + 1] * cs[p].x;
+        }
+        store8<T, WIDE>(out + (size_t)i * a.D, o, n);
+      }
+    }
+    if (more) {
+#pragma unroll
+      for (int i = 0; i < kForwardHeads; ++i) raw[i] = next[i];
     }
   }
 }
 
+// The tasks, tokens x shares of the batches, are dealt to the CTAs in turn.
 template <typename T, int G, bool WIDE>
-__global__ void __launch_bounds__(kThreads)
-backward_kernel(const Args a, float* partial) {      // partial: [2][CTAs][D], null where no weight's gradient is wanted
+__global__ void __launch_bounds__(kThreads, sizeof(T) == 2 ? 3 : 2)
+backward_kernel(const __grid_constant__ Args a, const int shares, float* partial) {      // partial: [2][CTAs][D], null where no weight's gradient is wanted
   constexpr int kTok = kThreads / G;
   __shared__ float sums[kThreads * 8];
   tc::pdl_wait();
   tc::pdl_trigger();
-  const int sub = threadIdx.x % G, col = sub * 8, n = min(8, a.D - col);
-#pragma unroll 1
-  for (int which = 0; which < 2; ++which) {
-    const Side& s = a.side[which];
-    const unsigned blocks = (unsigned)(s.heads + kHeads - 1) / kHeads, tasks = (unsigned)((a.n_tok + kTok - 1) / kTok) * blocks;
-    const bool norm = s.w != nullptr;
-    float w[8], acc[8] = {};
-    load_weight<T>(s, col, n, w);
-    for (unsigned task = blockIdx.x; task < tasks; task += gridDim.x) {
-      const int tok = (int)(task / blocks) * kTok + threadIdx.x / G, h0 = (int)(task % blocks) * kHeads, heads = min(kHeads, s.heads - h0);
-      const bool on = tok < a.n_tok && n > 0;
-      Eight<T> rx[kHeads], rg[kHeads];
+  const int sub = threadIdx.x % G, col = sub * 8, n = min(8, a.D - col), batches = batches_of(a.side[0].heads, a.side[1].heads, kBackwardHeads);
+  const unsigned tasks = (unsigned)((a.n_tok + kTok - 1) / kTok) * (unsigned)shares;
+  const float inv_d = 1.f / (float)a.D;
+  float w[8], acc[2][8] = {};
+  int side = -1;
+  for (unsigned task = blockIdx.x; task < tasks; task += gridDim.x) {
+    const int share = (int)(task % (unsigned)shares), tok = (int)(task / (unsigned)shares) * kTok + threadIdx.x / G;
+    const int first = (int)((long long)batches * share / shares), last = (int)((long long)batches * (share + 1) / shares);
+    const bool on = tok < a.n_tok && n > 0;
+    float2 cs[4] = {};
+    for (int b = first; b < last; ++b) {
+      const Batch now = batch_at<kBackwardHeads>(a, b);
+      const Side& s = a.side[now.which];
+      const bool norm = s.w != nullptr;
+      Eight<T> rx[kBackwardHeads], rg[kBackwardHeads];
+      {
+        const T* px = static_cast<const T*>(s.x) + tok * s.row + now.h0 * s.head + col;
+        const T* pg = static_cast<const T*>(s.g) + tok * s.g_row + now.h0 * s.g_head + col;
 #pragma unroll
-      for (int i = 0; i < kHeads; ++i) {
-        rx[i].zero();
-        rg[i].zero();
-        if (on && i < heads) {
-          load8<T, WIDE>(rg[i], static_cast<const T*>(s.g) + tok * s.g_row + (h0 + i) * s.g_head + col, n);
-          if (norm) load8<T, WIDE>(rx[i], static_cast<const T*>(s.x) + tok * s.row + (h0 + i) * s.head + col, n);
+        for (int i = 0; i < kBackwardHeads; ++i) {
+          rx[i].zero();
+          rg[i].zero();
+          if (on && i < now.heads) {
+            load8<T, WIDE>(rg[i], pg + i * s.g_head, n);
+            if (norm) load8<T, WIDE>(rx[i], px + i * s.head, n);
+          }
         }
       }
-      float2 cs[4] = {};
-      if (on) load_angles(a, tok, sub * 4, a.D >> 1, cs);
+      if (b == first && on) load_angles(a, tok, sub * 4, a.D >> 1, cs);
+      if (now.which != side) {
+        side = now.which;
+        load_weight<T, WIDE>(s, col, n, w);
+      }
+      T* out = static_cast<T*>(s.out) + ((size_t)tok * s.heads + now.h0) * a.D + col;
 #pragma unroll
-      for (int i = 0; i < kHeads; ++i) {
+      for (int i = 0; i < kBackwardHeads; ++i) {
         float gv[8], xv[8], gy[8];
         rg[i].get(gv);
         rx[i].get(xv);
@@ -222,35 +290,40 @@ backward_kernel(const Args a, float* partial) {      // partial: [2][CTAs][D], n
         }
         if (norm) {      // uniform: every lane takes part in the shuffles
           float ss = 0.f, dot = 0.f;
+          bool any = false;
 #pragma unroll
           for (int e = 0; e < 8; ++e) {
             ss = fmaf(xv[e], xv[e], ss);
-            if (e < n) dot = fmaf(gy[e] * w[e], xv[e], dot);      // pairs beyond D have no angle
+            if (WIDE || e < n) {      // pairs beyond D have no angle
+              dot = fmaf(gy[e] * w[e], xv[e], dot);
+              any |= gy[e] != 0.f;
+            }
           }
           ss = group_sum<G>(ss);
           dot = group_sum<G>(dot);
           // a row whose gradient is 0 gives 0, also where the row (of no sequence, say) is infinite or not a number
-          bool any = false;
-#pragma unroll
-          for (int e = 0; e < 8; ++e) any |= e < n && gy[e] != 0.f;
           const unsigned lanes = __ballot_sync(0xffffffffu, any);
-          if (on && i < heads && ((lanes >> ((threadIdx.x & 31) / G * G)) & ((1u << G) - 1u)) != 0u) {
-            const float inv_d = 1.f / (float)a.D, r = rsqrtf(ss * inv_d + a.eps), k = r * r * r * inv_d * dot;
+          if (on && i < now.heads && ((lanes >> ((threadIdx.x & 31) / G * G)) & ((1u << G) - 1u)) != 0u) {
+            const float r = rsqrtf(fmaf(ss, inv_d, a.eps)), k = r * r * r * inv_d * dot;
 #pragma unroll
             for (int e = 0; e < 8; ++e) {
-              if (e < n) acc[e] = fmaf(gy[e], xv[e] * r, acc[e]);
+              const float add = (WIDE || e < n) ? gy[e] * (xv[e] * r) : 0.f;
+              if (now.which) acc[1][e] += add; else acc[0][e] += add;
               gy[e] = r * gy[e] * w[e] - k * xv[e];
             }
           }
         }
-        if (on && i < heads) store8<T, WIDE>(static_cast<T*>(s.out) + ((size_t)tok * s.heads + h0 + i) * a.D + col, gy, n);
+        if (on && i < now.heads) store8<T, WIDE>(out + (size_t)i * a.D, gy, n);
       }
     }
-    if (partial == nullptr || !norm) continue;      // uniform
+  }
+  if (partial == nullptr) return;
+#pragma unroll
+  for (int which = 0; which < 2; ++which) {
     __syncthreads();
     float4* mine = reinterpret_cast<float4*>(sums + (threadIdx.x / G) * (8 * G) + col);
-    mine[0] = make_float4(acc[0], acc[1], acc[2], acc[3]);
-    mine[1] = make_float4(acc[4], acc[5], acc[6], acc[7]);
+    mine[0] = make_float4(acc[which][0], acc[which][1], acc[which][2], acc[which][3]);
+    mine[1] = make_float4(acc[which][4], acc[which][5], acc[which][6], acc[which][7]);
     __syncthreads();
     if (threadIdx.x < a.D) {
       float t = 0.f;
@@ -286,11 +359,24 @@ weight_grad_kernel(const float* partial, void* gw0, void* gw1, int rows, int D, 
   else static_cast<T*>(gw)[at] = Elem<T>::from_float(s);
 }
 
-// backward: four CTAs on each SM, which walk over the tasks of q, then of k
+static long long token_blocks(long long n_tok, int D) {
+  const long long per = kThreads / (D <= 64 ? 8 : 16);
+  return (n_tok + per - 1) / per;
+}
+// into how many shares a token's batches go, so that there are about `want` CTAs or tasks
+static int shares_of(long long blocks, int batches, long long want) {
+  const long long s = (want + blocks - 1) / blocks;
+  return s < 1 ? 1 : s < batches ? (int)s : batches;
+}
+
+// backward: three CTAs on each SM, four tasks for each of them where there are so many
+constexpr int kBackwardCtas = 3 * kSms;
+static int backward_shares(long long n_tok, long long q_heads, long long k_heads, int D) {
+  return shares_of(token_blocks(n_tok, D), batches_of(q_heads, k_heads, kBackwardHeads), 4 * kBackwardCtas);
+}
 static unsigned backward_ctas(long long n_tok, long long q_heads, long long k_heads, int D) {
-  const long long per = kThreads / (D <= 64 ? 8 : 16), heads = q_heads > k_heads ? q_heads : k_heads;
-  const long long tasks = (n_tok + per - 1) / per * ((heads + kHeads - 1) / kHeads);
-  return (unsigned)(tasks < 4 * kSms ? tasks : 4 * kSms);
+  const long long tasks = token_blocks(n_tok, D) * backward_shares(n_tok, q_heads, k_heads, D);
+  return (unsigned)(tasks < kBackwardCtas ? tasks : kBackwardCtas);
 }
 
 static bool wide(const Args& a, int size, bool backward) {
@@ -299,7 +385,7 @@ static bool wide(const Args& a, int size, bool backward) {
   const int unit = 16 / size;      // elements of 16 bytes
   for (const Side& s : a.side) {
     if (s.heads == 0) continue;
-    if (off(s.x) || off(s.out) || s.row % unit || s.head % unit) return false;
+    if (off(s.x) || off(s.out) || off(s.w) || s.row % unit || s.head % unit) return false;
     if (backward && (off(s.g) || s.g_row % unit || s.g_head % unit)) return false;
   }
   return true;
@@ -308,12 +394,12 @@ static bool wide(const Args& a, int size, bool backward) {
 template <typename T>
 static cudaError_t launch_forward(const Args& a, cudaStream_t s) {
   const int G = a.D <= 64 ? 8 : 16;
-  const long long heads = (a.side[0].heads + kHeads - 1) / kHeads + (a.side[1].heads + kHeads - 1) / kHeads;
-  const long long ctas = (a.n_tok + kThreads / G - 1) / (kThreads / G) * heads;
-  if (ctas > 0x7fffffffLL) return cudaErrorInvalidValue;
+  const long long blocks = token_blocks(a.n_tok, a.D);
+  const int shares = shares_of(blocks, batches_of(a.side[0].heads, a.side[1].heads, kForwardHeads), 8 * kSms);
+  if (blocks * shares > 0x7fffffffLL) return cudaErrorInvalidValue;
   const bool w = wide(a, sizeof(T), false);
   auto kern = G == 8 ? (w ? forward_kernel<T, 8, true> : forward_kernel<T, 8, false>) : (w ? forward_kernel<T, 16, true> : forward_kernel<T, 16, false>);
-  return tc::launch_pdl(kern, (unsigned)ctas, kThreads, 0, s, a);
+  return tc::launch_pdl(kern, (unsigned)(blocks * shares), kThreads, 0, s, a, shares);
 }
 
 template <typename T>
@@ -323,7 +409,8 @@ static cudaError_t launch_backward(const Args& a, void* const (&gw)[2], float* p
   auto kern = a.D <= 64 ? (w ? backward_kernel<T, 8, true> : backward_kernel<T, 8, false>) : (w ? backward_kernel<T, 16, true> : backward_kernel<T, 16, false>);
   const bool any = gw[0] != nullptr || gw[1] != nullptr;
   *launches = 1;
-  cudaError_t e = tc::launch_pdl(kern, ctas, kThreads, 0, s, a, any ? partial : nullptr);
+  cudaError_t e = tc::launch_pdl(kern, ctas, kThreads, 0, s, a, backward_shares(a.n_tok, a.side[0].heads, a.side[1].heads, a.D),
+                                 any ? partial : nullptr);
   if (e != cudaSuccess || !any) return e;
   *launches = 2;
   cudaLaunchAttribute attr;
