@@ -33,11 +33,10 @@ constexpr long long kPieceBytes = 256ll << 20;
 struct BackwardPlan {
   bool tc;
   int cols, pieces;               // columns of a piece (the last may have fewer)
-  int dx_splits, dw_splits;       // most shares of k of any piece
-  size_t coef, scale, G, x, acc_dx, acc_dw, total;      // offsets in bytes
+  int dx_splits;                  // CUDA cores: most shares of k of any piece
+  size_t coef, scale, G, x, acc_dx, acc_dw, parts, total;      // offsets in bytes
 };
 
-int shares(bool tc, long long rows, long long cols, long long k) { return tc ? tc_splits(rows, cols, k) : simt_splits(rows, cols, k); }
 int piece_cols(const BackwardPlan& b, const attn_lce_shape_t* s, int i) { return i + 1 < b.pieces ? b.cols : s->V - (b.pieces - 1) * b.cols; }
 
 BackwardPlan plan_backward(const attn_lce_shape_t* s, bool dx, bool dw) {
@@ -51,13 +50,16 @@ BackwardPlan plan_backward(const attn_lce_shape_t* s, bool dx, bool dw) {
   pieces = (s->V + cols - 1) / cols;
   b.cols = (int)(cols < s->V ? cols : s->V);
   b.pieces = (int)pieces;
-  b.dx_splits = shares(b.tc, n, s->d, b.cols);      // the first piece's, the longest in k
-  b.dw_splits = 1;
-  size_t dw_floats = 0;
+  b.dx_splits = b.tc ? 1 : simt_splits(n, s->d, b.cols);      // the first piece's, the longest in k
+  size_t dw_floats = 0, parts = 0;
   for (int i = 0; i < b.pieces; i += b.pieces > 1 ? b.pieces - 1 : 1) {      // all but the last are alike
-    const int c = piece_cols(b, s, i), sp = shares(b.tc, c, s->d, n);
-    if (sp > b.dw_splits) b.dw_splits = sp;
-    if (sp > 1 && (size_t)sp * c * s->d > dw_floats) dw_floats = (size_t)sp * c * s->d;
+    const int c = piece_cols(b, s, i);
+    if (b.tc) {
+      for (const size_t bytes : {dx ? tc_parts_bytes(n, s->d, c) : 0, dw ? tc_parts_bytes(c, s->d, n) : 0}) parts = bytes > parts ? bytes : parts;
+    } else {
+      const int sp = simt_splits(c, s->d, n);
+      if (sp > 1 && (size_t)sp * c * s->d > dw_floats) dw_floats = (size_t)sp * c * s->d;
+    }
   }
   size_t at = 0;
   auto take = [&](size_t bytes) { const size_t here = at; at += up(bytes); return here; };
@@ -67,6 +69,7 @@ BackwardPlan plan_backward(const attn_lce_shape_t* s, bool dx, bool dw) {
   b.x = take(dw ? (size_t)n * s->d * size : 0);
   b.acc_dx = take(dx && (b.pieces > 1 || b.dx_splits > 1) ? (size_t)b.dx_splits * n * s->d * 4 : 0);
   b.acc_dw = take(dw ? dw_floats * 4 : 0);
+  b.parts = take(parts);
   b.total = at;
   return b;
 }
@@ -130,9 +133,14 @@ int attn_b200_linear_ce_forward(const attn_lce_shape_t* shape, const void* x, co
     const ForwardScratch f = plan_forward(shape);
     char* base = static_cast<char*>(scratch);
     const Scores sc{reinterpret_cast<Partial*>(base + f.partial), reinterpret_cast<float*>(base + f.logit), f.tiles};
-    e = on_tensor_cores(shape) ? tc_scores(p, sc, cs, &why) : simt_scores(p, sc, cs);
+    if (on_tensor_cores(shape)) {
+      e = tc_scores(p, sc, cs, &launches, &why);
+    } else {
+      e = simt_scores(p, sc, cs);
+      ++launches;
+    }
     if (e == cudaSuccess) e = launch_finish(p, sc, loss, lse, cs);
-    launches = 2;
+    ++launches;
   }
   if (e == cudaSuccess && shape->reduction != RED_NONE) {
     e = launch_total(p, loss, shape->reduction, value, counted, cs);
@@ -183,23 +191,24 @@ int attn_b200_linear_ce_backward(const attn_lce_shape_t* shape, const void* x, c
     piece.ld = (b.cols + 7) / 8 * 8;
     piece.is_first = i == 0;
     piece.is_last = i + 1 == b.pieces;
-    then([&] { return b.tc ? tc_piece_grad(p, piece, lse, c, G, cs, &why) : simt_piece_grad(p, piece, lse, c, (float*)G, cs); });
+    if (b.tc) {
+      float* const parts = reinterpret_cast<float*>(base + b.parts);
+      if (e == cudaSuccess) e = tc_piece_grad(p, piece, lse, c, G, cs, &launches, &why);
+      if (dw != nullptr && e == cudaSuccess) e = tc_piece_dw(p, piece, c, G, base + b.x, parts, dw, cs, &launches, &why);
+      if (dx != nullptr && e == cudaSuccess) e = tc_piece_dx(p, piece, c, G, parts, acc_dx, dx, cs, &launches, &why);
+      continue;
+    }
+    then([&] { return simt_piece_grad(p, piece, lse, c, (float*)G, cs); });
     if (dw != nullptr) {
-      const int sp = shares(b.tc, piece.cols, p.d, p.n);
-      void* const rows = static_cast<char*>(dw) + size * piece.first * p.d;
-      then([&] {
-        return b.tc ? tc_piece_dw(p, piece, c, G, base + b.x, sp, acc_dw, dw, cs, &why)
-                    : simt_piece_dw(p, piece, c, (const float*)G, base + b.x, sp, acc_dw, dw, cs);
-      });
-      if (sp > 1) then([&] { return launch_sum_splits(acc_dw, sp, (long long)piece.cols * p.d, c.scale, rows, p.dtype, cs); });
+      const int sp = simt_splits(piece.cols, p.d, p.n);
+      then([&] { return simt_piece_dw(p, piece, c, (const float*)G, base + b.x, sp, acc_dw, dw, cs); });
+      if (sp > 1)
+        then([&] { return launch_sum_splits(acc_dw, sp, (long long)piece.cols * p.d, c.scale, static_cast<char*>(dw) + size * piece.first * p.d, p.dtype, cs); });
     }
     if (dx != nullptr) {
-      int sp = shares(b.tc, p.n, p.d, piece.cols);
+      int sp = simt_splits(p.n, p.d, piece.cols);
       if (sp > b.dx_splits) sp = b.dx_splits;
-      then([&] {
-        return b.tc ? tc_piece_dx(p, piece, c, G, sp, b.dx_splits > 1, acc_dx, dx, cs, &why)
-                    : simt_piece_dx(p, piece, c, (const float*)G, sp, b.dx_splits > 1, acc_dx, dx, cs);
-      });
+      then([&] { return simt_piece_dx(p, piece, c, (const float*)G, sp, b.dx_splits > 1, acc_dx, dx, cs); });
     }
   }
   if (dx != nullptr && b.dx_splits > 1)

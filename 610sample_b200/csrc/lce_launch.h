@@ -48,18 +48,20 @@ struct Piece { int first, cols, ld; bool is_first, is_last; };
 // result = *scale x the sum of `splits` planes of `count` values, in order
 cudaError_t launch_sum_splits(const float* acc, int splits, long long count, const float* scale, void* result, int dtype, cudaStream_t stream);
 
-// dx: acc [splits][n, d] floats, where there are several pieces or splits; `keep` leaves the sum there after the last piece.  dW: acc [splits][piece, d], likewise.  x is launch_counted_rows' copy.
-
-// tensor cores: f16 / bf16, d a multiple of 8, 16-byte aligned tensors; G in the input type
+// tensor cores: f16 / bf16, d a multiple of 8, 16-byte aligned tensors; G in the input type.  acc [n, d] floats, where there are several
+// pieces; parts: tc_parts_bytes of a product's rows, columns and length in k.  x is launch_counted_rows' copy in dW.  `launches` is added to.
 int tc_tiles(int V);
-int tc_splits(long long rows, long long cols, long long k);
-cudaError_t tc_scores(const Problem& p, const Scores& s, cudaStream_t stream, const char** err);
-cudaError_t tc_piece_grad(const Problem& p, const Piece& piece, const float* lse, const Coefficients& c, void* G, cudaStream_t stream, const char** err);
-cudaError_t tc_piece_dx(const Problem& p, const Piece& piece, const Coefficients& c, const void* G, int splits, bool keep, float* acc, void* dx,
-                        cudaStream_t stream, const char** err);
-cudaError_t tc_piece_dw(const Problem& p, const Piece& piece, const Coefficients& c, const void* G, const void* x, int splits, float* acc,
-                        void* dw, cudaStream_t stream, const char** err);
+size_t tc_parts_bytes(long long rows, long long cols, long long k);
+cudaError_t tc_scores(const Problem& p, const Scores& s, cudaStream_t stream, int* launches, const char** err);
+cudaError_t tc_piece_grad(const Problem& p, const Piece& piece, const float* lse, const Coefficients& c, void* G, cudaStream_t stream, int* launches,
+                          const char** err);
+cudaError_t tc_piece_dx(const Problem& p, const Piece& piece, const Coefficients& c, const void* G, float* parts, float* acc, void* dx,
+                        cudaStream_t stream, int* launches, const char** err);
+cudaError_t tc_piece_dw(const Problem& p, const Piece& piece, const Coefficients& c, const void* G, const void* x, float* parts, void* dw,
+                        cudaStream_t stream, int* launches, const char** err);
 
+// dx: acc [splits][n, d] floats, where there are several pieces or splits; `keep` leaves the sum there after the last piece.
+// dW: acc [splits][piece, d], likewise.
 // CUDA cores: every type and size; G in float
 int simt_tiles(int V);
 int simt_splits(long long rows, long long cols, long long k);

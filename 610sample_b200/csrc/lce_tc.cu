@@ -8,10 +8,16 @@
 //
 // A pair of CTAs (a cluster) owns a tile of 256 rows x up to 256 columns: either holds 128 rows of A and half of B's columns, one
 // tcgen05.mma.cta_group::2 reads both.  A single CTA's 128 x 256 tile would stream 96 bytes per clock from L2 and read 96 more from
-// shared memory for the product, above either's rate; the pair needs 64 of each.  Tiles are dealt to the pairs in turn; a warp
+// shared memory for the product, above either's rate; the pair needs 64 of each.  A warp
 // loads through a ring of six stages of 64 in k, one (in rank 0) issues the products, eight finish a tile from tensor memory while
 // the next one accumulates in the other half of it.  The order of the tiles runs along the axis of the smaller operand first, so
 // that the larger one is read from HBM once and the smaller one stays in L2.
+//
+// DX and DW have few tiles with long sums: 96 of 256 blocks of k for 74 pairs, in the 16384 x 32000 case's dW, are two rounds, 65 % busy.  There the
+// tiles of the last round are each shared out along k among several pairs (plan_shares), and a small kernel behind adds the parts in
+// order (join_kernel).  Whole rounds stay as they are: pairs that are at the same place in k read the same rows of G and x from L2;
+// equal, contiguous shares of all blocks left no pair idle, but took dW's product from 178 to 168 us only, and dx's from 146 to 167 to
+// 187, since G then came from HBM several times.
 #include "lce_launch.h"
 #include "tc_common.cuh"
 
@@ -47,7 +53,6 @@ struct GemmMaps { CUtensorMap a, b, out; };
 
 struct GemmArgs {
   int m_tiles, n_tiles, k_blocks;
-  int splits, split_blocks;      // DX, DW: shares of the blocks in k, each with its own sum
   int tile_n;                    // columns of a tile, a multiple of 32
   int rows, cols;                // of the result
   int m_fast;                    // tiles in sequence along the rows
@@ -58,9 +63,11 @@ struct GemmArgs {
   float* target_logit;
   const float *lse, *coef;
   // DX, DW
-  float* acc;                    // [splits][rows, cols], where there are several pieces or splits
+  float* acc;                    // DX: [rows, cols], where there are several pieces
   int acc_in, acc_out;           // add it; leave the sum there instead of in the result
   const float* scale;
+  int full, rest, splits, split_blocks;      // tiles taken whole; the others, each in `splits` shares of `split_blocks` blocks of k
+  float* parts;                  // [rest x splits][2 CTAs][128][256], where there are several shares
   unsigned int* status;
 };
 
@@ -77,7 +84,6 @@ lce_gemm_kernel(const __grid_constant__ GemmMaps maps, const GemmArgs g) {
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const uint32_t rank = cluster_rank();
   const int pair = blockIdx.x >> 1, pairs = gridDim.x >> 1;
-  const int plane = g.m_tiles * g.n_tiles, tiles = plane * g.splits;
 
   auto bar_full = [&](int s) { return smem_u32(&ctl->full[s]); };
   auto bar_empty = [&](int s) { return smem_u32(&ctl->empty[s]); };
@@ -108,9 +114,20 @@ lce_gemm_kernel(const __grid_constant__ GemmMaps maps, const GemmArgs g) {
   pdl_wait();
   pdl_trigger();
 
-  auto tile_at = [&](int t, int& mt, int& nt, int& split) {
-    split = t / plane;
-    t -= split * plane;
+  // what the pairs work on in turn: the tiles taken whole, then the shares of the others, all first shares first
+  const int items = g.full + g.rest * g.splits;
+  auto item_at = [&](int i, int& t, int& first_block, int& blocks) {
+    t = i;
+    first_block = 0;
+    blocks = g.k_blocks;
+    if (kByColumns && i >= g.full) {
+      const int split = (i - g.full) / g.rest;
+      t = i - split * g.rest;
+      first_block = split * g.split_blocks;
+      blocks = min(g.split_blocks, g.k_blocks - first_block);
+    }
+  };
+  auto tile_at = [&](int t, int& mt, int& nt) {
     if (g.m_fast) { nt = t / g.m_tiles; mt = t - nt * g.m_tiles; }
     else { mt = t / g.n_tiles; nt = t - mt * g.n_tiles; }
   };
@@ -121,10 +138,10 @@ lce_gemm_kernel(const __grid_constant__ GemmMaps maps, const GemmArgs g) {
       const uint32_t stage_bytes = kOperandBytes + (kByColumns ? kOperandBytes : (uint32_t)half_n * 128u);
       bool ok = true;
       int it = 0;
-      for (int t = pair; t < tiles && ok; t += pairs) {
-        int mt, nt, split;
-        tile_at(t, mt, nt, split);
-        const int first_block = split * g.split_blocks, blocks = min(g.split_blocks, g.k_blocks - first_block);
+      for (int item = pair; item < items && ok; item += pairs) {
+        int t, mt, nt, first_block, blocks;
+        item_at(item, t, first_block, blocks);
+        tile_at(t, mt, nt);
         const int m0 = mt * kTileM + (int)rank * 128, n0 = nt * g.tile_n + (int)rank * half_n;
         for (int kb = 0; kb < blocks; ++kb, ++it) {
           const int s = it % kStages;
@@ -160,7 +177,9 @@ lce_gemm_kernel(const __grid_constant__ GemmMaps maps, const GemmArgs g) {
       const uint32_t idesc = make_idesc(kTileM, g.tile_n, Pack<T>::kIsBf16, USE == DW ? 1 : 0, kByColumns ? 1 : 0);
       bool ok = true;
       int it = 0, i = 0;
-      for (int t = pair; t < tiles && ok; t += pairs, ++i) {
+      for (int item = pair; item < items && ok; item += pairs, ++i) {
+        int t, first_block, blocks;
+        item_at(item, t, first_block, blocks);
         const int buf = i & 1;
         if (i >= 2) {
           ok = __all_sync(0xffffffffu, mbar_wait(bar_acc_empty(buf), ((i >> 1) & 1) ^ 1, abort_flag, g.status, wait_code(KCODE, 2)));
@@ -168,7 +187,6 @@ lce_gemm_kernel(const __grid_constant__ GemmMaps maps, const GemmArgs g) {
           tc_fence_after_sync();
         }
         const uint32_t acc = tmem_base + (uint32_t)buf * 256u;
-        const int first_block = t / plane * g.split_blocks, blocks = min(g.split_blocks, g.k_blocks - first_block);
         for (int kb = 0; kb < blocks; ++kb, ++it) {
           const int s = it % kStages;
           ok = __all_sync(0xffffffffu, mbar_wait(bar_full(s), (it / kStages) & 1, abort_flag, g.status, wait_code(KCODE, 3)));
@@ -197,9 +215,10 @@ lce_gemm_kernel(const __grid_constant__ GemmMaps maps, const GemmArgs g) {
     if constexpr (kByColumns) scale = from_l2(g.scale);
     bool ok = true;
     int i = 0;
-    for (int t = pair; t < tiles && ok; t += pairs, ++i) {
-      int mt, nt, split;
-      tile_at(t, mt, nt, split);
+    for (int item = pair; item < items && ok; item += pairs, ++i) {
+      int t, mt, nt, first_block, blocks;
+      item_at(item, t, first_block, blocks);
+      tile_at(t, mt, nt);
       const int buf = i & 1, r0 = mt * kTileM + (int)rank * 128, r = r0 + row;
       const int col0 = nt * g.tile_n + half * half_n;      // this half's first column
       const uint32_t acc = lane_addr + (uint32_t)buf * 256u + (uint32_t)(half * half_n);
@@ -259,7 +278,10 @@ lce_gemm_kernel(const __grid_constant__ GemmMaps maps, const GemmArgs g) {
           g.partial[(size_t)nt * g.rows + r] = Partial{m_all, l_all};
         }
       } else {
-        const bool to_acc = kByColumns && g.acc_out;
+        const bool to_acc = USE == DX && g.acc_out;
+        const bool part = kByColumns && item >= g.full && g.splits > 1;      // a share of a tile
+        float* part_row = nullptr;
+        if (part) part_row = g.parts + (((size_t)(item - g.full) * 2 + rank) * 128 + row) * 256 + half * 128;
 #pragma unroll 1
         for (int c = 0; c < 128; c += 64) {
           uint32_t v[4][16];
@@ -283,8 +305,12 @@ lce_gemm_kernel(const __grid_constant__ GemmMaps maps, const GemmArgs g) {
                 if (target == c + e) f[e] -= coef;
             }
           } else {
-            if ((g.acc_in || to_acc) && in) {
-              float4* at = reinterpret_cast<float4*>(g.acc + ((size_t)split * g.rows + r) * g.cols + col);
+            if (part) {
+              float4* at = reinterpret_cast<float4*>(part_row + c);
+#pragma unroll
+              for (int q = 0; q < 16; ++q) __stcg(at + q, make_float4(f[4 * q], f[4 * q + 1], f[4 * q + 2], f[4 * q + 3]));
+            } else if (USE == DX && (g.acc_in || to_acc) && in) {
+              float4* at = reinterpret_cast<float4*>(g.acc + (size_t)r * g.cols + col);
 #pragma unroll
               for (int q = 0; q < 16; ++q)
                 if (col + 4 * q < g.cols) {                // cols is a multiple of 8
@@ -298,7 +324,7 @@ lce_gemm_kernel(const __grid_constant__ GemmMaps maps, const GemmArgs g) {
 #pragma unroll
             for (int e = 0; e < 64; ++e) f[e] *= scale;
           }
-          if (!to_acc) {
+          if (!to_acc && !part) {
             // through shared memory; the store before must have read it
             if (quarter == 0 && lane == 0) bulk_wait_group_read_all();
             named_barrier_sync(3 + half, 128);
@@ -329,6 +355,37 @@ lce_gemm_kernel(const __grid_constant__ GemmMaps maps, const GemmArgs g) {
   }
 }
 
+// The tiles in several shares.  A CTA has eight rows of one CTA's half of a tile; the parts are read once.
+template <typename T>
+__global__ void __launch_bounds__(256)
+join_kernel(const GemmArgs g, T* out) {
+  pdl_wait();
+  pdl_trigger();
+  const int tile = (int)(blockIdx.x >> 5), t = g.full + tile, rank = (int)(blockIdx.x >> 4) & 1, row0 = (int)(blockIdx.x & 15) * 8;
+  int mt, nt;
+  if (g.m_fast) { nt = t / g.m_tiles; mt = t - nt * g.m_tiles; }
+  else { mt = t / g.n_tiles; nt = t - mt * g.n_tiles; }
+  const float scale = from_l2(g.scale);
+#pragma unroll
+  for (int i = threadIdx.x; i < 8 * 64; i += 256) {
+    const int row = row0 + (i >> 6), c = (i & 63) * 4, r = mt * kTileM + rank * 128 + row, col = nt * kTileN + c;
+    if (r >= g.rows || col >= g.cols) continue;
+    float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 4
+    for (int q = 0; q < g.splits; ++q) {
+      const float4 x = from_l2(reinterpret_cast<const float4*>(g.parts + (((size_t)(q * g.rest + tile) * 2 + rank) * 128 + row) * 256 + c));
+      v.x += x.x; v.y += x.y; v.z += x.z; v.w += x.w;
+    }
+    float4* acc = reinterpret_cast<float4*>(g.acc + (size_t)r * g.cols + col);
+    if (g.acc_in) {
+      const float4 x = from_l2(acc);
+      v.x += x.x; v.y += x.y; v.z += x.z; v.w += x.w;
+    }
+    if (g.acc_out) *acc = v;
+    else *reinterpret_cast<uint2*>(out + (size_t)r * g.cols + col) = make_uint2(Pack<T>::pack(v.x * scale, v.y * scale), Pack<T>::pack(v.z * scale, v.w * scale));
+  }
+}
+
 // ---- host ---------------------------------------------------------------------------------------
 typedef CUresult (*EncodeTiledFn)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*, const cuuint32_t*,
                                   const cuuint32_t*, CUtensorMapInterleave, CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
@@ -356,40 +413,63 @@ static bool encode(CUtensorMap* map, const void* p, bool bf16, long long rows, l
             CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
+static int blocks_of(long long k) { return (int)((k + kBlockK - 1) / kBlockK); }
+static long long tiles_of(long long rows, long long cols) { return (rows + kTileM - 1) / kTileM * ((cols + kTileN - 1) / kTileN); }
+
+// DX and DW: the tiles of the last, part-filled round in shares along k, where that is shorter.  In blocks of k (0.28 us): a round of the shares takes
+// split_blocks; shared tiles cost the launch behind them, 20, and a quarter of a block for every part that is written and read.  At least 8 blocks a share.
+struct SharePlan { int full, rest, splits, split_blocks; };
+static SharePlan plan_shares(long long rows, long long cols, long long k) {
+  const int pairs = kSms / 2, tiles = (int)tiles_of(rows, cols), blocks = blocks_of(k);
+  SharePlan best{tiles, 0, 1, blocks};
+  const int rest = tiles % pairs;
+  float least = (float)blocks;
+  for (int s = 2; rest > 0 && rest * s <= 2 * pairs && blocks / s >= 8; ++s) {
+    const int each = (blocks + s - 1) / s, shares = (blocks + each - 1) / each;      // none without blocks
+    const float cost = (float)each * ((rest * shares + pairs - 1) / pairs) + 20.f + 0.25f * rest * shares;
+    if (cost < least) {
+      least = cost;
+      best = SharePlan{tiles - rest, rest, shares, each};
+    }
+  }
+  return best;
+}
+size_t tc_parts_bytes(long long rows, long long cols, long long k) {
+  const SharePlan s = plan_shares(rows, cols, k);
+  return s.splits > 1 ? (size_t)s.rest * s.splits * kTileM * kTileN * sizeof(float) : 0;
+}
+
 template <int USE>
-static cudaError_t launch_use(const GemmMaps& maps, GemmArgs g, int dtype, long long k, cudaStream_t stream) {
+static cudaError_t launch_use(const GemmMaps& maps, GemmArgs g, int dtype, long long k, void* out, cudaStream_t stream, int* launches) {
   g.m_tiles = (g.rows + kTileM - 1) / kTileM;
   g.n_tiles = (g.cols + g.tile_n - 1) / g.tile_n;
-  g.k_blocks = (int)((k + kBlockK - 1) / kBlockK);
+  g.k_blocks = blocks_of(k);
   g.m_fast = g.rows < g.cols;      // A, of `rows` rows, is the smaller operand
-  if (g.splits < 1) g.splits = 1;
-  g.split_blocks = (g.k_blocks + g.splits - 1) / g.splits;
-  g.splits = (g.k_blocks + g.split_blocks - 1) / g.split_blocks;      // a share without blocks would never complete
-  const long long tiles = (long long)g.m_tiles * g.n_tiles * g.splits;
-  if (tiles > 0x7fffffffLL) return cudaErrorInvalidValue;
-  const int pairs = (int)(tiles < kSms / 2 ? tiles : kSms / 2);
+  const long long tiles = (long long)g.m_tiles * g.n_tiles;
+  if (tiles > 0x3fffffffLL) return cudaErrorInvalidValue;
+  SharePlan plan{(int)tiles, 0, 1, g.k_blocks};
+  if (USE == DX || USE == DW) plan = plan_shares(g.rows, g.cols, k);
+  g.full = plan.full; g.rest = plan.rest; g.splits = plan.splits; g.split_blocks = plan.split_blocks;
+  const int items = g.full + g.rest * g.splits, pairs = items < kSms / 2 ? items : kSms / 2;
   static std::atomic<unsigned long long> smem_set[2];
   auto kern = dtype == 1 ? lce_gemm_kernel<__nv_bfloat16, USE> : lce_gemm_kernel<__half, USE>;
-  const cudaError_t e = set_smem_once(kern, kSmemBytes, smem_set[dtype == 1]);
-  return e != cudaSuccess ? e : launch_pdl_cluster(kern, (unsigned)pairs * 2, kThreads, kSmemBytes, 2, stream, maps, g);
+  cudaError_t e = set_smem_once(kern, kSmemBytes, smem_set[dtype == 1]);
+  if (e == cudaSuccess) e = launch_pdl_cluster(kern, (unsigned)pairs * 2, kThreads, kSmemBytes, 2, stream, maps, g);
+  ++*launches;
+  if (g.splits > 1 && e == cudaSuccess) {
+    const unsigned ctas = (unsigned)g.rest * 32;
+    e = dtype == 1 ? launch_pdl(join_kernel<__nv_bfloat16>, ctas, 256u, 0, stream, g, (__nv_bfloat16*)out)
+                   : launch_pdl(join_kernel<__half>, ctas, 256u, 0, stream, g, (__half*)out);
+    ++*launches;
+  }
+  return e;
 }
 
 static const char* const kMapError = "cuTensorMapEncodeTiled refused a tensor";
 
 int tc_tiles(int V) { return (V + kTileN - 1) / kTileN; }
 
-// Where the tiles are too few for the pairs, k is shared out, down to 16 blocks (1024 in k) a share, and the shares' sums are added
-// by a kernel of their own.  No share is without blocks.
-int tc_splits(long long rows, long long cols, long long k) {
-  const long long tiles = ((rows + kTileM - 1) / kTileM) * ((cols + kTileN - 1) / kTileN), blocks = (k + kBlockK - 1) / kBlockK;
-  long long s = (kSms / 2) / tiles;
-  if (s > blocks / 16) s = blocks / 16;
-  if (s < 2) return 1;
-  const long long each = (blocks + s - 1) / s;
-  return (int)((blocks + each - 1) / each);
-}
-
-cudaError_t tc_scores(const Problem& p, const Scores& s, cudaStream_t stream, const char** err) {
+cudaError_t tc_scores(const Problem& p, const Scores& s, cudaStream_t stream, int* launches, const char** err) {
   GemmMaps maps;
   GemmArgs g = {};
   const bool bf = p.dtype == 1;
@@ -404,10 +484,11 @@ cudaError_t tc_scores(const Problem& p, const Scores& s, cudaStream_t stream, co
   g.partial = s.partial;
   g.target_logit = s.target_logit;
   g.status = p.status;
-  return launch_use<LSE>(maps, g, p.dtype, p.d, stream);
+  return launch_use<LSE>(maps, g, p.dtype, p.d, nullptr, stream, launches);
 }
 
-cudaError_t tc_piece_grad(const Problem& p, const Piece& piece, const float* lse, const Coefficients& c, void* G, cudaStream_t stream, const char** err) {
+cudaError_t tc_piece_grad(const Problem& p, const Piece& piece, const float* lse, const Coefficients& c, void* G, cudaStream_t stream, int* launches,
+                          const char** err) {
   GemmMaps maps;
   GemmArgs g = {};
   const bool bf = p.dtype == 1;
@@ -424,11 +505,11 @@ cudaError_t tc_piece_grad(const Problem& p, const Piece& piece, const float* lse
   g.lse = lse;
   g.coef = c.coef;
   g.status = p.status;
-  return launch_use<GRAD>(maps, g, p.dtype, p.d, stream);
+  return launch_use<GRAD>(maps, g, p.dtype, p.d, nullptr, stream, launches);
 }
 
-cudaError_t tc_piece_dx(const Problem& p, const Piece& piece, const Coefficients& c, const void* G, int splits, bool keep, float* acc, void* dx,
-                        cudaStream_t stream, const char** err) {
+cudaError_t tc_piece_dx(const Problem& p, const Piece& piece, const Coefficients& c, const void* G, float* parts, float* acc, void* dx,
+                        cudaStream_t stream, int* launches, const char** err) {
   GemmMaps maps;
   GemmArgs g = {};
   const bool bf = p.dtype == 1;
@@ -440,17 +521,17 @@ cudaError_t tc_piece_dx(const Problem& p, const Piece& piece, const Coefficients
     return cudaErrorInvalidValue;
   }
   g.rows = p.n; g.cols = p.d;
-  g.splits = splits;
+  g.parts = parts;
   g.acc = acc;
   g.acc_in = !piece.is_first;
-  g.acc_out = !piece.is_last || keep;
+  g.acc_out = !piece.is_last;
   g.scale = c.scale;
   g.status = p.status;
-  return launch_use<DX>(maps, g, p.dtype, piece.cols, stream);
+  return launch_use<DX>(maps, g, p.dtype, piece.cols, dx, stream, launches);
 }
 
-cudaError_t tc_piece_dw(const Problem& p, const Piece& piece, const Coefficients& c, const void* G, const void* x, int splits, float* acc,
-                        void* dw, cudaStream_t stream, const char** err) {
+cudaError_t tc_piece_dw(const Problem& p, const Piece& piece, const Coefficients& c, const void* G, const void* x, float* parts, void* dw,
+                        cudaStream_t stream, int* launches, const char** err) {
   GemmMaps maps;
   GemmArgs g = {};
   const bool bf = p.dtype == 1;
@@ -462,12 +543,10 @@ cudaError_t tc_piece_dw(const Problem& p, const Piece& piece, const Coefficients
     return cudaErrorInvalidValue;
   }
   g.rows = piece.cols; g.cols = p.d;
-  g.splits = splits;
-  g.acc = acc;
-  g.acc_out = splits > 1;
+  g.parts = parts;
   g.scale = c.scale;
   g.status = p.status;
-  return launch_use<DW>(maps, g, p.dtype, p.n, stream);
+  return launch_use<DW>(maps, g, p.dtype, p.n, out, stream, launches);
 }
 
 }  // namespace lce

@@ -72,7 +72,7 @@ def test_scratch_does_not_grow_with_the_logits(capi):
     size = lambda n, d, V, dx=1, dw=1, dtype=capi.ATTN_BF16: capi.lib().attn_b200_linear_ce_backward_scratch_bytes(
         ctypes.byref(_shape(capi, n=n, d=d, V=V, dtype=dtype)), dx, dw)
     n, d, V = 16384, 768, 128 * 1024
-    assert size(n, d, V) <= (256 << 20) + 4 * n * d + 2 * n * d + 4 * n + 4096 < 2 * n * V
+    assert size(n, d, V) <= (256 << 20) + 4 * n * d + 2 * n * d + 4 * n + (37 << 20) + 4096 < 2 * n * V
     assert size(n, d, V, 1, 0) < size(n, d, V) and size(n, d, V, 0, 1) < size(n, d, V)
     assert size(1, 8, 2) >= 4 + 4 + 16 + 16
     assert capi.lib().attn_b200_linear_ce_forward_scratch_bytes(ctypes.byref(_shape(capi, n=n, d=d, V=V))) <= 8 * n * (V // 256) + 4 * n + 512
@@ -195,6 +195,13 @@ def test_peaked_rows(lce, dtype):
 def test_pieces_and_shares_of_k(lce, n, d, V):
     # several pieces of the vocabulary; one row block against a long vocabulary; a long sum over rows for few classes
     check(lce, n, d, V, torch.bfloat16)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("n, d, V", [(5000, 768, 3001), (700, 1000, 20000), (2000, 264, 8192), (9000, 512, 700), (300, 2048, 30000), (16500, 64, 8200)])
+def test_tiles_in_several_shares(lce, dtype, n, d, V):
+    check(lce, n, d, V, dtype, "none")
 
 
 @pytest.mark.gpu
