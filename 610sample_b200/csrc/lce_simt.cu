@@ -1,7 +1,8 @@
 // The matrix products of the linear cross entropy on the CUDA cores, for float32 and for what the tensor-core kernel does not take
 // (widths that are no multiple of 8).  The same four uses as there (lce_tc.cu); G is kept in float.  All arithmetic is in fp32.
-// A CTA of 256 threads computes 128 x 128 results, 8 x 8 a thread, over blocks of 8 in k that go through shared memory, the next one
-// on its way into registers meanwhile.  Bound by the FMA pipe.
+// A CTA of 256 threads computes 128 x 128 results, 8 x 8 a thread, over blocks of 16 in k that go through shared memory, the next one
+// on its way into registers meanwhile.  A thread brings eight elements of either operand, along whichever axis is dense, with 16-byte loads
+// where that axis' extent and the addresses allow it.  Bound by the FMA pipe.
 #include "attn_common.cuh"
 #include "lce_launch.h"
 #include "tc_common.cuh"
@@ -12,10 +13,10 @@ namespace lce {
 using tc::from_l2;
 
 enum Use { LSE = 0, GRAD = 1, DX = 2, DW = 3 };
-constexpr int kTile = 128, kBlock = 8, kPitch = kTile + 4;
+constexpr int kTile = 128, kBlock = 16, kPitch = kTile + 4;
 
 // element (i, k) of an operand at p[i * si + k * sk]; one of the strides is 1
-template <typename T> struct Operand { const T* p; long long si, sk; };
+template <typename T> struct Operand { const T* p; long long si, sk; int wide; };      // wide: runs of eight are 16-byte aligned
 
 struct SimtArgs {
   int rows, cols, k;
@@ -33,22 +34,41 @@ struct SimtArgs {
   const float* scale;
 };
 
-// the four elements of a [128][8] block that this thread brings: along k, or along i where that is the dense axis
+// The eight elements of a [128][16] block that this thread brings: along k of row t / 2, or along i at k = t / 16.
 template <typename T>
-__device__ __forceinline__ void fetch(const Operand<T>& o, int i0, int k0, int n_i, int n_k, float (&v)[4], bool k_dense) {
-  const int t = threadIdx.x;
+__device__ __forceinline__ void fetch(const Operand<T>& o, int i0, int k0, int n_i, int n_k, float (&v)[8], bool k_dense) {
+  const int t = threadIdx.x, i = i0 + (k_dense ? t >> 1 : (t & 15) * 8), k = k0 + (k_dense ? (t & 1) * 8 : t >> 4);
+  const T* p = o.p + i * o.si + k * o.sk;
+  if (o.wide && (k_dense ? i < n_i && k + 8 <= n_k : k < n_k && i + 8 <= n_i)) {
+    if constexpr (sizeof(T) == 4) {
+      const float4 a = from_l2(reinterpret_cast<const float4*>(p)), b = from_l2(reinterpret_cast<const float4*>(p) + 1);
+      v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w; v[4] = b.x; v[5] = b.y; v[6] = b.z; v[7] = b.w;
+    } else {
+      const uint4 q = from_l2(reinterpret_cast<const uint4*>(p));
+      const uint32_t w[4] = {q.x, q.y, q.z, q.w};
 #pragma unroll
-  for (int e = 0; e < 4; ++e) {
-    const int i = i0 + (k_dense ? t >> 1 : (t & 31) * 4 + e), k = k0 + (k_dense ? (t & 1) * 4 + e : t >> 5);
-    v[e] = i < n_i && k < n_k ? Elem<T>::to_float(o.p[i * o.si + k * o.sk]) : 0.f;
+      for (int e = 0; e < 4; ++e) {
+        const float2 f = tc::Pack<T>::unpack(w[e]);
+        v[2 * e] = f.x; v[2 * e + 1] = f.y;
+      }
+    }
+    return;
+  }
+#pragma unroll
+  for (int e = 0; e < 8; ++e) {
+    const bool in = k_dense ? i < n_i && k + e < n_k : k < n_k && i + e < n_i;
+    v[e] = in ? Elem<T>::to_float(p[e]) : 0.f;
   }
 }
-__device__ __forceinline__ void put(float* s, const float (&v)[4], bool k_dense) {
+__device__ __forceinline__ void put(float* s, const float (&v)[8], bool k_dense) {
   const int t = threadIdx.x;
+  if (k_dense) {
 #pragma unroll
-  for (int e = 0; e < 4; ++e) {
-    const int i = k_dense ? t >> 1 : (t & 31) * 4 + e, k = k_dense ? (t & 1) * 4 + e : t >> 5;
-    s[k * kPitch + i] = v[e];
+    for (int e = 0; e < 8; ++e) s[((t & 1) * 8 + e) * kPitch + (t >> 1)] = v[e];
+  } else {
+    float4* at = reinterpret_cast<float4*>(s + (t >> 4) * kPitch + (t & 15) * 8);
+    at[0] = make_float4(v[0], v[1], v[2], v[3]);
+    at[1] = make_float4(v[4], v[5], v[6], v[7]);
   }
 }
 
@@ -62,8 +82,12 @@ lce_simt_kernel(const Operand<TA> A, const Operand<TB> B, const SimtArgs g, T* o
   const int k_begin = split * g.split_k, k_end = min(g.k, k_begin + g.split_k);
   const int ty = threadIdx.x >> 4, tx = threadIdx.x & 15;      // rows ty * 8 + i, columns tx * 4 + j and 64 + tx * 4 + j
   const bool ka = A.sk == 1, kb = B.sk == 1;
-  float acc[8][8] = {};
-  float va[4], vb[4];
+  float2 sum[8][4];
+#pragma unroll
+  for (int i = 0; i < 8; ++i)
+#pragma unroll
+    for (int j = 0; j < 4; ++j) sum[i][j] = make_float2(0.f, 0.f);
+  float va[8], vb[8];
   fetch(A, r0, k_begin, g.rows, k_end, va, ka);
   fetch(B, c0, k_begin, g.cols, k_end, vb, kb);
   int buf = 0;
@@ -77,17 +101,22 @@ lce_simt_kernel(const Operand<TA> A, const Operand<TB> B, const SimtArgs g, T* o
     }
 #pragma unroll
     for (int k = 0; k < kBlock; ++k) {
-      float a[8], b[8];
+      float a[8];
       *reinterpret_cast<float4*>(a) = *reinterpret_cast<const float4*>(&as[buf][k * kPitch + ty * 8]);
       *reinterpret_cast<float4*>(a + 4) = *reinterpret_cast<const float4*>(&as[buf][k * kPitch + ty * 8 + 4]);
-      *reinterpret_cast<float4*>(b) = *reinterpret_cast<const float4*>(&bs[buf][k * kPitch + tx * 4]);
-      *reinterpret_cast<float4*>(b + 4) = *reinterpret_cast<const float4*>(&bs[buf][k * kPitch + 64 + tx * 4]);
+      const float4 b0 = *reinterpret_cast<const float4*>(&bs[buf][k * kPitch + tx * 4]), b1 = *reinterpret_cast<const float4*>(&bs[buf][k * kPitch + 64 + tx * 4]);
+      const float2 b[4] = {make_float2(b0.x, b0.y), make_float2(b0.z, b0.w), make_float2(b1.x, b1.y), make_float2(b1.z, b1.w)};
 #pragma unroll
       for (int i = 0; i < 8; ++i)
 #pragma unroll
-        for (int j = 0; j < 8; ++j) acc[i][j] = fmaf(a[i], b[j], acc[i][j]);
+        for (int j = 0; j < 4; ++j) sum[i][j] = __ffma2_rn(make_float2(a[i], a[i]), b[j], sum[i][j]);
     }
   }
+  float acc[8][8];
+#pragma unroll
+  for (int i = 0; i < 8; ++i)
+#pragma unroll
+    for (int j = 0; j < 4; ++j) { acc[i][2 * j] = sum[i][j].x; acc[i][2 * j + 1] = sum[i][j].y; }
   auto col_of = [&](int j) { return c0 + (j >> 2) * 64 + tx * 4 + (j & 3); };
 #pragma unroll
   for (int i = 0; i < 8; ++i) {
@@ -136,12 +165,15 @@ lce_simt_kernel(const Operand<TA> A, const Operand<TB> B, const SimtArgs g, T* o
   }
 }
 
+// a share of k: whole blocks, so that runs of eight that are aligned in the first share are so in every one
+static long long share_of(long long k, long long splits) { return ((k + splits - 1) / splits + kBlock - 1) / kBlock * kBlock; }
+
 template <int USE, typename TA, typename TB, typename T>
 static cudaError_t launch_use(const Operand<TA>& A, const Operand<TB>& B, SimtArgs g, T* out, cudaStream_t stream) {
   g.tiles_m = (g.rows + kTile - 1) / kTile;
   const long long tiles = g.tiles_m * ((g.cols + kTile - 1) / kTile);
   if (g.splits < 1) g.splits = 1;
-  g.split_k = (g.k + g.splits - 1) / g.splits;
+  g.split_k = (int)share_of(g.k, g.splits);
   if (tiles > 0x7fffffffLL || g.splits > 65535) return cudaErrorInvalidValue;
   cudaLaunchAttribute attr;
   attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
@@ -164,12 +196,13 @@ int simt_splits(long long rows, long long cols, long long k) {
   if (s > k / 64) s = k / 64;
   if (s > 256) s = 256;
   if (s < 2) return 1;
-  const long long each = (k + s - 1) / s;
+  const long long each = share_of(k, s);
   return (int)((k + each - 1) / each);
 }
 
-template <typename T> static Operand<T> rows_of(const void* p, long long ld) { return {static_cast<const T*>(p), ld, 1}; }
-template <typename T> static Operand<T> columns_of(const void* p, long long ld) { return {static_cast<const T*>(p), 1, ld}; }
+static int wide(const void* p, long long ld, int size) { return reinterpret_cast<uintptr_t>(p) % 16 == 0 && ld * size % 16 == 0; }
+template <typename T> static Operand<T> rows_of(const void* p, long long ld) { return {static_cast<const T*>(p), ld, 1, wide(p, ld, sizeof(T))}; }
+template <typename T> static Operand<T> columns_of(const void* p, long long ld) { return {static_cast<const T*>(p), 1, ld, wide(p, ld, sizeof(T))}; }
 
 template <typename T>
 static cudaError_t scores(const Problem& p, const Scores& s, cudaStream_t stream) {

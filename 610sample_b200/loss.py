@@ -4,7 +4,7 @@
 
 computes `F.cross_entropy(F.linear(x, weight).float(), targets)`, but the [n, V] logits exist only tile by tile: the
 forward reduces each tile to a maximum and a sum per row, the backward forms the gradient of a piece of the
-vocabulary at a time, in at most 256 MB, whatever n and V are.  Logits are summed and used in float32, never
+vocabulary at a time, in at most 512 MB (or 1024 columns), whatever V is.  Logits are summed and used in float32, never
 rounded to the input type.  The reference takes the loss of whole logits (e2e/ttt_pytorch/model.py:540-671).
 There is no fallback: importing this module fails if the compiled extension `attention_cuda` is missing.
 """

@@ -1,7 +1,7 @@
 #!/usr/bin/env python
 """End-to-end test-time-training (TTT) step benchmark: the caller of the attention path.
 
-    python bench_ttt.py [--gpus N] [--steps K] [--warmup W] [--impl ours|reference] [--small]
+    python bench_ttt.py [--gpus N] [--steps K] [--warmup W] [--impl ours|reference] [--small] [--loss logits|linear]
 
 Workload: a random-init 12-layer pre-norm decoder, d_model 768,
 12 heads (D = 64), GELU MLP 3072, vocabulary 32000, sequence 2048, batch 8 per GPU, bf16,
@@ -16,7 +16,8 @@ The pattern (functional forward with a parameter dict, `autograd.grad(..., creat
 (`e2e/ttt_pytorch/model.py:540-671`); the model itself is the plain decoder BASELINE names,
 not the reference's SwiGLU/RoPE model.  Attention goes through `flash_attention_v7`
 (`--impl ours`) or through the reference's math attention (`--impl reference`, on the CPU,
-on a reduced sample that is stated in the output).
+on a reduced sample that is stated in the output).  `--loss linear` takes the loss through
+`linear_cross_entropy`, which does not keep the logits; the default keeps them, as the reference does.
 
 Prints one JSON line: metric `ttt_tokens_per_s`.
 """
@@ -63,7 +64,7 @@ def init_params(cfg, device, dtype, seed=0):
     return slow, fast
 
 
-def forward_loss(cfg, slow, fast, ids, targets, attention):
+def forward_loss(cfg, slow, fast, ids, targets, attention, linear_loss=None):
     """Mean cross entropy of the decoder with the given fast weights."""
     import torch
     import torch.nn.functional as F
@@ -83,18 +84,20 @@ def forward_loss(cfg, slow, fast, ids, targets, attention):
         h = F.layer_norm(x, (d,), fast[p + "ln2.w"], fast[p + "ln2.b"])
         x = x + F.linear(F.gelu(F.linear(h, fast[p + "fc1"])), fast[p + "fc2"])
     x = F.layer_norm(x, (d,), slow["ln_f.w"], slow["ln_f.b"])
+    if linear_loss is not None:
+        return linear_loss(x, slow["head"], targets)
     logits = F.linear(x, slow["head"])
     return F.cross_entropy(logits.float().view(B * N, -1), targets.reshape(B * N))
 
 
-def ttt_step(cfg, slow, fast, ids, targets, attention):
+def ttt_step(cfg, slow, fast, ids, targets, attention, linear_loss=None):
     """One meta step; returns the outer loss (call .backward() on it)."""
     import torch
     names = list(fast.keys())
-    inner = forward_loss(cfg, slow, fast, ids, targets, attention)
+    inner = forward_loss(cfg, slow, fast, ids, targets, attention, linear_loss)
     grads = torch.autograd.grad(inner, [fast[n] for n in names], create_graph=True)
     updated = {n: fast[n] - INNER_LR * g for n, g in zip(names, grads)}
-    return forward_loss(cfg, slow, updated, ids, targets, attention)
+    return forward_loss(cfg, slow, updated, ids, targets, attention, linear_loss)
 
 
 def make_batch(cfg, device, seed):
@@ -164,7 +167,10 @@ def measure(args, init_process_group=True):
     local = int(os.environ.get("LOCAL_RANK", "0"))
     cfg = dict(SMALL if args.small else FULL)
     reference = args.impl == "reference"
-    sample = None
+    linear = getattr(args, "loss", "logits") == "linear"
+    linear_loss = sample = None
+    if linear and reference:
+        raise SystemExit("--loss linear needs the kernels: it goes with --impl ours")
     if reference:
         # CPU arm: the reference's math attention; a reduced sample of the workload, stated below
         if rank != 0:
@@ -188,6 +194,8 @@ def measure(args, init_process_group=True):
         sys.path.insert(0, os.path.join(ROOT, "610sample_b200"))
         import attention_cuda
         from attention import FlashAttentionV7, flash_attention_v7
+        if linear:
+            from loss import linear_cross_entropy as linear_loss
         timer = AttentionTimer(attention_cuda)
         dtype = torch.bfloat16
         N = cfg["seq"]
@@ -202,7 +210,7 @@ def measure(args, init_process_group=True):
     def step():
         for p in params:
             p.grad = None
-        loss = ttt_step(cfg, slow, fast, ids, targets, attention)
+        loss = ttt_step(cfg, slow, fast, ids, targets, attention, linear_loss)
         loss.backward()
         if world > 1:
             flat = torch.cat([p.grad.reshape(-1) for p in params])
@@ -254,7 +262,7 @@ def measure(args, init_process_group=True):
             "impl": args.impl,
             "config": {"workload": "ttt_step_12L_d768_h12_seq2048_b8" if not args.small else "ttt_step_small",
                        **{k: cfg[k] for k in ("layers", "d_model", "heads", "d_ff", "vocab", "seq", "batch")},
-                       "inner_lr": INNER_LR, "sample": sample},
+                       "inner_lr": INNER_LR, "sample": sample, **({"loss": "linear"} if linear else {})},
             "outer_loss": float(loss.detach()), "peak_memory_mb": peak_mb,
         }
         if attn_ms is not None:
@@ -282,6 +290,7 @@ def main():
     ap.add_argument("--warmup", type=int, default=2)
     ap.add_argument("--impl", default="ours", choices=["ours", "reference"])
     ap.add_argument("--small", action="store_true", help="2-layer toy configuration (tests)")
+    ap.add_argument("--loss", default="logits", choices=["logits", "linear"], help="cross entropy of kept logits, or linear_cross_entropy")
     run(ap.parse_args())
 
 

@@ -237,7 +237,7 @@ int attn_b200_packed_qk_norm_rope_backward(const attn_rope_shape_t* shape, const
 
 /* ---- Cross entropy of a linear layer --------------------------------------------------------------
  * z = x W^T, loss_i = log sum_j exp(z_ij) - z_i,targets[i], without z being kept: the forward reduces it tile by tile, the
- * backward forms its gradient for a piece of the vocabulary at a time (at most 256 MB, or 1024 columns).  x: [n, d], w: [V, d]
+ * backward forms its gradient for a piece of the vocabulary at a time (at most 512 MB, or 1024 columns).  x: [n, d], w: [V, d]
  * dense, of one type, 16-byte aligned; f16 / bf16 with d a multiple of 8 run on the tensor cores, all else on the CUDA cores in
  * fp32.  A row whose target is ignore_index has loss 0 and gradients 0 and does not count in the mean, whatever x holds there; a
  * target outside [0, V) otherwise gives NaN.  The reference takes the loss of whole logits

@@ -72,7 +72,7 @@ def test_scratch_does_not_grow_with_the_logits(capi):
     size = lambda n, d, V, dx=1, dw=1, dtype=capi.ATTN_BF16: capi.lib().attn_b200_linear_ce_backward_scratch_bytes(
         ctypes.byref(_shape(capi, n=n, d=d, V=V, dtype=dtype)), dx, dw)
     n, d, V = 16384, 768, 128 * 1024
-    assert size(n, d, V) <= (256 << 20) + 4 * n * d + 2 * n * d + 4 * n + (37 << 20) + 4096 < 2 * n * V
+    assert size(n, d, V) <= (512 << 20) + 4 * n * d + 2 * n * d + 4 * n + (37 << 20) + 4096 < 2 * n * V
     assert size(n, d, V, 1, 0) < size(n, d, V) and size(n, d, V, 0, 1) < size(n, d, V)
     assert size(1, 8, 2) >= 4 + 4 + 16 + 16
     assert capi.lib().attn_b200_linear_ce_forward_scratch_bytes(ctypes.byref(_shape(capi, n=n, d=d, V=V))) <= 8 * n * (V // 256) + 4 * n + 512
@@ -191,7 +191,7 @@ def test_peaked_rows(lce, dtype):
 
 
 @pytest.mark.gpu
-@pytest.mark.parametrize("n, d, V", [(33000, 64, 9000), (3000, 128, 100003), (8, 64, 100003), (20000, 8, 3)])
+@pytest.mark.parametrize("n, d, V", [(33000, 64, 17000), (3000, 128, 100003), (8, 64, 100003), (20000, 8, 3)])
 def test_pieces_and_shares_of_k(lce, n, d, V):
     # several pieces of the vocabulary; one row block against a long vocabulary; a long sum over rows for few classes
     check(lce, n, d, V, torch.bfloat16)
@@ -206,7 +206,7 @@ def test_tiles_in_several_shares(lce, dtype, n, d, V):
 
 @pytest.mark.gpu
 def test_pieces_on_cuda_cores(lce):
-    check(lce, 33000, 16, 5000, torch.float32)
+    check(lce, 33000, 16, 9000, torch.float32)
 
 
 @pytest.mark.gpu
@@ -357,3 +357,24 @@ def test_gradient_against_differences(lce):
         up, down = (lce(*moved(s * h), y, reduction="none").double().sum() for s in (1, -1))
         want = float((grad.double() * direction.double()).sum())
         assert abs(float(up - down) / (2 * h) - want) <= 5e-3 * float(grad.double().norm() * direction.double().norm()) / math.sqrt(direction.numel()) * 3
+
+
+@pytest.mark.gpu
+def test_meta_step_of_the_benchmark(lce):
+    # the whole second-order step with this loss against the one that keeps its logits, as that one's test compares two attentions
+    root = os.path.dirname(PKG_DIR)
+    if root not in sys.path:
+        sys.path.insert(0, root)
+    bt = importlib.import_module("bench_ttt")
+    cfg, dev = dict(bt.SMALL), torch.device("cuda")
+    attention = importlib.import_module("attention").flash_attention_v7
+    grads = []
+    for loss in (None, lce):
+        slow, fast = bt.init_params(cfg, dev, torch.bfloat16, seed=1)
+        ids, targets = bt.make_batch(cfg, dev, seed=2)
+        out = bt.ttt_step(cfg, slow, fast, ids, targets, lambda q, k, v: attention(q, k, v, cfg["seq"], 0), loss)
+        out.backward()
+        grads.append((float(out.detach()), {n: p.grad.float() for n, p in {**slow, **fast}.items()}))
+    assert abs(grads[0][0] - grads[1][0]) < 0.02
+    for n, g in grads[0][1].items():
+        assert torch.allclose(grads[1][1][n], g, atol=5e-2 * max(1.0, float(g.abs().max())), rtol=5e-2), n
