@@ -326,6 +326,7 @@ cudaError_t launch_tc(int op, int dtype, const Geometry& g, const Tensors& t, cu
 namespace tc {
 
 cudaError_t launch_packed_fwd(int is_bf16, const TmaMaps& maps, const PackedGeometry& g, const Tensors& t, cudaStream_t s);
+cudaError_t launch_packed_fwd_pairs(int is_bf16, const TmaMaps& maps, const PackedGeometry& g, const Tensors& t, cudaStream_t s);
 cudaError_t launch_packed_bwd(int is_bf16, const TmaMaps& maps, const PackedGeometry& g, const Tensors& t, cudaStream_t s, int* launches);
 
 // D_i of a packed batch: dO [n_tok, heads, D] in strides, O dense, out [heads, n_tok].  Eight or sixteen lanes own a row,
@@ -367,6 +368,16 @@ static cudaError_t launch_packed_rowdot(const Tensors& t, const PackedGeometry& 
 
 }  // namespace tc
 
+// Forward: pairs of query tiles (packed_fwd.cu) or single ones, two CTAs to an SM (attn_tc_fwd.cu).  A pair's CTA is faster in its stride and costs more
+// besides, so it is for long sequences, of which the host knows the mean length, and for a full set of CTAs.  Pairs / single tiles, in us:
+// 12 heads of 64, 16384 rows in 1, 2, 4, 8, 16, 24, 40 sequences 484 / 552, 321 / 360, 182 / 192, 125 / 129, 139 / 142, 99 / 97, 92 / 86; 4096 rows in 1, 2, 4
+// 51 / 51, 40 / 47, 30 / 29; 2048 rows in one (108 CTAs) 28 / 17.  16 and 4 heads of 128, 16384 rows in 1, 2, 4, 8, 16 932 / 999, 570 / 589, 312 / 304, 212 / 200,
+// 236 / 221; 4096 rows in one 76 / 87.
+static bool forward_in_pairs(const PackedGeometry& g) {
+  const long long n_seq = g.pair_cap - plan_pairs(g.N_q, 0);
+  return (long long)g.pair_cap * g.q_heads >= 5 * kSms / 4 && g.N_q >= n_seq * (g.D <= 64 ? 1024 : 4096);
+}
+
 cudaError_t launch_packed_tc(int op, int dtype, const PackedGeometry& g, const Tensors& t, const PackedLayout& lay, cudaStream_t s,
                              int* launches, const char** err) {
   using namespace tc;
@@ -376,8 +387,10 @@ cudaError_t launch_packed_tc(int op, int dtype, const PackedGeometry& g, const T
   const TensorId ids[PI_COUNT] = {T_Q, T_K, T_V, T_dO};
   const void* ins[PI_COUNT] = {t.Q, t.K, t.V, t.dO};
   bool ok = true;
+  const bool pairs = op == OP_FORWARD && forward_in_pairs(g);
   for (int i = 0; i < n_in && ok; ++i)
-    ok = encode_strided(&maps.m[ids[i]], ins[i], bf, i == PI_K || i == PI_V ? g.kv_heads : g.q_heads, g.N_q, g.D, lay.of[i].row, lay.of[i].head, 64);
+    ok = encode_strided(&maps.m[ids[i]], ins[i], bf, i == PI_K || i == PI_V ? g.kv_heads : g.q_heads, g.N_q, g.D, lay.of[i].row, lay.of[i].head,
+                        pairs ? 128 : 64);
   auto out = [&](int id, void* p, int heads) {
     ok = ok && encode_strided(&maps.out[id], p, bf, heads, g.N_q, g.D, (long long)heads * g.D, g.D, 128);
   };
@@ -394,7 +407,7 @@ cudaError_t launch_packed_tc(int op, int dtype, const PackedGeometry& g, const T
   }
   if (op == OP_FORWARD) {
     *launches = 1;
-    return launch_packed_fwd(bf, maps, g, t, s);
+    return pairs ? launch_packed_fwd_pairs(bf, maps, g, t, s) : launch_packed_fwd(bf, maps, g, t, s);
   }
   *launches = 1;
   const cudaError_t e = bf ? launch_packed_rowdot<__nv_bfloat16>(t, g, lay.of[PI_dO], s) : launch_packed_rowdot<__half>(t, g, lay.of[PI_dO], s);

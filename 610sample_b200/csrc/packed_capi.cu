@@ -45,6 +45,8 @@ PackedGeometry make_geometry(const attn_packed_shape_t* s, const int32_t* plan) 
   g.cap = (int)plan_tiles(s->n_tok, s->n_seq);
   g.row_tiles = reinterpret_cast<const PackedTile*>(plan + kPlanHeader);
   g.col_tiles = g.row_tiles + g.cap;
+  g.pair_tiles = g.col_tiles + g.cap;
+  g.pair_cap = (int)plan_pairs(s->n_tok, s->n_seq);
   g.q_heads = s->q_heads;
   g.kv_heads = s->kv_heads;
   g.group = s->q_heads / s->kv_heads;

@@ -7,8 +7,8 @@
 // sequence are listed too; they get zeros.  Short sequences pay for that with part-filled tiles: tiles of 128
 // consecutive rows over several sequences would need up to 128 / length times fewer of them, but mix the rows of
 // two sequences in one product, where 0 * inf and 0 * NaN of a neighbour's masked keys reach the sums.
-// The entries are sorted by the length of a tile's stream, longest first, once for query tiles and once for key
-// tiles.  Kernels bound every entry on reading it: a plan that is not one gives wrong results, but no
+// The entries are sorted by the length of a tile's stream, longest first, once for query tiles, once for key tiles and
+// once for pairs of query tiles (256 rows).  Kernels bound every entry on reading it: a plan that is not one gives wrong results, but no
 // access outside of the tensors.
 #pragma once
 
@@ -19,21 +19,26 @@ namespace attn {
 constexpr int kPlanRows = 128;      // rows of a stationary tile
 constexpr int kPlanHeader = 8;      // ints: tiles, longest sequence, n_tok, n_seq, 4 unused
 
-// rows [row0, min(row0 + 128, end)) of the sequence [begin, end); begin < 0: rows of no sequence; row0 < 0: unused entry
+// rows [row0, min(row0 + 128, end)), in the list of pairs 256, of the sequence [begin, end); begin < 0: rows of no sequence; row0 < 0: unused entry
 struct alignas(16) PackedTile { int row0, begin, end, unused; };
 
 // Entries of either list: a sequence's last tile and the gaps in front and behind take one more each than
 // n_tok / 128.
 __host__ __device__ inline long long plan_tiles(long long n_tok, long long n_seq) { return n_tok / kPlanRows + n_seq + 2; }
 
-// A plan: header | query tiles | key tiles | row behind each sequence, and its tiles so far (n_seq ints each)
-inline long long plan_ints(long long n_tok, long long n_seq) { return kPlanHeader + 8 * plan_tiles(n_tok, n_seq) + 2 * n_seq; }
+__host__ __device__ inline long long plan_pairs(long long n_tok, long long n_seq) { return n_tok / (2 * kPlanRows) + n_seq + 2; }
+
+// A plan: header | query tiles | key tiles | pairs | row behind each sequence, and its tiles so far (n_seq ints each)
+inline long long plan_ints(long long n_tok, long long n_seq) {
+  return kPlanHeader + 8 * plan_tiles(n_tok, n_seq) + 4 * plan_pairs(n_tok, n_seq) + 2 * n_seq;
+}
 
 struct PackedGeometry : Geometry {
   static constexpr bool kPacked = true;
   const PackedTile* row_tiles;
   const PackedTile* col_tiles;
-  int cap;                  // entries of a list
+  const PackedTile* pair_tiles;
+  int cap, pair_cap;        // entries of either list, and of that of the pairs
   int group;                // query heads per key/value head
   int q_heads, kv_heads;
 };

@@ -2,7 +2,7 @@
 // one CTA.  Offsets are taken as they come: each is cut to [0, n_tok] and to no less than those before it, so that the
 // sequences never overlap.
 //   pass 1  running maximum of the offsets and running count of tiles, 1024 sequences at a time, kept in the plan
-//   pass 2  a histogram of the tiles by the length of their stream (in tiles; both lists have the same one)
+//   pass 2  histograms of the tiles (both lists have the same one) and of the pairs by the length of their stream, in tiles
 //   pass 3  every tile to its place, longest streams first
 // Made once per batch and shared by all layers and both directions, so what counts is that it is one short launch.
 #include "packed_geometry.cuh"
@@ -33,17 +33,18 @@ __device__ __forceinline__ int block_scan(int v, int* warp_sums, Op op, int iden
 
 __global__ void __launch_bounds__(kPlanThreads)
 packed_plan_kernel(const int* cu, int* plan, int n_tok, int n_seq) {
-  __shared__ int warp_sums[32], place[kPlanBins], shared_max, shared_longest;
-  const int cap = (int)plan_tiles(n_tok, n_seq);
+  __shared__ int warp_sums[32], place[kPlanBins], pair_place[kPlanBins], shared_max, shared_longest;
+  const int cap = (int)plan_tiles(n_tok, n_seq), pair_cap = (int)plan_pairs(n_tok, n_seq);
   PackedTile* const rows = reinterpret_cast<PackedTile*>(plan + kPlanHeader);
   PackedTile* const cols = rows + cap;
-  int* const ends = reinterpret_cast<int*>(cols + cap);      // row behind sequence i
+  PackedTile* const pairs = cols + cap;
+  int* const ends = reinterpret_cast<int*>(pairs + pair_cap);      // row behind sequence i
   int* const counts = ends + n_seq;                           // tiles of the sequences up to and with i
   const int tid = threadIdx.x;
   // streams of up to cap tiles fall into the bins `shift` apart
   int shift = 0;
   while ((n_tok / kPlanRows >> shift) >= kPlanBins - 1) ++shift;
-  for (int i = tid; i < kPlanBins; i += kPlanThreads) place[i] = 0;
+  for (int i = tid; i < kPlanBins; i += kPlanThreads) place[i] = pair_place[i] = 0;
   if (tid == 0) shared_longest = 0;
   auto cut = [&](int v) { return min(max(v, 0), n_tok); };
   const int first = cut(cu[0]);
@@ -85,21 +86,26 @@ packed_plan_kernel(const int* cu, int* plan, int n_tok, int n_seq) {
     int begin, end, k, n;
     find(t, begin, end, k, n);
     atomicAdd(&place[kPlanBins - 1 - (k >> shift)], 1);
+    if (k % 2 == 0) atomicAdd(&pair_place[kPlanBins - 1 - (k >> shift)], 1);
   }
   __syncthreads();
-  {
-    const int a = place[2 * tid], b = place[2 * tid + 1];
+  for (int which = 0; which < 2; ++which) {
+    int* const bins = which ? pair_place : place;
+    const int a = bins[2 * tid], b = bins[2 * tid + 1];
     const int through = block_scan(a + b, warp_sums, [](int x, int y) { return x + y; }, 0);
-    place[2 * tid] = through - a - b;
-    place[2 * tid + 1] = through - b;
+    bins[2 * tid] = through - a - b;
+    bins[2 * tid + 1] = through - b;
+    if (which && tid == kPlanThreads - 1) shared_max = through;
   }
   __syncthreads();
+  const int pair_count = shared_max;
   for (int t = tid; t < tiles; t += kPlanThreads) {
     int begin, end, k, n;
     find(t, begin, end, k, n);
     const int at = atomicAdd(&place[kPlanBins - 1 - (k >> shift)], 1);
     rows[at] = PackedTile{begin + k * kPlanRows, begin, end, 0};
     cols[at] = PackedTile{begin + (n - 1 - k) * kPlanRows, begin, end, 0};
+    if (k % 2 == 0) pairs[atomicAdd(&pair_place[kPlanBins - 1 - (k >> shift)], 1)] = PackedTile{begin + k * kPlanRows, begin, end, 0};
   }
   for (int t = tid; t < cap - tiles; t += kPlanThreads) {
     PackedTile e{-1, -1, -1, 0};
@@ -107,6 +113,13 @@ packed_plan_kernel(const int* cu, int* plan, int n_tok, int n_seq) {
     else if (t < front + back) e = PackedTile{last + (t - front) * kPlanRows, -1, n_tok, 0};
     rows[tiles + t] = e;
     cols[tiles + t] = e;
+  }
+  const int pair_front = (front + 1) / 2, pair_back = (back + 1) / 2;
+  for (int t = tid; t < pair_cap - pair_count; t += kPlanThreads) {
+    PackedTile e{-1, -1, -1, 0};
+    if (t < pair_front) e = PackedTile{t * 2 * kPlanRows, -1, first, 0};
+    else if (t < pair_front + pair_back) e = PackedTile{last + (t - pair_front) * 2 * kPlanRows, -1, n_tok, 0};
+    pairs[pair_count + t] = e;
   }
   if (tid == 0) {
     plan[0] = tiles; plan[1] = shared_longest; plan[2] = n_tok; plan[3] = n_seq;

@@ -78,8 +78,8 @@ def test_refused_pointers(capi):
     assert L.attn_b200_packed_plan(good, 4, 1, odd, None) == -1
     assert L.attn_b200_packed_plan(good, -4, 1, good, None) == -1
     assert L.attn_b200_packed_plan_ints(-1, 2) == 0
-    assert L.attn_b200_packed_plan_ints(0, 0) == 8 + 8 * 2
-    assert L.attn_b200_packed_plan_ints(1000, 3) == 8 + 8 * (1000 // 128 + 3 + 2) + 2 * 3
+    assert L.attn_b200_packed_plan_ints(0, 0) == 8 + 8 * 2 + 4 * 2
+    assert L.attn_b200_packed_plan_ints(1000, 3) == 8 + 8 * (1000 // 128 + 3 + 2) + 4 * (1000 // 256 + 3 + 2) + 2 * 3
 
 
 def test_empty_batch_needs_no_device(capi):
@@ -217,6 +217,55 @@ def test_many_tiles(packed, dtype, D):
     check(packed, [517, 1, 1200, 90, 64, 64, 3, 260, 31], 24, 8, D, dtype, tail=9)
 
 
+# long sequences, for which the forward takes its query tiles in pairs: mean lengths from 1024 (D <= 64) and 4096 on, 185 pairs and more
+PAIRS = [([1500, 700, 2300, 1], 24, 12, 64), ([1100, 1281], 32, 4, 32), ([4200], 16, 4, 128), ([129, 8100], 12, 4, 80)]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("lens, H, Hkv, D", PAIRS)
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+def test_long_sequences(packed, lens, H, Hkv, D, dtype):
+    check(packed, lens, H, Hkv, D, dtype, front=3, tail=1)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("window", [0, 1, 2, 100, 127, 128, 129, 256, 300, 1000])
+@pytest.mark.parametrize("lens, H, Hkv, D", PAIRS[:1] + PAIRS[2:3])
+def test_long_sequences_with_windows(packed, lens, H, Hkv, D, window):
+    check(packed, lens, H, Hkv, D, torch.bfloat16, window=window, tail=300)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("n", [1025, 1152, 1153, 1279, 1280, 1281, 1407, 1408, 1409])
+def test_last_rows_of_a_pair(packed, n):
+    check(packed, [n, n], 24, 8, 64, torch.bfloat16, amp=3.0)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("lens, D, dtype", [([1300, 900, 1200], 64, torch.bfloat16), ([4100, 4300], 128, torch.float16)])
+@pytest.mark.parametrize("bad", [math.nan, math.inf, -math.inf])
+def test_long_sequences_do_not_touch_one_another(packed, lens, D, dtype, bad):
+    cu = offsets(lens, 5)
+    n_tok = cu[-1] + 9
+    q, k, v, _ = tensors(n_tok, 24, 4, D, dtype)
+    plan = packed.packed_plan(torch.tensor(cu, dtype=torch.int32, device="cuda"), n_tok)
+    clean = packed.packed_attention(q, k, v, plan)
+    for t in (q, k, v):
+        for a, b in ((0, 5), (cu[1], cu[2]), (cu[-1], n_tok)):
+            t[a:b] = bad
+    dirty = packed.packed_attention(q, k, v, plan)
+    for i in range(len(lens)):
+        a, b = cu[i], cu[i + 1]
+        assert torch.equal(clean[a:b], dirty[a:b]) if i != 1 else bool(dirty[a:b].isnan().all()) or bad == -math.inf
+    assert not bool(dirty[:5].any()) and not bool(dirty[cu[-1]:].any())
+    # a key that is not a number reaches the rows that see it
+    q, k, v, _ = tensors(n_tok, 24, 4, D, dtype)
+    at = cu[0] + 700
+    k[at] = math.nan
+    o = packed.packed_attention(q, k, v, plan)
+    assert bool(o[at:cu[1]].isnan().all()) and not bool(o[:at].isnan().any()) and not bool(o[cu[1]:].isnan().any())
+
+
 @pytest.mark.gpu
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16, torch.float32])
 def test_peaked_rows(packed, dtype):
@@ -227,6 +276,11 @@ def test_peaked_rows(packed, dtype):
 def test_a_thousand_short_sequences(packed):
     lens = [(7 * i) % 23 for i in range(1500)]      # more than a pass of the plan takes at a time
     check(packed, lens, 2, 1, 32, torch.bfloat16, front=1, tail=1)
+
+
+def gaps_of(cu, n_tok, step):
+    first, last = (min(max(c, 0), n_tok) for c in (cu[0], max(cu)))
+    return [(r, -1, first) for r in range(0, first, step)] + [(r, -1, n_tok) for r in range(last, n_tok, step)]
 
 
 def plain_plan(cu, n_tok):
@@ -241,8 +295,7 @@ def plain_plan(cu, n_tok):
         for t in range(n):
             rows[(a + 128 * t, a, b)] = t + 1
             cols[(a + 128 * t, a, b)] = n - t
-    gaps = [(r, -1, fixed[0]) for r in range(0, fixed[0], 128)] + [(r, -1, n_tok) for r in range(fixed[-1], n_tok, 128)]
-    return rows, cols, gaps, max([b - a for a, b in zip(fixed[:-1], fixed[1:])], default=0)
+    return rows, cols, gaps_of(cu, n_tok, 128), max([b - a for a, b in zip(fixed[:-1], fixed[1:])], default=0)
 
 
 @pytest.mark.gpu
@@ -267,6 +320,13 @@ def test_plan(packed, cu, n_tok, dtype):
             shift += 1
         bins = [(x - 1) >> shift for x in work]
         assert bins == sorted(bins, reverse=True)      # longest streams first
+    pair_cap = n_tok // 256 + len(cu) - 1 + 2
+    e = [tuple(x[:3]) for x in t[8 + 8 * cap:8 + 8 * cap + 4 * pair_cap].view(pair_cap, 4).tolist()]
+    want = {k: v for k, v in rows.items() if (k[0] - k[1]) % 256 == 0}
+    n, wide_gaps = len(want), gaps_of(cu, n_tok, 256)
+    assert sorted(e[:n]) == sorted(want) and e[n:n + len(wide_gaps)] == wide_gaps and all(x[0] == -1 for x in e[n + len(wide_gaps):])
+    bins = [(want[x] - 1) >> shift for x in e[:n]]
+    assert bins == sorted(bins, reverse=True)
 
 
 @pytest.mark.gpu
