@@ -109,7 +109,7 @@ coefficients_kernel(const float* grad, const float* counted, const int64_t* targ
     return kind == 0 ? 0.f : kind == 1 ? (reduction == RED_NONE ? from_l2(grad + i) : common) : NAN;
   };
   float unit = 1.f, times = 1.f;
-  if (relative) {
+  if (relative) {      // the largest factor: of all rows where they have their own, which takes one CTA
     float top = 0.f;
     if (reduction == RED_NONE) {
 #pragma unroll 4
@@ -125,12 +125,13 @@ coefficients_kernel(const float* grad, const float* counted, const int64_t* targ
     if (top > 0.f && top < INFINITY) { unit = top; times = 32768.f; }
   }
 #pragma unroll 4
-  for (int i = threadIdx.x; i < n; i += 1024) coef[i] = factor(i) / unit * times;
-  if (threadIdx.x == 0) *scale = unit / times;
+  for (int i = blockIdx.x * 1024 + threadIdx.x; i < n; i += gridDim.x * 1024) coef[i] = factor(i) / unit * times;
+  if (blockIdx.x == 0 && threadIdx.x == 0) *scale = unit / times;
 }
 
 cudaError_t launch_coefficients(const Problem& p, const float* grad, const float* counted, int reduction, const Coefficients& c, cudaStream_t stream) {
-  return tc::launch_pdl(coefficients_kernel, 1u, 1024u, 0, stream, grad, counted, p.targets, c.coef, c.scale, p.n, p.V, reduction, p.dtype == 0 ? 1 : 0,
+  const unsigned ctas = p.dtype == 0 && reduction == RED_NONE ? 1u : (unsigned)((p.n + 1023) / 1024 < kSms ? (p.n + 1023) / 1024 : kSms);
+  return tc::launch_pdl(coefficients_kernel, ctas, 1024u, 0, stream, grad, counted, p.targets, c.coef, c.scale, p.n, p.V, reduction, p.dtype == 0 ? 1 : 0,
                         p.ignore_index);
 }
 
