@@ -887,7 +887,7 @@ static cudaError_t launch_packed_kind(const TmaMaps& maps, PackedGeometry g, con
   g.BH = kCol ? g.kv_heads : g.q_heads;
   const long long ctas = (long long)g.BH * g.cap;
   if (ctas > 0x7fffffffLL) return cudaErrorInvalidValue;
-  g.head_group = packed_head_group(g, 2ll * (kCol ? g.q_heads : g.kv_heads) * g.N_q * g.D * 2);
+  g.head_group = packed_head_group(g, ctas, 2ll * (kCol ? g.q_heads : g.kv_heads) * g.N_q * g.D * 2);
   const size_t smem = DUAL ? half_sm_smem(Kernel::CF::kSmemBytes) : whole_sm_smem(Kernel::CF::kSmemBytes);
   static std::atomic<unsigned long long> smem_set{0};
   auto kern = tile_kernel<Kernel, PackedGeometry>;

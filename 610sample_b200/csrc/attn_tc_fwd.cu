@@ -655,7 +655,7 @@ static cudaError_t launch_packed_fwd_one(const TmaMaps& maps, const PackedGeomet
   PackedGeometry g = g_in;
   g.BH = g.q_heads;
   const long long ctas = (long long)g.BH * g.cap;
-  g.head_group = packed_head_group(g, 2ll * g.kv_heads * g.N_kv * g.D * 2);
+  g.head_group = packed_head_group(g, ctas, 2ll * g.kv_heads * g.N_kv * g.D * 2);
   if (ctas > 0x7fffffffLL) return cudaErrorInvalidValue;
   static std::atomic<unsigned long long> smem_set[2];
   if (ctas >= 2 * kSms) {

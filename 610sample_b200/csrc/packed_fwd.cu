@@ -437,7 +437,7 @@ cudaError_t launch_one(const TmaMaps& maps, const PackedGeometry& g_in, const Te
   g.BH = g.q_heads;
   const long long ctas = (long long)g.BH * g.pair_cap;
   if (ctas > 0x7fffffffLL) return cudaErrorInvalidValue;
-  g.head_group = packed_head_group(g, 2ll * g.kv_heads * g.N_kv * g.D * 2);
+  g.head_group = packed_head_group(g, ctas, 2ll * g.kv_heads * g.N_kv * g.D * 2);
   static std::atomic<unsigned long long> smem_set{0};
   auto kern = packed_fwd_kernel<DT, T>;
   const cudaError_t e = set_smem_once(kern, CF::kSmemBytes, smem_set);

@@ -52,8 +52,9 @@ __device__ __forceinline__ int packed_cap(const PackedGeometry& g) { return g.ca
 // Heads of a group of the CTAs' order (Geometry::head_group): all of them where the streamed tensors of all heads, of `bytes`, fit L2 together
 // with the rest, so that the longest streams of all heads come first; else as many as 16 MB hold.  Groups of four of twelve heads left the SMs idle for
 // 18 % of the forward's and 13 to 17 % of the backward's time (16384 rows in 19 sequences, 12 heads of 64).
-inline int packed_head_group(const PackedGeometry& g, long long bytes) {
-  if (bytes <= (64ll << 20)) return g.BH;
+// So do a few CTAs, whose longest ones decide (8192 rows in 7 sequences, 32 and 8 heads of 128, dK/dV: 584 CTAs, 281 us, 365 head by head).
+inline int packed_head_group(const PackedGeometry& g, long long ctas, long long bytes) {
+  if (ctas < 8 * kSms || bytes <= (64ll << 20)) return g.BH;
   const long long n = (16ll << 20) * g.BH / bytes;
   return n < 1 ? 1 : n < g.BH ? (int)n : g.BH;
 }
