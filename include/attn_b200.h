@@ -272,8 +272,9 @@ int attn_b200_last_launch_count(void);
  * forever: each wait has an iteration limit, after which the kernel records its
  * code here and returns.  Code = (kernel id + 1) << 8 | wait id, kernel ids:
  * 4 / 5 / 6 double-backward scalar + g_dO / g_Q / g_K + g_V kernel, 18 / 19
- * backward row / column kernel, 20 forward, 0x6f the primitive self-test (codes
- * 0x7001..0x7003); wait id 15 = the launch gave the kernel less shared memory
+ * backward row / column kernel, 20 forward, 21 forward of packed batches by pairs of tiles,
+ * 32 to 35 the linear cross entropy's products (scores, gradient of the logits, dx, dW), 0x6f the
+ * primitive self-test (codes 0x7001..0x7003); wait id 15 = the launch gave the kernel less shared memory
  * than its layout needs. */
 int attn_b200_device_status(uint32_t* code);
 
