@@ -372,7 +372,11 @@ struct PackedQKNormRopeBackward : public torch::autograd::Function<PackedQKNormR
     // aliases of the inputs, so that the derivatives are partial ones even where the inputs depend on one another
     auto alias = [&](const torch::Tensor& t) { return keep_graph && t.requires_grad() ? t.view_as(t) : t.detach().requires_grad_(true); };
     for (int side = 0; side < 2; ++side) {
-      const torch::Tensor g = alias(s[side]), x = alias(s[2 + side]);
+      // a row without a gradient that is not a number, or whose position is outside of the table, gives 0 here too
+      const torch::Tensor still = (s[side].detach() == 0).all(-1, true);
+      const torch::Tensor dead = still & s[2 + side].detach().isfinite().all(-1, true).logical_not();
+      const torch::Tensor turn = torch::where(still.unsqueeze(-1) & angles.isnan(), torch::zeros({}, angles.options()), angles);
+      const torch::Tensor g = alias(s[side]), x = alias(s[2 + side]), kept = torch::where(dead, torch::zeros({}, x.options()), x);
       variable_list first_wrt{x}, wrt{g, x};
       torch::Tensor w;
       if (s[4 + side].numel() > 0) {
@@ -380,7 +384,7 @@ struct PackedQKNormRopeBackward : public torch::autograd::Function<PackedQKNormR
         first_wrt.push_back(w);
         wrt.push_back(w);
       }
-      const variable_list first = torch::autograd::grad({rope_formula(x, w, angles, a.eps)}, first_wrt, {g}, true, true);
+      const variable_list first = torch::autograd::grad({rope_formula(kept, w, turn, a.eps)}, first_wrt, {g}, true, true);
       variable_list of, with;
       for (size_t i = 0; i < first.size(); ++i) {
         const torch::Tensor& t = tangents[i == 0 ? side : 2 + side];

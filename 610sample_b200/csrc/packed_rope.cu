@@ -283,6 +283,11 @@ backward_kernel(const __grid_constant__ Args a, const int shares, float* partial
         float gv[8], xv[8], gy[8];
         rg[i].get(gv);
         rx[i].get(xv);
+        // a row whose gradient is 0 gives 0, also where the row (of no sequence, say) is infinite or not a number, or its
+        // position is outside of the table
+        bool any = false;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) any |= gv[e] != 0.f;
 #pragma unroll
         for (int p = 0; p < 4; ++p) {
           gy[2 * p] = gv[2 * p] * cs[p].x + gv[2 * p + 1] * cs[p].y;
@@ -290,20 +295,16 @@ backward_kernel(const __grid_constant__ Args a, const int shares, float* partial
         }
         if (norm) {      // uniform: every lane takes part in the shuffles
           float ss = 0.f, dot = 0.f;
-          bool any = false;
 #pragma unroll
           for (int e = 0; e < 8; ++e) {
             ss = fmaf(xv[e], xv[e], ss);
-            if (WIDE || e < n) {      // pairs beyond D have no angle
-              dot = fmaf(gy[e] * w[e], xv[e], dot);
-              any |= gy[e] != 0.f;
-            }
+            if (WIDE || e < n) dot = fmaf(gy[e] * w[e], xv[e], dot);      // pairs beyond D have no angle
           }
           ss = group_sum<G>(ss);
           dot = group_sum<G>(dot);
-          // a row whose gradient is 0 gives 0, also where the row (of no sequence, say) is infinite or not a number
           const unsigned lanes = __ballot_sync(0xffffffffu, any);
-          if (on && i < now.heads && ((lanes >> ((threadIdx.x & 31) / G * G)) & ((1u << G) - 1u)) != 0u) {
+          any = ((lanes >> ((threadIdx.x & 31) / G * G)) & ((1u << G) - 1u)) != 0u;
+          if (on && i < now.heads && any) {
             const float r = rsqrtf(fmaf(ss, inv_d, a.eps)), k = r * r * r * inv_d * dot;
 #pragma unroll
             for (int e = 0; e < 8; ++e) {
@@ -312,6 +313,10 @@ backward_kernel(const __grid_constant__ Args a, const int shares, float* partial
               gy[e] = r * gy[e] * w[e] - k * xv[e];
             }
           }
+        }
+        if (!any) {
+#pragma unroll
+          for (int e = 0; e < 8; ++e) gy[e] = 0.f;
         }
         if (on && i < now.heads) store8<T, WIDE>(out + (size_t)i * a.D, gy, n);
       }

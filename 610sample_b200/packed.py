@@ -62,7 +62,7 @@ def packed_qk_norm_rope(q, k, q_weight, k_weight, freqs, positions, sections=Non
 
     q_weight, k_weight: (D,), of the type of q and k or float32; None: no norm, only the rotation.
     freqs: `qk_prep.rope_table(...)`, float32 (rows, D / 2, 2); positions: (n_tok,) or (axes, n_tok), int32 or int64, rows of
-    freqs; one outside of it gives NaN.  sections: how many of the D / 2 pairs turn with each axis, in order (up to four
+    freqs; one outside of it gives NaN, and a gradient of 0 where the result's is 0.  sections: how many of the D / 2 pairs turn with each axis, in order (up to four
     axes: time, height and width of a video's patches, say); None for positions of one axis.
     q and k may be slices of one projection's result.  D even, up to 128; fp16, bf16 or fp32.  Computed in float32 and
     rounded once (`qk_norm_rope` rounds where the reference's separate operations do).  Twice differentiable in q, k and the

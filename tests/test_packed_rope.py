@@ -233,6 +233,40 @@ def test_rows_without_gradient_have_no_influence(packed, rope_table):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("D", [64, 128, 20])
+@pytest.mark.parametrize("with_weights", [True, False])
+def test_padding_behind_the_last_sequence_has_no_influence(packed, rope_table, dtype, D, with_weights):
+    # rows that nothing reads: positions outside of the table, anything in q and k; first and second derivative
+    table = rope_table(D, 500, device="cuda")
+    q, k, w, g, pos, sec = inputs(90, 4, 2, D, dtype)
+    u, v, uw, _, _, _ = inputs(90, 4, 2, D, dtype, seed=5)
+    w = w if with_weights else [None, None]
+    for t in (*g, u, v):
+        t[60:] = 0
+
+    def passes():
+        leaves = [t.detach().clone().requires_grad_(True) for t in (q, k, *w) if t is not None]
+        gl = [t.detach().clone().requires_grad_(True) for t in g]
+        outs = packed.packed_qk_norm_rope(*leaves, *([None] * (4 - len(leaves))), table, pos, sec)
+        plain = torch.autograd.grad(outs, leaves, gl, retain_graph=True)
+        first = torch.autograd.grad(outs, leaves, gl, create_graph=True)
+        second = torch.autograd.grad(first, leaves + gl, [u, v, *uw][:len(leaves)], allow_unused=True)
+        return [*plain, *first, *[t for t in second if t is not None]]
+    want = passes()
+    pos[60:75], pos[75:] = -1, 2 ** 31 - 1
+    q[60:70] = math.nan
+    k[65:80] = math.inf
+    got = passes()
+    assert len(got) == len(want)
+    for a, b in zip(got, want):
+        assert bool(a.isfinite().all()) or a.shape[0] == 90
+        assert torch.equal(a[:60], b[:60]) if a.shape[0] == 90 else torch.equal(a, b)
+    for a in got[:2]:
+        assert not bool(a[60:].any())
+
+
+@pytest.mark.gpu
 def test_refused_calls(packed, rope_table):
     q, k, w, g, pos, sec = inputs(20, 4, 2, 32, torch.bfloat16)
     t = rope_table(32, 500, device="cuda")
