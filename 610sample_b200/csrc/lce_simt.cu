@@ -133,9 +133,10 @@ lce_simt_kernel(const Operand<TA> A, const Operand<TB> B, const SimtArgs g, T* o
       }
 #pragma unroll
       for (int o = 8; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));      // the 16 threads of a row
+      const float ref = m == -INFINITY ? 0.f : m;      // logits of -inf alone: every term 0
       float l = 0.f;
 #pragma unroll
-      for (int j = 0; j < 8; ++j) l += exp2f(fmaf(acc[i][j], kLog2e, -m));
+      for (int j = 0; j < 8; ++j) l += exp2f(fmaf(acc[i][j], kLog2e, -ref));
 #pragma unroll
       for (int o = 8; o > 0; o >>= 1) l += __shfl_xor_sync(0xffffffffu, l, o);
       if (in && tx == 0) g.partial[(size_t)nt * g.rows + r] = Partial{m, l};

@@ -13,11 +13,14 @@
 // the next one accumulates in the other half of it.  The order of the tiles runs along the axis of the smaller operand first, so
 // that the larger one is read from HBM once and the smaller one stays in L2.
 //
-// DX and DW have few tiles with long sums: 96 of 256 blocks of k for 74 pairs, in the 16384 x 32000 case's dW, are two rounds, 65 % busy.  There the
-// tiles of the last round are each shared out along k among several pairs (plan_shares), and a small kernel behind adds the parts in
-// order (join_kernel).  Whole rounds stay as they are: pairs that are at the same place in k read the same rows of G and x from L2;
-// equal, contiguous shares of all blocks left no pair idle, but took dW's product from 178 to 168 us only, and dx's from 146 to 167 to
-// 187, since G then came from HBM several times.
+// DX and DW have few tiles with long sums: dW of a piece of 8192 classes x 768 from 16384 rows is 96 tiles of 256 blocks of k for 74 pairs, two
+// rounds, 65 % busy.  There the tiles of the last round are each shared out along k among several pairs (plan_shares), and a small kernel behind
+// adds the parts in order (join_kernel).  Whole rounds stay as they are: pairs that are at the same place in k read the same rows of G and x from
+// L2; equal, contiguous shares of all blocks left no pair idle, but took dW's product from 178 to 168 us only (that size), and dx's from
+// 146 to between 167 and 187, since G then came from HBM several times.
+//
+// 16384 x 768 x 32000, bf16, each by itself: LSE 490 to 517 us (1 600 TFLOP/s, tensor pipe 87 % active); for a piece of 16128 classes GRAD 295 to 321
+// (1 320, 68 %: it writes 475 MB), DW 250 to 275 (1 550, 83 %), DX 240 to 264 (1 610, 87 %), join 12 each.  In a loop the board is at its power limit.
 #include "lce_launch.h"
 #include "tc_common.cuh"
 
@@ -261,10 +264,10 @@ lce_gemm_kernel(const __grid_constant__ GemmMaps maps, const GemmArgs g) {
           float mx = z[0];
 #pragma unroll
           for (int e = 1; e < 16; ++e) mx = fmaxf(mx, z[e]);
-          const float m_new = fmaxf(m, mx * kLog2e);
+          const float m_new = fmaxf(m, mx * kLog2e), ref = m_new == -INFINITY ? 0.f : m_new;      // logits of -inf alone: every term 0
           float sum = 0.f;
 #pragma unroll
-          for (int e = 0; e < 16; ++e) sum += ex2(fmaf(z[e], kLog2e, -m_new));
+          for (int e = 0; e < 16; ++e) sum += ex2(fmaf(z[e], kLog2e, -ref));
           l = fmaf(l, m == -INFINITY ? 0.f : ex2(m - m_new), sum);
           m = m_new;
         }
@@ -274,7 +277,7 @@ lce_gemm_kernel(const __grid_constant__ GemmMaps maps, const GemmArgs g) {
         if (half == 0 && in) {
           const float2 o = halves[buf * 128 + row];
           const float m_all = fmaxf(m, o.x);
-          const float l_all = fmaf(l, ex2(m - m_all), o.y * (o.x == -INFINITY ? 0.f : ex2(o.x - m_all)));
+          const float l_all = fmaf(l, m == -INFINITY ? 0.f : ex2(m - m_all), o.y * (o.x == -INFINITY ? 0.f : ex2(o.x - m_all)));
           g.partial[(size_t)nt * g.rows + r] = Partial{m_all, l_all};
         }
       } else {

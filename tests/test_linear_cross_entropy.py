@@ -224,6 +224,26 @@ def test_ignored_rows_have_no_influence(lce, dtype, d, bad):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("dtype, d", [(torch.bfloat16, 64), (torch.float32, 64), (torch.bfloat16, 60)])
+@pytest.mark.parametrize("out", [(0, 300), (300, 600), (3, 20), (500, 900)])
+def test_logits_of_minus_infinity_count_nothing(lce, dtype, d, out):
+    # classes whose weights are the type's lowest value: their logits overflow to -inf for rows of positive x
+    x, w, y, g = inputs(140, d, 900, dtype)
+    x = x.abs() + 0.5
+    keep = torch.ones(900, dtype=torch.bool, device="cuda")
+    keep[out[0]:out[1]] = False
+    index = torch.cumsum(keep, 0) - 1
+    y = torch.where((y >= 0) & ~keep[y.clamp(min=0)], int(keep.nonzero()[0]), y)
+    w[~keep] = torch.finfo(dtype).min
+    got = both_passes(lce, x, w, y, g, "none")
+    want, bound = reference(x, w[keep], torch.where(y >= 0, index[y.clamp(min=0)], y), g, -100, "none")
+    tiny = torch.finfo(dtype).smallest_normal * torch.finfo(dtype).eps
+    assert not bool(got[2][~keep].any())
+    for a, b, e in zip((got[0], got[1], got[2][keep]), want, bound):
+        assert bool(((a.double() - b).abs() <= e + tiny).all())
+
+
+@pytest.mark.gpu
 def test_nothing_counts(lce):
     x, w, y, g = inputs(20, 32, 50, torch.bfloat16)
     y.fill_(-100)
