@@ -51,7 +51,8 @@ def packed_attention(q, k, v, plan, window_size=None):
     Key j is visible to query i of the same sequence when j <= i and, with a `window_size`, i < j + window_size.
     The softmax scale is 1 / sqrt(D).  Rows that see no key (of no sequence, or a window of 0) give 0.  What
     rows of other sequences or of none hold, infinities and NaN too, has no influence on a sequence's result;
-    within a sequence, an infinite or NaN key or value may reach the queries of up to 127 rows before it as well.
+    within a sequence, an infinite or NaN row of k or v (or, in the backward, of q or the gradient) may reach rows that it is
+    masked for as well, up to 255 before the first or behind the last one that it is not.
     Returns O: (n_tok, H, D), dense."""
     return _attention_cuda.packed_attention(q, k, v, plan.tensor, plan.n_tok, plan.n_seq, window_size, plan.max_seqlen)
 
