@@ -224,6 +224,23 @@ def test_ignored_rows_have_no_influence(lce, dtype, d, bad):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("reduction", ["none", "sum", "mean"])
+def test_a_factor_of_all_rows_is_not_rounded(lce, dtype, reduction):
+    # a factor just below the middle of two numbers of the type.  Rounded in every row, it alone would put the gradients off by u = half a
+    # step; the roundings of G and of the results are independent and evenly spread, each off by at most u / sqrt(3) in the 2-norm
+    u = torch.finfo(dtype).eps / 2
+    n = 400
+    x, w, y, _ = inputs(n, 128, 2000, dtype, ignored=0.0)
+    factor = (1 + u) * (1 - 2.0 ** -20)
+    g = torch.full((n,), factor, device="cuda") if reduction == "none" else torch.tensor(factor * (n if reduction == "mean" else 1), device="cuda")
+    got = both_passes(lce, x, w, y, g, reduction)
+    want, _ = reference(x, w, y, g, -100, reduction)
+    for a, b in zip(got[1:], want[1:]):
+        assert float((a.double() - b).norm() / b.norm()) <= u * math.sqrt(2 / 3)
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("dtype, d", [(torch.bfloat16, 64), (torch.float32, 64), (torch.bfloat16, 60)])
 @pytest.mark.parametrize("out", [(0, 300), (300, 600), (3, 20), (500, 900)])
 def test_logits_of_minus_infinity_count_nothing(lce, dtype, d, out):
