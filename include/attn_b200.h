@@ -207,7 +207,8 @@ int attn_b200_packed_backward(const attn_packed_shape_t* shape, const int32_t* p
 /* The step in front of packed attention: per (token, head) RMS normalisation with a learned weight and rotation by positions
  * that are given per token, on up to four axes, of Q and K in one pass.  Pair i of a row, elements 2i and 2i + 1, is turned by
  * row positions[axis][token] of freqs, float32 [table_rows, D / 2, 2] = (cos, sin); axis 0 has the first section[0] pairs, axis 1
- * the next section[1], and so on, D / 2 in all.  A position outside of the table gives NaN.  Arithmetic in fp32, rounded once
+ * the next section[1], and so on, D / 2 in all.  A position outside of the table gives NaN (in
+ * the backward a row whose gradient is 0 gives 0 whatever its position and content).  Arithmetic in fp32, rounded once
  * (attn_b200_qk_norm_rope has the rounding points of the reference's separate operations instead).
  * q: [n_tok, q_heads, D], k: [n_tok, k_heads, D] in strides of elements, results dense; weights [D], null for no norm, of the type of
  * q and k or (weight_float) float32; positions [axes][n_tok], axis_stride elements apart, int32 or (positions64) int64.  D even, up to

@@ -450,6 +450,108 @@ def test_captured_plan_and_passes(packed):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("H, Hkv, D", [(16, 16, 64), (32, 8, 128)])
+def test_captured_long_sequences(packed, H, Hkv, D):
+    # forwards of pairs of tiles; lengths of another replay
+    n = 8300
+    q, k, v, do = tensors(n, H, Hkv, D, torch.bfloat16)
+    cu = torch.tensor([0, 8200], dtype=torch.int32, device="cuda")
+
+    def step():
+        return both_passes(packed, q, k, v, do, packed.packed_plan(cu, n), None)
+    step()
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = step()
+    for lens in ([0, 8200], [5, 8300], [0, 1]):
+        cu.copy_(torch.tensor(lens, dtype=torch.int32))
+        graph.replay()
+        for x, y in zip(out, step()):
+            assert torch.equal(x, y)
+
+
+@pytest.mark.gpu
+def test_captured_second_derivative(packed):
+    # with the length of the longest sequence given, nothing waits for the host
+    n, H, Hkv, D = 260, 4, 2, 64
+    leaves = [t.requires_grad_(True) for t in tensors(n, H, Hkv, D, torch.bfloat16)]
+    tangents = tensors(n, H, Hkv, D, torch.bfloat16, seed=3)[:3]
+    cu = torch.tensor([0, 100, 256], dtype=torch.int32, device="cuda")
+
+    def step(leaves):
+        first = torch.autograd.grad(packed.packed_attention(*leaves[:3], packed.packed_plan(cu, n, max_seqlen=200)), leaves[:3], leaves[3], create_graph=True)
+        return torch.autograd.grad(first, leaves, tangents)
+    side = torch.cuda.Stream()
+    with torch.cuda.stream(side):
+        step(leaves)
+        torch.cuda.synchronize()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, stream=side):
+            out = step(leaves)
+    for lens in ([0, 100, 256], [3, 200, 260], [0, 0, 190]):
+        cu.copy_(torch.tensor(lens, dtype=torch.int32))
+        graph.replay()
+        torch.cuda.synchronize()
+        for x, y in zip(out, step([t.detach().requires_grad_(True) for t in leaves])):
+            assert torch.equal(x, y)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_some_gradients_and_their_layouts(packed, dtype):
+    q, k, v, do = tensors(300, 4, 2, 64, dtype)
+    plan = packed.packed_plan(torch.tensor([0, 130, 290], dtype=torch.int64, device="cuda"), 300)
+    want = both_passes(packed, q, k, v, torch.ones_like(do), plan, None)
+    # the gradient of a sum has strides of 0; each input alone; the same graph twice
+    for i in range(3):
+        leaves = [t.detach().clone() for t in (q, k, v)]
+        leaves[i].requires_grad_(True)
+        o = packed.packed_attention(*leaves, plan)
+        for _ in range(2):
+            assert torch.equal(torch.autograd.grad(o.sum(), leaves[i], retain_graph=True)[0], want[1 + i])
+    # a gradient laid out by heads
+    leaves = [t.detach().clone().requires_grad_(True) for t in (q, k, v)]
+    o = packed.packed_attention(*leaves, plan)
+    by_heads = do.transpose(0, 1).contiguous().transpose(0, 1)
+    for a, b in zip(torch.autograd.grad(o, leaves, by_heads), both_passes(packed, q, k, v, do, plan, None)[1:]):
+        assert torch.equal(a, b)
+    # one tensor in all three places
+    x = k.detach().clone().requires_grad_(True)
+    got = torch.autograd.grad(packed.packed_attention(x, x, x, plan), x, do[:, :2])[0]
+    parts = both_passes(packed, k, k, k, do[:, :2], plan, None)[1:]
+    assert float((got.float() - sum(t.float() for t in parts)).norm() / got.float().norm()) <= 2 * torch.finfo(dtype).eps
+
+
+@pytest.mark.gpu
+def test_second_derivative_without_rows_or_keys(packed):
+    for n, cu, window, longest in ((0, [0], None, None), (5, [0], None, None), (5, [0, 0, 0], None, None), (70, [0, 70], 0, None), (70, [0, 70], None, 0)):
+        leaves = [t.requires_grad_(True) for t in tensors(n, 4, 2, 32, torch.bfloat16)]
+        plan = packed.packed_plan(torch.tensor(cu, dtype=torch.int32, device="cuda"), n, max_seqlen=longest)
+        first = torch.autograd.grad(packed.packed_attention(*leaves[:3], plan, window), leaves[:3], leaves[3], create_graph=True)
+        for t, x in zip(torch.autograd.grad(first, leaves, [torch.ones_like(f) for f in first]), leaves):
+            assert t.shape == x.shape and not bool(t.any())
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("n, H, Hkv, D, dtype, window, bad", [
+    (300, 4, 2, 64, torch.bfloat16, 150, 120), (300, 4, 2, 128, torch.bfloat16, 150, 120), (300, 4, 2, 64, torch.float32, 150, 120),
+    (4100, 16, 16, 64, torch.bfloat16, 1500, 1100), (8200, 16, 4, 128, torch.bfloat16, 1500, 1100)])
+def test_scores_of_minus_infinity_count_nothing(packed, n, H, Hkv, D, dtype, window, bad):
+    # keys 1 .. bad: products below the range of float, as beside them finite ones of -1e4 with probabilities of 0 too.  Every row
+    # sees another key, with the window some behind whole tiles of these
+    q, k, v, do = tensors(n, H, Hkv, D, dtype)
+    q, k = torch.full_like(q, 2.0 ** 64), k * 2.0 ** -64
+    plan = packed.packed_plan(torch.tensor([0, n], dtype=torch.int32, device="cuda"), n)
+    out = []
+    for low in (-2.0 ** 66, -1250 * 2.0 ** -64):
+        k[1:bad + 1] = low
+        out.append(both_passes(packed, q, k, v, do, plan, window))
+    for a, b in zip(*out):
+        assert bool(a.isfinite().all()) and torch.equal(a, b)
+
+
+@pytest.mark.gpu
 def test_two_streams_at_once(packed):
     cases = []
     for seed, lens in ((1, [300, 400]), (2, [650, 50])):
