@@ -69,8 +69,8 @@ variable_list loss_backward(const torch::Tensor& g_in, const torch::Tensor& x_in
 // Second backward, out of ordinary operations over pieces of the rows: with tangents u on dx and v on dw, T = u W^T + x v^T,
 // P = exp(z - lse), c the rows' factors, r_i = sum_j P_ij T_ij:
 //   to c_i: r_i - T_i,y      H = c P (T - r), G = c (P - onehot)      to x: H W + G v      to W: H^T x + G^T u
-// Products of half types are summed and kept in float; H and G are rounded to the input type, relative to their largest element
-// (fp16 would lose factors like 1 / n to its range).
+// Products of half types are summed and kept in float; H and G are rounded to the input type, in bf16 relative to the largest factor (one that
+// all rows share would be rounded in the same direction everywhere), in fp16 to their own largest elements (its range).
 variable_list loss_double_backward(const torch::Tensor& u_in, const torch::Tensor& v_in, const torch::Tensor& g, const torch::Tensor& x,
                                    const torch::Tensor& w, const torch::Tensor& targets, const torch::Tensor& lse, const torch::Tensor& counted_rows,
                                    const LossArgs& a) {
@@ -84,6 +84,11 @@ variable_list loss_double_backward(const torch::Tensor& u_in, const torch::Tenso
   torch::Tensor gx = torch::zeros_like(x), gw = torch::zeros(w.sizes(), w.options().dtype(at::kFloat)), gc = torch::zeros({n}, c.options());
   const bool half = x.scalar_type() != at::kFloat;
   auto mm = [&](const torch::Tensor& p, const torch::Tensor& q) { return half ? at::mm(p, q, at::kFloat) : at::mm(p, q); };
+  auto unit = [&](const torch::Tensor& t, float largest) {
+    const torch::Tensor top = t.numel() > 0 ? t.abs().amax() : torch::zeros({}, t.options());
+    return torch::where((top > 0) & (top < std::numeric_limits<float>::infinity()), largest / top, torch::ones({}, top.options()));
+  };
+  const torch::Tensor common = x.scalar_type() == at::kBFloat16 ? unit(c, 1.f) : torch::ones({}, c.options());
   const int64_t step = std::max<int64_t>(1, std::min<int64_t>(n, (int64_t(1) << 28) / V));
   for (int64_t i = 0; i < n; i += step) {
     const int64_t e = std::min(n, i + step);
@@ -100,15 +105,8 @@ variable_list loss_double_backward(const torch::Tensor& u_in, const torch::Tenso
     torch::Tensor G = P.scatter_add_(1, y, torch::full({}, -1.f, P.options()).expand_as(y)).mul_(cs);
     H = torch::where(mask, H, zero);
     G = torch::where(mask, G, zero);
-    torch::Tensor sh = torch::ones({}, c.options()), sg = sh;
-    if (x.scalar_type() == at::kHalf) {
-      auto unit = [&](const torch::Tensor& t) {
-        const torch::Tensor top = t.abs().amax();
-        return torch::where((top > 0) & (top < std::numeric_limits<float>::infinity()), 32768.f / top, torch::ones({}, top.options()));
-      };
-      sh = unit(H);
-      sg = unit(G);
-    }
+    const bool fp16 = x.scalar_type() == at::kHalf;
+    const torch::Tensor sh = fp16 ? unit(H, 32768.f) : common, sg = fp16 ? unit(G, 32768.f) : common;
     const torch::Tensor Ht = (H * sh).to(x.scalar_type()), Gt = (G * sg).to(x.scalar_type());
     torch::Tensor to_x = mm(Ht, w) / sh;
     if (v_in.defined()) to_x.add_(mm(Gt, v_in) / sg);

@@ -384,6 +384,28 @@ def test_second_derivative(lce, dtype, tol, reduction):
 
 
 @pytest.mark.gpu
+def test_a_factor_of_all_rows_is_not_rounded_in_the_second_derivative(lce):
+    # the factor below the middle of two numbers, as above.  H = c P (T - r) and G = c (P - onehot) are rounded element by element, and the
+    # results: each off by u / sqrt(3) / m in the mean square, m the mantissa, over [1, 2) 0.408 u; 15 % more for how they really lie
+    n, d, V, u = 300, 128, 1500, 2.0 ** -8
+    x, w, y, _ = inputs(n, d, V, torch.bfloat16, ignored=0.0)
+    tx, tw, _, _ = inputs(n, d, V, torch.bfloat16, seed=8)
+    factor = (1 + u) * (1 - 2.0 ** -20)
+    leaves = [x.requires_grad_(True), w.requires_grad_(True)]
+    first = torch.autograd.grad(lce(x, w, y, reduction="sum"), leaves, torch.tensor(factor, device="cuda"), create_graph=True)
+    got = torch.autograd.grad(first, leaves, (tx, tw))
+    x, w, tx, tw = (t.detach().double() for t in (x, w, tx, tw))
+    P, T = torch.softmax(x @ w.T, 1), tx @ w.T + x @ tw.T
+    H = factor * P * (T - (P * T).sum(1, keepdim=True))
+    G = factor * (P - torch.nn.functional.one_hot(y, V))
+    want = (H @ w + G @ tw, H.T @ x + G.T @ tx)
+    squares = lambda a, b: ((a * a) @ (b * b).sum(1)).sum()
+    spread = (squares(H, w) + squares(G, tw), squares(H.T, x) + squares(G.T, tx))
+    for a, b, e in zip(got, want, spread):
+        assert float((a.double() - b).norm()) <= 0.47 * u * float((e + (b * b).sum()).sqrt())
+
+
+@pytest.mark.gpu
 def test_gradient_against_differences(lce):
     # h = 2^-7: truncation h^2 / 6 of a third derivative of the first's size (1e-5), rounding of the sum of 100 losses over 2 h (2e-4)
     x, w, y, _ = inputs(100, 40, 300, torch.float32)
