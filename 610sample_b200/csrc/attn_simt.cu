@@ -449,6 +449,17 @@ __device__ __forceinline__ void simt_tile(const Geo& g, const Tensors& t, const 
             if constexpr (KIND == K_HVP_COL) op[2][at] = h.g_dp;
           }
         }
+      if constexpr (kPacked) {
+        // a query that sees one key, the first of its sequence or with a window of 1 every one: dP - D is 0, which sums in two orders need not be
+        const int q0 = SP::kCol ? s0 : r0;
+        if (g.window == 1 || (q0 <= work.begin && work.begin < q0 + (SP::kCol ? TT : TS))) {
+#pragma unroll
+          for (int a = 0; a < RA; ++a)
+#pragma unroll
+            for (int b = 0; b < CB; ++b)
+              if (g.window == 1 || q0 + (SP::kCol ? col0 + 8 * b : row0 + 4 * a) == work.begin) op[SP::kCol][op_at(row0 + 4 * a, col0 + 8 * b)] *= 0.f;
+        }
+      }
     }
     __syncthreads();
     auto add = [&](int o, int which, int z) { out_fma<DC, RA>(op[which], strm[z], lay, row0, chunk0, chunks, out[o]); };

@@ -520,6 +520,11 @@ __device__ __forceinline__ void fb_kernel<KIND, D, T, SPLIT, DUAL, Geo>::run(con
     };
     if constexpr (CF::kCol) { if (n_iter > 0) publish_stat(0, fetch_stat(0)); }
 
+    // A query of a packed batch that sees one key has P = 1 and dP - D = 0, which the product and the row-dot, sums in two orders, need
+    // not give: its dS counts as 0 (times 0, so that what is not a number stays).  The first query of a sequence is column 0 of its first
+    // tile, beside key 0; with a window of 1 it is every query, and the results are multiplied.
+    [[maybe_unused]] auto only_key = [&](int j0) { return gidx == work.begin && j0 == work.begin; };
+
     if constexpr (CF::kWholeRow) {
       // ---- row kind: the eight math warps form two groups of four; group w takes the tiles of
       // parity w (= score buffer w), a thread its whole row of the tile (64 scores).  While one
@@ -598,7 +603,8 @@ __device__ __forceinline__ void fb_kernel<KIND, D, T, SPLIT, DUAL, Geo>::run(con
               float2 dv = nDv;
               if constexpr (CF::kCol) dv = *reinterpret_cast<const float2*>(cs + 64 + hh * 32 + ch * 16 + e);
               const float2 dpd = __fadd2_rn(make_float2(__uint_as_float(d_[ch][e]), __uint_as_float(d_[ch][e + 1])), dv);
-              const float2 ds = __fmul2_rn(pw[hh * 16 + ch * 8 + (e >> 1)], dpd);
+              float2 ds = __fmul2_rn(pw[hh * 16 + ch * 8 + (e >> 1)], dpd);
+              if (kPacked && CF::kCol && hh + ch + e == 0 && only_key(j0)) ds.x *= 0.f;
               kds[ch][e >> 1] = Pack<T>::pack(ds.x, ds.y);
             }
           // dS, in the column kind behind P, over the dP columns this thread has just read (the layout
@@ -693,7 +699,8 @@ __device__ __forceinline__ void fb_kernel<KIND, D, T, SPLIT, DUAL, Geo>::run(con
               float2 dv = nDv;
               if constexpr (CF::kCol) dv = *reinterpret_cast<const float2*>(cs + 64 + cc);
               const float2 dpd = __fadd2_rn(make_float2(__uint_as_float(d_[ch][e]), __uint_as_float(d_[ch][e + 1])), dv);
-              const float2 ds = __fmul2_rn(p_[ch * 8 + (e >> 1)], dpd);
+              float2 ds = __fmul2_rn(p_[ch * 8 + (e >> 1)], dpd);
+              if (kPacked && CF::kCol && ch + e == 0 && half == 0 && only_key(j0)) ds.x *= 0.f;
               kds[ch][e >> 1] = Pack<T>::pack(ds.x, ds.y);
             }
           // over the dP columns this thread has read: [P^T (column kind) | dS]
@@ -732,6 +739,7 @@ __device__ __forceinline__ void fb_kernel<KIND, D, T, SPLIT, DUAL, Geo>::run(con
         float mul = 1.f;
         if constexpr (KIND == FB_BWD_ROW) mul = g.scale;
         else mul = (o == 0) ? 1.f : g.scale;
+        if (kPacked && (CF::kCol ? o == 1 && g.window == 1 : vspan == 1)) mul = 0.f;
         const uint32_t tile = staging + (uint32_t)o * kAtoms * kAtomBytesStat;
         uint32_t v[kChunks][16];
 #pragma unroll

@@ -428,6 +428,32 @@ def test_refused_calls_on_the_device(packed):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16, torch.float32])
+@pytest.mark.parametrize("H, Hkv, D", [(6, 2, 64), (4, 4, 128), (5, 1, 80)])
+def test_one_visible_key_takes_no_gradient_of_scores(packed, dtype, H, Hkv, D):
+    # P = 1 whatever the score is: dq and dk are 0, not nearly
+    for lens, window in (([1], None), ([1, 1, 0, 1], None), ([70, 1, 200], 1)):
+        cu = offsets(lens)
+        q, k, v, do = tensors(cu[-1] + 2, H, Hkv, D, dtype)
+        plan = packed.packed_plan(torch.tensor(cu, dtype=torch.int32, device="cuda"), cu[-1] + 2)
+        o, dq, dk, dv = both_passes(packed, q, k, v, do, plan, window)
+        assert not bool(dq.any()) and not bool(dk.any()) and bool(dv[:cu[-1]].flatten(1).any(1).all())
+        assert torch.equal(o[:cu[-1]], v[:cu[-1]].repeat_interleave(H // Hkv, 1))
+    # the first row of a sequence, beside rows that see more; a score that is not a number stays one
+    cu = [0, 130, 137, 400]
+    q, k, v, do = tensors(400, H, Hkv, D, dtype)
+    plan = packed.packed_plan(torch.tensor(cu, dtype=torch.int32, device="cuda"), 400)
+    dq = both_passes(packed, q, k, v, do, plan, None)[1]
+    assert (dq == 0).flatten(1).all(1).nonzero().flatten().tolist() == cu[:-1]
+    do[:] = 0
+    do[130] = 1
+    assert not any(bool(t.any()) for t in both_passes(packed, q, k, v, do, plan, None)[1:3])
+    q[130, 0, 3] = math.nan
+    o, dq, dk, dv = both_passes(packed, q, k, v, do, plan, None)
+    assert bool(o[130, 0].isnan().all()) and bool(dq[130, 0].isnan().all()) and bool(dk[130, 0].isnan().any())
+
+
+@pytest.mark.gpu
 def test_captured_plan_and_passes(packed):
     n, H, Hkv, D = 700, 4, 2, 64
     q, k, v, do = tensors(n, H, Hkv, D, torch.bfloat16)
