@@ -49,6 +49,7 @@ PackedGeometry make_geometry(const attn_packed_shape_t* s, const int32_t* plan) 
   g.pair_cap = (int)plan_pairs(s->n_tok, s->n_seq);
   g.q_heads = s->q_heads;
   g.kv_heads = s->kv_heads;
+  g.n_seq = s->n_seq;
   g.group = s->q_heads / s->kv_heads;
   return g;
 }

@@ -40,7 +40,7 @@ struct PackedGeometry : Geometry {
   const PackedTile* pair_tiles;
   int cap, pair_cap;        // entries of either list, and of that of the pairs
   int group;                // query heads per key/value head
-  int q_heads, kv_heads;
+  int q_heads, kv_heads, n_seq;
 };
 
 // what the kernels that serve both kinds of geometry ask for; a plain one has its heads on both sides alike

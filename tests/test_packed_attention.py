@@ -454,6 +454,39 @@ def test_one_visible_key_takes_no_gradient_of_scores(packed, dtype, H, Hkv, D):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("H, Hkv, D", [(6, 2, 32), (4, 4, 128), (5, 1, 80)])
+@pytest.mark.parametrize("window", [None, 3])
+def test_gradients_of_sequences_of_few_rows(packed, dtype, H, Hkv, D, window):
+    # D without the rounding of O: what is left is dS and the result, rounded once each (u = half a step), and P, dP and D in float, relatively
+    # within 2^-16 for D + 8 terms of scores below 16.  In fp16 dS is also off by half of its smallest step, 2^-25
+    lens = [7, 2, 0, 8, 5, 1, 3, 4, 6]
+    cu, u, s = offsets(lens, 2), torch.finfo(dtype).eps / 2, 1 / math.sqrt(D)
+    q, k, v, do = tensors(cu[-1] + 3, H, Hkv, D, dtype, seed=2, amp=1.4)
+    plan = packed.packed_plan(torch.tensor(cu, dtype=torch.int32, device="cuda"), cu[-1] + 3)
+    got = both_passes(packed, q, k, v, do, plan, window)[1:3]
+    eta = torch.finfo(dtype).smallest_normal * torch.finfo(dtype).eps
+    want, err = [torch.zeros_like(t, dtype=torch.float64) for t in (q, k)], [torch.zeros_like(t, dtype=torch.float64) for t in (q, k)]
+    for a, b in zip(cu[:-1], cu[1:]):
+        i = torch.arange(b - a, device="cuda")
+        seen = (i[None] <= i[:, None]) & (i[:, None] < i[None] + (window or b - a))
+        for h in range(H if b > a else 0):
+            qh, kh, vh, gh = (t[a:b, x].double() for t, x in ((q, h), (k, h * Hkv // H), (v, h * Hkv // H), (do, h)))
+            P = torch.softmax((qh @ kh.T * s).masked_fill(~seen, -math.inf), -1)
+            dP = gh @ vh.T
+            dS = P * (dP - (P * dP).sum(-1, keepdim=True))
+            size = P * (gh.abs() @ vh.abs().T + (P * (gh.abs() @ vh.abs().T)).sum(-1, keepdim=True))
+            eS = (u * dS.abs() + 2.0 ** -16 * size) * 1.01 + eta * seen
+            want[0][a:b, h] = dS @ kh * s
+            want[1][a:b, h * Hkv // H] += dS.T @ qh * s
+            err[0][a:b, h] = eS @ kh.abs() * s
+            err[1][a:b, h * Hkv // H] += eS.T @ qh.abs() * s
+    for x, w, e in zip(got, want, err):
+        worst = ((x.double() - w).abs() / (e + 1.01 * u * w.abs() + eta)).max()
+        assert bool(worst <= 1), float(worst)
+
+
+@pytest.mark.gpu
 def test_captured_plan_and_passes(packed):
     n, H, Hkv, D = 700, 4, 2, 64
     q, k, v, do = tensors(n, H, Hkv, D, torch.bfloat16)
