@@ -29,7 +29,7 @@ NVCC_FLAGS = ["-gencode", "arch=compute_100a,code=sm_100a", "-lineinfo", "-O3", 
 CU_SOURCES = ["attn_capi.cu", "attn_prep.cu", "attn_simt.cu", "attn_tc.cu", "attn_tc_fb.cu", "attn_tc_fwd.cu", "attn_tc_hvp_row.cu", "attn_tc_hvp_col.cu",
               "packed_capi.cu", "packed_plan.cu", "packed_rope.cu", "packed_fwd.cu", "lce_capi.cu", "lce_tc.cu", "lce_rows.cu", "lce_simt.cu"]
 EXT_SOURCES = ["attention_ext.cpp", "packed_ext.cpp", "loss_ext.cpp"]
-HEADERS = ["attn_common.cuh", "attn_launch.h", "capi_common.h", "packed_geometry.cuh", "packed_launch.h", "lce_launch.h", "simt_split.h", "tc_primitives.cuh", "tc_common.cuh", os.path.join(INCLUDE, "attn_b200.h")]
+HEADERS = ["attn_common.cuh", "attn_launch.h", "capi_common.h", "packed_geometry.cuh", "packed_launch.h", "packed_order.h", "lce_launch.h", "simt_split.h", "tc_primitives.cuh", "tc_common.cuh", os.path.join(INCLUDE, "attn_b200.h")]
 
 
 def _nvcc() -> str:

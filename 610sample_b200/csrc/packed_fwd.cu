@@ -14,7 +14,7 @@
 // D <= 64: there is room for P beside S, so the next scores come as soon as these are in registers; a warp for either row tile issues
 // its products.  What counts then is to keep the special-function unit busy (8 clocks for a warp's exponentials: 2 048 for 256 x 128 scores),
 // which one warp of a tile on each scheduler does to 60 % and two do better: two threads a row, half of the columns each, which agree on
-// the row's reference through shared memory.
+// the row's reference through shared memory.  The order of the issuing warps is in packed_order.h.
 //
 // One sequence of 8192, 16 heads, causal: D = 128 (4 key heads) 242 us, 1 136 TFLOP/s, 69 % of the measured peak (single tiles 252); D = 64 178 us,
 // 771 TFLOP/s, the special-function unit 70 % busy (201).  Tried on the way, beside 231 and 196 us of another board with one thread a row and one
@@ -22,6 +22,7 @@
 // then exponentiate, at the same time); exponentials strictly in turn 241 and 211; a quarter or half of them by polynomial on the FMA pipe no
 // faster and 257 and 224; 208 registers a thread 239 and 201; two threads a row 247 and 186.
 #include "packed_launch.h"
+#include "packed_order.h"
 #include "tc_common.cuh"
 
 namespace attn {
@@ -96,16 +97,14 @@ packed_fwd_kernel(const __grid_constant__ TmaMaps maps, const PackedGeometry g, 
   if (r0 < 0 || r0 >= g.N_q) return;
   const int end = min(max(entry.z, r0 + 1), g.N_q), row_end = min(r0 + 256, end), begin = min(entry.y, r0);
   const int lo = begin < 0 ? r0 : max(begin, r0 - g.window + 1);
-  const int tiles = begin < 0 || g.window == 0 ? 0 : (row_end - lo + kKeys - 1) / kKeys;
-  if (tiles == 0) {      // rows of no sequence, or that see nothing
+  if (begin < 0 || g.window == 0) {      // rows of no sequence, or that see nothing
     store_packed_rows<true>(t.out_O, 0u, r0, row_end, head, g.q_heads, g.D, kThreads);
     if (threadIdx.x < 256 && r0 + (int)threadIdx.x < row_end) t.out_L[(size_t)head * g.N_q + r0 + threadIdx.x] = -INFINITY;
     return;
   }
-  // streamed tiles [from[x], to[x]) of row tile x; B may have no rows, and with a window its first keys come later
-  auto first_of = [&](int x) { return x == 0 ? 0 : (max(lo, r0 + 128 - g.window + 1) - lo) / kKeys; };
-  auto behind_of = [&](int x) { return x == 1 ? (row_end > r0 + 128 ? tiles : 0) : (min(r0 + 128, row_end) - lo + kKeys - 1) / kKeys; };
-  const int from_b = first_of(1), to_a = behind_of(0), to_b = behind_of(1);
+  // B may have no rows, and with a window its first keys come later
+  const ProductOrder order = pair_order(r0, row_end, lo, g.window, kKeys);
+  const int tiles = order.tiles;
 
   auto bar_slot_full = [&](int s) { return smem_u32(&ctl->slot_full[s]); };
   auto bar_slot_empty = [&](int s) { return smem_u32(&ctl->slot_empty[s]); };
@@ -139,7 +138,7 @@ packed_fwd_kernel(const __grid_constant__ TmaMaps maps, const PackedGeometry g, 
       tma_load_3d(ring + s * CF::kTileBytes + a * kAtomBytes, &maps.m[(i & 1) ? T_V : T_K], a * 64, lo + j * kKeys, kv_head, bar);
   };
   if (warp == kLoadWarp && lane == 0) {
-    const int q_tiles = to_b > 0 ? 2 : 1;
+    const int q_tiles = order.to(1) > 0 ? 2 : 1;
     mbar_arrive_expect_tx(bar_q, q_tiles * CF::kTileBytes);
     for (int x = 0; x < q_tiles; ++x)
 #pragma unroll
@@ -192,16 +191,8 @@ packed_fwd_kernel(const __grid_constant__ TmaMaps maps, const PackedGeometry g, 
       constexpr uint32_t idesc_s = make_idesc(128, kKeys, Pack<T>::kIsBf16, 0, 0);
       const uint32_t idesc_o = make_idesc(128, g.D, Pack<T>::kIsBf16, 0, 1);
       auto step = [](int ks) { return (uint64_t)(((ks >> 2) * kAtomBytes + (ks & 3) * 32) >> 4); };
-      auto from_of = [&](int x) { return x == 0 ? 0 : from_b; };
-      auto to_of = [&](int x) { return x == 0 ? to_a : to_b; };
-      auto on = [&](int x, int j) { return j >= from_of(x) && j < to_of(x); };
-      // item i of the ring; one that this warp has waited for is not asked for again (a satisfied wait takes some 90 clocks)
-      int known = -1;
-      auto arrived = [&](int i) {
-        if (i <= known) return true;
-        known = i;
-        return wait(bar_slot_full(i % kSlots), (i / kSlots) & 1, 3);
-      };
+      Arrivals known;
+      auto arrived = [&](int i) { return known(i, [&](int n) { return wait(bar_slot_full(n % kSlots), (n / kSlots) & 1, 3); }); };
       // an item that a row tile does not use: its slot is given back all the same
       auto skip = [&](int i) {
         const bool here = arrived(i);
@@ -225,7 +216,7 @@ packed_fwd_kernel(const __grid_constant__ TmaMaps maps, const PackedGeometry g, 
         return true;
       };
       auto outputs = [&](int x, int j, bool release) {
-        if (!arrived(2 * j + 1) || !wait(smem_u32(&ctl->p_full[x]), (j - from_of(x)) & 1, 5 + x)) return false;
+        if (!arrived(2 * j + 1) || !wait(smem_u32(&ctl->p_full[x]), (j - order.from(x)) & 1, 5 + x)) return false;
         tc_fence_after_sync();
         const int s = (2 * j + 1) % kSlots;
         const uint64_t dv = smem_desc_sw128(ring + s * CF::kTileBytes, kAtomBytes, 1024);
@@ -233,45 +224,27 @@ packed_fwd_kernel(const __grid_constant__ TmaMaps maps, const PackedGeometry g, 
         if (elect_one()) {
 #pragma unroll
           for (int ks = 0; ks < kKeys / 16; ++ks)
-            mma_ts(o_tmem, p_tmem + 8 * ks, dv + (uint64_t)((ks * 2048) >> 4), idesc_o, j > from_of(x) || ks > 0);
+            mma_ts(o_tmem, p_tmem + 8 * ks, dv + (uint64_t)((ks * 2048) >> 4), idesc_o, j > order.from(x) || ks > 0);
           if (CF::kOwnP) mma_commit(smem_u32(&ctl->pv_done[x]));
-          if (j + 1 == to_of(x)) mma_commit(smem_u32(&ctl->acc_done[x]));
+          if (j + 1 == order.to(x)) mma_commit(smem_u32(&ctl->acc_done[x]));
           if (release) mma_commit(bar_slot_empty(s));
         }
         __syncwarp();
         return true;
       };
-      bool ok = wait(bar_q, 0, 4);
+      if (!wait(bar_q, 0, 4)) return;
       if constexpr (CF::kOwnP) {
-        // a warp for either row tile: the next scores as soon as these are in registers
-        const int x = warp - kIssueWarp, from = from_of(x), to = to_of(x);
-        for (int i = 0; i < 2 * from && ok; ++i) ok = skip(i);
-        if (to > from && ok) ok = scores(x, from, true);
-        for (int j = from; j < to && ok; ++j) {
-          if (j + 1 < to) ok = wait(smem_u32(&ctl->s_free[x]), (j - from) & 1, 9) && scores(x, j + 1, true);
-          ok = ok && outputs(x, j, true);
-        }
-        for (int i = 2 * max(from, to); i < 2 * tiles && ok; ++i) ok = skip(i);
+        auto free = [&](int x, int j) { return wait(smem_u32(&ctl->s_free[x]), (j - order.from(x)) & 1, 9); };
+        issue_one_row_tile(order, warp - kIssueWarp, skip, free, scores, outputs);
       } else {
-        // one warp for both, so that one tile's products run while the other one's scores are exponentiated: P lies over the scores, and the
-        // next ones come right behind the product that reads it
-        if (ok && on(0, 0)) ok = scores(0, 0, !on(1, 0));
-        if (ok && on(1, 0)) ok = scores(1, 0, true);
-        for (int j = 0; j < tiles && ok; ++j) {      // every tile of the stream belongs to A, to B or to both
-          const bool next = j + 1 < tiles;
-          ok = arrived(2 * j + 1) && (!next || arrived(2 * j + 2));      // while P is still being made
-          if (ok && on(0, j)) ok = outputs(0, j, !on(1, j));
-          if (ok && next && on(0, j + 1)) ok = scores(0, j + 1, !on(1, j + 1));
-          if (ok && on(1, j)) ok = outputs(1, j, true);
-          if (ok && next && on(1, j + 1)) ok = scores(1, j + 1, true);
-        }
+        issue_both_row_tiles(order, arrived, scores, outputs);
       }
     });
   }
   } else {
     if constexpr (kThreads == 640) registers_up<104>();
     const int x = warp / CF::kTileWarps, half = kHalves == 2 ? (warp >> 2) & 1 : 0, quarter = warp & 3, row = quarter * 32 + lane, i = r0 + 128 * x + row;
-    const int from = x == 0 ? 0 : from_b, to = x == 0 ? to_a : to_b;
+    const int from = order.from(x), to = order.to(x);
     const uint32_t lane_addr = tmem_base + ((uint32_t)(quarter * 32) << 16);
     const uint32_t s_addr = lane_addr + 128 * x + kCols * half, o_addr = lane_addr + CF::kO + DT * x + DT / kHalves * half;
     const uint32_t p_addr = lane_addr + CF::kP + CF::kPStride * x + kCols / 2 * half;

@@ -5,6 +5,7 @@ import ctypes
 import importlib
 import math
 import os
+import subprocess
 import sys
 
 import pytest
@@ -685,3 +686,12 @@ def test_gradient_against_differences(packed):
             f.append((packed.packed_attention(*args, plan, 70).double() * do.double()).sum())
         slope, want = float((f[0] - f[1]) / (2 * h)), float((grads[i].double() * dirs[i].double()).sum())
         assert abs(slope - want) <= 5e-3 * float(grads[i].double().norm())
+
+
+def test_products_wait_for_their_items(tmp_path):
+    # the order of the paired forward's issuing warps, walked through on the CPU
+    here = os.path.dirname(os.path.abspath(__file__))
+    program = str(tmp_path / "packed_order")
+    subprocess.run(["g++", "-std=c++17", "-O1", "-Wall", "-Werror", "-I" + os.path.join(PKG_DIR, "csrc"), os.path.join(here, "host", "packed_order.cpp"), "-o", program], check=True)
+    done = subprocess.run([program], capture_output=True, text=True, timeout=120)
+    assert done.returncode == 0, done.stdout + done.stderr
