@@ -368,53 +368,99 @@ static cudaError_t launch_packed_rowdot(const Tensors& t, const PackedGeometry& 
   return launch_pdl(kern, (unsigned)ctas, 256, 0, s, (const T*)t.dO, (const T*)t.O, t.Dv, g.N_q, g.q_heads, g.D, st.row, st.head);
 }
 
-// The same for the first rows of every sequence, of at most kFirstRows keys: D_i = sum_j P_ij dP_ij.  A row of few keys is often nearly all on one,
-// where dP - D is a small difference; with D from the rounded O dq and dk of one sequence of 7 rows were 1.9 % from 64 bits in bf16.  Beside
-// many rows of many keys that is lost in the norm, so the rest is not worth a second product.  A CTA has a sequence and a head, a warp a row.
-// Bound by latency: 16384 rows in 19 sequences, 12 heads, forward and backward 462 us without it, 465 with it.
-constexpr int kFirstRows = 8;
+// The same for the rows that see at most kFewKeys keys, from P and dP: D_i = sum_j P_ij dP_ij.  A row of few keys is often nearly all on one,
+// where dP - D is a small difference, and D from the rounded O costs more than the rounding of dS.  These are the first rows of every sequence, and with a
+// window of no more than kFewKeys all rows (then nothing else gives D).  Eight or sixteen lanes own a row, 16 bytes each; a CTA has a head's first rows
+// of a sequence, or its rows of a tile of the plan.
+// bf16, 1024 rows, unit variance times 1.4 in q and k, dq off by (2-norm, the roundings emulated in 64 bits) with D from O / this, windows of 2, 4, 8, 9, 16,
+// 64, none: 5.8e-3, 4.5e-3, 3.8e-3, 3.8e-3, 3.5e-3, 3.0e-3, 2.8e-3 / 2.4e-3 throughout.  Backward, 16384 rows of 12 heads of 64 and 8192 of 32 and 8 of 128, in us: window 2
+// 133 and 250 (113 and 211 with D from O), 8 147 and 297 (117 and 214), 16 171 and 370 (117 and 214): every key costs all rows a step, so eight, where it matters most.
+constexpr int kFewKeys = 8;
 
-template <typename T>
-__global__ void __launch_bounds__(32 * kFirstRows)
-packed_first_rows_kernel(const PackedGeometry g, const Tensors t, const PackedLayout lay) {
+template <typename T, int G>
+__global__ void __launch_bounds__(256)
+packed_few_keys_kernel(const PackedGeometry g, const Tensors t, const PackedLayout lay) {
   pdl_wait();
   pdl_trigger();
-  const int seq = (int)(blockIdx.x / (unsigned)g.q_heads), h = (int)(blockIdx.x - (unsigned)seq * g.q_heads), lane = threadIdx.x & 31;
-  const int* plan = reinterpret_cast<const int*>(g.row_tiles) - kPlanHeader;
-  const int* ends = reinterpret_cast<const int*>(g.pair_tiles + g.pair_cap);
-  const int begin = from_l2(seq == 0 ? plan + 4 : ends + seq - 1), end = min(from_l2(ends + seq), g.N_q), i = begin + (int)(threadIdx.x >> 5);
-  if (begin < 0 || begin >= end || i >= end) return;
-  const bool in = lane * 4 < g.D;
-  auto load = [&](const void* p, int which, int row, int head, float (&v)[4]) {
-    v[0] = v[1] = v[2] = v[3] = 0.f;
-    if (!in) return;
-    const uint2 w = from_l2(reinterpret_cast<const uint2*>(static_cast<const T*>(p) + row * lay.of[which].row + head * lay.of[which].head + lane * 4));
-    const float2 a = widen_pair<T>(w.x), b = widen_pair<T>(w.y);
-    v[0] = a.x; v[1] = a.y; v[2] = b.x; v[3] = b.y;
-  };
-  float q[4], d[4], sum = 0.f;
-  load(t.Q, PI_Q, i, h, q);
-  load(t.dO, PI_dO, i, h, d);
-  const float L2 = from_l2(t.L + (size_t)h * g.N_q + i) * kLog2e;
-#pragma unroll 2
-  for (int j = max(begin, i - g.window + 1); j <= i; ++j) {
-    float k[4], v[4];
-    load(t.K, PI_K, j, h / g.group, k);
-    load(t.V, PI_V, j, h / g.group, v);
-    float s = 0.f, dp = 0.f;
-#pragma unroll
-    for (int e = 0; e < 4; ++e) { s = fmaf(q[e], k[e], s); dp = fmaf(d[e], v[e], dp); }
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) { s += __shfl_xor_sync(0xffffffffu, s, o); dp += __shfl_xor_sync(0xffffffffu, dp, o); }
-    sum = fmaf(ex2(fmaf(s, g.scale_log2e, -L2)), dp, sum);
+  constexpr int kRows = 256 / G;
+  const int unit = (int)(blockIdx.x / (unsigned)g.q_heads), h = (int)(blockIdx.x - (unsigned)unit * g.q_heads);
+  int begin, first, last;
+  if (g.window <= kFewKeys) {
+    PackedWork w;
+    if (!packed_work(g, false, unit, w) || w.lo == w.hi) return;
+    begin = w.begin; first = w.r0; last = w.row_end;
+  } else {
+    const int* plan = reinterpret_cast<const int*>(g.row_tiles) - kPlanHeader;
+    const int* ends = reinterpret_cast<const int*>(g.pair_tiles + g.pair_cap);
+    begin = first = from_l2(unit == 0 ? plan + 4 : ends + unit - 1);
+    last = min(from_l2(ends + unit), g.N_q);
+    if (begin < 0 || begin >= last) return;
+    last = min(last, begin + kFewKeys);
   }
-  if (lane == 0) t.Dv[(size_t)h * g.N_q + i] = sum;
+  __shared__ uint4 keys[2][kRows + kFewKeys][G];      // K and V of the rows that `kRows` queries see; each is used up to kFewKeys times
+  const int sub = threadIdx.x % G;
+  const bool on = sub * 8 < g.D;
+  auto load = [&](const void* p, int which, int row, int head) {
+    return from_l2(reinterpret_cast<const uint4*>(static_cast<const T*>(p) + row * lay.of[which].row + head * lay.of[which].head + sub * 8));
+  };
+  for (int r = first; r < last; r += kRows) {      // uniform over the CTA: barriers and shuffles need every thread
+    const int base = max(begin, r - kFewKeys + 1), group = (int)threadIdx.x / G, i = r + group;
+    const bool row = i < last;
+    const int lo = max(begin, i - g.window + 1);
+    uint4 q4 = make_uint4(0u, 0u, 0u, 0u), d4 = q4;
+    if (row && on) { q4 = load(t.Q, PI_Q, i, h); d4 = load(t.dO, PI_dO, i, h); }
+    const float L2 = row ? from_l2(t.L + (size_t)h * g.N_q + i) * kLog2e : 0.f;
+    __syncthreads();
+    for (int j = base + group; j < min(r + kRows, last); j += kRows)
+      if (on) {
+        keys[0][j - base][sub] = load(t.K, PI_K, j, h / g.group);
+        keys[1][j - base][sub] = load(t.V, PI_V, j, h / g.group);
+      }
+    __syncthreads();
+    const uint32_t q[4] = {q4.x, q4.y, q4.z, q4.w}, d[4] = {d4.x, d4.y, d4.z, d4.w};
+    float sum = 0.f;
+#pragma unroll 4
+    for (int n = 0; n < kFewKeys; ++n) {
+      const int j = lo + n;
+      if (!__any_sync(0xffffffffu, row && j <= i)) break;
+      float s = 0.f, dp = 0.f;
+      if (row && on && j <= i) {
+        const uint4 k4 = keys[0][j - base][sub], v4 = keys[1][j - base][sub];
+        const uint32_t k[4] = {k4.x, k4.y, k4.z, k4.w}, v[4] = {v4.x, v4.y, v4.z, v4.w};
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const float2 a = widen_pair<T>(q[e]), b = widen_pair<T>(k[e]), x = widen_pair<T>(d[e]), y = widen_pair<T>(v[e]);
+          s = fmaf(a.y, b.y, fmaf(a.x, b.x, s));
+          dp = fmaf(x.y, y.y, fmaf(x.x, y.x, dp));
+        }
+      }
+#pragma unroll
+      for (int o = G / 2; o > 0; o >>= 1) { s += __shfl_xor_sync(0xffffffffu, s, o); dp += __shfl_xor_sync(0xffffffffu, dp, o); }
+      if (j <= i) sum = fmaf(ex2(fmaf(s, g.scale_log2e, -L2)), dp, sum);
+    }
+    if (row && sub == 0) t.Dv[(size_t)h * g.N_q + i] = sum;
+  }
 }
 
 template <typename T>
-static cudaError_t launch_packed_first_rows(const Tensors& t, const PackedGeometry& g, const PackedLayout& lay, cudaStream_t s) {
-  const long long ctas = (long long)g.n_seq * g.q_heads;      // no more than the tiles of the batch
-  return ctas == 0 ? cudaSuccess : launch_pdl(packed_first_rows_kernel<T>, (unsigned)ctas, 32u * kFirstRows, 0, s, g, t, lay);
+static cudaError_t launch_packed_few_keys(const Tensors& t, const PackedGeometry& g, const PackedLayout& lay, cudaStream_t s) {
+  const long long ctas = (long long)(g.window <= kFewKeys ? g.cap : g.n_seq) * g.q_heads;      // no more than the tiles of the batch
+  auto kern = g.D <= 64 ? packed_few_keys_kernel<T, 8> : packed_few_keys_kernel<T, 16>;
+  return launch_pdl(kern, (unsigned)ctas, 256u, 0, s, g, t, lay);
+}
+
+template <typename T>
+static cudaError_t launch_packed_dots(const Tensors& t, const PackedGeometry& g, const PackedLayout& lay, cudaStream_t s, int* launches) {
+  *launches = 0;
+  cudaError_t e = cudaSuccess;
+  if (g.window > kFewKeys) {
+    e = launch_packed_rowdot<T>(t, g, lay.of[PI_dO], s);
+    ++*launches;
+    if (g.n_seq == 0) return e;
+  }
+  if (e == cudaSuccess) e = launch_packed_few_keys<T>(t, g, lay, s);
+  ++*launches;
+  return e;
 }
 
 }  // namespace tc
@@ -460,9 +506,7 @@ cudaError_t launch_packed_tc(int op, int dtype, const PackedGeometry& g, const T
     *launches = 1;
     return pairs ? launch_packed_fwd_pairs(bf, maps, g, t, s) : launch_packed_fwd(bf, maps, g, t, s);
   }
-  *launches = g.n_seq > 0 ? 2 : 1;
-  cudaError_t e = bf ? launch_packed_rowdot<__nv_bfloat16>(t, g, lay.of[PI_dO], s) : launch_packed_rowdot<__half>(t, g, lay.of[PI_dO], s);
-  if (e == cudaSuccess) e = bf ? launch_packed_first_rows<__nv_bfloat16>(t, g, lay, s) : launch_packed_first_rows<__half>(t, g, lay, s);
+  const cudaError_t e = bf ? launch_packed_dots<__nv_bfloat16>(t, g, lay, s, launches) : launch_packed_dots<__half>(t, g, lay, s, launches);
   return e != cudaSuccess ? e : launch_packed_bwd(bf, maps, g, t, s, launches);
 }
 

@@ -695,3 +695,30 @@ def test_products_wait_for_their_items(tmp_path):
     subprocess.run(["g++", "-std=c++17", "-O1", "-Wall", "-Werror", "-I" + os.path.join(PKG_DIR, "csrc"), os.path.join(here, "host", "packed_order.cpp"), "-o", program], check=True)
     done = subprocess.run([program], capture_output=True, text=True, timeout=120)
     assert done.returncode == 0, done.stdout + done.stderr
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("H, Hkv, D", [(6, 2, 32), (4, 4, 128), (5, 1, 80), (2, 1, 64)])
+@pytest.mark.parametrize("window", [2, 3, 5, 7, 8])
+def test_gradients_under_narrow_windows(packed, dtype, H, Hkv, D, window):
+    # every row sees few keys, whichever place it has in its sequence: the bound of test_gradients_of_sequences_of_few_rows, D without the rounding of O
+    lens = [300, 5, 0, 128, 129, 16, 1, 17]
+    cu, u, s, f = offsets(lens, 3), torch.finfo(dtype).eps / 2, 1 / math.sqrt(D), 2.0 ** -16
+    n = cu[-1] + 40
+    q, k, v, do = tensors(n, H, Hkv, D, dtype, seed=4, amp=1.4)
+    plan = packed.packed_plan(torch.tensor(cu, dtype=torch.int32, device="cuda"), n)
+    got = both_passes(packed, q, k, v, do, plan, window)[1:3]
+    eta = torch.finfo(dtype).smallest_normal * torch.finfo(dtype).eps
+    at = torch.arange(n, device="cuda")
+    seq = torch.bucketize(at, torch.tensor(cu, device="cuda"), right=True)
+    seen = (seq[None] == seq[:, None]) & (at[None] <= at[:, None]) & (at[:, None] < at[None] + window) & (at >= cu[0]) & (at < cu[-1])
+    q, k, v, do = (t.double().transpose(0, 1) for t in (q, k.repeat_interleave(H // Hkv, 1), v.repeat_interleave(H // Hkv, 1), do))
+    P = torch.softmax((q @ k.transpose(1, 2) * s).masked_fill(~seen, -math.inf), -1).nan_to_num(0.0)
+    dP, size = do @ v.transpose(1, 2), do.abs() @ v.abs().transpose(1, 2)
+    dS = P * (dP - (P * dP).sum(-1, keepdim=True))
+    eS = (u * dS.abs() + f * P * (size + (P * size).sum(-1, keepdim=True))) * 1.01 + eta * seen
+    group = lambda t: t.view(Hkv, H // Hkv, n, D).sum(1)
+    for x, w, e in zip(got, (dS @ k * s, group(dS.transpose(1, 2) @ q * s)), (eS @ k.abs() * s, group(eS.transpose(1, 2) @ q.abs() * s))):
+        worst = ((x.double().transpose(0, 1) - w).abs() / (e + 1.01 * u * w.abs() + eta)).max()
+        assert bool(worst <= 1), float(worst)
