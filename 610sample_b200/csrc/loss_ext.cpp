@@ -1,6 +1,8 @@
 // Module `attention_cuda`: cross entropy of a linear layer without kept logits, twice differentiable.
 #include "ext_common.h"
 
+#include <ATen/Context.h>
+
 namespace ext {
 
 namespace {
@@ -83,7 +85,16 @@ variable_list loss_double_backward(const torch::Tensor& u_in, const torch::Tenso
   c = torch::where(counted, c.expand({n}), torch::zeros({}, c.options()));
   torch::Tensor gx = torch::zeros_like(x), gw = torch::zeros(w.sizes(), w.options().dtype(at::kFloat)), gc = torch::zeros({n}, c.options());
   const bool half = x.scalar_type() != at::kFloat;
-  auto mm = [&](const torch::Tensor& p, const torch::Tensor& q) { return half ? at::mm(p, q, at::kFloat) : at::mm(p, q); };
+  // Whatever the process allows its own products: TF32 operands would leave P = exp(z - lse), of logits in full float, without a sum of 1, and half
+  // products that may be summed in fp16 have no float result.  The guard speaks for cuBLAS alone; where cuBLASLt is preferred, float goes through double.
+  const at::NoTF32Guard full_float;
+  auto& context = at::globalContext();
+  const at::ScalarType wide = !half ? at::kDouble : at::kFloat;
+  const bool widen = half ? x.scalar_type() == at::kHalf && context.allowFP16AccumulationCuBLAS() : context.blasPreferredBackend() != at::BlasBackend::Cublas;
+  auto mm = [&](const torch::Tensor& p, const torch::Tensor& q) {
+    if (widen) return at::mm(p.to(wide), q.to(wide)).to(at::kFloat);
+    return half ? at::mm(p, q, at::kFloat) : at::mm(p, q);
+  };
   auto unit = [&](const torch::Tensor& t, float largest) {
     const torch::Tensor top = t.numel() > 0 ? t.abs().amax() : torch::zeros({}, t.options());
     return torch::where((top > 0) & (top < std::numeric_limits<float>::infinity()), largest / top, torch::ones({}, top.options()));

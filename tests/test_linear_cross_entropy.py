@@ -437,3 +437,37 @@ def test_meta_step_of_the_benchmark(lce):
     assert abs(grads[0][0] - grads[1][0]) < 0.02
     for n, g in grads[0][1].items():
         assert torch.allclose(grads[1][1][n], g, atol=5e-2 * max(1.0, float(g.abs().max())), rtol=5e-2), n
+
+
+def second_of(lce, x, w, y, g, u, v, reduction):
+    """((d/dg, d/dx, d/dw) of <first gradients, (u, v)>, the same in 64 bits)"""
+    leaves = [t.detach().requires_grad_(True) for t in (x, w, g)]
+    first = torch.autograd.grad(lce(leaves[0], leaves[1], y, reduction=reduction), leaves[:2], leaves[2], create_graph=True)
+    got = torch.autograd.grad(first, leaves, (u, v))
+    d = [t.detach().double().requires_grad_(True) for t in leaves]
+    f64 = torch.autograd.grad(torch.nn.functional.cross_entropy(d[0] @ d[1].T, y, reduction=reduction), d[:2], d[2], create_graph=True)
+    return got, torch.autograd.grad(f64, d, (u.double(), v.double()))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype, tol", [(torch.float32, 2e-5), (torch.float16, 3e-3)])
+def test_second_derivative_under_the_callers_precision(lce, dtype, tol):
+    # the tolerances of test_second_derivative, whatever the process allows its own products
+    matmul = torch.backends.cuda.matmul
+    x, w, y, _ = inputs(300, 256, 700, dtype, ignored=0.2)
+    u, v, _, _ = inputs(300, 256, 700, dtype, seed=8)
+    g = torch.tensor(1.3, device="cuda")
+    before = torch.get_float32_matmul_precision(), matmul.allow_fp16_accumulation, matmul.allow_fp16_reduced_precision_reduction, torch.backends.cuda.preferred_blas_library()
+    try:
+        for precision in ("high", "medium"):
+            for library in ("cublas", "cublaslt"):
+                torch.set_float32_matmul_precision(precision)
+                torch.backends.cuda.preferred_blas_library(library)
+                matmul.allow_fp16_accumulation = matmul.allow_fp16_reduced_precision_reduction = True
+                for a, b in zip(*second_of(lce, x, w, y, g, u, v, "mean")):
+                    assert float((a.double() - b).norm() / b.norm()) <= tol, (precision, library)
+                assert torch.get_float32_matmul_precision() == precision and matmul.allow_fp16_accumulation      # left as they were
+    finally:
+        torch.set_float32_matmul_precision(before[0])
+        matmul.allow_fp16_accumulation, matmul.allow_fp16_reduced_precision_reduction = before[1:3]
+        torch.backends.cuda.preferred_blas_library(before[3])
