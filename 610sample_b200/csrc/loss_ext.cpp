@@ -87,6 +87,8 @@ variable_list loss_double_backward(const torch::Tensor& u_in, const torch::Tenso
   const bool half = x.scalar_type() != at::kFloat;
   // Whatever the process allows its own products: TF32 operands would leave P = exp(z - lse), of logits in full float, without a sum of 1, and half
   // products that may be summed in fp16 have no float result.  The guard speaks for cuBLAS alone; where cuBLASLt is preferred, float goes through double.
+  // Autocast would round the operands of float products.
+  const c10::impl::ExcludeDispatchKeyGuard as_they_are(c10::autocast_dispatch_keyset);
   const at::NoTF32Guard full_float;
   auto& context = at::globalContext();
   const at::ScalarType wide = !half ? at::kDouble : at::kFloat;

@@ -471,3 +471,15 @@ def test_second_derivative_under_the_callers_precision(lce, dtype, tol):
         torch.set_float32_matmul_precision(before[0])
         matmul.allow_fp16_accumulation, matmul.allow_fp16_reduced_precision_reduction = before[1:3]
         torch.backends.cuda.preferred_blas_library(before[3])
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype, tol", [(torch.float32, 2e-5), (torch.float16, 3e-3)])
+def test_second_derivative_under_autocast(lce, dtype, tol):
+    x, w, y, _ = inputs(300, 256, 700, dtype, ignored=0.2)
+    u, v, _, _ = inputs(300, 256, 700, dtype, seed=8)
+    with torch.autocast("cuda", torch.bfloat16):
+        got = second_of(lce, x, w, y, torch.tensor(1.3, device="cuda"), u, v, "mean")[0]
+    want = second_of(lce, x, w, y, torch.tensor(1.3, device="cuda"), u, v, "mean")[1]
+    for a, b in zip(got, want):
+        assert float((a.double() - b).norm() / b.norm()) <= tol
