@@ -251,7 +251,7 @@ qk_norm_rope_bwd_kernel(const T* x, const T* weight, const float* freqs, const T
   using PR = Pairs<T>;
   using P = typename PR::P;
   constexpr int kTok = kPrepThreads / G;
-  __shared__ float sums[kPrepThreads * 8];
+  __shared__ __align__(16) float sums[kPrepThreads * 8];
   tc::pdl_wait();
   tc::pdl_trigger();
   const unsigned head_blocks = (unsigned)(H + kPrepHeads - 1) / kPrepHeads;

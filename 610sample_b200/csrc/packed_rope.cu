@@ -243,7 +243,7 @@ template <typename T, int G, bool WIDE>
 __global__ void __launch_bounds__(kThreads, sizeof(T) == 2 ? 3 : 2)
 backward_kernel(const __grid_constant__ Args a, const int shares, float* partial) {      // partial: [2][CTAs][D], null where no weight's gradient is wanted
   constexpr int kTok = kThreads / G;
-  __shared__ float sums[kThreads * 8];
+  __shared__ __align__(16) float sums[kThreads * 8];
   tc::pdl_wait();
   tc::pdl_trigger();
   const int sub = threadIdx.x % G, col = sub * 8, n = min(8, a.D - col), batches = batches_of(a.side[0].heads, a.side[1].heads, kBackwardHeads);
