@@ -15,9 +15,10 @@ def sources():
 
 def test_shared_arrays_used_by_16_bytes_are_aligned():
     for name, text in sources().items():
-        for decl in re.findall(r"__shared__\s+([^;]*);", text):
-            if "__align__" in decl or re.match(r"(u?int4|float4|PackedTile)\b", decl):
-                continue
-            for array in re.findall(r"\b(\w+)\s*\[", decl):
-                wide = re.search(r"reinterpret_cast<(const )?(float4|uint4|int4)\s*\*>\(&?%s\b" % array, text)
-                assert wide is None, f"{name}: {array} is read or written by 16 bytes, and declared with less: {decl}"
+        for kernel in text.split("__global__"):
+            for decl in re.findall(r"__shared__\s+([^;]*);", kernel):
+                if "__align__" in decl or re.match(r"(u?int4|float4|PackedTile)\b", decl):
+                    continue
+                for array in re.findall(r"\b(\w+)\s*\[", decl):
+                    wide = re.search(r"reinterpret_cast<(const )?(float4|uint4|int4)\s*\*>\(&?%s\b" % array, kernel)
+                    assert wide is None, f"{name}: {array} is read or written by 16 bytes, and declared with less: {decl}"
