@@ -6,7 +6,7 @@
 //   DX     G [n, piece]           W [piece, d], read by columns    dx (float between pieces)
 //   DW     G [n, piece], by columns   x [n, d], by columns         dW rows of the piece
 //
-// A pair of CTAs (a cluster) owns a tile of 256 rows x up to 256 columns: either holds 128 rows of A and half of B's columns, one
+// A pair of CTAs (a cluster) owns a tile of 256 rows x 256 columns: either holds 128 rows of A and half of B's columns, one
 // tcgen05.mma.cta_group::2 reads both.  A single CTA's 128 x 256 tile would stream 96 bytes per clock from L2 and read 96 more from
 // shared memory for the product, above either's rate; the pair needs 64 of each.  A warp
 // loads through a ring of six stages of 64 in k, one (in rank 0) issues the products, eight finish a tile from tensor memory while
@@ -35,6 +35,7 @@ using namespace tc;
 enum Use { LSE = 0, GRAD = 1, DX = 2, DW = 3 };
 
 constexpr int kTileM = 256, kTileN = 256, kBlockK = 64;
+constexpr int kHalfN = kTileN / 2;                             // columns of B in one CTA, and of a result in one half of its epilogue
 constexpr int kStages = 6;
 constexpr uint32_t kOperandBytes = 128 * 128;                  // 128 rows (or columns) of 64 in k, of A or of B, in one CTA
 constexpr uint32_t kStageBytes = 2 * kOperandBytes;
@@ -56,7 +57,6 @@ struct GemmMaps { CUtensorMap a, b, out; };
 
 struct GemmArgs {
   int m_tiles, n_tiles, k_blocks;
-  int tile_n;                    // columns of a tile, a multiple of 32
   int rows, cols;                // of the result
   int m_fast;                    // tiles in sequence along the rows
   // LSE, GRAD
@@ -134,25 +134,23 @@ lce_gemm_kernel(const __grid_constant__ GemmMaps maps, const GemmArgs g) {
     if (g.m_fast) { nt = t / g.m_tiles; mt = t - nt * g.m_tiles; }
     else { mt = t / g.n_tiles; nt = t - mt * g.n_tiles; }
   };
-  const int half_n = g.tile_n >> 1;      // columns of B in this CTA
 
   if (warp == kLoadWarp) {
     if (lane == 0) {
-      const uint32_t stage_bytes = kOperandBytes + (kByColumns ? kOperandBytes : (uint32_t)half_n * 128u);
       bool ok = true;
       int it = 0;
       for (int item = pair; item < items && ok; item += pairs) {
         int t, mt, nt, first_block, blocks;
         item_at(item, t, first_block, blocks);
         tile_at(t, mt, nt);
-        const int m0 = mt * kTileM + (int)rank * 128, n0 = nt * g.tile_n + (int)rank * half_n;
+        const int m0 = mt * kTileM + (int)rank * 128, n0 = nt * kTileN + (int)rank * kHalfN;
         for (int kb = 0; kb < blocks; ++kb, ++it) {
           const int s = it % kStages;
           if (it >= kStages) {
             ok = mbar_wait(bar_empty(s), ((it / kStages) & 1) ^ 1, abort_flag, g.status, wait_code(KCODE, 1));
             if (!ok) break;
           }
-          if (rank == 0) mbar_arrive_expect_tx(bar_full(s), 2 * stage_bytes);
+          if (rank == 0) mbar_arrive_expect_tx(bar_full(s), 2 * kStageBytes);
           const uint32_t bar = map_rank(bar_full(s), 0), a = smem_base + s * kStageBytes, b = a + kOperandBytes;
           const int k0 = (first_block + kb) * kBlockK;
           if constexpr (USE == DW) {
@@ -177,7 +175,7 @@ lce_gemm_kernel(const __grid_constant__ GemmMaps maps, const GemmArgs g) {
     }
   } else if (warp == kIssueWarp) {
     if (rank == 0) {
-      const uint32_t idesc = make_idesc(kTileM, g.tile_n, Pack<T>::kIsBf16, USE == DW ? 1 : 0, kByColumns ? 1 : 0);
+      const uint32_t idesc = make_idesc(kTileM, kTileN, Pack<T>::kIsBf16, USE == DW ? 1 : 0, kByColumns ? 1 : 0);
       bool ok = true;
       int it = 0, i = 0;
       for (int item = pair; item < items && ok; item += pairs, ++i) {
@@ -223,15 +221,15 @@ lce_gemm_kernel(const __grid_constant__ GemmMaps maps, const GemmArgs g) {
       item_at(item, t, first_block, blocks);
       tile_at(t, mt, nt);
       const int buf = i & 1, r0 = mt * kTileM + (int)rank * 128, r = r0 + row;
-      const int col0 = nt * g.tile_n + half * half_n;      // this half's first column
-      const uint32_t acc = lane_addr + (uint32_t)buf * 256u + (uint32_t)(half * half_n);
+      const int col0 = nt * kTileN + half * kHalfN;      // this half's first column
+      const uint32_t acc = lane_addr + (uint32_t)buf * 256u + (uint32_t)(half * kHalfN);
       const bool in = r < g.rows;
       int target = -1;                                     // column of this row's target, counted from col0
       float lse2 = 0.f, coef = 0.f;
       if constexpr (USE == LSE || USE == GRAD) {
         if (in) {
           const int64_t y = from_l2(reinterpret_cast<const long long*>(g.targets) + r) - g.first_col - col0;
-          if (y >= 0 && y < half_n) target = (int)y;
+          if (y >= 0 && y < kHalfN) target = (int)y;
           if constexpr (USE == GRAD) { lse2 = from_l2(g.lse + r) * kLog2e; coef = from_l2(g.coef + r); }
         }
       }
@@ -247,8 +245,8 @@ lce_gemm_kernel(const __grid_constant__ GemmMaps maps, const GemmArgs g) {
 
       if constexpr (USE == LSE) {
         float m = -INFINITY, l = 0.f;
-        const int left = g.cols - col0;                    // valid columns of this half, where less than half_n
-        for (int c = 0; c < half_n; c += 16) {
+        const int left = g.cols - col0;                    // valid columns of this half, where less than kHalfN
+        for (int c = 0; c < kHalfN; c += 16) {
           uint32_t v[16];
           tmem_ld16(acc + c, v);
           tmem_ld_wait(v);
@@ -445,7 +443,7 @@ size_t tc_parts_bytes(long long rows, long long cols, long long k) {
 template <int USE>
 static cudaError_t launch_use(const GemmMaps& maps, GemmArgs g, int dtype, long long k, void* out, cudaStream_t stream, int* launches) {
   g.m_tiles = (g.rows + kTileM - 1) / kTileM;
-  g.n_tiles = (g.cols + g.tile_n - 1) / g.tile_n;
+  g.n_tiles = (g.cols + kTileN - 1) / kTileN;
   g.k_blocks = blocks_of(k);
   g.m_fast = g.rows < g.cols;      // A, of `rows` rows, is the smaller operand
   const long long tiles = (long long)g.m_tiles * g.n_tiles;
@@ -476,8 +474,7 @@ cudaError_t tc_scores(const Problem& p, const Scores& s, cudaStream_t stream, in
   GemmMaps maps;
   GemmArgs g = {};
   const bool bf = p.dtype == 1;
-  g.tile_n = kTileN;
-  if (!encode(&maps.a, p.x, bf, p.n, p.d, p.d, 128) || !encode(&maps.b, p.w, bf, p.V, p.d, p.d, g.tile_n / 2)) {
+  if (!encode(&maps.a, p.x, bf, p.n, p.d, p.d, 128) || !encode(&maps.b, p.w, bf, p.V, p.d, p.d, kHalfN)) {
     *err = kMapError;
     return cudaErrorInvalidValue;
   }
@@ -495,7 +492,6 @@ cudaError_t tc_piece_grad(const Problem& p, const Piece& piece, const float* lse
   GemmMaps maps;
   GemmArgs g = {};
   const bool bf = p.dtype == 1;
-  g.tile_n = kTileN;
   const void* w = static_cast<const uint16_t*>(p.w) + (size_t)piece.first * p.d;
   if (!encode(&maps.a, p.x, bf, p.n, p.d, p.d, 128) || !encode(&maps.b, w, bf, piece.cols, p.d, p.d, 128) ||
       !encode(&maps.out, G, bf, p.n, piece.cols, piece.ld, 128)) {
@@ -516,7 +512,6 @@ cudaError_t tc_piece_dx(const Problem& p, const Piece& piece, const Coefficients
   GemmMaps maps;
   GemmArgs g = {};
   const bool bf = p.dtype == 1;
-  g.tile_n = kTileN;
   const void* w = static_cast<const uint16_t*>(p.w) + (size_t)piece.first * p.d;
   if (!encode(&maps.a, G, bf, p.n, piece.cols, piece.ld, 128) || !encode(&maps.b, w, bf, piece.cols, p.d, p.d, 64) ||
       !encode(&maps.out, dx, bf, p.n, p.d, p.d, 128)) {
@@ -538,7 +533,6 @@ cudaError_t tc_piece_dw(const Problem& p, const Piece& piece, const Coefficients
   GemmMaps maps;
   GemmArgs g = {};
   const bool bf = p.dtype == 1;
-  g.tile_n = kTileN;
   void* out = static_cast<uint16_t*>(dw) + (size_t)piece.first * p.d;
   if (!encode(&maps.a, G, bf, p.n, piece.cols, piece.ld, 64) || !encode(&maps.b, x, bf, p.n, p.d, p.d, 64) ||
       !encode(&maps.out, out, bf, piece.cols, p.d, p.d, 128)) {

@@ -567,13 +567,6 @@ __device__ __forceinline__ float max3(float a, float b, float c) {
   return m;
 }
 
-// not a number where any of the three is not
-__device__ __forceinline__ float max3_nan(float a, float b, float c) {
-  float m;
-  asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(m) : "f"(a), "f"(b), "f"(c));
-  return m;
-}
-
 // Scores of one row that are not visible, as zeros: element i is number `first` + i of the row's visible range [0, span).  A pass
 // of its own for the tiles that have such elements: within the loop of the exponentials its three instructions for an
 // element are executed in every tile.

@@ -1,4 +1,5 @@
-"""What the kernels' sources promise beyond what a compiler checks: alignment of shared arrays that are used 16 bytes at a time."""
+"""What the kernels' sources promise beyond what a compiler checks: alignment of shared arrays that are used 16 bytes at a time, and no
+helper without a caller."""
 import os
 import re
 
@@ -22,3 +23,13 @@ def test_shared_arrays_used_by_16_bytes_are_aligned():
                 for array in re.findall(r"\b(\w+)\s*\[", decl):
                     wide = re.search(r"reinterpret_cast<(const )?(float4|uint4|int4)\s*\*>\(&?%s\b" % array, kernel)
                     assert wide is None, f"{name}: {array} is read or written by 16 bytes, and declared with less: {decl}"
+
+
+def test_device_helpers_have_callers():
+    texts = sources()
+    everything = "\n".join(texts.values())
+    for name, text in texts.items():
+        for helper in re.findall(r"__device__ __forceinline__ [\w:<>, \t*&]*?\b(\w+)\(", text):
+            uses = len(re.findall(r"\b%s\b" % helper, everything))
+            definitions = len(re.findall(r"__device__ __forceinline__ [\w:<>, \t*&]*?\b%s(?:<\w+>)?\(" % helper, everything))
+            assert uses > definitions, f"{name}: {helper} has no caller"
