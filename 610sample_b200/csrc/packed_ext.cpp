@@ -5,6 +5,7 @@
 
 #include <ATen/cuda/CUDAGraphsUtils.cuh>
 
+#include <algorithm>
 #include <limits>
 
 namespace ext {
@@ -94,51 +95,90 @@ variable_list packed_backward(const torch::Tensor& dO_in, const torch::Tensor& q
   return {dQ, dK, dV};
 }
 
-// Second backward: the sequences as rows of a padded batch, through the double-backward kernels of flash_attention.  A
-// padded row has zeros everywhere and comes behind its sequence's rows, which do not see it, so it adds nothing.  The longest
-// sequence's length is read from the plan unless the caller has given it, which waits for the device.
+// The sequences that one call of the second backward takes, each padded to `width` rows.
+struct PaddedGroup { torch::Tensor starts, ends; int64_t width; };
+
+// So that no call has more than `most` padded rows (or one sequence).  With lengths from the host, if given, sequences of like lengths go together;
+// else every sequence counts as one of `width`.
+std::vector<PaddedGroup> padded_groups(const torch::Tensor& starts, const torch::Tensor& ends, const std::vector<int64_t>& lens, int64_t width, int64_t most) {
+  const int64_t n_seq = ends.size(0);
+  if (n_seq * width <= most) return {{starts, ends, width}};
+  std::vector<PaddedGroup> groups;
+  if (lens.empty()) {
+    const int64_t each = std::max<int64_t>(1, most / width);
+    for (int64_t i = 0; i < n_seq; i += each) groups.push_back({starts.slice(0, i, std::min(n_seq, i + each)), ends.slice(0, i, std::min(n_seq, i + each)), width});
+    return groups;
+  }
+  std::vector<int64_t> order;
+  for (int64_t i = 0; i < n_seq; ++i)
+    if (lens[i] > 0) order.push_back(i);
+  std::stable_sort(order.begin(), order.end(), [&](int64_t a, int64_t b) { return lens[a] > lens[b]; });
+  const torch::Tensor by_length = torch::tensor(order, torch::kLong).to(ends.device());
+  for (int64_t i = 0, e; i < (int64_t)order.size(); i = e) {
+    const int64_t longest = lens[order[i]];
+    for (e = i + 1; e < (int64_t)order.size() && 2 * lens[order[e]] >= longest && (e + 1 - i) * longest <= most; ++e) { }
+    const torch::Tensor which = by_length.slice(0, i, e);
+    groups.push_back({starts.index_select(0, which), ends.index_select(0, which), longest});
+  }
+  return groups;
+}
+
+// Second backward: the sequences as rows of padded batches, through the double-backward kernels of flash_attention.  A
+// padded row has zeros everywhere and comes behind its sequence's rows, which do not see it, so it adds nothing.  The lengths are
+// read from the plan unless the caller has given the longest one, which waits for the device.
 variable_list packed_double_backward(const torch::Tensor& g_dq, const torch::Tensor& g_dk, const torch::Tensor& g_dv, const torch::Tensor& dO,
                                      const torch::Tensor& q, const torch::Tensor& k, const torch::Tensor& v, const torch::Tensor& O,
                                      const torch::Tensor& L, const torch::Tensor& plan, int64_t n_seq, int64_t window, int64_t max_seqlen) {
   at::AutoGradMode off(false);
   c10::cuda::CUDAGuard guard(q.device());
   const int64_t n_tok = q.size(0), Hq = q.size(1), Hkv = k.size(1), group = Hq / Hkv;
-  variable_list zero{torch::zeros_like(q), torch::zeros_like(q), torch::zeros_like(k), torch::zeros_like(v)};
-  if (n_tok == 0 || n_seq == 0) return zero;
+  // a row more than the result's, where every padded row goes
+  auto fresh_zeros = [&](const torch::Tensor& like) { return torch::zeros({n_tok + 1, like.size(1), like.size(2)}, like.options()); };
+  const variable_list out{fresh_zeros(q), fresh_zeros(q), fresh_zeros(k), fresh_zeros(v)};
+  auto results = [&]() {
+    variable_list r;
+    for (const torch::Tensor& t : out) r.push_back(t.slice(0, 0, n_tok));
+    return r;
+  };
+  if (n_tok == 0 || n_seq == 0 || max_seqlen == 0) return results();
+  const torch::Tensor ends = plan.slice(0, plan.numel() - 2 * n_seq, plan.numel() - n_seq).to(at::kLong);
+  const torch::Tensor starts = torch::cat({plan.slice(0, 4, 5).to(at::kLong), ends.slice(0, 0, n_seq - 1)});
+  std::vector<int64_t> lens;
+  int64_t longest = max_seqlen;
   if (max_seqlen < 0) {
     TORCH_CHECK(at::cuda::currentStreamCaptureStatusMayInitCtx() == at::cuda::CaptureStatus::None,
                 "the second derivative of packed_attention needs packed_plan(..., max_seqlen=...) while a graph is being captured");
-    max_seqlen = plan[1].item<int32_t>();
+    const torch::Tensor host = (ends - starts).cpu();
+    lens.assign(host.data_ptr<int64_t>(), host.data_ptr<int64_t>() + n_seq);
+    longest = *std::max_element(lens.begin(), lens.end());
+    if (longest == 0) return results();
   }
-  const int64_t width = std::min(max_seqlen, n_tok);
-  if (width == 0) return zero;
-  const torch::Tensor ends = plan.slice(0, plan.numel() - 2 * n_seq, plan.numel() - n_seq).to(at::kLong);
-  const torch::Tensor starts = torch::cat({plan.slice(0, 4, 5).to(at::kLong), ends.slice(0, 0, n_seq - 1)});
-  const torch::Tensor at = starts.unsqueeze(1) + torch::arange(width, ends.options()).unsqueeze(0);      // [n_seq, width]
-  const torch::Tensor in = at < ends.unsqueeze(1);
-  const torch::Tensor from = torch::where(in, at, torch::zeros_like(at)).reshape({-1});
-  const torch::Tensor in4 = in.view({n_seq, width, 1, 1});
-  // [n_tok, H, D] -> [n_seq, Hq, width, D]
-  auto pad = [&](const torch::Tensor& t) {
-    torch::Tensor p = t.index_select(0, from).view({n_seq, width, t.size(1), t.size(2)});
-    p = torch::where(in4, p, torch::zeros({}, p.options())).permute({0, 2, 1, 3});
-    return t.size(1) == Hq ? p.contiguous() : p.unsqueeze(2).expand({n_seq, Hkv, group, width, t.size(2)}).reshape({n_seq, Hq, width, t.size(2)});
-  };
-  const torch::Tensor Lp = torch::where(in.view({n_seq, 1, width}), L.index_select(1, from).view({Hq, n_seq, width}).permute({1, 0, 2}),
-                                        torch::zeros({}, L.options())).contiguous();
-  const int seen = (int)std::min<int64_t>(window, std::numeric_limits<int32_t>::max());
-  const variable_list r = v7_double_backward_cuda(pad(g_dq), pad(g_dk), pad(g_dv), pad(dO), pad(q), pad(k), pad(v), pad(O), Lp, seen, 0, 0, 0);
-  // a row of no sequence is where every padded row goes, and gets zeros
-  const torch::Tensor to = torch::where(in, at, torch::full_like(at, n_tok)).reshape({-1});
-  auto unpad = [&](const torch::Tensor& t, const torch::Tensor& like) {
-    torch::Tensor p = t;
-    if (like.size(1) != Hq) p = p.view({n_seq, Hkv, group, width, like.size(2)}).to(at::kFloat).sum(2).to(like.scalar_type());
-    p = p.permute({0, 2, 1, 3}).reshape({n_seq * width, like.size(1), like.size(2)});
-    torch::Tensor out = torch::zeros({n_tok + 1, like.size(1), like.size(2)}, like.options());
-    out.index_copy_(0, to, p);
-    return out.slice(0, 0, n_tok);
-  };
-  return {unpad(r[0], q), unpad(r[1], q), unpad(r[2], k), unpad(r[3], v)};
+  // at most twice the batch's rows in a call: memory goes with the batch, and a batch that is half padding is not cut
+  for (const PaddedGroup& part : padded_groups(starts, ends, lens, std::min(longest, n_tok), std::max<int64_t>(2 * n_tok, 4096))) {
+    const int64_t n = part.ends.size(0), width = part.width;
+    const torch::Tensor at = part.starts.unsqueeze(1) + torch::arange(width, ends.options()).unsqueeze(0);      // [n, width]
+    const torch::Tensor in = at < part.ends.unsqueeze(1);
+    const torch::Tensor from = torch::where(in, at, torch::zeros_like(at)).reshape({-1});
+    const torch::Tensor in4 = in.view({n, width, 1, 1});
+    // [n_tok, H, D] -> [n, Hq, width, D]
+    auto pad = [&](const torch::Tensor& t) {
+      torch::Tensor p = t.index_select(0, from).view({n, width, t.size(1), t.size(2)});
+      p = torch::where(in4, p, torch::zeros({}, p.options())).permute({0, 2, 1, 3});
+      return t.size(1) == Hq ? p.contiguous() : p.unsqueeze(2).expand({n, Hkv, group, width, t.size(2)}).reshape({n, Hq, width, t.size(2)});
+    };
+    const torch::Tensor Lp = torch::where(in.view({n, 1, width}), L.index_select(1, from).view({Hq, n, width}).permute({1, 0, 2}),
+                                          torch::zeros({}, L.options())).contiguous();
+    const int seen = (int)std::min<int64_t>(window, std::numeric_limits<int32_t>::max());
+    const variable_list r = v7_double_backward_cuda(pad(g_dq), pad(g_dk), pad(g_dv), pad(dO), pad(q), pad(k), pad(v), pad(O), Lp, seen, 0, 0, 0);
+    const torch::Tensor to = torch::where(in, at, torch::full_like(at, n_tok)).reshape({-1});
+    for (int i = 0; i < 4; ++i) {
+      torch::Tensor p = r[i];
+      const int64_t heads = out[i].size(1), D = out[i].size(2);
+      if (heads != Hq) p = p.view({n, Hkv, group, width, D}).to(at::kFloat).sum(2).to(out[i].scalar_type());
+      out[i].index_copy_(0, to, p.permute({0, 2, 1, 3}).reshape({n * width, heads, D}));
+    }
+  }
+  return results();
 }
 
 struct PackedAttentionBackward : public torch::autograd::Function<PackedAttentionBackward> {

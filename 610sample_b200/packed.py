@@ -6,8 +6,8 @@
 
 Attention is causal within each sequence, optionally within a sliding window, with grouped heads: `q` has a
 multiple of the heads of `k` and `v`, head h of `q` reading head h // (heads of q / heads of k).  It is
-differentiable to second order, as `flash_attention_v7`; the second derivative runs on rows padded to the
-longest sequence.  There is no counterpart in the reference, whose batches are dense [B, H, N, D]
+differentiable to second order, as `flash_attention_v7`; the second derivative runs on sequences of like lengths, padded to the
+longest of them, in memory that goes with the batch's rows.  There is no counterpart in the reference, whose batches are dense [B, H, N, D]
 (e2e/ttt_pytorch/model.py:174-191).  `packed_qk_norm_rope` is the step in front of it, as `qk_norm_rope` is
 for dense batches, with positions given per token.  There is no fallback: importing this module fails if the compiled
 extension `attention_cuda` is missing.
@@ -37,8 +37,8 @@ def packed_plan(cu_seqlens, n_tok, max_seqlen=None):
     on the device, by one launch on the current stream: nothing waits for the host, and a plan made inside a
     captured graph is made anew by each replay.  A later change of `cu_seqlens` does not change the plan.
     max_seqlen: length of the longest sequence, or an upper bound, if the caller knows it; only the second
-    derivative uses it, which else reads it from the device.  Sequences longer than a given one are not
-    covered by the second derivative."""
+    derivative uses it, which else reads the lengths from the device.  With it every sequence costs as much there as one of
+    that length.  Sequences longer than a given one are not covered by the second derivative."""
     if max_seqlen is not None and max_seqlen < 0:
         raise ValueError("max_seqlen must be >= 0")
     return PackedPlan(_attention_cuda.packed_plan(cu_seqlens, n_tok), n_tok, cu_seqlens.numel() - 1, max_seqlen)

@@ -722,3 +722,43 @@ def test_gradients_under_narrow_windows(packed, dtype, H, Hkv, D, window):
     for x, w, e in zip(got, (dS @ k * s, group(dS.transpose(1, 2) @ q * s)), (eS @ k.abs() * s, group(eS.transpose(1, 2) @ q.abs() * s))):
         worst = ((x.double().transpose(0, 1) - w).abs() / (e + 1.01 * u * w.abs() + eta)).max()
         assert bool(worst <= 1), float(worst)
+
+
+def second_derivatives(packed, leaves, cu, n, window, tangents, known):
+    plan = packed.packed_plan(torch.tensor(cu, dtype=torch.int32, device="cuda"), n, max_seqlen=known)
+    leaves = [t.detach().requires_grad_(True) for t in leaves]
+    first = torch.autograd.grad(packed.packed_attention(*leaves[:3], plan, window), leaves[:3], leaves[3], create_graph=True)
+    return torch.autograd.grad(first, leaves, tangents)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("known", [None, 700, 800])
+@pytest.mark.parametrize("dtype, tol", [(torch.float32, 2e-5), (torch.bfloat16, 3e-2)])
+@pytest.mark.parametrize("window", [None, 25])
+def test_second_derivative_of_unlike_lengths(packed, dtype, tol, known, window):
+    # a long sequence beside short and empty ones, several calls of the dense kernels: the tolerances of test_second_derivative
+    lens, H, Hkv, D = [3, 0, 11, 700, 1, 90, 0, 60, 200, 7, 7, 7], 4, 2, 32
+    cu = offsets(lens, 2)
+    n = cu[-1] + 3
+    leaves, g2 = tensors(n, H, Hkv, D, dtype), tensors(n, H, Hkv, D, dtype, seed=9)[:3]
+    got = second_derivatives(packed, leaves, cu, n, window, g2, known)
+    d = [t.double().cpu().requires_grad_(True) for t in leaves]
+    o = _math_attention(*d[:3], cu, window)
+    want = torch.autograd.grad(torch.autograd.grad(o, d[:3], d[3][2:cu[-1]], create_graph=True), d, [t.double().cpu() for t in g2])
+    for x, w in zip(got, want):
+        assert float((x.double().cpu() - w).norm() / w.norm()) <= tol
+        assert not bool(x[:2].any()) and not bool(x[cu[-1]:].any())
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("known", [None, 2048])
+def test_second_derivative_takes_memory_by_rows(packed, known):
+    # one document beside 600 short ones: no more than 40 tensors of twice the batch's rows, where rows padded to the longest one take 1.2 GB each
+    lens, H, D = [5] * 300 + [2048] + [11] * 300, 8, 64
+    cu = offsets(lens)
+    leaves, g2 = tensors(cu[-1], H, H, D, torch.bfloat16), tensors(cu[-1], H, H, D, torch.bfloat16, seed=9)[:3]
+    torch.cuda.synchronize()
+    torch.cuda.reset_peak_memory_stats()
+    before = torch.cuda.memory_allocated()
+    second_derivatives(packed, leaves, cu, cu[-1], None, g2, known)
+    assert torch.cuda.max_memory_allocated() - before <= 40 * 2 * leaves[0].numel() * 2
