@@ -178,6 +178,11 @@ variable_list packed_double_backward(const torch::Tensor& g_dq, const torch::Ten
       out[i].index_copy_(0, to, p.permute({0, 2, 1, 3}).reshape({n * width, heads, D}));
     }
   }
+  // a given length that is too small would leave rows out of the sums without a word
+  if (max_seqlen > 0 && max_seqlen < n_tok) {
+    const torch::Tensor longer = plan.select(0, 1) > max_seqlen;
+    for (torch::Tensor t : out) t.masked_fill_(longer, std::numeric_limits<double>::quiet_NaN());
+  }
   return results();
 }
 

@@ -38,7 +38,7 @@ def packed_plan(cu_seqlens, n_tok, max_seqlen=None):
     captured graph is made anew by each replay.  A later change of `cu_seqlens` does not change the plan.
     max_seqlen: length of the longest sequence, or an upper bound, if the caller knows it; only the second
     derivative uses it, which else reads the lengths from the device.  With it every sequence costs as much there as one of
-    that length.  Sequences longer than a given one are not covered by the second derivative."""
+    that length, and where one is longer all of the second derivative is NaN.  0 says that none is needed: it is 0."""
     if max_seqlen is not None and max_seqlen < 0:
         raise ValueError("max_seqlen must be >= 0")
     return PackedPlan(_attention_cuda.packed_plan(cu_seqlens, n_tok), n_tok, cu_seqlens.numel() - 1, max_seqlen)

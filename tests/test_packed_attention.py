@@ -762,3 +762,16 @@ def test_second_derivative_takes_memory_by_rows(packed, known):
     before = torch.cuda.memory_allocated()
     second_derivatives(packed, leaves, cu, cu[-1], None, g2, known)
     assert torch.cuda.max_memory_allocated() - before <= 40 * 2 * leaves[0].numel() * 2
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_second_derivative_of_a_longer_sequence_than_given_is_not_a_number(packed, dtype):
+    cu, n = [0, 40, 110, 111], 115
+    leaves, g2 = tensors(n, 4, 2, 32, dtype), tensors(n, 4, 2, 32, dtype, seed=9)[:3]
+    for known in (1, 40, 69):
+        assert all(bool(t.isnan().all()) for t in second_derivatives(packed, leaves, cu, n, None, g2, known))
+    want = second_derivatives(packed, leaves, cu, n, None, g2, None)
+    for known in (70, 114, 115, 2 ** 40):
+        for a, b in zip(second_derivatives(packed, leaves, cu, n, None, g2, known), want):
+            assert bool(a.isfinite().all()) and float((a.float() - b.float()).norm() / b.float().norm()) <= 4 * torch.finfo(dtype).eps
