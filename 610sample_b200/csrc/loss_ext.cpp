@@ -3,6 +3,8 @@
 
 #include <ATen/Context.h>
 
+#include <limits>
+
 namespace ext {
 
 namespace {
@@ -79,7 +81,8 @@ variable_list loss_double_backward(const torch::Tensor& u_in, const torch::Tenso
   at::AutoGradMode off(false);
   c10::cuda::CUDAGuard guard(x.device());
   const int64_t n = x.size(0), V = w.size(0);
-  const torch::Tensor counted = targets != a.ignore_index;
+  // a target that is no class: taken out of the sums, and not a number in the end
+  const torch::Tensor wrong = (targets != a.ignore_index) & ((targets < 0) | (targets >= V)), counted = (targets != a.ignore_index) & ~wrong;
   torch::Tensor c = g.to(at::kFloat);
   if (a.reduction == ATTN_REDUCE_MEAN) c = c / counted_rows;
   c = torch::where(counted, c.expand({n}), torch::zeros({}, c.options()));
@@ -127,6 +130,11 @@ variable_list loss_double_backward(const torch::Tensor& u_in, const torch::Tenso
     gw.add_(mm(Ht.t(), xs) / sh);
     if (us.defined()) gw.add_(mm(Gt.t(), us) / sg);
   }
+  // as in the first backward: the row's, and all that is summed over it
+  const double nan = std::numeric_limits<double>::quiet_NaN();
+  gx.masked_fill_(wrong.unsqueeze(1), nan);
+  gw.masked_fill_(wrong.any(), nan);
+  gc.masked_fill_(wrong, nan);
   torch::Tensor gg;
   if (a.reduction == ATTN_REDUCE_NONE) gg = gc;
   else if (a.reduction == ATTN_REDUCE_SUM) gg = gc.sum();

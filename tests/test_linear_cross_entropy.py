@@ -483,3 +483,18 @@ def test_second_derivative_under_autocast(lce, dtype, tol):
     want = second_of(lce, x, w, y, torch.tensor(1.3, device="cuda"), u, v, "mean")[1]
     for a, b in zip(got, want):
         assert float((a.double() - b).norm() / b.norm()) <= tol
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16, torch.float32])
+def test_no_such_class_is_not_a_number_in_the_second_derivative(lce, dtype):
+    # as the loss and the first gradients: the row's, and all that sums over it
+    for wrong in (50, -1, 1 << 40):
+        x, w, y, g = inputs(40, 32, 50, dtype, ignored=0.2)
+        y[3] = wrong
+        leaves = [t.detach().requires_grad_(True) for t in (x, w, g)]
+        first = torch.autograd.grad(lce(leaves[0], leaves[1], y, reduction="none"), leaves[:2], leaves[2], create_graph=True)
+        assert first[0].isnan().any(1).nonzero().flatten().tolist() == [3] and bool(first[1].isnan().any())
+        gx, gw, gg = torch.autograd.grad(first, leaves, [t.detach() for t in inputs(40, 32, 50, dtype, seed=8)[:2]])
+        assert gx.isnan().all(1).nonzero().flatten().tolist() == [3] and gg.isnan().nonzero().flatten().tolist() == [3] and bool(gw.isnan().all())
+        assert not bool(gx[y == -100].any()) and not bool(gg[y == -100].any())
