@@ -27,27 +27,32 @@ finish_kernel(const Partial* partial, const float* target_logit, const int64_t* 
   tc::pdl_wait();
   tc::pdl_trigger();
   const int x = threadIdx.x & 31, y = threadIdx.x >> 5, r = blockIdx.x * 32 + x;
-  float m = -INFINITY, l = 0.f;
+  float m = -INFINITY, part = 0.f;
   if (r < n)
 #pragma unroll 8
     for (int t = y; t < tiles; t += kRowGroups) {
       const float2 v = from_l2(reinterpret_cast<const float2*>(partial) + (size_t)t * n + r);
       const float m_new = fmaxf(m, v.x);
-      l = l * (m == m_new ? 1.f : exp2f(m - m_new)) + v.y * (v.x == m_new ? 1.f : exp2f(v.x - m_new));
+      part = part * (m == m_new ? 1.f : exp2f(m - m_new)) + v.y * (v.x == m_new ? 1.f : exp2f(v.x - m_new));
       m = m_new;
     }
   ms[y][x] = m;
-  ls[y][x] = l;
+  ls[y][x] = part;
   __syncthreads();
   if (y != 0 || r >= n) return;
   float top = ms[0][x];
   for (int i = 1; i < kRowGroups; ++i) top = fmaxf(top, ms[i][x]);
   float sum = 0.f;
   for (int i = 0; i < kRowGroups; ++i) sum += ls[i][x] * (ms[i][x] == top ? 1.f : exp2f(ms[i][x] - top));
-  const float v = (top + log2f(sum)) * kLn2;
-  lse[r] = v;
+  const float over = log2f(sum);
+  lse[r] = (top + over) * kLn2;
   const int kind = row_kind(target_of(targets, r), ignore_index, V);
-  loss[r] = kind == 0 ? 0.f : kind == 1 ? v - from_l2(target_logit + r) : NAN;
+  float l = kind == 0 ? 0.f : NAN;
+  if (kind == 1) {      // not lse - z: where the target has nearly all of the sum, that would be the rounding of lse.  Below 0 only by rounding
+    l = (fmaf(-from_l2(target_logit + r), kLog2e, top) + over) * kLn2;
+    if (l < 0.f) l = 0.f;
+  }
+  loss[r] = l;
 }
 
 cudaError_t launch_finish(const Problem& p, const Scores& s, float* loss, float* lse, cudaStream_t stream) {

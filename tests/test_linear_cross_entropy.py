@@ -498,3 +498,24 @@ def test_no_such_class_is_not_a_number_in_the_second_derivative(lce, dtype):
         gx, gw, gg = torch.autograd.grad(first, leaves, [t.detach() for t in inputs(40, 32, 50, dtype, seed=8)[:2]])
         assert gx.isnan().all(1).nonzero().flatten().tolist() == [3] and gg.isnan().nonzero().flatten().tolist() == [3] and bool(gw.isnan().all())
         assert not bool(gx[y == -100].any()) and not bool(gg[y == -100].any())
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype, d", [(torch.bfloat16, 256), (torch.float16, 256), (torch.float32, 256), (torch.bfloat16, 252)])
+@pytest.mark.parametrize("low, high", [(0.5, 8.0), (8.0, 40.0), (40.0, 500.0), (500.0, 30000.0)])
+def test_losses_of_sure_rows(lce, dtype, d, low, high):
+    # logits of 0 but for the target's, all exact: log(1 + (V - 1) e^-top), near 0 beside logits that are not.  A term of the sum goes through up to five
+    # exponentials of 2^-22 each: its own, the two moves of its part's reference (from 0 or -7 to the target), the joins of halves and of tiles; the sums of 256
+    # terms and the logarithm are within 2^-22 beside them, and the difference of target and maximum within 2^-22 of itself
+    w = torch.eye(d, device="cuda", dtype=dtype)
+    y = torch.arange(300, device="cuda") % d
+    top = torch.linspace(low, high, 300, device="cuda").to(dtype).unsqueeze(1)
+    x = w[y] * top
+    for z in (x, x - w[(y + 1) % d] * 7):      # another class below the others
+        got = lce(z, w, y, reduction="none").double()
+        want = torch.nn.functional.cross_entropy(z.double() @ w.double().T, y, reduction="none")
+        assert bool((got >= 0).all()) and float(((got - want).abs() / (6 * 2.0 ** -22 + 2.0 ** -22 * want)).max()) <= 1, float((got - want).abs().max())
+    # and of rows that are sure of another class: top, with the same share of its own size
+    got = lce(x, w, (y + 3) % d, reduction="none").double()
+    want = torch.nn.functional.cross_entropy(x.double() @ w.double().T, (y + 3) % d, reduction="none")
+    assert float(((got - want).abs() / (6 * 2.0 ** -22 + 2.0 ** -22 * want)).max()) <= 1
