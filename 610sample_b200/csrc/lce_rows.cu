@@ -45,7 +45,7 @@ finish_kernel(const Partial* partial, const float* target_logit, const int64_t* 
   float sum = 0.f;
   for (int i = 0; i < kRowGroups; ++i) sum += ls[i][x] * (ms[i][x] == top ? 1.f : exp2f(ms[i][x] - top));
   const float over = log2f(sum);
-  lse[r] = (top + over) * kLn2;
+  lse[r] = (float)(((double)top + over) / kLog2e);      // maxima are multiples of kLog2e: a row of one logit gives that logit
   const int kind = row_kind(target_of(targets, r), ignore_index, V);
   float l = kind == 0 ? 0.f : NAN;
   if (kind == 1) {      // not lse - z: where the target has nearly all of the sum, that would be the rounding of lse.  Below 0 only by rounding

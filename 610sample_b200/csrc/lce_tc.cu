@@ -225,12 +225,12 @@ lce_gemm_kernel(const __grid_constant__ GemmMaps maps, const GemmArgs g) {
       const uint32_t acc = lane_addr + (uint32_t)buf * 256u + (uint32_t)(half * kHalfN);
       const bool in = r < g.rows;
       int target = -1;                                     // column of this row's target, counted from col0
-      float lse2 = 0.f, coef = 0.f;
+      float lse = 0.f, coef = 0.f;
       if constexpr (USE == LSE || USE == GRAD) {
         if (in) {
           const int64_t y = from_l2(reinterpret_cast<const long long*>(g.targets) + r) - g.first_col - col0;
           if (y >= 0 && y < kHalfN) target = (int)y;
-          if constexpr (USE == GRAD) { lse2 = from_l2(g.lse + r) * kLog2e; coef = from_l2(g.coef + r); }
+          if constexpr (USE == GRAD) { lse = from_l2(g.lse + r); coef = from_l2(g.coef + r); }
         }
       }
       // the eight warps go on, or give up, together: the barriers below need all of them
@@ -299,7 +299,12 @@ lce_gemm_kernel(const __grid_constant__ GemmMaps maps, const GemmArgs g) {
           if constexpr (USE == GRAD) {
             // a row that does not count has a factor of 0 and G = 0, whatever its logits are
 #pragma unroll
-            for (int e = 0; e < 64; ++e) f[e] = coef == 0.f ? 0.f : ex2(fmaf(f[e], kLog2e, -lse2)) * coef;
+            for (int e = 0; e < 64; e += 2) {      // the difference first: exact where a row is sure of a class, so that P is 1 there
+              const float2 t = __fmul2_rn(__fadd2_rn(make_float2(f[e], f[e + 1]), make_float2(-lse, -lse)), make_float2(kLog2e, kLog2e));
+              const float2 p = __fmul2_rn(make_float2(ex2(t.x), ex2(t.y)), make_float2(coef, coef));
+              f[e] = coef == 0.f ? 0.f : p.x;
+              f[e + 1] = coef == 0.f ? 0.f : p.y;
+            }
             if (__any_sync(0xffffffffu, (uint32_t)(target - c) < 64u)) {
 #pragma unroll
               for (int e = 0; e < 64; ++e)

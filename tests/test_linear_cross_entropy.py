@@ -519,3 +519,20 @@ def test_losses_of_sure_rows(lce, dtype, d, low, high):
     got = lce(x, w, (y + 3) % d, reduction="none").double()
     want = torch.nn.functional.cross_entropy(x.double() @ w.double().T, (y + 3) % d, reduction="none")
     assert float(((got - want).abs() / (6 * 2.0 ** -22 + 2.0 ** -22 * want)).max()) <= 1
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype, d", [(torch.bfloat16, 256), (torch.float16, 256), (torch.float32, 256), (torch.bfloat16, 252)])
+@pytest.mark.parametrize("low, high", [(8.0, 24.0), (24.0, 100.0), (100.0, 500.0), (500.0, 30000.0)])
+def test_gradients_of_sure_rows(lce, dtype, d, low, high):
+    # the rows above; with W = 1, dx is G.  At the target G = -(V - 1) e^-top / (1 + ...), of which the log-sum-exp, rounded once, knows half a step (top 2^-24
+    # and less), beside the 2^-22 of the exponential that is the target's share of its sum; it is top itself where both are below a quarter of a step, from 24
+    # on.  The exponential of the difference is off by 2^-22
+    w = torch.eye(d, device="cuda", dtype=dtype)
+    y = torch.arange(300, device="cuda") % d
+    top = torch.linspace(low, high, 300, device="cuda").to(dtype).unsqueeze(1)
+    x = w[y] * top
+    dx = both_passes(lce, x, w, y, torch.ones(300, device="cuda"), "none")[1].double()
+    want = torch.softmax(x.double() @ w.double().T, 1) - w[y].double()
+    bound = 2.0 ** -22 + (top.double() * 2.0 ** -24 + 2.0 ** -22 if low < 24 else 0.0) + (torch.finfo(dtype).eps + 2.0 ** -20) * want.abs()
+    assert float(((dx - want).abs() / bound).max()) <= 1, float((dx - want).abs().max())
