@@ -702,7 +702,7 @@ static cudaError_t launch_two(const Geometry& g, const Tensors& t, cudaStream_t 
 
 // Packed batches.  Where there are few tiles, a cluster of 2 to 8 CTAs shares a tile's stream, as above; the host knows only an upper bound
 // of the tiles, a part-filled one and an unused one for every sequence, and no length, so the rule is a round of twice the SMs' places for that
-// bound.  1031 rows in 5 sequences, window 100, 6 and 2 heads of 80, forward and backward: 117 to 126 us, without clusters 134, by four always 213, by eight 407.
+// bound.  1031 rows in 5 sequences, window 100, 6 and 2 heads of 80, forward and backward: 117 to 131 us, without clusters 134, by four always 213, by eight 407.
 template <int KIND, int DC>
 static int packed_split(long long ctas) {
   const long long s = 2ll * kSms * (DC == 1 ? 2 : 1) / (ctas > 0 ? ctas : 1);

@@ -2,8 +2,10 @@
 // (widths that are no multiple of 8).  The same four uses as there (lce_tc.cu); G is kept in float.  All arithmetic is in fp32.
 // A CTA of 256 threads computes 128 x 128 results, 8 x 8 a thread, over blocks of 16 in k that go through shared memory, the next one
 // on its way into registers meanwhile.  A thread brings eight elements of either operand, along whichever axis is dense, with 16-byte loads
-// where that axis' extent and the addresses allow it.  Bound by the FMA pipe; at 333 x 200 x 5003 the
-// launches with gradients, nine of 80 to 290 CTAs, take 151 us, four products of 9 us at the pipe's rate.
+// where that axis' extent and the addresses allow it.  At 333 x 200 x 5003 the launches with gradients, nine of 80 to 290 CTAs, take 151 us.  The four
+// products, 9 us each at the FMA pipe's rate, take 32 to 38: one CTA of eight warps an SM issues in 37 % of the cycles (packed multiply-adds, of two
+// cycles, in 25 %) and else waits for shared memory or the next block, and the SMs are idle for a quarter of the time at either end.  With many tiles,
+// 2048 x 770 x 32000 in bf16, the forward takes 3.25 ms, 31 TFLOP/s, and with gradients 14.6.
 #include "attn_common.cuh"
 #include "lce_launch.h"
 #include "tc_common.cuh"

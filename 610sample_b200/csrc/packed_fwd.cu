@@ -16,8 +16,8 @@
 // which one warp of a tile on each scheduler does to 60 % and two do better: two threads a row, half of the columns each, which agree on
 // the row's reference through shared memory.  The order of the issuing warps is in packed_order.h.
 //
-// One sequence of 8192, 16 heads, causal: D = 128 (4 key heads) 242 us, 1 136 TFLOP/s, 69 % of the measured peak (single tiles 252); D = 64 178 us,
-// 771 TFLOP/s, the special-function unit 70 % busy (201).  Tried on the way, beside 231 and 196 us of another board with one thread a row and one
+// One sequence of 8192, 16 heads, causal: D = 128 (4 key heads) 239 us, 1 151 TFLOP/s, 70 % of the measured peak (single tiles 252); D = 64 177 us,
+// 778 TFLOP/s, the special-function unit 70 % busy (201).  Tried on the way, beside 231 and 196 us of another board with one thread a row and one
 // issuing warp: P handed over in halves 257 and 220; two issuing warps and halves 310 and 198 (both tiles then wait for the tensor pipe, and
 // then exponentiate, at the same time); exponentials strictly in turn 241 and 211; a quarter or half of them by polynomial on the FMA pipe no
 // faster and 257 and 224; 208 registers a thread 239 and 201; two threads a row 247 and 186.

@@ -3,7 +3,8 @@
 //
 // A plan, made on the device from the sequences' offsets (packed_plan.cu), lists the stationary tiles of a
 // batch: up to 128 rows of ONE sequence each, so that a sequence's result depends neither on what lies
-// beside it (also where that is infinite or not a number) nor on where it lies in the batch.  Rows of no
+// beside it (also where that is infinite or not a number) nor on where it lies in the batch; but which kernels a batch
+// takes goes by its size and mean length, and with them the order of sums: a sequence by itself may differ in the last bits.  Rows of no
 // sequence are listed too; they get zeros.  Short sequences pay for that with part-filled tiles: tiles of 128
 // consecutive rows over several sequences would need up to 128 / length times fewer of them, but mix the rows of
 // two sequences in one product, where 0 * inf and 0 * NaN of a neighbour's masked keys reach the sums.
