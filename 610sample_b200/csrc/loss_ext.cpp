@@ -82,7 +82,7 @@ variable_list loss_double_backward(const torch::Tensor& u_in, const torch::Tenso
   c10::cuda::CUDAGuard guard(x.device());
   const int64_t n = x.size(0), V = w.size(0);
   // a target that is no class: taken out of the sums, and not a number in the end
-  const torch::Tensor wrong = (targets != a.ignore_index) & ((targets < 0) | (targets >= V)), counted = (targets != a.ignore_index) & ~wrong;
+  const torch::Tensor classes = targets.clamp(0, V - 1), named = targets != a.ignore_index, wrong = named & (classes != targets), counted = named ^ wrong;
   torch::Tensor c = g.to(at::kFloat);
   if (a.reduction == ATTN_REDUCE_MEAN) c = c / counted_rows;
   c = torch::where(counted, c.expand({n}), torch::zeros({}, c.options()));
@@ -111,7 +111,7 @@ variable_list loss_double_backward(const torch::Tensor& u_in, const torch::Tenso
     const torch::Tensor mask = counted.slice(0, i, e).unsqueeze(1), zero = torch::zeros({}, c.options());
     auto rows = [&](const torch::Tensor& t) { return torch::where(mask, t.slice(0, i, e), torch::zeros({}, t.options())); };
     const torch::Tensor xs = rows(x), us = u_in.defined() ? rows(u_in) : torch::Tensor(), cs = c.slice(0, i, e).unsqueeze(1);
-    const torch::Tensor y = torch::where(counted.slice(0, i, e), targets.slice(0, i, e), torch::zeros({}, targets.options())).clamp(0, V - 1).unsqueeze(1);
+    const torch::Tensor y = classes.slice(0, i, e).unsqueeze(1);
     torch::Tensor P = torch::exp(mm(xs, w.t()) - lse.slice(0, i, e).unsqueeze(1));
     torch::Tensor T = us.defined() ? mm(us, w.t()) : torch::zeros_like(P);
     if (v_in.defined()) T.add_(mm(xs, v_in.t()));
