@@ -141,8 +141,9 @@ variable_list packed_double_backward(const torch::Tensor& g_dq, const torch::Ten
     return r;
   };
   if (n_tok == 0 || n_seq == 0 || max_seqlen == 0) return results();
-  const torch::Tensor ends = plan.slice(0, plan.numel() - 2 * n_seq, plan.numel() - n_seq).to(at::kLong);
-  const torch::Tensor starts = torch::cat({plan.slice(0, 4, 5).to(at::kLong), ends.slice(0, 0, n_seq - 1)});
+  // bounded as in the kernels: what is no plan (the memory of one that a captured graph has yet to make) must not index outside of the rows
+  const torch::Tensor ends = plan.slice(0, plan.numel() - 2 * n_seq, plan.numel() - n_seq).to(at::kLong).clamp_(0, n_tok);
+  const torch::Tensor starts = torch::cat({plan.slice(0, 4, 5).to(at::kLong).clamp_(0, n_tok), ends.slice(0, 0, n_seq - 1)});
   std::vector<int64_t> lens;
   int64_t longest = max_seqlen;
   if (max_seqlen < 0) {
@@ -151,7 +152,7 @@ variable_list packed_double_backward(const torch::Tensor& g_dq, const torch::Ten
     const torch::Tensor host = (ends - starts).cpu();
     lens.assign(host.data_ptr<int64_t>(), host.data_ptr<int64_t>() + n_seq);
     longest = *std::max_element(lens.begin(), lens.end());
-    if (longest == 0) return results();
+    if (longest <= 0) return results();
   }
   // at most twice the batch's rows in a call: memory goes with the batch, and a batch that is half padding is not cut
   for (const PaddedGroup& part : padded_groups(starts, ends, lens, std::min(longest, n_tok), std::max<int64_t>(2 * n_tok, 4096))) {

@@ -775,3 +775,21 @@ def test_second_derivative_of_a_longer_sequence_than_given_is_not_a_number(packe
     for known in (70, 114, 115, 2 ** 40):
         for a, b in zip(second_derivatives(packed, leaves, cu, n, None, g2, known), want):
             assert bool(a.isfinite().all()) and float((a.float() - b.float()).norm() / b.float().norm()) <= 4 * torch.finfo(dtype).eps
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("known", [None, 100])
+def test_second_derivative_of_no_plan_stays_within_the_rows(packed, known):
+    # offsets outside of the rows, large and negative ones, as memory holds them that no plan has been written to
+    n, cu = 300, [0, 100, 200, 300]
+    leaves, g2 = tensors(n, 2, 2, 32, torch.float32), tensors(n, 2, 2, 32, torch.float32, seed=9)[:3]
+    for wrong in ([2 ** 31 - 1, 7, -5], [-2 ** 31, -2 ** 31, 2 ** 31 - 1], [301, 5000, 2 ** 30], [0, 0, 0], [-1, -1, -1]):
+        plan = packed.packed_plan(torch.tensor(cu, dtype=torch.int32, device="cuda"), n, max_seqlen=known)
+        x = [t.detach().requires_grad_(True) for t in leaves]
+        first = torch.autograd.grad(packed.packed_attention(*x[:3], plan), x[:3], x[3], create_graph=True)
+        with torch.no_grad():
+            plan.tensor.data[4] = wrong[0]
+            plan.tensor.data[-6:-3] = torch.tensor(wrong, dtype=torch.int32)
+        for t, like in zip(torch.autograd.grad(first, x, g2), x):
+            assert t.shape == like.shape
+        torch.cuda.synchronize()
