@@ -753,7 +753,8 @@ def test_second_derivative_of_unlike_lengths(packed, dtype, tol, known, window):
 @pytest.mark.gpu
 @pytest.mark.parametrize("known", [None, 2048])
 def test_second_derivative_takes_memory_by_rows(packed, known):
-    # one document beside 600 short ones: no more than 40 tensors of twice the batch's rows, where rows padded to the longest one take 1.2 GB each
+    # one document beside 600 short ones: no more than 40 tensors of twice the batch's rows or of 128 MB, where rows padded to the longest one take 1.2 GB each
+    # (15.4 GB in all)
     lens, H, D = [5] * 300 + [2048] + [11] * 300, 8, 64
     cu = offsets(lens)
     leaves, g2 = tensors(cu[-1], H, H, D, torch.bfloat16), tensors(cu[-1], H, H, D, torch.bfloat16, seed=9)[:3]
@@ -761,7 +762,7 @@ def test_second_derivative_takes_memory_by_rows(packed, known):
     torch.cuda.reset_peak_memory_stats()
     before = torch.cuda.memory_allocated()
     second_derivatives(packed, leaves, cu, cu[-1], None, g2, known)
-    assert torch.cuda.max_memory_allocated() - before <= 40 * 2 * leaves[0].numel() * 2
+    assert torch.cuda.max_memory_allocated() - before <= 40 * max(2 * leaves[0].numel() * 2, 128 << 20)
 
 
 @pytest.mark.gpu
