@@ -19,8 +19,8 @@ _REDUCTIONS = {"none": 0, "sum": 1, "mean": 2}
 def linear_cross_entropy(x, weight, targets, ignore_index=-100, reduction="mean"):
     """x: (..., d); weight: (V, d), both fp16, bf16 or fp32 CUDA tensors of one type; targets: int64, (...).
 
-    A row whose target is `ignore_index` has loss and gradients 0 and does not count in the mean; what x holds there,
-    infinities and NaN too, has no influence.  A target outside [0, V) otherwise gives a NaN loss (and no fault).
+    A row whose target is `ignore_index` has loss and, beside finite weights, gradients 0 and does not count in the mean; what x
+    holds there, infinities and NaN too, has no influence.  A target outside [0, V) otherwise gives a NaN loss (and no fault).
     reduction: "mean" over the rows that count (NaN if none does), "sum", or "none" (the losses, shaped as targets).
     Returns float32.  Half types with d a multiple of 8 run on the tensor cores, all else on the CUDA cores.
     Twice differentiable in x and weight; the second derivative is computed by PyTorch operations, in pieces of rows."""
