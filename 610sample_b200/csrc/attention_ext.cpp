@@ -384,6 +384,7 @@ c10::optional<torch::Tensor> qk_norm_rope_diff(const torch::Tensor& x, c10::opti
 PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   register_packed(m);
   register_loss(m);
+  register_layers(m);
   m.def("qk_norm_rope", &qk_norm_rope_cuda, "fused RMS norm + rotary embedding + [n_tok,H,d] -> [1,H,n_tok,d]",
         py::arg("x"), py::arg("weight"), py::arg("freqs"), py::arg("pos0") = 0, py::arg("eps") = 1e-6, py::arg("norm_from") = 0);
   m.def("qk_norm_rope_diff", &qk_norm_rope_diff, "qk_norm_rope, twice differentiable (None: a call for the Python function)",

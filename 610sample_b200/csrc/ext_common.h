@@ -117,6 +117,7 @@ inline bool wants_graph(std::initializer_list<const torch::Tensor*> inputs) {
 
 void register_packed(pybind11::module& m);
 void register_loss(pybind11::module& m);
+void register_layers(pybind11::module& m);
 
 }  // namespace ext
 

@@ -1,0 +1,389 @@
+// Layer norm of rows, y = (x - mean) r w + b with r = 1 / sqrt(variance + eps), and its two backward passes, in fp32, each result rounded once.
+//
+//   first    c = g w:  dx = r (c - m(c) - xh m(c xh)),  dw = sum g xh,  db = sum g            (xh = (x - mean) r, m: mean over the row)
+//   second   along tangents (u, uw, ub) of (x, w, b), P = r (u - m(u) - xh m(u xh)) is the tangent of xh:
+//            to g: w P + uw xh + ub        to w: sum g P
+//            to x: r (q - m(q) - xh m(q xh)) - r^2 xh (m(c u) - m(c) m(u) - m(c xh) m(u xh)),  q = g uw - r (c m(u xh) + u m(c xh))
+//            m(q) and m(q xh) follow from the means of c, u, g uw and their products with xh, so one round of sums over the row does
+//
+// Every pass reads its rows once: a row stays in the registers of a group of 32 to 1024 threads, up to 32 elements each, so that the variance is that of
+// the centred row.  Bound by memory.  Sums over the rows stay in registers while a group goes from row to row, its next row on the way; a
+// kernel behind adds what the CTAs have, in order.
+#pragma once
+
+#include "attn_common.cuh"
+#include "layer_launch.h"
+#include "tc_common.cuh"
+
+namespace attn {
+namespace layer {
+
+using tc::from_l2;
+
+constexpr int kNormThreads = 256;
+
+struct NormArgs {
+  int n, d;
+  bool param_float;
+  float eps;
+  const void *x, *w, *b, *g, *u, *uw, *ub;
+  void *y, *gx;
+  float *mean, *rstd;
+  float* partial;                // [CTAs][sums][d]
+  long long ldx, ldg, ldu;
+};
+
+// How a row lies in a group: `tpr` threads with `vectors` times eight elements each; wide: with 16-byte loads
+struct NormPlan { int tpr, vectors; bool wide; };
+
+// Eight elements of a row at a time.  WIDE: in sequence, with 16-byte loads; else one by one, neighbouring threads on neighbouring elements, for any
+// width and alignment.
+template <typename T, int TPR, bool WIDE>
+struct Lanes {
+  static __device__ __forceinline__ int column(int t, int v, int e) { return WIDE ? (v * TPR + t) * 8 + e : (v * 8 + e) * TPR + t; }
+  static __device__ __forceinline__ bool inside(int t, int v, int e, int d) { return column(t, v, WIDE ? 0 : e) < d; }      // WIDE: d is a multiple of 8
+  static constexpr int kWords = sizeof(T) == 4 ? 8 : 4;
+  struct Raw { uint32_t w[WIDE ? kWords : 8]; };
+
+  static __device__ __forceinline__ Raw load(const T* row, int t, int v, int d) {
+    Raw r;
+    if constexpr (WIDE) {
+      if (inside(t, v, 0, d)) {
+        const uint4* p = reinterpret_cast<const uint4*>(row + column(t, v, 0));
+#pragma unroll
+        for (int q = 0; q < kWords / 4; ++q) {
+          const uint4 a = from_l2(p + q);
+          r.w[4 * q] = a.x; r.w[4 * q + 1] = a.y; r.w[4 * q + 2] = a.z; r.w[4 * q + 3] = a.w;
+        }
+      } else {
+#pragma unroll
+        for (int q = 0; q < kWords; ++q) r.w[q] = 0u;
+      }
+    } else {
+#pragma unroll
+      for (int e = 0; e < 8; ++e) r.w[e] = inside(t, v, e, d) ? __float_as_uint(Elem<T>::to_float(row[column(t, v, e)])) : 0u;
+    }
+    return r;
+  }
+  static __device__ __forceinline__ void values(const Raw& r, float (&f)[8]) {
+    if constexpr (WIDE && sizeof(T) == 2) {
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const float2 a = tc::Pack<T>::unpack(r.w[e]);
+        f[2 * e] = a.x; f[2 * e + 1] = a.y;
+      }
+    } else {
+#pragma unroll
+      for (int e = 0; e < 8; ++e) f[e] = __uint_as_float(r.w[e]);
+    }
+  }
+  static __device__ __forceinline__ void store(T* row, int t, int v, int d, const float (&f)[8]) {
+    if constexpr (WIDE) {
+      if (!inside(t, v, 0, d)) return;
+      uint4* p = reinterpret_cast<uint4*>(row + column(t, v, 0));
+      if constexpr (sizeof(T) == 4) {
+        p[0] = make_uint4(__float_as_uint(f[0]), __float_as_uint(f[1]), __float_as_uint(f[2]), __float_as_uint(f[3]));
+        p[1] = make_uint4(__float_as_uint(f[4]), __float_as_uint(f[5]), __float_as_uint(f[6]), __float_as_uint(f[7]));
+      } else {
+        p[0] = make_uint4(tc::Pack<T>::pack(f[0], f[1]), tc::Pack<T>::pack(f[2], f[3]), tc::Pack<T>::pack(f[4], f[5]), tc::Pack<T>::pack(f[6], f[7]));
+      }
+    } else {
+#pragma unroll
+      for (int e = 0; e < 8; ++e)
+        if (inside(t, v, e, d)) row[column(t, v, e)] = Elem<T>::from_float(f[e]);
+    }
+  }
+};
+// a parameter's (or its tangent's) elements of the same columns, float or of the rows' type; `fill` where there is none
+template <typename L, typename T, bool WIDE>
+__device__ __forceinline__ void parameter(const void* p, bool is_float, int t, int v, int d, float fill, float (&f)[8]) {
+  if (p == nullptr) {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) f[e] = fill;
+    return;
+  }
+  if (WIDE && !L::inside(t, v, 0, d)) {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) f[e] = 0.f;
+    return;
+  }
+  if (sizeof(T) == 4 || is_float) {
+    const float* at = static_cast<const float*>(p);
+    if constexpr (WIDE) {
+      const float4 a = reinterpret_cast<const float4*>(at + L::column(t, v, 0))[0], b = reinterpret_cast<const float4*>(at + L::column(t, v, 0))[1];
+      f[0] = a.x; f[1] = a.y; f[2] = a.z; f[3] = a.w; f[4] = b.x; f[5] = b.y; f[6] = b.z; f[7] = b.w;
+    } else {
+#pragma unroll
+      for (int e = 0; e < 8; ++e) f[e] = L::inside(t, v, e, d) ? at[L::column(t, v, e)] : 0.f;
+    }
+  } else if constexpr (sizeof(T) == 2) {
+    const T* at = static_cast<const T*>(p);
+    if constexpr (WIDE) {
+      const uint4 a = *reinterpret_cast<const uint4*>(at + L::column(t, v, 0));
+      const uint32_t w[4] = {a.x, a.y, a.z, a.w};
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const float2 b = tc::Pack<T>::unpack(w[e]);
+        f[2 * e] = b.x; f[2 * e + 1] = b.y;
+      }
+    } else {
+#pragma unroll
+      for (int e = 0; e < 8; ++e) f[e] = L::inside(t, v, e, d) ? Elem<T>::to_float(at[L::column(t, v, e)]) : 0.f;
+    }
+  }
+}
+
+// Sums over the TPR threads of a group; all threads of the CTA call it.  `turn` alternates between two places in shared memory.
+template <int TPR, int THREADS, int K>
+__device__ __forceinline__ void group_sum(float (&v)[K], float* shared, int& turn) {
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1)
+#pragma unroll
+    for (int k = 0; k < K; ++k) v[k] += __shfl_xor_sync(0xffffffffu, v[k], o);
+  if constexpr (TPR > 32) {
+    constexpr int kWarps = THREADS / 32, kMine = TPR / 32;
+    float* s = shared + turn * K * kWarps;
+    turn ^= 1;
+    const int warp = threadIdx.x >> 5, first = warp / kMine * kMine;
+    if ((threadIdx.x & 31) == 0)
+#pragma unroll
+      for (int k = 0; k < K; ++k) s[k * kWarps + warp] = v[k];
+    __syncthreads();
+#pragma unroll
+    for (int k = 0; k < K; ++k) {
+      float sum = 0.f;
+#pragma unroll
+      for (int w = 0; w < kMine; ++w) sum += s[k * kWarps + first + w];
+      v[k] = sum;
+    }
+  }
+}
+template <int TPR> constexpr int kThreadsOf = TPR > kNormThreads ? TPR : kNormThreads;
+
+template <typename T, int TPR, int V, bool WIDE>
+__global__ void __launch_bounds__(kThreadsOf<TPR>, 1)
+norm_forward_kernel(const NormArgs a) {
+  constexpr int kThreads = kThreadsOf<TPR>;
+  __shared__ float sums[2 * (kThreads / 32)];
+  typedef Lanes<T, TPR, WIDE> L;
+  tc::pdl_wait();
+  tc::pdl_trigger();
+  const int t = threadIdx.x % TPR;
+  const long long row = blockIdx.x * (long long)(kThreads / TPR) + threadIdx.x / TPR;
+  const bool in = row < a.n;
+  const T* x = static_cast<const T*>(a.x) + (in ? row : 0) * a.ldx;
+  float f[V][8], s[1] = {0.f};
+#pragma unroll
+  for (int v = 0; v < V; ++v) L::values(L::load(x, t, v, a.d), f[v]);
+#pragma unroll
+  for (int v = 0; v < V; ++v)
+#pragma unroll
+    for (int e = 0; e < 8; ++e) s[0] += f[v][e];      // 0 outside
+  int turn = 0;
+  const float over = 1.f / (float)a.d;
+  group_sum<TPR, kThreads>(s, sums, turn);
+  const float mean = s[0] * over;
+  s[0] = 0.f;
+#pragma unroll
+  for (int v = 0; v < V; ++v)
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      f[v][e] = L::inside(t, v, e, a.d) ? f[v][e] - mean : 0.f;
+      s[0] = fmaf(f[v][e], f[v][e], s[0]);
+    }
+  group_sum<TPR, kThreads>(s, sums, turn);
+  const float r = 1.f / sqrtf(s[0] * over + a.eps);
+  if (!in) return;
+  if (t == 0 && a.mean != nullptr) { a.mean[row] = mean; a.rstd[row] = r; }
+#pragma unroll
+  for (int v = 0; v < V; ++v) {
+    float w[8], b[8];
+    parameter<L, T, WIDE>(a.w, a.param_float, t, v, a.d, 1.f, w);
+    parameter<L, T, WIDE>(a.b, a.param_float, t, v, a.d, 0.f, b);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) f[v][e] = fmaf(f[v][e] * r, w[e], b[e]);
+    L::store(static_cast<T*>(a.y) + row * a.d, t, v, a.d, f[v]);
+  }
+}
+
+// ORDER 1: dx, sums dw and db.  ORDER 2: the gradients of g and x, sum dw.
+template <typename T, int TPR, int V, bool WIDE, int ORDER>
+__global__ void __launch_bounds__(kThreadsOf<TPR>, 1)
+norm_backward_kernel(const NormArgs a) {
+  constexpr int kThreads = kThreadsOf<TPR>, kGroups = kThreads / TPR, kSums = ORDER == 1 ? 2 : 1, kMeans = ORDER == 1 ? 2 : 7;
+  __shared__ float sums[2 * kMeans * (kThreads / 32)];
+  typedef Lanes<T, TPR, WIDE> L;
+  tc::pdl_wait();
+  tc::pdl_trigger();
+  const int t = threadIdx.x % TPR, group = threadIdx.x / TPR;
+  const long long stride = (long long)gridDim.x * kGroups;
+  float total[kSums][V][8];
+#pragma unroll
+  for (int k = 0; k < kSums; ++k)
+#pragma unroll
+    for (int v = 0; v < V; ++v)
+#pragma unroll
+      for (int e = 0; e < 8; ++e) total[k][v][e] = 0.f;
+  int turn = 0;
+  const float over = 1.f / (float)a.d;
+  typename L::Raw rx[V], rg[V], ru[ORDER == 2 ? V : 1];
+  float mean, r;
+  auto fetch = [&](long long row) {
+    const long long at = row < a.n ? row : 0;
+#pragma unroll
+    for (int v = 0; v < V; ++v) {
+      rx[v] = L::load(static_cast<const T*>(a.x) + at * a.ldx, t, v, a.d);
+      rg[v] = L::load(static_cast<const T*>(a.g) + at * a.ldg, t, v, a.d);
+      if constexpr (ORDER == 2)
+        if (a.u != nullptr) ru[v] = L::load(static_cast<const T*>(a.u) + at * a.ldu, t, v, a.d);
+    }
+    mean = from_l2(a.mean + at);
+    r = from_l2(a.rstd + at);
+  };
+  // all groups of a CTA go the same number of rounds: they meet in the sums
+  const long long first = blockIdx.x * (long long)kGroups;
+  if (first < a.n) fetch(first + group);
+  for (long long base = first; base < a.n; base += stride) {
+    const long long row = base + group;
+    const bool in = row < a.n;
+    float xh[V][8], c[V][8], u[ORDER == 2 ? V : 1][8];
+    const float rs = r;
+    float m[kMeans];
+#pragma unroll
+    for (int k = 0; k < kMeans; ++k) m[k] = 0.f;
+#pragma unroll
+    for (int v = 0; v < V; ++v) {
+      float x[8], g[8], w[8];
+      L::values(rx[v], x);
+      L::values(rg[v], g);
+      parameter<L, T, WIDE>(a.w, a.param_float, t, v, a.d, 1.f, w);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) xh[v][e] = L::inside(t, v, e, a.d) ? (x[e] - mean) * r : 0.f;      // g is 0 outside
+      if constexpr (ORDER == 1) {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          c[v][e] = g[e] * w[e];
+          m[0] += c[v][e];
+          m[1] = fmaf(c[v][e], xh[v][e], m[1]);
+          if (in) {
+            total[0][v][e] = fmaf(g[e], xh[v][e], total[0][v][e]);
+            total[1][v][e] += g[e];
+          }
+        }
+      } else {
+        float uw[8];
+        parameter<L, T, WIDE>(a.uw, a.param_float, t, v, a.d, 0.f, uw);
+        if (a.u != nullptr) L::values(ru[v], u[v]);
+        else
+#pragma unroll
+          for (int e = 0; e < 8; ++e) u[v][e] = 0.f;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          const float h = xh[v][e], cc = g[e] * w[e], q = g[e] * uw[e], uu = u[v][e];
+          c[v][e] = g[e];
+          m[0] += cc;
+          m[1] = fmaf(cc, h, m[1]);
+          m[2] += uu;
+          m[3] = fmaf(uu, h, m[3]);
+          m[4] = fmaf(cc, uu, m[4]);
+          m[5] += q;
+          m[6] = fmaf(q, h, m[6]);
+        }
+      }
+    }
+    if (base + stride < a.n) fetch(row + stride);
+    group_sum<TPR, kThreads>(m, sums, turn);
+#pragma unroll
+    for (int k = 0; k < kMeans; ++k) m[k] *= over;
+    if (!in) continue;
+    if constexpr (ORDER == 1) {
+      if (a.gx != nullptr) {
+#pragma unroll
+        for (int v = 0; v < V; ++v) {
+#pragma unroll
+          for (int e = 0; e < 8; ++e) c[v][e] = rs * (c[v][e] - m[0] - xh[v][e] * m[1]);
+          L::store(static_cast<T*>(a.gx) + row * a.d, t, v, a.d, c[v]);
+        }
+      }
+    } else {
+      const float mc = m[0], mch = m[1], mu = m[2], muh = m[3];
+      const float mq = m[5] - rs * (mc * muh + mu * mch), mqh = m[6] - 2.f * rs * mch * muh, turned = rs * rs * (m[4] - mc * mu - mch * muh);
+#pragma unroll
+      for (int v = 0; v < V; ++v) {
+        float w[8], uw[8], ub[8], gg[8], gx[8];
+        parameter<L, T, WIDE>(a.w, a.param_float, t, v, a.d, 1.f, w);
+        parameter<L, T, WIDE>(a.uw, a.param_float, t, v, a.d, 0.f, uw);
+        parameter<L, T, WIDE>(a.ub, a.param_float, t, v, a.d, 0.f, ub);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          const float h = xh[v][e], g = c[v][e], uu = u[v][e], moved = rs * (uu - mu - h * muh);
+          gg[e] = fmaf(w[e], moved, fmaf(uw[e], h, ub[e]));
+          const float q = fmaf(-rs, g * w[e] * muh + uu * mch, g * uw[e]);
+          gx[e] = rs * (q - mq - h * mqh) - h * turned;
+          total[0][v][e] = fmaf(g, moved, total[0][v][e]);
+        }
+        if (a.y != nullptr) L::store(static_cast<T*>(a.y) + row * a.d, t, v, a.d, gg);
+        if (a.gx != nullptr) L::store(static_cast<T*>(a.gx) + row * a.d, t, v, a.d, gx);
+      }
+    }
+  }
+  if (a.partial == nullptr) return;
+  // the CTA's groups, one after the other, into its row of the partial sums
+  __shared__ __align__(16) float joined[kGroups > 1 ? kSums * TPR * V * 8 : 4];
+  float* out = a.partial + (size_t)blockIdx.x * kSums * a.d;
+  for (int q = kGroups - 1; q >= 0; --q) {
+    if (group == q)
+#pragma unroll
+      for (int k = 0; k < kSums; ++k)
+#pragma unroll
+        for (int v = 0; v < V; ++v)
+#pragma unroll
+          for (int e = 0; e < 8; ++e) {
+            float s = total[k][v][e];
+            const int at = ((k * V + v) * 8 + e) * TPR + t;
+            if (q < kGroups - 1) s += joined[at];
+            if (q > 0) joined[at] = s;
+            else if (L::inside(t, v, e, a.d)) out[(size_t)k * a.d + L::column(t, v, e)] = s;
+          }
+    __syncthreads();
+  }
+}
+
+// ---- host ---------------------------------------------------------------------------------------
+template <typename T, int TPR, int V, bool WIDE, int ORDER>
+inline cudaError_t launch_norm(const NormArgs& a, unsigned ctas, cudaStream_t stream) {
+  if constexpr (ORDER == 0) return tc::launch_pdl(norm_forward_kernel<T, TPR, V, WIDE>, ctas, (unsigned)kThreadsOf<TPR>, 0, stream, a);
+  else return tc::launch_pdl(norm_backward_kernel<T, TPR, V, WIDE, ORDER>, ctas, (unsigned)kThreadsOf<TPR>, 0, stream, a);
+}
+template <typename T, bool WIDE, int ORDER>
+inline cudaError_t launch_plan(const NormPlan& p, const NormArgs& a, unsigned ctas, cudaStream_t stream) {
+  if (p.tpr == 32) {
+    if constexpr (WIDE) {
+      if (p.vectors == 2) return launch_norm<T, 32, 2, WIDE, ORDER>(a, ctas, stream);
+      if (p.vectors == 3) return launch_norm<T, 32, 3, WIDE, ORDER>(a, ctas, stream);
+    }
+    return p.vectors == 1 ? launch_norm<T, 32, 1, WIDE, ORDER>(a, ctas, stream) : launch_norm<T, 32, 4, WIDE, ORDER>(a, ctas, stream);
+  }
+  if (p.tpr == 128) {
+    if constexpr (WIDE) {
+      if (p.vectors == 2) return launch_norm<T, 128, 2, WIDE, ORDER>(a, ctas, stream);
+      if (p.vectors == 3) return launch_norm<T, 128, 3, WIDE, ORDER>(a, ctas, stream);
+    }
+    return launch_norm<T, 128, 4, WIDE, ORDER>(a, ctas, stream);
+  }
+  if (p.tpr == 512) return launch_norm<T, 512, 2, WIDE, ORDER>(a, ctas, stream);
+  return p.vectors <= 2 ? launch_norm<T, 1024, 2, WIDE, ORDER>(a, ctas, stream) : launch_norm<T, 1024, 4, WIDE, ORDER>(a, ctas, stream);
+}
+template <int ORDER>
+inline cudaError_t launch_typed(const NormPlan& p, const NormArgs& a, int dtype, unsigned ctas, cudaStream_t stream) {
+  if (dtype == ATTN_F16) return p.wide ? launch_plan<__half, true, ORDER>(p, a, ctas, stream) : launch_plan<__half, false, ORDER>(p, a, ctas, stream);
+  if (dtype == ATTN_BF16) return p.wide ? launch_plan<__nv_bfloat16, true, ORDER>(p, a, ctas, stream) : launch_plan<__nv_bfloat16, false, ORDER>(p, a, ctas, stream);
+  return p.wide ? launch_plan<float, true, ORDER>(p, a, ctas, stream) : launch_plan<float, false, ORDER>(p, a, ctas, stream);
+}
+
+cudaError_t launch_norm_forward(const NormPlan& p, const NormArgs& a, int dtype, unsigned ctas, cudaStream_t stream);
+cudaError_t launch_norm_first(const NormPlan& p, const NormArgs& a, int dtype, unsigned ctas, cudaStream_t stream);
+cudaError_t launch_norm_second(const NormPlan& p, const NormArgs& a, int dtype, unsigned ctas, cudaStream_t stream);
+
+}  // namespace layer
+}  // namespace attn

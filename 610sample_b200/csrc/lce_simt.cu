@@ -8,19 +8,15 @@
 // 2048 x 770 x 32000 in bf16, the forward takes 3.25 ms, 31 TFLOP/s, and with gradients 14.6.
 #include "attn_common.cuh"
 #include "lce_launch.h"
-#include "tc_common.cuh"
+#include "simt_product.cuh"
 
 namespace attn {
 namespace lce {
 
+using namespace simt;
 using tc::from_l2;
 
 enum Use { LSE = 0, GRAD = 1, DX = 2, DW = 3 };
-constexpr int kTile = 128, kBlock = 16, kPitch = kTile + 4;
-
-// element (i, k) of an operand at p[i * si + k * sk]; one of the strides is 1
-template <typename T> struct Operand { const T* p; long long si, sk; int wide; };      // wide: runs of eight are 16-byte aligned
-
 struct SimtArgs {
   int rows, cols, k;
   int splits, split_k;           // DX, DW: shares of k
@@ -37,44 +33,6 @@ struct SimtArgs {
   const float* scale;
 };
 
-// The eight elements of a [128][16] block that this thread brings: along k of row t / 2, or along i at k = t / 16.
-template <typename T>
-__device__ __forceinline__ void fetch(const Operand<T>& o, int i0, int k0, int n_i, int n_k, float (&v)[8], bool k_dense) {
-  const int t = threadIdx.x, i = i0 + (k_dense ? t >> 1 : (t & 15) * 8), k = k0 + (k_dense ? (t & 1) * 8 : t >> 4);
-  const T* p = o.p + i * o.si + k * o.sk;
-  if (o.wide && (k_dense ? i < n_i && k + 8 <= n_k : k < n_k && i + 8 <= n_i)) {
-    if constexpr (sizeof(T) == 4) {
-      const float4 a = from_l2(reinterpret_cast<const float4*>(p)), b = from_l2(reinterpret_cast<const float4*>(p) + 1);
-      v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w; v[4] = b.x; v[5] = b.y; v[6] = b.z; v[7] = b.w;
-    } else {
-      const uint4 q = from_l2(reinterpret_cast<const uint4*>(p));
-      const uint32_t w[4] = {q.x, q.y, q.z, q.w};
-#pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        const float2 f = tc::Pack<T>::unpack(w[e]);
-        v[2 * e] = f.x; v[2 * e + 1] = f.y;
-      }
-    }
-    return;
-  }
-#pragma unroll
-  for (int e = 0; e < 8; ++e) {
-    const bool in = k_dense ? i < n_i && k + e < n_k : k < n_k && i + e < n_i;
-    v[e] = in ? Elem<T>::to_float(p[e]) : 0.f;
-  }
-}
-__device__ __forceinline__ void put(float* s, const float (&v)[8], bool k_dense) {
-  const int t = threadIdx.x;
-  if (k_dense) {
-#pragma unroll
-    for (int e = 0; e < 8; ++e) s[((t & 1) * 8 + e) * kPitch + (t >> 1)] = v[e];
-  } else {
-    float4* at = reinterpret_cast<float4*>(s + (t >> 4) * kPitch + (t & 15) * 8);
-    at[0] = make_float4(v[0], v[1], v[2], v[3]);
-    at[1] = make_float4(v[4], v[5], v[6], v[7]);
-  }
-}
-
 template <int USE, typename TA, typename TB, typename T>
 __global__ void __launch_bounds__(256)
 lce_simt_kernel(const Operand<TA> A, const Operand<TB> B, const SimtArgs g, T* out) {
@@ -86,35 +44,10 @@ lce_simt_kernel(const Operand<TA> A, const Operand<TB> B, const SimtArgs g, T* o
   const int ty = threadIdx.x >> 4, tx = threadIdx.x & 15;      // rows ty * 8 + i, columns tx * 4 + j and 64 + tx * 4 + j
   const bool ka = A.sk == 1, kb = B.sk == 1;
   float2 sum[8][4];
-#pragma unroll
-  for (int i = 0; i < 8; ++i)
-#pragma unroll
-    for (int j = 0; j < 4; ++j) sum[i][j] = make_float2(0.f, 0.f);
-  float va[8], vb[8];
-  fetch(A, r0, k_begin, g.rows, k_end, va, ka);
-  fetch(B, c0, k_begin, g.cols, k_end, vb, kb);
+  clear(sum);
   int buf = 0;
-  for (int k0 = k_begin; k0 < k_end; k0 += kBlock, buf ^= 1) {
-    put(as[buf], va, ka);
-    put(bs[buf], vb, kb);
-    __syncthreads();
-    if (k0 + kBlock < k_end) {
-      fetch(A, r0, k0 + kBlock, g.rows, k_end, va, ka);
-      fetch(B, c0, k0 + kBlock, g.cols, k_end, vb, kb);
-    }
-#pragma unroll
-    for (int k = 0; k < kBlock; ++k) {
-      float a[8];
-      *reinterpret_cast<float4*>(a) = *reinterpret_cast<const float4*>(&as[buf][k * kPitch + ty * 8]);
-      *reinterpret_cast<float4*>(a + 4) = *reinterpret_cast<const float4*>(&as[buf][k * kPitch + ty * 8 + 4]);
-      const float4 b0 = *reinterpret_cast<const float4*>(&bs[buf][k * kPitch + tx * 4]), b1 = *reinterpret_cast<const float4*>(&bs[buf][k * kPitch + 64 + tx * 4]);
-      const float2 b[4] = {make_float2(b0.x, b0.y), make_float2(b0.z, b0.w), make_float2(b1.x, b1.y), make_float2(b1.z, b1.w)};
-#pragma unroll
-      for (int i = 0; i < 8; ++i)
-#pragma unroll
-        for (int j = 0; j < 4; ++j) sum[i][j] = __ffma2_rn(make_float2(a[i], a[i]), b[j], sum[i][j]);
-    }
-  }
+  accumulate(as, bs, buf, k_begin, k_end, [&](int k0, float (&v)[8]) { fetch(A, r0, k0, g.rows, k_end, v, ka); },
+             [&](int k0, float (&v)[8]) { fetch(B, c0, k0, g.cols, k_end, v, kb); }, ka, kb, sum);
   float acc[8][8];
 #pragma unroll
   for (int i = 0; i < 8; ++i)
@@ -169,9 +102,6 @@ lce_simt_kernel(const Operand<TA> A, const Operand<TB> B, const SimtArgs g, T* o
   }
 }
 
-// a share of k: whole blocks, so that runs of eight that are aligned in the first share are so in every one
-static long long share_of(long long k, long long splits) { return ((k + splits - 1) / splits + kBlock - 1) / kBlock * kBlock; }
-
 template <int USE, typename TA, typename TB, typename T>
 static cudaError_t launch_use(const Operand<TA>& A, const Operand<TB>& B, SimtArgs g, T* out, cudaStream_t stream) {
   g.tiles_m = (g.rows + kTile - 1) / kTile;
@@ -203,10 +133,6 @@ int simt_splits(long long rows, long long cols, long long k) {
   const long long each = share_of(k, s);
   return (int)((k + each - 1) / each);
 }
-
-static int wide(const void* p, long long ld, int size) { return reinterpret_cast<uintptr_t>(p) % 16 == 0 && ld * size % 16 == 0; }
-template <typename T> static Operand<T> rows_of(const void* p, long long ld) { return {static_cast<const T*>(p), ld, 1, wide(p, ld, sizeof(T))}; }
-template <typename T> static Operand<T> columns_of(const void* p, long long ld) { return {static_cast<const T*>(p), 1, ld, wide(p, ld, sizeof(T))}; }
 
 template <typename T>
 static cudaError_t scores(const Problem& p, const Scores& s, cudaStream_t stream) {

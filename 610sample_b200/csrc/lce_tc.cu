@@ -14,7 +14,7 @@
 // that the larger one is read from HBM once and the smaller one stays in L2.
 //
 // DX and DW have few tiles with long sums: dW of a piece of 8192 classes x 768 from 16384 rows is 96 tiles of 256 blocks of k for 74 pairs, two
-// rounds, 65 % busy.  There the tiles of the last round are each shared out along k among several pairs (plan_shares), and a small kernel behind
+// rounds, 65 % busy.  There the tiles of the last round are each shared out along k among several pairs (product_common.cuh), and a small kernel behind
 // adds the parts in order (join_kernel).  Whole rounds stay as they are: pairs that are at the same place in k read the same rows of G and x from
 // L2; equal, contiguous shares of all blocks left no pair idle, but took dW's product from 178 to 168 us only (that size), and dx's from
 // 146 to between 167 and 187, since G then came from HBM several times.
@@ -25,19 +25,17 @@
 // Logits are as exact as the tensor cores' own sums, which lose a little toward 0 with every block of k: 6e-7 of a logit at d = 768 and 2.1e-6 at 2048 (a
 // library's product the same), 3e-7 and 1e-6 of the loss; the CUDA cores' 1e-8.
 #include "lce_launch.h"
+#include "product_common.cuh"
 #include "tc_common.cuh"
-
-#include <cstdio>
-#include <mutex>
 
 namespace attn {
 namespace lce {
 
 using namespace tc;
+using namespace product;
 
 enum Use { LSE = 0, GRAD = 1, DX = 2, DW = 3 };
 
-constexpr int kTileM = 256, kTileN = 256, kBlockK = 64;
 constexpr int kHalfN = kTileN / 2;                             // columns of B in one CTA, and of a result in one half of its epilogue
 constexpr int kStages = 6;
 constexpr uint32_t kOperandBytes = 128 * 128;                  // 128 rows (or columns) of 64 in k, of A or of B, in one CTA
@@ -396,55 +394,12 @@ join_kernel(const GemmArgs g, T* out) {
 }
 
 // ---- host ---------------------------------------------------------------------------------------
-typedef CUresult (*EncodeTiledFn)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*, const cuuint32_t*,
-                                  const cuuint32_t*, CUtensorMapInterleave, CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
-static EncodeTiledFn encode_fn() {
-  static EncodeTiledFn fn = nullptr;
-  static std::once_flag once;
-  std::call_once(once, [] {
-    void* p = nullptr;
-    cudaDriverEntryPointQueryResult q;
-    if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &p, cudaEnableDefault, &q) == cudaSuccess && q == cudaDriverEntryPointSuccess)
-      fn = reinterpret_cast<EncodeTiledFn>(p);
-  });
-  return fn;
-}
-
-// [rows][cols] with `ld` elements from row to row, boxes of 64 columns x `box_rows`; outside of it loads give zeros and stores nothing
-static bool encode(CUtensorMap* map, const void* p, bool bf16, long long rows, long long cols, long long ld, int box_rows) {
-  const EncodeTiledFn fn = encode_fn();
-  if (fn == nullptr) return false;
-  cuuint64_t dims[2] = {(cuuint64_t)cols, (cuuint64_t)rows};
-  cuuint64_t strides[1] = {(cuuint64_t)ld * 2};
-  cuuint32_t box[2] = {64, (cuuint32_t)box_rows};
-  cuuint32_t estr[2] = {1, 1};
-  return fn(map, bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 2, const_cast<void*>(p), dims, strides, box, estr,
-            CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
-}
-
-static int blocks_of(long long k) { return (int)((k + kBlockK - 1) / kBlockK); }
 static long long tiles_of(long long rows, long long cols) { return (rows + kTileM - 1) / kTileM * ((cols + kTileN - 1) / kTileN); }
 
-// DX and DW: the tiles of the last, part-filled round in shares along k, where that is shorter.  In blocks of k (0.28 us): a round of the shares takes
-// split_blocks; shared tiles cost the launch behind them, 20, and a quarter of a block for every part that is written and read.  At least 8 blocks a share.
-struct SharePlan { int full, rest, splits, split_blocks; };
-static SharePlan plan_shares(long long rows, long long cols, long long k) {
-  const int pairs = kSms / 2, tiles = (int)tiles_of(rows, cols), blocks = blocks_of(k);
-  SharePlan best{tiles, 0, 1, blocks};
-  const int rest = tiles % pairs;
-  float least = (float)blocks;
-  for (int s = 2; rest > 0 && rest * s <= 2 * pairs && blocks / s >= 8; ++s) {
-    const int each = (blocks + s - 1) / s, shares = (blocks + each - 1) / each;      // none without blocks
-    const float cost = (float)each * ((rest * shares + pairs - 1) / pairs) + 20.f + 0.25f * rest * shares;
-    if (cost < least) {
-      least = cost;
-      best = SharePlan{tiles - rest, rest, shares, each};
-    }
-  }
-  return best;
-}
+// DX and DW
+static SharePlan shares_of(long long rows, long long cols, long long k) { return plan_shares((int)tiles_of(rows, cols), blocks_of(k)); }
 size_t tc_parts_bytes(long long rows, long long cols, long long k) {
-  const SharePlan s = plan_shares(rows, cols, k);
+  const SharePlan s = shares_of(rows, cols, k);
   return s.splits > 1 ? (size_t)s.rest * s.splits * kTileM * kTileN * sizeof(float) : 0;
 }
 
@@ -457,7 +412,7 @@ static cudaError_t launch_use(const GemmMaps& maps, GemmArgs g, int dtype, long 
   const long long tiles = (long long)g.m_tiles * g.n_tiles;
   if (tiles > 0x3fffffffLL) return cudaErrorInvalidValue;
   SharePlan plan{(int)tiles, 0, 1, g.k_blocks};
-  if (USE == DX || USE == DW) plan = plan_shares(g.rows, g.cols, k);
+  if (USE == DX || USE == DW) plan = shares_of(g.rows, g.cols, k);
   g.full = plan.full; g.rest = plan.rest; g.splits = plan.splits; g.split_blocks = plan.split_blocks;
   const int items = g.full + g.rest * g.splits, pairs = items < kSms / 2 ? items : kSms / 2;
   static std::atomic<unsigned long long> smem_set[2];

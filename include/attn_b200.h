@@ -264,6 +264,92 @@ size_t attn_b200_linear_ce_backward_scratch_bytes(const attn_lce_shape_t* shape,
 int attn_b200_linear_ce_backward(const attn_lce_shape_t* shape, const void* x, const void* w, const int64_t* targets, const float* lse,
                                  const float* grad, const float* counted, void* dx, void* dw, void* scratch, void* stream);
 
+/* ---- Matrix products of a layer ----------------------------------------------------------------------
+ * One call is one launch (two where a long sum is shared out) of up to ATTN_PRODUCT_COUNT results, each the sum of up to ATTN_PRODUCT_PAIRS
+ * products of the same sizes, summed in fp32:
+ *   ATTN_FORM_NT   out[i, j] = sum_k a[i, k] b[j, k]      (a layer's output)
+ *   ATTN_FORM_NN   out[i, j] = sum_k a[i, k] b[k, j]      (the gradient of its input)
+ *   ATTN_FORM_TN   out[i, j] = sum_k a[k, i] b[k, j]      (the gradient of its weight)
+ * and what follows them, in one rounding each:
+ *   ATTN_PRODUCT_PLAIN   z = sum + bias[j];  kept[0] = z (not with null);  out = activation(z) + residual.  Bias, activation, residual and
+ *                        kept with one result only
+ *   ATTN_PRODUCT_GATED   NT, one result, one pair: u = the product with b2 in place of b;  kept = (z, u) (not with null);
+ *                        out = activation(z) u
+ *   ATTN_PRODUCT_GATED_GRAD   NN, one result, without bias: given kept = (z, u), out = sum activation'(z) u, out2 = sum activation(z)
+ * Rows are `ld` elements apart, columns dense.  f16 and bf16 on the tensor cores: bases 16-byte aligned, strides multiples of 8;
+ * f32 on the CUDA cores, in any alignment of an element.  Values that are kept are cut to the type's finite range.  Only columns
+ * of a result are written, never what lies between them and the next row.  Inputs must not overlap outputs. */
+enum { ATTN_FORM_NT = 0, ATTN_FORM_NN = 1, ATTN_FORM_TN = 2 };
+enum { ATTN_PRODUCT_PLAIN = 0, ATTN_PRODUCT_GATED = 1, ATTN_PRODUCT_GATED_GRAD = 2 };
+enum { ATTN_ACT_NONE = 0, ATTN_ACT_SILU = 1, ATTN_ACT_GELU = 2, ATTN_ACT_GELU_TANH = 3 };
+enum { ATTN_PRODUCT_PAIRS = 4, ATTN_PRODUCT_COUNT = 3 };
+typedef struct attn_factors { const void *a, *b; int64_t lda, ldb; } attn_factors_t;
+typedef struct attn_product {
+  int32_t rows, cols, k;
+  int32_t pairs;
+  attn_factors_t pair[ATTN_PRODUCT_PAIRS];
+  void* out;
+  int64_t ldo;
+} attn_product_t;
+typedef struct attn_products {
+  int32_t dtype;         /* ATTN_F16 / ATTN_BF16 / ATTN_F32 */
+  int32_t form, kind, activation;
+  int32_t count;
+  int32_t reserved;
+  attn_product_t product[ATTN_PRODUCT_COUNT];
+  const void* bias;                     /* [cols] of the type */
+  const void* residual; int64_t ld_residual;
+  const void* b2; int64_t ldb2;
+  void* kept[2]; int64_t ld_kept[2];
+  void* out2; int64_t ldo2;
+} attn_products_t;
+
+/* A pair of a call of several may be of no length (k = 0): its result is 0.  scratch: 16-byte aligned, null where it takes none. */
+size_t attn_b200_products_scratch_bytes(const attn_products_t* call);
+int attn_b200_products(const attn_products_t* call, void* scratch, void* stream);
+
+/* Elementwise passes around those products in the backward passes, [n, m] in rows `ld` apart, f16 / bf16 / f32, computed in fp32:
+ *   FIRST          in g, z           out dz = g activation'(z)  (none without an activation);  sum: of dz over the rows
+ *   SECOND         in g, z, t        out t activation'(z), s = g activation''(z) t, dz;  sum: of s.  t is the tangent of z
+ *   GATED_SECOND   in gh, z, u, zt, ut, gh2 (or null)   out, with h = a(z) u, zt and ut the tangents of z and u, gh the gradient of h and gh2 a
+ *                  part of the gradient of h's tangent's factor:  ht = a' zt u + a ut,  gh a' u,  gh a,  gh (a'' zt u + a' ut) + gh2 a' u,
+ *                  gh a' zt + gh2 a
+ * sum: [m] of the type, or null; scratch is used with it. */
+enum { ATTN_ELEMENTS_FIRST = 0, ATTN_ELEMENTS_SECOND = 1, ATTN_ELEMENTS_GATED_SECOND = 2 };
+typedef struct attn_elements {
+  int32_t n, m;
+  int32_t dtype, activation, pass;
+  int32_t reserved;
+  const void* in[6]; int64_t ld_in[6];
+  void* out[5]; int64_t ld_out[5];
+  void* sum;
+} attn_elements_t;
+size_t attn_b200_elements_scratch_bytes(const attn_elements_t* e);
+int attn_b200_elements(const attn_elements_t* e, void* scratch, void* stream);
+
+/* ---- Layer norm ---------------------------------------------------------------------------------------
+ * y = (x - mean) / sqrt(variance + eps) w + b over rows of d, d up to 32768; x: [n, d], rows ldx apart (and the gradient's ldg, a tangent's
+ * ldu), results dense; w, b: [d], of the type of x or (param_float) float32, either null for none.  Arithmetic in fp32, rounded once. */
+typedef struct attn_norm_shape {
+  int32_t n, d;
+  int32_t dtype, param_float;
+  float eps;
+  int32_t reserved;
+  int64_t ldx, ldg, ldu;
+} attn_norm_shape_t;
+
+/* mean, rstd: [n] float32, what the backward takes; both null if not wanted */
+int attn_b200_layer_norm(const attn_norm_shape_t* shape, const void* x, const void* w, const void* b, void* y, float* mean, float* rstd,
+                         void* stream);
+/* dx in the type of x, dw and db in that of the parameters, each null if not wanted; scratch is used with dw or db */
+size_t attn_b200_layer_norm_backward_scratch_bytes(const attn_norm_shape_t* shape);
+int attn_b200_layer_norm_backward(const attn_norm_shape_t* shape, const void* x, const void* w, const void* g, const float* mean,
+                                  const float* rstd, void* dx, void* dw, void* db, void* scratch, void* stream);
+/* The derivative of <(dx, dw, db), (u, uw, ub)> with respect to g, x and w: gg, gx, gw, each null if not wanted; u, uw and ub null for 0 */
+int attn_b200_layer_norm_second_backward(const attn_norm_shape_t* shape, const void* x, const void* w, const void* g, const float* mean,
+                                         const float* rstd, const void* u, const void* uw, const void* ub, void* gg, void* gx, void* gw,
+                                         void* scratch, void* stream);
+
 /* Number of kernels the last successful call of the calling thread launched. */
 int attn_b200_last_launch_count(void);
 
@@ -274,7 +360,8 @@ int attn_b200_last_launch_count(void);
  * code here and returns.  Code = (kernel id + 1) << 8 | wait id, kernel ids:
  * 4 / 5 / 6 double-backward scalar + g_dO / g_Q / g_K + g_V kernel, 18 / 19
  * backward row / column kernel, 20 forward, 21 forward of packed batches by pairs of tiles,
- * 32 to 35 the linear cross entropy's products (scores, gradient of the logits, dx, dW), 0x6f the
+ * 32 to 35 the linear cross entropy's products (scores, gradient of the logits, dx, dW), 40 to 44 a layer's
+ * products (plain, with z kept, gated, with both kept, gated gradient), 0x6f the
  * primitive self-test (codes 0x7001..0x7003); wait id 15 = the launch gave the kernel less shared memory
  * than its layout needs. */
 int attn_b200_device_status(uint32_t* code);
