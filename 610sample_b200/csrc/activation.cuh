@@ -86,6 +86,87 @@ __device__ __forceinline__ void activate(float z, float& a, float& d1, float& d2
   if (z != z) a = d1 = d2 = z;      // the bound drops it
 }
 
+// The fast form of two elements at a time, in packed arithmetic: the products' epilogues compute it for every element of a tile, in the time that the
+// tensor cores take for the next one.  a(z), for any z; with GRAD its derivative too, for finite z.
+__device__ __forceinline__ float2 both(float v) { return make_float2(v, v); }
+template <int ACT, bool GRAD>
+__device__ __forceinline__ void activate2(float2 z, float2& a, float2& d) {
+  if constexpr (ACT == ACT_NONE) {
+    a = z;
+    d = both(1.f);
+  } else if constexpr (ACT == ACT_GELU) {
+    const float2 m = make_float2(fminf(fabsf(z.x), 40.f), fminf(fabsf(z.y), 40.f));      // what lies below 40 is 0; NaN comes back with z itself
+    const float2 t1 = __ffma2_rn(both(0.31f), m, both(1.f)), t = make_float2(fast_rcp(t1.x), fast_rcp(t1.y));
+    const float2 q = __fmul2_rn(__fmul2_rn(m, m), both(-0.5f * kLog2e)), e = make_float2(tc::ex2(q.x), tc::ex2(q.y));
+    float2 p = __ffma2_rn(both(-0.07392913f), t, both(0.18045032f));
+    p = __ffma2_rn(p, t, both(0.01574473f));
+    p = __ffma2_rn(p, t, both(0.13342978f));
+    p = __ffma2_rn(p, t, both(0.12044128f));
+    p = __ffma2_rn(p, t, both(0.1238607f));
+    const float2 below = __fmul2_rn(__fmul2_rn(e, t), p), half = __fmul2_rn(z, both(0.5f));
+    // max(z, 0) - |z| F(-|z|)
+    a = __ffma2_rn(make_float2(-m.x, -m.y), below, make_float2(fmaf(0.5f, fabsf(z.x), half.x), fmaf(0.5f, fabsf(z.y), half.y)));
+    if constexpr (GRAD) {
+      const float2 F = make_float2(z.x < 0.f ? below.x : 1.f - below.x, z.y < 0.f ? below.y : 1.f - below.y);
+      d = __ffma2_rn(__fmul2_rn(z, both(0.3989422804014327f)), e, F);
+    }
+  } else {
+    constexpr float kRoot = 1.5957691216057308f, kCube = 0.044715f;      // sqrt(8 / pi)
+    float2 c = z, u = z;
+    if constexpr (ACT == ACT_GELU_TANH) {
+      if constexpr (GRAD) c = make_float2(fminf(fmaxf(z.x, -30.f), 30.f), fminf(fmaxf(z.y, -30.f), 30.f));
+      u = __fmul2_rn(c, __ffma2_rn(__fmul2_rn(c, c), both(kRoot * kCube), both(kRoot)));
+    }
+    const float2 q = __fmul2_rn(u, both(-kLog2e)), e = __fadd2_rn(make_float2(tc::ex2(q.x), tc::ex2(q.y)), both(1.f));
+    const float2 s = make_float2(fast_rcp(e.x), fast_rcp(e.y));
+    a = __fmul2_rn(z, s);
+    if constexpr (GRAD) {      // a' = s + c u' s (1 - s)
+      float2 w = __fmul2_rn(c, s);
+      if constexpr (ACT == ACT_GELU_TANH) w = __fmul2_rn(w, __ffma2_rn(__fmul2_rn(c, c), both(3.f * kRoot * kCube), both(kRoot)));
+      d = __ffma2_rn(w, __fadd2_rn(both(1.f), make_float2(-s.x, -s.y)), s);
+    }
+  }
+}
+
+// What a gated product keeps of a half-precision call, 20 bits a value: 16 in a plane of the type's size, and 4 of either value in a plane of bytes.  A
+// product of two values that were rounded to the type, rounded again, would have gradients 3.0e-3 (bf16) from 64 bits in the 2-norm, where rounding the
+// gradients' own factors and results makes 2.4e-3; 4 more bits cost 1 byte beside 4.  bf16: sign, 8 bits of exponent, 11 of mantissa; f16, cut to its
+// range: 5 and 14.  They are cut off, and read as the middle of what they stand for.
+template <typename T> struct Kept;
+template <> struct Kept<__nv_bfloat16> {
+  static __device__ __forceinline__ uint32_t code(float v) { return __float_as_uint(v); }      // in the upper 20 bits
+  static __device__ __forceinline__ float value(uint32_t code) { return __uint_as_float(code); }
+};
+template <> struct Kept<__half> {
+  // the exponent moved to where 5 bits hold it: what is below goes to denormals, as in f16
+  static __device__ __forceinline__ uint32_t code(float v) {
+    float x = v * 0x1p-112f;
+    asm("min.NaN.f32 %0, %0, %1;" : "+f"(x) : "f"(65504.f * 0x1p-112f));
+    asm("max.NaN.f32 %0, %0, %1;" : "+f"(x) : "f"(-65504.f * 0x1p-112f));
+    const uint32_t b = __float_as_uint(x);
+    return (b & 0x80000000u) | (b << 3 & 0x7fffffffu);      // NaN beyond the largest exponent of a number
+  }
+  static __device__ __forceinline__ float value(uint32_t code) {
+    const float v = __uint_as_float((code & 0x80000000u) | (code & 0x7fffffffu) >> 3) * 0x1p112f;
+    return fabsf(v) >= 65536.f ? NAN : v;
+  }
+};
+// The planes' words of four values of either: the upper halves in pairs, and a word of bytes, bits of z low and of u high
+__device__ __forceinline__ uint32_t kept_high(uint32_t c0, uint32_t c1) { return __byte_perm(c0, c1, 0x7632); }
+__device__ __forceinline__ uint32_t kept_nibbles(const uint32_t (&c)[4]) {      // bits 12 to 15 of each, in the upper halves of bytes
+  return __byte_perm(__byte_perm(c[0], c[1], 0x0051), __byte_perm(c[2], c[3], 0x0051), 0x5410);
+}
+__device__ __forceinline__ uint32_t kept_low(const uint32_t (&z)[4], const uint32_t (&u)[4]) {
+  return (kept_nibbles(z) >> 4 & 0x0f0f0f0fu) | (kept_nibbles(u) & 0xf0f0f0f0u);
+}
+// the codes of value E of four from the halves' pair that holds it and the nibbles' word, 0xf0 or 0x0f of `low` in its place with the middle bit
+__device__ __forceinline__ uint32_t kept_z(uint32_t low) { return (low << 4 & 0xf0f0f0f0u) | 0x08080808u; }
+__device__ __forceinline__ uint32_t kept_u(uint32_t low) { return (low & 0xf0f0f0f0u) | 0x08080808u; }
+template <int E> __device__ __forceinline__ uint32_t kept_code(uint32_t high, uint32_t nibbles) {
+  constexpr uint32_t kHalf = (E & 1) ? 0x3200u : 0x1000u;      // the half's two bytes on top, the nibble's byte below; what is below that counts 2^-16
+  return __byte_perm(high, nibbles, kHalf | (4u + E) << 4 | (4u + E));
+}
+
 // f(tc::Int<activation>): the switch lies outside of the loops over elements
 template <typename F>
 __device__ __forceinline__ void with_activation(int act, F&& f) {
@@ -95,12 +176,17 @@ __device__ __forceinline__ void with_activation(int act, F&& f) {
   else f(tc::Int<ACT_NONE>{});
 }
 
-// A value that is kept for the backward in T: within its finite range, so that the derivatives there are those of a very large z.
-template <typename T> __device__ __forceinline__ float within(float v) { return v; }
-template <> __device__ __forceinline__ float within<__half>(float v) { return v > 65504.f ? 65504.f : v < -65504.f ? -65504.f : v; }
-template <> __device__ __forceinline__ float within<__nv_bfloat16>(float v) {
-  constexpr float kMost = 3.3895313892515355e38f;
-  return v > kMost ? kMost : v < -kMost ? -kMost : v;
+// Two values that are kept for the backward in T, within its finite range: the derivatives there are those of a very large z.
+template <typename T> __device__ __forceinline__ uint32_t pack_finite(float lo, float hi);
+template <> __device__ __forceinline__ uint32_t pack_finite<__half>(float lo, float hi) {
+  uint32_t r;
+  asm("cvt.rn.satfinite.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
+  return r;
+}
+template <> __device__ __forceinline__ uint32_t pack_finite<__nv_bfloat16>(float lo, float hi) {
+  uint32_t r;
+  asm("cvt.rn.satfinite.bf16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
+  return r;
 }
 
 }  // namespace attn

@@ -27,6 +27,19 @@ int check_matrix(const char* name, const void* p, int64_t ld, int cols, int dtyp
   return ATTN_OK;
 }
 
+int check_rows(const char* name, const void* p, int64_t ld, int m, int dtype) {
+  if (p == nullptr) return fail(ATTN_EINVAL, "%s is null", name);
+  if (ld < m || ld > (int64_t(1) << 36)) return fail(ATTN_EINVAL, "%s: rows are %lld elements apart, and %d long", name, (long long)ld, m);
+  if (reinterpret_cast<uintptr_t>(p) % size_of(dtype) != 0) return fail(ATTN_EINVAL, "%s is not aligned", name);
+  return ATTN_OK;
+}
+
+int check_low(const void* p, int64_t ld, int cols) {
+  if (p == nullptr || reinterpret_cast<uintptr_t>(p) % 32 != 0 || ld % 32 != 0 || ld < cols || ld > (int64_t(1) << 36))
+    return fail(ATTN_EINVAL, "kept_low: 32-byte aligned rows of at least %d bytes are needed", cols);
+  return ATTN_OK;
+}
+
 int check_products(const attn_products_t* c, bool pointers) {
   if (c == nullptr) return fail(ATTN_EINVAL, "call is null");
   if (!known_type(c->dtype)) return fail(ATTN_EUNSUPPORTED, "dtype %d: expected ATTN_F16, ATTN_BF16 or ATTN_F32", c->dtype);
@@ -72,12 +85,13 @@ int check_products(const attn_products_t* c, bool pointers) {
   if (first.rows == 0 || first.cols == 0) return ATTN_OK;
   int rc = ATTN_OK;
   if (c->bias != nullptr && reinterpret_cast<uintptr_t>(c->bias) % size_of(c->dtype) != 0) rc = fail(ATTN_EINVAL, "bias is not aligned");
-  if (rc == ATTN_OK && c->residual != nullptr) rc = check_matrix("residual", c->residual, c->ld_residual, first.cols, c->dtype);
+  if (rc == ATTN_OK && c->residual != nullptr) rc = check_rows("residual", c->residual, c->ld_residual, first.cols, c->dtype);
   if (rc == ATTN_OK && c->kind == ATTN_PRODUCT_GATED) rc = check_matrix("b2", c->b2, c->ldb2, first.k, c->dtype);
   const bool both = c->kind == ATTN_PRODUCT_GATED_GRAD || (c->kind == ATTN_PRODUCT_GATED && c->kept[0] != nullptr);
   for (int q = 0; q < 2 && rc == ATTN_OK; ++q)
-    if (both || (plain && q == 0 && c->kept[0] != nullptr)) rc = check_matrix("kept", c->kept[q], c->ld_kept[q], first.cols, c->dtype);
+    if (both || (plain && q == 0 && c->kept[0] != nullptr))  rc = check_matrix("kept", c->kept[q], c->ld_kept[q], first.cols, c->dtype);
   if (rc == ATTN_OK && c->kind == ATTN_PRODUCT_GATED_GRAD) rc = check_matrix("out2", c->out2, c->ldo2, first.cols, c->dtype);
+  if (rc == ATTN_OK && both && c->dtype != ATTN_F32) rc = check_low(c->kept_low, c->ld_low, first.cols);
   return rc;
 }
 
@@ -85,13 +99,6 @@ size_t parts_bytes(const attn_products_t& c) { return c.dtype == ATTN_F32 ? simt
 
 int inputs_of(int pass, int act) { return pass == ATTN_ELEMENTS_FIRST ? (act == ATTN_ACT_NONE ? 1 : 2) : pass == ATTN_ELEMENTS_SECOND ? 3 : 5; }
 int outputs_of(int pass, int act) { return pass == ATTN_ELEMENTS_FIRST ? (act == ATTN_ACT_NONE ? 0 : 1) : pass == ATTN_ELEMENTS_SECOND ? 3 : 5; }
-
-int check_rows(const char* name, const void* p, int64_t ld, int m, int dtype) {
-  if (p == nullptr) return fail(ATTN_EINVAL, "%s is null", name);
-  if (ld < m || ld > (int64_t(1) << 36)) return fail(ATTN_EINVAL, "%s: rows are %lld elements apart, and %d long", name, (long long)ld, m);
-  if (reinterpret_cast<uintptr_t>(p) % size_of(dtype) != 0) return fail(ATTN_EINVAL, "%s is not aligned", name);
-  return ATTN_OK;
-}
 
 int check_elements(const attn_elements_t* e, bool pointers) {
   if (e == nullptr) return fail(ATTN_EINVAL, "call is null");
@@ -106,6 +113,7 @@ int check_elements(const attn_elements_t* e, bool pointers) {
   for (int i = 0; i < 6 && rc == ATTN_OK; ++i)
     if (i < in || (e->pass == ATTN_ELEMENTS_GATED_SECOND && e->in[i] != nullptr)) rc = check_rows("an input", e->in[i], e->ld_in[i], e->m, e->dtype);
   for (int i = 0; i < out && rc == ATTN_OK; ++i) rc = check_rows("a result", e->out[i], e->ld_out[i], e->m, e->dtype);
+  if (rc == ATTN_OK && e->pass == ATTN_ELEMENTS_GATED_SECOND && e->dtype != ATTN_F32) rc = check_low(e->kept_low, e->ld_low, e->m);
   return rc;
 }
 
@@ -117,17 +125,10 @@ int check_norm(const attn_norm_shape_t* s) {
   return ATTN_OK;
 }
 
-// The fewest threads of 32, 128, 512 and 1024 that hold a row in up to 32 elements each (16 with 512 threads, and with 1024 where that will do: more do
-// not fit their registers)
-NormPlan plan_norm(int d, bool wide) {
-  const int vectors = (d + 7) / 8;
-  const int tpr = vectors <= 128 ? 32 : vectors <= 512 ? 128 : vectors <= 1024 ? 512 : 1024;
-  return {tpr, (vectors + tpr - 1) / tpr, wide};
-}
-unsigned groups_of(const NormPlan& p) { return p.tpr >= kNormThreads ? 1u : (unsigned)(kNormThreads / p.tpr); }
+unsigned groups_of(const NormPlan& p) { return p.tpr >= kNormThreads ? 1u : p.tpr == 96 ? 3u : (unsigned)(kNormThreads / p.tpr); }
 // rows of a backward pass go to so many CTAs, which each leave a row of partial sums
 unsigned backward_ctas(const attn_norm_shape_t* s, const NormPlan& p) {
-  const unsigned want = ((unsigned)s->n + groups_of(p) - 1) / groups_of(p), most = 2 * kSms;
+  const unsigned want = ((unsigned)s->n + groups_of(p) - 1) / groups_of(p), most = p.tpr > kNormThreads ? kSms : 2 * kSms;      // that run at a time
   return want < most ? want : most;
 }
 
@@ -200,6 +201,8 @@ int attn_b200_elements(const attn_elements_t* e, void* scratch, void* stream) {
     for (int i = 0; i < 6; ++i)
       if (i < in || e->pass == ATTN_ELEMENTS_GATED_SECOND) { a.in[i] = e->in[i]; a.ld_in[i] = e->ld_in[i]; }
     for (int i = 0; i < out; ++i) { a.out[i] = e->out[i]; a.ld_out[i] = e->ld_out[i]; }
+    a.low = e->kept_low;
+    a.ld_low = e->ld_low;
     a.partial = e->sum != nullptr ? static_cast<float*>(scratch) : nullptr;
     err = launch_elementwise(a, e->pass, e->activation, e->dtype, cs);
     ++launches;
@@ -222,7 +225,7 @@ int attn_b200_layer_norm(const attn_norm_shape_t* s, const void* x, const void* 
   rc = capi::begin(&status);
   if (rc != ATTN_OK) return rc;
   if (s->n == 0) return capi::done(cudaSuccess, "", nullptr, 0);
-  const NormPlan p = plan_norm(s->d, wide_norm(s, {w, b, y}) && wide_rows(s, x, s->ldx));
+  const NormPlan p = plan_norm(s->d, wide_norm(s, {w, b, y}) && wide_rows(s, x, s->ldx), false);
   NormArgs a = norm_args(s, x, w);
   a.b = b;
   a.y = y;
@@ -233,7 +236,7 @@ int attn_b200_layer_norm(const attn_norm_shape_t* s, const void* x, const void* 
 
 size_t attn_b200_layer_norm_backward_scratch_bytes(const attn_norm_shape_t* s) {
   if (check_norm(s) != ATTN_OK) return 0;
-  return (size_t)backward_ctas(s, plan_norm(s->d, true)) * 2 * s->d * sizeof(float);
+  return (size_t)backward_ctas(s, plan_norm(s->d, true, true)) * 2 * s->d * sizeof(float);
 }
 
 static int norm_backward(const attn_norm_shape_t* s, NormArgs a, bool wide, int order, void* sum0, void* sum1, void* scratch, void* stream) {
@@ -249,7 +252,7 @@ static int norm_backward(const attn_norm_shape_t* s, NormArgs a, bool wide, int 
       if (p != nullptr && e == cudaSuccess) e = cudaMemsetAsync(p, 0, (size_t)s->d * size_of(type), cs);
     return capi::done(e, "memset failed", nullptr, 0);
   }
-  const NormPlan p = plan_norm(s->d, wide);
+  const NormPlan p = plan_norm(s->d, wide, true);
   const unsigned ctas = backward_ctas(s, p);
   a.partial = sums ? static_cast<float*>(scratch) : nullptr;
   e = order == 1 ? launch_norm_first(p, a, s->dtype, ctas, cs) : launch_norm_second(p, a, s->dtype, ctas, cs);

@@ -20,6 +20,33 @@ constexpr int kElemCols = 256;
 template <typename T, bool WIDE>
 struct Columns {
   static __device__ __forceinline__ int at(int c0, int e) { return WIDE ? c0 + (int)(threadIdx.x & 31) * 8 + e : c0 + e * 32 + (int)(threadIdx.x & 31); }
+  // the same in two steps, so that several rows can be on their way at once
+  struct Raw { uint32_t w[WIDE && sizeof(T) == 2 ? 4 : 8]; };
+  static __device__ __forceinline__ Raw fetch(const void* p, long long ld, int r, int c0, int m) {
+    Raw raw;
+    if constexpr (WIDE && sizeof(T) == 2) {
+      const uint4 a = at(c0, 0) < m ? from_l2(reinterpret_cast<const uint4*>(static_cast<const T*>(p) + r * ld + at(c0, 0))) : make_uint4(0u, 0u, 0u, 0u);
+      raw.w[0] = a.x; raw.w[1] = a.y; raw.w[2] = a.z; raw.w[3] = a.w;
+    } else {
+      float f[8];
+      load(p, ld, r, c0, m, f);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) raw.w[e] = __float_as_uint(f[e]);
+    }
+    return raw;
+  }
+  static __device__ __forceinline__ void values(const Raw& raw, float (&f)[8]) {
+    if constexpr (WIDE && sizeof(T) == 2) {
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const float2 b = tc::Pack<T>::unpack(raw.w[e]);
+        f[2 * e] = b.x; f[2 * e + 1] = b.y;
+      }
+    } else {
+#pragma unroll
+      for (int e = 0; e < 8; ++e) f[e] = __uint_as_float(raw.w[e]);
+    }
+  }
   static __device__ __forceinline__ void load(const void* p, long long ld, int r, int c0, int m, float (&f)[8]) {
     const T* row = static_cast<const T*>(p) + r * ld;
     if constexpr (WIDE) {      // m is a multiple of 8
@@ -42,6 +69,20 @@ struct Columns {
 #pragma unroll
       for (int e = 0; e < 8; ++e) f[e] = at(c0, e) < m ? Elem<T>::to_float(row[at(c0, e)]) : 0.f;
     }
+  }
+  // z and u as a gated product keeps them, whose upper halves have been loaded as if they were values of the type
+  static __device__ __forceinline__ void with_low(const void* low, long long ld, int r, int c0, int m, float (&z)[8], float (&u)[8]) {
+    const uint8_t* row = static_cast<const uint8_t*>(low) + r * ld;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      const uint32_t b = at(c0, e) < m ? row[at(c0, e)] : 0u;
+      z[e] = Kept<T>::value(kept_code<0>(bits(z[e]), kept_z(b)));
+      u[e] = Kept<T>::value(kept_code<0>(bits(u[e]), kept_u(b)));
+    }
+  }
+  static __device__ __forceinline__ uint32_t bits(float v) {
+    const T h = Elem<T>::from_float(v);
+    return *reinterpret_cast<const uint16_t*>(&h);
   }
   static __device__ __forceinline__ void store(void* p, long long ld, int r, int c0, int m, const float (&f)[8]) {
     T* row = static_cast<T*>(p) + r * ld;
@@ -79,24 +120,52 @@ elementwise_kernel(const __grid_constant__ ElementArgs a) {
   for (int e = 0; e < 8; ++e) sum[e] = 0.f;
   auto load = [&](int i, int r, float (&f)[8]) { C::load(a.in[i], a.ld_in[i], r, c0, a.m, f); };
   auto store = [&](int i, int r, const float (&f)[8]) { C::store(a.out[i], a.ld_out[i], r, c0, a.m, f); };
+  if constexpr (PASS == PASS_FIRST) {
+    constexpr int kRows = sizeof(T) == 2 ? 4 : 2;      // of a thread, on their way at once
+    for (int r0 = (int)first + group; r0 < end; r0 += 8 * kRows) {
+      typename C::Raw rg[kRows], rz[ACT != ACT_NONE ? kRows : 1];
+#pragma unroll
+      for (int i = 0; i < kRows; ++i) {
+        const int r = min(r0 + 8 * i, end - 1);
+        rg[i] = C::fetch(a.in[0], a.ld_in[0], r, c0, a.m);
+        if constexpr (ACT != ACT_NONE) rz[i] = C::fetch(a.in[1], a.ld_in[1], r, c0, a.m);
+      }
+#pragma unroll
+      for (int i = 0; i < kRows; ++i) {
+        const int r = r0 + 8 * i;
+        if (r >= end) break;      // uniform within a warp
+        float g[8];
+        C::values(rg[i], g);
+        if constexpr (ACT != ACT_NONE) {
+          float z[8];
+          C::values(rz[i], z);
+#pragma unroll
+          for (int e = 0; e < 8; e += 2) {
+            if constexpr (kPrecise) {
+              float v, d1, d2;
+              activate<ACT, true, 1>(z[e], v, d1, d2);
+              g[e] *= d1;
+              activate<ACT, true, 1>(z[e + 1], v, d1, d2);
+              g[e + 1] *= d1;
+            } else {
+              float2 v, d;
+              activate2<ACT, true>(make_float2(z[e], z[e + 1]), v, d);
+              g[e] *= d.x;
+              g[e + 1] *= d.y;
+            }
+          }
+          store(0, r, g);
+        }
+#pragma unroll
+        for (int e = 0; e < 8; ++e) sum[e] += g[e];
+      }
+    }
+  } else
 #pragma unroll 2
   for (int r = (int)first + group; r < end; r += 8) {
     float g[8], z[8];
     load(0, r, g);
-    if constexpr (PASS == PASS_FIRST) {
-      if constexpr (ACT != ACT_NONE) {
-        load(1, r, z);
-#pragma unroll
-        for (int e = 0; e < 8; ++e) {
-          float v, d1, d2;
-          activate<ACT, kPrecise, 1>(z[e], v, d1, d2);
-          g[e] *= d1;
-        }
-        store(0, r, g);
-      }
-#pragma unroll
-      for (int e = 0; e < 8; ++e) sum[e] += g[e];
-    } else if constexpr (PASS == PASS_SECOND) {
+    if constexpr (PASS == PASS_SECOND) {
       float t[8], gg[8], s[8];
       load(1, r, z);
       load(2, r, t);
@@ -116,6 +185,7 @@ elementwise_kernel(const __grid_constant__ ElementArgs a) {
       float u[8], zt[8], ut[8], gh2[8], ht[8], ez[8], eu[8], dz[8], du[8];
       load(1, r, z);
       load(2, r, u);
+      if constexpr (!kPrecise) C::with_low(a.low, a.ld_low, r, c0, a.m, z, u);
       load(3, r, zt);
       load(4, r, ut);
       if (a.in[5] != nullptr) load(5, r, gh2);
@@ -151,20 +221,21 @@ elementwise_kernel(const __grid_constant__ ElementArgs a) {
 
 // column sums: out[k][c] = sum over the rows of partial [rows][kinds][d], in order; a CTA has 32 columns of one kind
 template <typename P>
-__global__ void __launch_bounds__(256)
+__global__ void __launch_bounds__(1024)
 sum_rows_kernel(const float* partial, int rows, int kinds, int d, P* out0, P* out1) {
-  __shared__ float s[8][32];
+  __shared__ float s[32][32];
   tc::pdl_wait();
   tc::pdl_trigger();
   const int x = threadIdx.x & 31, y = threadIdx.x >> 5, c = blockIdx.x * 32 + x, k = blockIdx.y;
   float v = 0.f;
   if (c < d)
-#pragma unroll 8
-    for (int i = y; i < rows; i += 8) v += from_l2(partial + ((size_t)i * kinds + k) * d + c);
+#pragma unroll 10
+    for (int i = y; i < rows; i += 32) v += from_l2(partial + ((size_t)i * kinds + k) * d + c);
   s[y][x] = v;
   __syncthreads();
   if (y != 0 || c >= d) return;
-  for (int i = 1; i < 8; ++i) v += s[i][x];
+#pragma unroll
+  for (int i = 1; i < 32; ++i) v += s[i][x];
   P* out = k == 0 ? out0 : out1;
   if (out != nullptr) out[c] = Elem<P>::from_float(v);
 }
@@ -175,7 +246,7 @@ cudaError_t launch_sum_rows(const float* partial, int rows, int kinds, int d, in
   attr.val.programmaticStreamSerializationAllowed = 1;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)((d + 31) / 32), (unsigned)kinds);
-  cfg.blockDim = dim3(256);
+  cfg.blockDim = dim3(1024);
   cfg.stream = stream;
   cfg.attrs = &attr;
   cfg.numAttrs = 1;

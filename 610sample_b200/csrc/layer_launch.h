@@ -26,6 +26,8 @@ struct ElementArgs {
   int chunk;                     // rows of a run, filled in by the launch
   const void* in[6];
   long long ld_in[6];
+  const void* low;               // the lower bits of z and u, half types of PASS_GATED_SECOND
+  long long ld_low;
   void* out[5];
   long long ld_out[5];
   float* partial;

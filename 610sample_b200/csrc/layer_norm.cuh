@@ -6,8 +6,7 @@
 //            to x: r (q - m(q) - xh m(q xh)) - r^2 xh (m(c u) - m(c) m(u) - m(c xh) m(u xh)),  q = g uw - r (c m(u xh) + u m(c xh))
 //            m(q) and m(q xh) follow from the means of c, u, g uw and their products with xh, so one round of sums over the row does
 //
-// Every pass reads its rows once: a row stays in the registers of a group of 32 to 1024 threads, up to 32 elements each, so that the variance is that of
-// the centred row.  Bound by memory.  Sums over the rows stay in registers while a group goes from row to row, its next row on the way; a
+// Every pass reads its rows once: a row stays in the registers of a group of 32 to 1024 threads, so that the variance is that of the centred row.  Bound by memory.  Sums over the rows stay in registers while a group goes from row to row, its next row on the way; a
 // kernel behind adds what the CTAs have, in order.
 #pragma once
 
@@ -33,8 +32,22 @@ struct NormArgs {
   long long ldx, ldg, ldu;
 };
 
-// How a row lies in a group: `tpr` threads with `vectors` times eight elements each; wide: with 16-byte loads
+// How a row lies in a group: `tpr` threads with `vectors` times eight elements each; wide: with 16-byte loads.  The fewest threads that hold it in
+// 32 elements each; in the backward passes, which keep sums and the next row beside it, in 16 up to 16384, and three warps for 768 and a little
+// less (dx and dw of 8195 x 4096 f16 with 32 elements each took 58 us, of 16384 x 768 bf16 with 24 43 to 56: one CTA an SM, or spills).
 struct NormPlan { int tpr, vectors; bool wide; };
+inline NormPlan plan_norm(int d, bool wide, bool backward) {
+  const int vectors = (d + 7) / 8;
+  if (!backward) {
+    const int tpr = vectors <= 128 ? 32 : vectors <= 512 ? 128 : vectors <= 2048 ? 512 : 1024;
+    return {tpr, (vectors + tpr - 1) / tpr, wide};
+  }
+  if (vectors <= 64) return {32, (vectors + 31) / 32, wide};
+  if (vectors <= 96) return {96, 1, wide};
+  int tpr = 64;
+  while (tpr < 1024 && vectors > 2 * tpr) tpr *= 2;
+  return {tpr, vectors > 2 * tpr ? 4 : 2, wide};
+}
 
 // Eight elements of a row at a time.  WIDE: in sequence, with 16-byte loads; else one by one, neighbouring threads on neighbouring elements, for any
 // width and alignment.
@@ -133,7 +146,7 @@ __device__ __forceinline__ void parameter(const void* p, bool is_float, int t, i
   }
 }
 
-// Sums over the TPR threads of a group; all threads of the CTA call it.  `turn` alternates between two places in shared memory.
+// Sums over the TPR threads of a group, all of which call it.  `turn` alternates between two places in shared memory.
 template <int TPR, int THREADS, int K>
 __device__ __forceinline__ void group_sum(float (&v)[K], float* shared, int& turn) {
 #pragma unroll
@@ -148,7 +161,7 @@ __device__ __forceinline__ void group_sum(float (&v)[K], float* shared, int& tur
     if ((threadIdx.x & 31) == 0)
 #pragma unroll
       for (int k = 0; k < K; ++k) s[k * kWarps + warp] = v[k];
-    __syncthreads();
+    tc::named_barrier_sync(1 + first / kMine, TPR);
 #pragma unroll
     for (int k = 0; k < K; ++k) {
       float sum = 0.f;
@@ -158,7 +171,7 @@ __device__ __forceinline__ void group_sum(float (&v)[K], float* shared, int& tur
     }
   }
 }
-template <int TPR> constexpr int kThreadsOf = TPR > kNormThreads ? TPR : kNormThreads;
+template <int TPR> constexpr int kThreadsOf = TPR > kNormThreads ? TPR : TPR == 96 ? 288 : kNormThreads;
 
 template <typename T, int TPR, int V, bool WIDE>
 __global__ void __launch_bounds__(kThreadsOf<TPR>, 1)
@@ -208,7 +221,7 @@ norm_forward_kernel(const NormArgs a) {
 
 // ORDER 1: dx, sums dw and db.  ORDER 2: the gradients of g and x, sum dw.
 template <typename T, int TPR, int V, bool WIDE, int ORDER>
-__global__ void __launch_bounds__(kThreadsOf<TPR>, 1)
+__global__ void __launch_bounds__(kThreadsOf<TPR>, ORDER == 1 && TPR <= kNormThreads ? 2 : 1)
 norm_backward_kernel(const NormArgs a) {
   constexpr int kThreads = kThreadsOf<TPR>, kGroups = kThreads / TPR, kSums = ORDER == 1 ? 2 : 1, kMeans = ORDER == 1 ? 2 : 7;
   __shared__ float sums[2 * kMeans * (kThreads / 32)];
@@ -226,104 +239,150 @@ norm_backward_kernel(const NormArgs a) {
       for (int e = 0; e < 8; ++e) total[k][v][e] = 0.f;
   int turn = 0;
   const float over = 1.f / (float)a.d;
-  typename L::Raw rx[V], rg[V], ru[ORDER == 2 ? V : 1];
-  float mean, r;
-  auto fetch = [&](long long row) {
-    const long long at = row < a.n ? row : 0;
+  // a row stays as it was read: what follows from it is computed before the sums over the row and again behind them, in fewer registers
+  struct Row { typename L::Raw x[V], g[V], u[ORDER == 2 ? V : 1]; float mean, r; };
+  auto fetch = [&](Row& row, long long at) {
 #pragma unroll
     for (int v = 0; v < V; ++v) {
-      rx[v] = L::load(static_cast<const T*>(a.x) + at * a.ldx, t, v, a.d);
-      rg[v] = L::load(static_cast<const T*>(a.g) + at * a.ldg, t, v, a.d);
+      row.x[v] = L::load(static_cast<const T*>(a.x) + at * a.ldx, t, v, a.d);
+      row.g[v] = L::load(static_cast<const T*>(a.g) + at * a.ldg, t, v, a.d);
       if constexpr (ORDER == 2)
-        if (a.u != nullptr) ru[v] = L::load(static_cast<const T*>(a.u) + at * a.ldu, t, v, a.d);
+        row.u[v] = a.u == nullptr ? typename L::Raw{} : L::load(static_cast<const T*>(a.u) + at * a.ldu, t, v, a.d);
     }
-    mean = from_l2(a.mean + at);
-    r = from_l2(a.rstd + at);
+    row.mean = from_l2(a.mean + at);
+    row.r = from_l2(a.rstd + at);
   };
-  // all groups of a CTA go the same number of rounds: they meet in the sums
-  const long long first = blockIdx.x * (long long)kGroups;
-  if (first < a.n) fetch(first + group);
-  for (long long base = first; base < a.n; base += stride) {
-    const long long row = base + group;
-    const bool in = row < a.n;
-    float xh[V][8], c[V][8], u[ORDER == 2 ? V : 1][8];
-    const float rs = r;
+  auto normed = [&](const Row& row, int v, float (&xh)[8]) {
+    L::values(row.x[v], xh);
+#pragma unroll
+    for (int e = 0; e < 8; e += 2) {
+      const float2 h = __fmul2_rn(__fadd2_rn(make_float2(xh[e], xh[e + 1]), make_float2(-row.mean, -row.mean)), make_float2(row.r, row.r));
+      xh[e] = h.x; xh[e + 1] = h.y;
+    }
+  };
+  auto as_read = [](typename L::Raw& raw) {      // keeps the compiler from holding on to the values instead
+#pragma unroll
+    for (int i = 0; i < (int)(sizeof(raw.w) / 4); ++i) asm volatile("" : "+r"(raw.w[i]));
+  };
+  // w in fp32, for as many threads as fill their registers with sums over the rows
+  constexpr bool kSharedW = TPR <= 512;
+  __shared__ __align__(16) float weight[kSharedW ? TPR * V * 8 : 4];
+  if constexpr (kSharedW) {
+    for (int i = threadIdx.x; i < TPR * V; i += kThreads) {
+      float w[8];
+      parameter<L, T, WIDE>(a.w, a.param_float, i % TPR, i / TPR, a.d, 1.f, w);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) weight[(i / TPR) * TPR * 8 + (e >> 2) * TPR * 4 + (i % TPR) * 4 + (e & 3)] = w[e];
+    }
+    __syncthreads();
+  }
+  auto weight_of = [&](int v, float (&w)[8]) {
+    if constexpr (kSharedW) {
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const float4 q = *reinterpret_cast<const float4*>(&weight[v * TPR * 8 + h * TPR * 4 + t * 4]);
+        w[4 * h] = q.x; w[4 * h + 1] = q.y; w[4 * h + 2] = q.z; w[4 * h + 3] = q.w;
+      }
+    } else {
+      parameter<L, T, WIDE>(a.w, a.param_float, t, v, a.d, 1.f, w);
+    }
+  };
+  Row next;
+  const long long first = blockIdx.x * (long long)kGroups + group;
+  if (first < a.n) fetch(next, first);
+  for (long long at = first; at < a.n; at += stride) {
+    Row row = next;
+    if (at + stride < a.n) fetch(next, at + stride);
     float m[kMeans];
 #pragma unroll
     for (int k = 0; k < kMeans; ++k) m[k] = 0.f;
+    [[maybe_unused]] float2 m0 = make_float2(0.f, 0.f), m1 = m0;
 #pragma unroll
     for (int v = 0; v < V; ++v) {
-      float x[8], g[8], w[8];
-      L::values(rx[v], x);
-      L::values(rg[v], g);
-      parameter<L, T, WIDE>(a.w, a.param_float, t, v, a.d, 1.f, w);
-#pragma unroll
-      for (int e = 0; e < 8; ++e) xh[v][e] = L::inside(t, v, e, a.d) ? (x[e] - mean) * r : 0.f;      // g is 0 outside
+      float xh[8], g[8], w[8];      // g and u are 0 outside of the row, and everything is a multiple of them
+      normed(row, v, xh);
+      L::values(row.g[v], g);
+      weight_of(v, w);
       if constexpr (ORDER == 1) {
 #pragma unroll
-        for (int e = 0; e < 8; ++e) {
-          c[v][e] = g[e] * w[e];
-          m[0] += c[v][e];
-          m[1] = fmaf(c[v][e], xh[v][e], m[1]);
-          if (in) {
-            total[0][v][e] = fmaf(g[e], xh[v][e], total[0][v][e]);
-            total[1][v][e] += g[e];
-          }
+        for (int e = 0; e < 8; e += 2) {
+          const float2 gg = make_float2(g[e], g[e + 1]), h = make_float2(xh[e], xh[e + 1]), c = __fmul2_rn(gg, make_float2(w[e], w[e + 1]));
+          m0 = __fadd2_rn(m0, c);
+          m1 = __ffma2_rn(c, h, m1);
+          const float2 t0 = __ffma2_rn(gg, h, make_float2(total[0][v][e], total[0][v][e + 1])), t1 = __fadd2_rn(gg, make_float2(total[1][v][e], total[1][v][e + 1]));
+          total[0][v][e] = t0.x; total[0][v][e + 1] = t0.y;
+          total[1][v][e] = t1.x; total[1][v][e + 1] = t1.y;
         }
       } else {
-        float uw[8];
+        float uw[8], u[8];
         parameter<L, T, WIDE>(a.uw, a.param_float, t, v, a.d, 0.f, uw);
-        if (a.u != nullptr) L::values(ru[v], u[v]);
-        else
-#pragma unroll
-          for (int e = 0; e < 8; ++e) u[v][e] = 0.f;
+        L::values(row.u[v], u);
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
-          const float h = xh[v][e], cc = g[e] * w[e], q = g[e] * uw[e], uu = u[v][e];
-          c[v][e] = g[e];
-          m[0] += cc;
-          m[1] = fmaf(cc, h, m[1]);
-          m[2] += uu;
-          m[3] = fmaf(uu, h, m[3]);
-          m[4] = fmaf(cc, uu, m[4]);
+          const float c = g[e] * w[e], q = g[e] * uw[e];
+          m[0] += c;
+          m[1] = fmaf(c, xh[e], m[1]);
+          m[2] += u[e];
+          m[3] = fmaf(u[e], xh[e], m[3]);
+          m[4] = fmaf(c, u[e], m[4]);
           m[5] += q;
-          m[6] = fmaf(q, h, m[6]);
+          m[6] = fmaf(q, xh[e], m[6]);
         }
       }
     }
-    if (base + stride < a.n) fetch(row + stride);
+    if constexpr (ORDER == 1) {
+      m[0] = m0.x + m0.y;
+      m[1] = m1.x + m1.y;
+    }
     group_sum<TPR, kThreads>(m, sums, turn);
 #pragma unroll
     for (int k = 0; k < kMeans; ++k) m[k] *= over;
-    if (!in) continue;
+#pragma unroll
+    for (int v = 0; v < V; ++v) {
+      as_read(row.x[v]);
+      as_read(row.g[v]);
+      if constexpr (ORDER == 2) as_read(row.u[v]);
+    }
+    const float r = row.r;
     if constexpr (ORDER == 1) {
       if (a.gx != nullptr) {
 #pragma unroll
         for (int v = 0; v < V; ++v) {
+          float xh[8], g[8], w[8];
+          normed(row, v, xh);
+          L::values(row.g[v], g);
+          weight_of(v, w);
 #pragma unroll
-          for (int e = 0; e < 8; ++e) c[v][e] = rs * (c[v][e] - m[0] - xh[v][e] * m[1]);
-          L::store(static_cast<T*>(a.gx) + row * a.d, t, v, a.d, c[v]);
+          for (int e = 0; e < 8; e += 2) {
+            float2 c = __ffma2_rn(make_float2(g[e], g[e + 1]), make_float2(w[e], w[e + 1]), make_float2(-m[0], -m[0]));
+            c = __fmul2_rn(__ffma2_rn(make_float2(xh[e], xh[e + 1]), make_float2(-m[1], -m[1]), c), make_float2(r, r));
+            g[e] = c.x; g[e + 1] = c.y;
+          }
+          L::store(static_cast<T*>(a.gx) + at * a.d, t, v, a.d, g);
         }
       }
     } else {
       const float mc = m[0], mch = m[1], mu = m[2], muh = m[3];
-      const float mq = m[5] - rs * (mc * muh + mu * mch), mqh = m[6] - 2.f * rs * mch * muh, turned = rs * rs * (m[4] - mc * mu - mch * muh);
+      const float mq = m[5] - r * (mc * muh + mu * mch), mqh = m[6] - 2.f * r * mch * muh, turned = r * r * (m[4] - mc * mu - mch * muh);
 #pragma unroll
       for (int v = 0; v < V; ++v) {
-        float w[8], uw[8], ub[8], gg[8], gx[8];
-        parameter<L, T, WIDE>(a.w, a.param_float, t, v, a.d, 1.f, w);
+        float xh[8], g[8], u[8], w[8], uw[8], ub[8], gg[8], gx[8];
+        normed(row, v, xh);
+        L::values(row.g[v], g);
+        L::values(row.u[v], u);
+        weight_of(v, w);
         parameter<L, T, WIDE>(a.uw, a.param_float, t, v, a.d, 0.f, uw);
         parameter<L, T, WIDE>(a.ub, a.param_float, t, v, a.d, 0.f, ub);
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
-          const float h = xh[v][e], g = c[v][e], uu = u[v][e], moved = rs * (uu - mu - h * muh);
-          gg[e] = fmaf(w[e], moved, fmaf(uw[e], h, ub[e]));
-          const float q = fmaf(-rs, g * w[e] * muh + uu * mch, g * uw[e]);
-          gx[e] = rs * (q - mq - h * mqh) - h * turned;
-          total[0][v][e] = fmaf(g, moved, total[0][v][e]);
+          const float h = xh[e], P = r * (u[e] - mu - h * muh);
+          gg[e] = fmaf(w[e], P, fmaf(uw[e], h, ub[e]));
+          const float q = fmaf(-r, g[e] * w[e] * muh + u[e] * mch, g[e] * uw[e]);
+          gx[e] = r * (q - mq - h * mqh) - h * turned;
+          total[0][v][e] = fmaf(g[e], P, total[0][v][e]);
         }
-        if (a.y != nullptr) L::store(static_cast<T*>(a.y) + row * a.d, t, v, a.d, gg);
-        if (a.gx != nullptr) L::store(static_cast<T*>(a.gx) + row * a.d, t, v, a.d, gx);
+        if (a.y != nullptr) L::store(static_cast<T*>(a.y) + at * a.d, t, v, a.d, gg);
+        if (a.gx != nullptr) L::store(static_cast<T*>(a.gx) + at * a.d, t, v, a.d, gx);
       }
     }
   }
@@ -358,21 +417,27 @@ inline cudaError_t launch_norm(const NormArgs& a, unsigned ctas, cudaStream_t st
 template <typename T, bool WIDE, int ORDER>
 inline cudaError_t launch_plan(const NormPlan& p, const NormArgs& a, unsigned ctas, cudaStream_t stream) {
   if (p.tpr == 32) {
-    if constexpr (WIDE) {
-      if (p.vectors == 2) return launch_norm<T, 32, 2, WIDE, ORDER>(a, ctas, stream);
-      if (p.vectors == 3) return launch_norm<T, 32, 3, WIDE, ORDER>(a, ctas, stream);
-    }
-    return p.vectors == 1 ? launch_norm<T, 32, 1, WIDE, ORDER>(a, ctas, stream) : launch_norm<T, 32, 4, WIDE, ORDER>(a, ctas, stream);
+    if (p.vectors == 1) return launch_norm<T, 32, 1, WIDE, ORDER>(a, ctas, stream);
+    if (p.vectors == 2) return launch_norm<T, 32, 2, WIDE, ORDER>(a, ctas, stream);
   }
-  if (p.tpr == 128) {
-    if constexpr (WIDE) {
-      if (p.vectors == 2) return launch_norm<T, 128, 2, WIDE, ORDER>(a, ctas, stream);
-      if (p.vectors == 3) return launch_norm<T, 128, 3, WIDE, ORDER>(a, ctas, stream);
+  if constexpr (ORDER == 0) {
+    if (p.tpr == 32 && p.vectors == 3) return launch_norm<T, 32, 3, WIDE, 0>(a, ctas, stream);
+    if (p.tpr == 32) return launch_norm<T, 32, 4, WIDE, 0>(a, ctas, stream);
+    if (p.tpr == 128) return p.vectors == 2   ? launch_norm<T, 128, 2, WIDE, 0>(a, ctas, stream)
+                             : p.vectors == 3 ? launch_norm<T, 128, 3, WIDE, 0>(a, ctas, stream)
+                                              : launch_norm<T, 128, 4, WIDE, 0>(a, ctas, stream);
+    if (p.tpr == 512) return p.vectors == 2 ? launch_norm<T, 512, 2, WIDE, 0>(a, ctas, stream) : launch_norm<T, 512, 4, WIDE, 0>(a, ctas, stream);
+    return launch_norm<T, 1024, 4, WIDE, 0>(a, ctas, stream);
+  } else {
+    switch (p.tpr) {
+      case 96: return launch_norm<T, 96, 1, WIDE, ORDER>(a, ctas, stream);
+      case 64: return launch_norm<T, 64, 2, WIDE, ORDER>(a, ctas, stream);
+      case 128: return launch_norm<T, 128, 2, WIDE, ORDER>(a, ctas, stream);
+      case 256: return launch_norm<T, 256, 2, WIDE, ORDER>(a, ctas, stream);
+      case 512: return launch_norm<T, 512, 2, WIDE, ORDER>(a, ctas, stream);
+      default: return p.vectors == 2 ? launch_norm<T, 1024, 2, WIDE, ORDER>(a, ctas, stream) : launch_norm<T, 1024, 4, WIDE, ORDER>(a, ctas, stream);
     }
-    return launch_norm<T, 128, 4, WIDE, ORDER>(a, ctas, stream);
   }
-  if (p.tpr == 512) return launch_norm<T, 512, 2, WIDE, ORDER>(a, ctas, stream);
-  return p.vectors <= 2 ? launch_norm<T, 1024, 2, WIDE, ORDER>(a, ctas, stream) : launch_norm<T, 1024, 4, WIDE, ORDER>(a, ctas, stream);
 }
 template <int ORDER>
 inline cudaError_t launch_typed(const NormPlan& p, const NormArgs& a, int dtype, unsigned ctas, cudaStream_t stream) {

@@ -44,6 +44,22 @@ torch::Tensor handed(const Matrix& m, at::IntArrayRef sizes) {
   return t.sizes() == sizes ? t : t.view(sizes);
 }
 
+// What a gated product keeps (attn_products_t): of half types z and u in rows of whole sectors, and a plane of bytes
+struct KeptPlanes {
+  Matrix z, u;
+  torch::Tensor low;
+  int64_t ld_low = 0;
+};
+KeptPlanes kept_planes(int64_t rows, int64_t cols, const torch::Tensor& like) {
+  if (like.scalar_type() == at::kFloat) return {result(rows, cols, like), result(rows, cols, like), torch::Tensor(), 0};
+  const int64_t pitch = (cols + 15) / 16 * 16, bytes = (cols + 31) / 32 * 32;
+  auto plane = [&] { return Matrix{fresh({rows, pitch}, like.scalar_type(), like), pitch}; };
+  return {plane(), plane(), fresh({rows, bytes}, at::kByte, like), bytes};
+}
+KeptPlanes kept_planes(const torch::Tensor& z, const torch::Tensor& u, const torch::Tensor& low) {
+  return {{z, z.size(1)}, {u, u.size(1)}, low, low.defined() ? low.size(1) : 0};
+}
+
 std::vector<int64_t> with_columns(const torch::Tensor& x, int64_t cols) {
   std::vector<int64_t> sizes = x.sizes().vec();
   sizes.back() = cols;
@@ -86,6 +102,12 @@ struct Products {
     if (m.t.defined()) { c.kept[i] = const_cast<void*>(m.data()); c.ld_kept[i] = m.ld; }
     return *this;
   }
+  Products& kept(const KeptPlanes& k) {
+    if (!k.z.t.defined()) return *this;
+    kept(0, k.z).kept(1, k.u);
+    if (k.low.defined()) { c.kept_low = k.low.data_ptr(); c.ld_low = k.ld_low; }
+    return *this;
+  }
   void run(const char* what) {
     if (c.count == 0) return;
     const int64_t bytes = (int64_t)attn_b200_products_scratch_bytes(&c);
@@ -108,6 +130,10 @@ struct Elements {
   Elements& in(int i, const Matrix& m) {
     if (m.t.defined()) { e.in[i] = m.data(); e.ld_in[i] = m.ld; }
     return *this;
+  }
+  Elements& kept(int i, const KeptPlanes& k) {
+    if (k.low.defined()) { e.kept_low = k.low.data_ptr(); e.ld_low = k.ld_low; }
+    return in(i, k.z).in(i + 1, k.u);
   }
   Elements& out(int i, const Matrix& m) {
     e.out[i] = m.t.data_ptr();
@@ -323,31 +349,29 @@ void check_gated(const torch::Tensor& x, const torch::Tensor& wg, const torch::T
   TORCH_CHECK(!r.defined() || r.sizes() == at::IntArrayRef(with_columns(x, wd.size(0))), "residual must have the shape of the result");
 }
 
-// {y, z, u, h}; z = x wg^T and u = x wu^T where they are to be kept, h = a(z) u
+// {y, z, u, their lower bits, h}; z = x wg^T and u = x wu^T where they are to be kept, h = a(z) u
 variable_list gated_forward(const torch::Tensor& x_in, const torch::Tensor& wg_in, const torch::Tensor& wu_in, const torch::Tensor& wd_in,
                             const torch::Tensor& r_in, int64_t activation, bool keep) {
   c10::cuda::CUDAGuard guard(x_in.device());
   begin_call(x_in);
   const int64_t d = columns_of(x_in), n = x_in.numel() / d, f = wg_in.size(0), m = wd_in.size(0);
   const Matrix x = matrix(x_in), wg = matrix(wg_in), wu = matrix(wu_in), wd = matrix(wd_in), h = result(n, f, x_in), y = result(n, m, x_in);
-  Matrix r, z, u;
+  Matrix r;
+  KeptPlanes kept;
   if (r_in.defined()) r = matrix(r_in);
-  if (keep) {
-    z = result(n, f, x_in);
-    u = result(n, f, x_in);
-  }
+  if (keep) kept = kept_planes(n, f, x_in);
   Products inner(x_in, ATTN_FORM_NT, ATTN_PRODUCT_GATED, activation);
-  inner.add(h, n, f, d, {{&x, &wg}}).kept(0, z).kept(1, u);
+  inner.add(h, n, f, d, {{&x, &wg}}).kept(kept);
   inner.c.b2 = wu.data();
   inner.c.ldb2 = wu.ld;
   inner.run("gated_feed_forward");
   Products(x_in, ATTN_FORM_NT).add(y, n, m, f, {{&h, &wd}}).residual(r).run("gated_feed_forward");
-  return {handed(y, with_columns(x_in, m)), z.t, u.t, h.t};
+  return {handed(y, with_columns(x_in, m)), kept.z.t, kept.u.t, kept.low, h.t};
 }
 
 // {dx, dwg, dwu, dwd}, undefined where not wanted.  The gradient of h exists in the product's epilogue only, where it becomes those of z and u.
 variable_list gated_backward(const torch::Tensor& g_in, const torch::Tensor& x_in, const torch::Tensor& wg_in, const torch::Tensor& wu_in,
-                             const torch::Tensor& wd_in, const torch::Tensor& z_in, const torch::Tensor& u_in, const torch::Tensor& h_in,
+                             const torch::Tensor& wd_in, const KeptPlanes& kept, const torch::Tensor& h_in,
                              int64_t activation, bool want_x, bool want_g, bool want_u, bool want_d) {
   variable_list out(4);
   if (!want_x && !want_g && !want_u && !want_d) return out;
@@ -361,7 +385,7 @@ variable_list gated_backward(const torch::Tensor& g_in, const torch::Tensor& x_i
     dz = result(n, f, x_in);
     du = result(n, f, x_in);
     Products inner(x_in, ATTN_FORM_NN, ATTN_PRODUCT_GATED_GRAD, activation);
-    inner.add(dz, n, f, m, {{&g, &wd}}).kept(0, matrix(z_in)).kept(1, matrix(u_in));
+    inner.add(dz, n, f, m, {{&g, &wd}}).kept(kept);
     inner.c.out2 = du.t.data_ptr();
     inner.c.ldo2 = du.ld;
     inner.run("gated_feed_forward backward");
@@ -389,7 +413,7 @@ variable_list gated_backward(const torch::Tensor& g_in, const torch::Tensor& x_i
 //   ez = gh a' u, eu = gh a (those of zt, ut);  dz = gh (a'' zt u + a' ut) + gh2 a' u, du = gh a' zt + gh2 a (those of z, u):
 //   to g: ht wd^T + h ud^T     to x: dz wg + du wu + ez ug + eu uu     to wg: dz^T x + ez^T ux     to wu: du^T x + eu^T ux     to wd: g^T ht
 variable_list gated_second(variable_list t, const torch::Tensor& g_in, const torch::Tensor& x_in, const torch::Tensor& wg_in, const torch::Tensor& wu_in,
-                           const torch::Tensor& wd_in, const torch::Tensor& z_in, const torch::Tensor& u_in, const torch::Tensor& h_in, int64_t activation) {
+                           const torch::Tensor& wd_in, const KeptPlanes& kept, const torch::Tensor& h_in, int64_t activation) {
   c10::cuda::CUDAGuard guard(x_in.device());
   begin_call(x_in);
   const char* what = "gated_feed_forward second backward";
@@ -413,7 +437,7 @@ variable_list gated_second(variable_list t, const torch::Tensor& g_in, const tor
     Products(x_in, ATTN_FORM_NN).add(gh2, n, f, m, {{&g, &ud}}).run(what);
   }
   const Matrix ht = result(n, f, x_in), ez = result(n, f, x_in), eu = result(n, f, x_in), dz = result(n, f, x_in), du = result(n, f, x_in);
-  Elements(x_in, n, f, ATTN_ELEMENTS_GATED_SECOND, activation).in(0, gh).in(1, matrix(z_in)).in(2, matrix(u_in)).in(3, zt).in(4, ut).in(5, gh2)
+  Elements(x_in, n, f, ATTN_ELEMENTS_GATED_SECOND, activation).in(0, gh).kept(1, kept).in(3, zt).in(4, ut).in(5, gh2)
       .out(0, ht).out(1, ez).out(2, eu).out(3, dz).out(4, du).run(torch::Tensor(), what);
   const Matrix gg = result(n, m, x_in), gx = result(n, d, x_in), gwg = result(f, d, x_in), gwu = result(f, d, x_in), gwd = result(m, f, x_in);
   Products(x_in, ATTN_FORM_NT).add(gg, n, m, f, {{&ht, &wd}, {&h, &ud}}).run(what);
@@ -424,19 +448,21 @@ variable_list gated_second(variable_list t, const torch::Tensor& g_in, const tor
 
 struct GatedBackward : public torch::autograd::Function<GatedBackward> {
   static variable_list forward(AutogradContext* ctx, const torch::Tensor& g, const torch::Tensor& x, const torch::Tensor& wg, const torch::Tensor& wu,
-                               const torch::Tensor& wd, const torch::Tensor& z, const torch::Tensor& u, const torch::Tensor& h, int64_t activation) {
+                               const torch::Tensor& wd, const torch::Tensor& z, const torch::Tensor& u, const Maybe& low_in, const torch::Tensor& h,
+                               int64_t activation) {
+    const torch::Tensor low = or_nothing(low_in);
     ctx->set_materialize_grads(false);
     ctx->saved_data["activation"] = activation;
-    ctx->save_for_backward({g, x, wg, wu, wd, z, u, h});
-    return gated_backward(g, x, wg, wu, wd, z, u, h, activation, true, true, true, true);
+    ctx->save_for_backward({g, x, wg, wu, wd, z, u, low, h});
+    return gated_backward(g, x, wg, wu, wd, kept_planes(z, u, low), h, activation, true, true, true, true);
   }
 
   static variable_list backward(AutogradContext* ctx, variable_list t) {
-    variable_list out(9);      // g, x, wg, wu, wd, z, u, h, activation
+    variable_list out(10);      // g, x, wg, wu, wd, z, u, low, h, activation
     if (!t[0].defined() && !t[1].defined() && !t[2].defined() && !t[3].defined()) return out;
     TORCH_CHECK(!at::GradMode::is_enabled(), "gated_feed_forward has no third derivative: call the second backward without create_graph");
     const variable_list s = ctx->get_saved_variables();
-    variable_list r = gated_second(t, s[0], s[1], s[2], s[3], s[4], s[5], s[6], s[7], ctx->saved_data["activation"].toInt());
+    variable_list r = gated_second(t, s[0], s[1], s[2], s[3], s[4], kept_planes(s[5], s[6], s[7]), s[8], ctx->saved_data["activation"].toInt());
     for (int i = 0; i < 5; ++i) out[i] = std::move(r[i]);
     return out;
   }
@@ -450,7 +476,7 @@ struct Gated : public torch::autograd::Function<Gated> {
     ctx->set_materialize_grads(false);
     ctx->saved_data["activation"] = activation;
     ctx->saved_data["residual"] = r.defined();
-    ctx->save_for_backward({x, wg, wu, wd, out[1], out[2], out[3]});
+    ctx->save_for_backward({x, wg, wu, wd, out[1], out[2], out[3], out[4]});
     return out[0];
   }
 
@@ -461,8 +487,8 @@ struct Gated : public torch::autograd::Function<Gated> {
     const int64_t activation = ctx->saved_data["activation"].toInt();
     TORCH_CHECK(!has_tangent({&g[0], &s[0], &s[1], &s[2], &s[3]}), "gated_feed_forward has no forward-mode derivative");
     variable_list r = at::GradMode::is_enabled()
-                          ? GatedBackward::apply(g[0], s[0], s[1], s[2], s[3], s[4], s[5], s[6], activation)
-                          : gated_backward(g[0], s[0], s[1], s[2], s[3], s[4], s[5], s[6], activation, ctx->needs_input_grad(0), ctx->needs_input_grad(1),
+                          ? GatedBackward::apply(g[0], s[0], s[1], s[2], s[3], s[4], s[5], maybe(s[6]), s[7], activation)
+                          : gated_backward(g[0], s[0], s[1], s[2], s[3], kept_planes(s[4], s[5], s[6]), s[7], activation, ctx->needs_input_grad(0), ctx->needs_input_grad(1),
                                            ctx->needs_input_grad(2), ctx->needs_input_grad(3));
     for (int i = 0; i < 4; ++i) out[i] = std::move(r[i]);
     if (ctx->saved_data["residual"].toBool()) out[4] = g[0];

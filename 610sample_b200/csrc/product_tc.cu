@@ -6,16 +6,18 @@
 //   TN     [k, rows], by columns  [k, cols], by columns
 //
 // A pair of CTAs (a cluster) owns a tile of 256 x 256: either holds 128 rows of A and half of B's columns, and one tcgen05.mma.cta_group::2
-// reads both.  A warp loads through a ring of stages of 64 in k, one (in rank 0) issues the products, eight finish a tile from tensor memory
+// reads both.  A warp loads through a ring of stages of 64 in k, one (in rank 0) issues the products, sixteen finish a tile from tensor memory
 // while the next one accumulates in the other half of it.  A result is the sum of up to four products, one behind the other along k.
 //
-// kind    what the eight warps do with a tile, 64 columns at a time in 16 KB of shared memory per buffer and half of the warps
-// PLAIN   z = sum + bias, activation, residual.  The residual is loaded into the buffer that the result leaves from
-// KEEP    the same with z kept
-// GATED   128 columns: CTA 0 holds rows of Wg as its half of B and CTA 1 the same rows of Wu, so that columns j and 128 + j of the accumulator are z and u
-// KEPT    the same with z and u kept (three buffers)
-// GRAD    z and u are loaded into the buffers that their gradients leave from
-// A buffer's next input is asked for as soon as its last result has been read, so it is on its way while the next tile accumulates.
+// kind    what the sixteen warps do with a tile
+// PLAIN   z = sum + bias, activation, residual; z is kept or not
+// GATED   128 columns: CTA 0 holds rows of Wg as its half of B and CTA 1 the same rows of Wu, so that columns j and 128 + j of the accumulator are z and u,
+//         which are kept or not
+// GRAD    reads z and u, and leaves their gradients
+// A warp has 32 rows and a quarter of the columns, a thread one of the rows, 16 columns at a time.  Results leave through shared memory by TMA, 4 KB of each
+// warp's own, so that no warp waits for another one.  Stored from registers, 32 rows to an instruction, they take 70 cycles of the shared memory's
+// pipe each, which the products read their operands through (with z kept 64 us, 16384 x 768 x 2048).  In GRAD z and u come by TMA, 32 columns at a time for each
+// four warps, and their gradients leave from where they lay: loads of 32 rows to an instruction are 32 requests, of which an SM has too few in flight.
 //
 // The tiles of several results are one list, so that three small ones (the weights' gradients of a gated block at 16384 x 768 x 2048: 24 tiles each
 // of 256 blocks of k) fill the 74 pairs once.  Where the last round of tiles stays short of them, its tiles are shared out along k and a small kernel behind adds
@@ -31,55 +33,56 @@ namespace layer {
 using namespace tc;
 using namespace product;
 
-enum Kind { PLAIN = 0, KEEP = 1, GATED = 2, KEPT = 3, GRAD = 4 };
+enum Kind { PLAIN = 0, GATED = 1, GRAD = 2 };
 
 constexpr int kHalfN = kTileN / 2;
 constexpr uint32_t kOperandBytes = 128 * 128;                  // 128 rows (or columns) of 64 in k, of A or of B, in one CTA
 constexpr uint32_t kStageBytes = 2 * kOperandBytes;
-constexpr uint32_t kBufferBytes = 128 * 128;                   // [128 rows][64 columns] of a result or an input
-constexpr int kEpilogueWarps = 8, kLoadWarp = 8, kIssueWarp = 9, kThreads = 320;
+constexpr int kEpilogueWarps = 16, kLoadWarp = 16, kIssueWarp = 17, kThreads = 576;
 constexpr int KPRODUCT = 40;                                   // kernel id inside device status codes: 40 + kind
 
-template <int KIND> constexpr int kBuffersOf = KIND == KEPT ? 3 : KIND == KEEP || KIND == GRAD ? 2 : 1;
-template <int KIND> constexpr int kStagesOf = 7 - kBuffersOf<KIND>;
+template <int KIND> constexpr int kStagesOf = KIND == GRAD ? 4 : 5;
+constexpr int kParts = kEpilogueWarps / 4;
+constexpr uint32_t kStagingBytes = 4096;                       // of a warp, for results on their way out (not GRAD)
+// z, u and their lower bits, [128 rows][32 columns], for each part
+constexpr uint32_t kPlaneBytes = 128 * 64, kLowBytes = 128 * 32, kInputBytes = 2 * kPlaneBytes + kLowBytes;
+
+template <int KIND> constexpr uint32_t kSideOf = KIND == GRAD ? kParts * kInputBytes : kEpilogueWarps * kStagingBytes;
 
 template <int STAGES>
 struct Control {
   uint64_t full[STAGES], empty[STAGES];        // full: rank 0's counts both CTAs' loads
   uint64_t acc_full[2], acc_empty[2];          // acc_empty: rank 0's counts both CTAs' warps
-  uint64_t in_full[2];                         // inputs of the epilogue, by half
+  uint64_t in_full[kParts];                    // GRAD
   uint32_t tmem_base;
   volatile uint32_t abort_flag;
 };
-template <int KIND> constexpr uint32_t smem_bytes() {
-  return kStagesOf<KIND> * kStageBytes + 2 * kBuffersOf<KIND> * kBufferBytes + sizeof(Control<kStagesOf<KIND>>) + 1024;
-}
-static_assert(smem_bytes<PLAIN>() <= 232448 && smem_bytes<KEEP>() <= 232448 && smem_bytes<KEPT>() <= 232448, "shared memory");
+template <int KIND> constexpr uint32_t kSmemOf = kStagesOf<KIND> * kStageBytes + kSideOf<KIND> + sizeof(Control<kStagesOf<KIND>>) + 1024;
+static_assert(kSmemOf<PLAIN> <= 232448 && kSmemOf<GRAD> <= 232448, "shared memory");
 
-struct Maps {
-  CUtensorMap a[kMaxFactors], b[kMaxFactors];
-  CUtensorMap out[kMaxProducts];
-  CUtensorMap side[2];           // PLAIN, KEEP: residual, z.  KEPT, GRAD: z, u
-  CUtensorMap out2;              // GRAD
+// side: z (PLAIN); z, u and their lower bits (GATED, and GRAD, which loads them)
+struct Maps { CUtensorMap a[kMaxFactors], b[kMaxFactors], out[kMaxProducts], side[3]; };
+
+// rows `ld` elements apart; wide: runs of 16 elements start at 32 bytes (2), at 16 (1), or anywhere (0)
+struct Rows {
+  void* p;
+  long long ld;
+  int wide;
 };
-
 struct Result {
   int rows, cols;
   int m_tiles, n_tiles, m_fast;  // m_fast: tiles in sequence along the rows
   int tile_end;                  // in the list of all tiles
   int first_factor, factor_blocks, blocks;      // blocks of k of one product of the sum, and of all of them
-  void* out;
-  long long ldo;
+  Rows out;
 };
 struct ProductArgs {
   Result result[kMaxProducts];
   int results, act;
   int full, rest, splits, split_blocks;      // tiles taken whole; the others, each in `splits` shares of `split_blocks` blocks of k
   float* parts;                  // [rest x splits][2 CTAs][128][256], where there are several shares
-  const void *bias, *residual;
-  long long ld_residual;
-  void* z;
-  long long ld_z;
+  const void* bias;
+  Rows residual, kept;           // kept: z of PLAIN; of GATED, whether z and u are
   unsigned int* status;
 };
 
@@ -101,62 +104,58 @@ __device__ __forceinline__ void tile_at(const Result& r, int tiles_before, int t
 }
 __device__ __forceinline__ int tiles_before(const ProductArgs& g, int p) { return p == 0 ? 0 : g.result[p - 1].tile_end; }
 
-// bias[col .. col + 16) in fp32; zeros outside
+// 16 elements of a row, `left` of which are inside
 template <typename T>
-__device__ __forceinline__ void bias16(const void* bias, int col, int cols, float (&b)[16]) {
-  const T* p = static_cast<const T*>(bias) + col;
-  if (col + 16 <= cols && reinterpret_cast<uintptr_t>(bias) % 16 == 0) {      // col is a multiple of 16
+__device__ __forceinline__ void get16(const Rows& t, long long row, int col, int left, uint32_t (&w)[8]) {
+  const T* p = static_cast<const T*>(t.p) + row * t.ld + col;
+  if (left >= 16 && t.wide == 2) {
+    asm volatile("ld.global.v8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
+                 : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3]), "=r"(w[4]), "=r"(w[5]), "=r"(w[6]), "=r"(w[7])
+                 : "l"(p)
+                 : "memory");
+  } else if (left >= 16 && t.wide == 1) {
+    const uint4 a = reinterpret_cast<const uint4*>(p)[0], b = reinterpret_cast<const uint4*>(p)[1];
+    w[0] = a.x; w[1] = a.y; w[2] = a.z; w[3] = a.w; w[4] = b.x; w[5] = b.y; w[6] = b.z; w[7] = b.w;
+  } else {
+    const uint16_t* h = reinterpret_cast<const uint16_t*>(p);
 #pragma unroll
-    for (int q = 0; q < 2; ++q) {
-      const uint4 v = reinterpret_cast<const uint4*>(p)[q];
-      const uint32_t w[4] = {v.x, v.y, v.z, v.w};
-#pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        const float2 f = Pack<T>::unpack(w[e]);
-        b[8 * q + 2 * e] = f.x; b[8 * q + 2 * e + 1] = f.y;
-      }
-    }
-    return;
+    for (int e = 0; e < 8; ++e) w[e] = (2 * e < left ? (uint32_t)h[2 * e] : 0u) | (2 * e + 1 < left ? (uint32_t)h[2 * e + 1] << 16 : 0u);
   }
-#pragma unroll
-  for (int e = 0; e < 16; ++e) b[e] = col + e < cols ? Elem<T>::to_float(p[e]) : 0.f;
+}
+__device__ __forceinline__ void load_shared16(uint32_t at, uint32_t* w) {
+  asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3]) : "r"(at) : "memory");
 }
 
-template <typename T>
-__device__ __forceinline__ void unpack16(const uint32_t (&w)[8], float (&f)[16]) {
-#pragma unroll
-  for (int e = 0; e < 8; ++e) {
-    const float2 v = Pack<T>::unpack(w[e]);
-    f[2 * e] = v.x; f[2 * e + 1] = v.y;
-  }
+__device__ __forceinline__ void store_shared16(uint32_t at, uint32_t w0, uint32_t w1, uint32_t w2, uint32_t w3) {
+  asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(at), "r"(w0), "r"(w1), "r"(w2), "r"(w3) : "memory");
 }
-template <typename T>
-__device__ __forceinline__ void put16(uint32_t buffer, int row, int col, const float (&f)[16]) {
-  uint32_t w[8];
+// 16-byte chunk `c` of a row in a tile of rows of 64 bytes and of 32, in the swizzle of that width
+__device__ __forceinline__ uint32_t sw64(int row, int c) { return (uint32_t)row * 64u + ((uint32_t)(c ^ (row >> 1 & 3)) << 4); }
+__device__ __forceinline__ uint32_t sw32(int row, int c) { return (uint32_t)row * 32u + ((uint32_t)(c ^ (row >> 2 & 1)) << 4); }
+// 16 elements of a row: of 64 columns, or of 32
+__device__ __forceinline__ void stage16(uint32_t tile, bool of64, int row, int col, const uint32_t (&w)[8]) {
 #pragma unroll
-  for (int e = 0; e < 8; ++e) w[e] = Pack<T>::pack(f[2 * e], f[2 * e + 1]);
-  store_op16(buffer, row, col, w);
+  for (int h = 0; h < 2; ++h)
+    store_shared16(tile + (of64 ? sw128_offset(row, col + 8 * h) : sw64(row, (col >> 3) + h)), w[4 * h], w[4 * h + 1], w[4 * h + 2], w[4 * h + 3]);
 }
+
+// bias[col .. col + 16), packed; `left` of them are inside
 template <typename T>
-__device__ __forceinline__ void keep16(uint32_t buffer, int row, int col, const float (&f)[16]) {
-  float v[16];
-#pragma unroll
-  for (int e = 0; e < 16; ++e) v[e] = within<T>(f[e]);
-  put16<T>(buffer, row, col, v);
+__device__ __forceinline__ void bias16(const void* bias, int col, int left, uint32_t (&w)[8]) {
+  get16<T>(Rows{const_cast<void*>(bias), 0, reinterpret_cast<uintptr_t>(bias) % 16 == 0 ? 1 : 0}, 0, col, left, w);
 }
 
 template <typename T, int FORM, int KIND>
 __global__ void __launch_bounds__(kThreads, 1)
 product_kernel(const __grid_constant__ Maps maps, const __grid_constant__ ProductArgs g) {
-  constexpr int kStages = kStagesOf<KIND>, kBuffers = kBuffersOf<KIND>;
-  constexpr bool kAByColumns = FORM == ATTN_FORM_TN, kBByColumns = FORM != ATTN_FORM_NT, kGate = KIND == GATED || KIND == KEPT;
-  constexpr int kChunks = kGate ? 1 : 2;                         // of 64 columns of a result, for either half
-  constexpr int KCODE = KPRODUCT + KIND;
+  constexpr bool kAByColumns = FORM == ATTN_FORM_TN, kBByColumns = FORM != ATTN_FORM_NT, kGate = KIND == GATED;
+  constexpr int kColumns = kGate ? 32 : 64;                      // of a result, for each warp
+  constexpr int KCODE = KPRODUCT + KIND, kStages = kStagesOf<KIND>;
   extern __shared__ __align__(1024) uint8_t smem_raw[];
   const uint32_t smem_base = (smem_u32(smem_raw) + 1023u) & ~1023u;
-  const uint32_t buffers = smem_base + kStages * kStageBytes;
+  const uint32_t side = smem_base + kStages * kStageBytes;
   typedef Control<kStages> Ctl;
-  Ctl* ctl = reinterpret_cast<Ctl*>(smem_raw + (smem_base - smem_u32(smem_raw)) + kStages * kStageBytes + 2 * kBuffers * kBufferBytes);
+  Ctl* ctl = reinterpret_cast<Ctl*>(smem_raw + (smem_base - smem_u32(smem_raw)) + kStages * kStageBytes + kSideOf<KIND>);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const uint32_t rank = cluster_rank();
   const int pair = blockIdx.x >> 1, pairs = gridDim.x >> 1;
@@ -165,7 +164,6 @@ product_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Produc
   auto bar_empty = [&](int s) { return smem_u32(&ctl->empty[s]); };
   auto bar_acc_full = [&](int b) { return smem_u32(&ctl->acc_full[b]); };
   auto bar_acc_empty = [&](int b) { return smem_u32(&ctl->acc_empty[b]); };
-  auto bar_in_full = [&](int h) { return smem_u32(&ctl->in_full[h]); };
 
   if (warp == kLoadWarp && lane == 0) {
     for (int s = 0; s < kStages; ++s) {
@@ -175,8 +173,8 @@ product_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Produc
     for (int b = 0; b < 2; ++b) {
       mbar_init(bar_acc_full(b), 1);
       mbar_init(bar_acc_empty(b), 2 * kEpilogueWarps);
-      mbar_init(bar_in_full(b), 1);
     }
+    for (int q = 0; q < kParts; ++q) mbar_init(smem_u32(&ctl->in_full[q]), 1);
     ctl->abort_flag = 0u;
     fence_barrier_init();
     fence_proxy_async_smem();
@@ -271,180 +269,236 @@ product_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Produc
       }
     }
   } else {
-    const int quarter = warp & 3, half = warp >> 2;
+    const int quarter = warp & 3, part = warp >> 2;          // of the rows, and of the columns
     const int row = quarter * 32 + lane;
-    const bool leader = quarter == 0 && lane == 0;
     const uint32_t lane_addr = tmem_base + ((uint32_t)(quarter * 32) << 16);
-    const uint32_t buf0 = buffers + (uint32_t)(half * kBuffers) * kBufferBytes, buf1 = buf0 + kBufferBytes, buf2 = buf1 + kBufferBytes;
-    const bool inputs = KIND == GRAD || ((KIND == PLAIN || KIND == KEEP) && g.residual != nullptr);
-    // the leader: inputs of chunk c of item i, where there is such an item and it is a whole tile (the join kernel finishes the others).  Boxes may
-    // lie outside of the tensor, and are zeros there
-    auto ask = [&](int i, int c) {
+    const bool residual = KIND == PLAIN && g.residual.p != nullptr, keep = KIND != GRAD && g.kept.p != nullptr;
+    // GRAD: one thread of a part asks for the inputs of 32 columns of an item.  Boxes may lie outside of the planes, and are zeros there
+    const uint32_t in_z = side + part * kInputBytes, in_u = in_z + kPlaneBytes, in_low = in_u + kPlaneBytes, bar_in = smem_u32(&ctl->in_full[part]);
+    auto fetch = [&](int i, int c) {
       if (i >= items) return;
       const Item item = item_at(g, i);
-      if (item.part) return;
-      const int p = result_of(g, item.t);
       int mt, nt;
-      tile_at(g.result[p], tiles_before(g, p), item.t, mt, nt);
-      const int r0 = mt * kTileM + (int)rank * 128, col = nt * kTileN + half * kHalfN + 64 * c;
-      const uint32_t bar = map_rank(bar_in_full(half), rank);
-      mbar_arrive_expect_tx(bar_in_full(half), (KIND == GRAD ? 2 : 1) * kBufferBytes);
-      tma_load_2d_pair(buf0, &maps.side[0], col, r0, bar);
-      if constexpr (KIND == GRAD) tma_load_2d_pair(buf1, &maps.side[1], col, r0, bar);
+      tile_at(g.result[0], 0, item.t, mt, nt);
+      const int col = nt * kTileN + part * kColumns + c, r0 = mt * kTileM + (int)rank * 128;
+      const uint32_t bar = map_rank(bar_in, rank);
+      mbar_arrive_expect_tx(bar_in, kInputBytes);
+      tma_load_2d_pair(in_z, &maps.side[0], col, r0, bar);
+      tma_load_2d_pair(in_u, &maps.side[1], col, r0, bar);
+      tma_load_2d_pair(in_low, &maps.side[2], col, r0, bar);
     };
-    if (inputs && leader) ask(pair, 0);
-    // A wait for inputs that gives up is this half's alone: it goes on, with what is there, to the next tile, where all warps hear of it
+    // what the warp has written to its staging leaves it
+    const uint32_t staging = side + (uint32_t)warp * kStagingBytes;
+    auto leave = [&](auto&& store, bool inside) {
+      fence_proxy_async_smem();
+      __syncwarp();
+      if (lane == 0 && inside) {
+        store();
+        bulk_commit_group();
+      }
+    };
+    const bool leader = quarter == 0 && lane == 0;
+    if (KIND == GRAD && leader) fetch(pair, 0);
+    // GRAD: the four warps of a part meet, so they go on or give up together; a wait for inputs that gives up goes on to the next tile, where all hear of it
     bool ok = true, alive = true;
-    int n = 0, asked = 0;                                  // asked: chunks with inputs so far
+    int n = 0, fetched = 0;
     for (int i = pair; i < items && ok; i += pairs, ++n) {
       const Item item = item_at(g, i);
       const int p = result_of(g, item.t);
       const Result& r = g.result[p];
       int mt, nt;
       tile_at(r, tiles_before(g, p), item.t, mt, nt);
-      const int buf = n & 1, r0 = mt * kTileM + (int)rank * 128;
-      // this half's first column, of the result and of the accumulator
-      const int col0 = kGate ? nt * kHalfN + half * 64 : nt * kTileN + half * kHalfN;
-      const uint32_t acc = lane_addr + (uint32_t)buf * 256u + (uint32_t)(kGate ? half * 64 : half * kHalfN);
-      // the eight warps go on, or give up, together: the barriers below need all of them
-      ok = named_barrier_all(1, 32 * kEpilogueWarps, mbar_wait(bar_acc_full(buf), (n >> 1) & 1, abort_flag, g.status, wait_code(KCODE, 4)) && alive);
+      const int buf = n & 1;
+      const int r0 = mt * kTileM + (int)rank * 128 + quarter * 32;      // the warp's first row
+      const long long at = r0 + lane;
+      const bool in = at < r.rows;
+      const int col0 = (kGate ? nt * kHalfN : nt * kTileN) + part * kColumns;      // the warp's first column
+      const uint32_t acc = lane_addr + (uint32_t)buf * 256u + (uint32_t)(part * kColumns);
+      // the residual of the next two runs of 16 columns; each is asked for anew once it has been used
+      uint32_t next[2][KIND == PLAIN ? 8 : 1];
+      auto ask = [&](int c, int q) {
+        const int col = col0 + c + 16 * q, left = r.cols - col;
+        if constexpr (KIND == PLAIN)
+          if (residual && in && !item.part && left > 0) get16<T>(g.residual, at, col, left, next[q]);
+      };
+      ask(0, 0);
+      ask(0, 1);
+      ok = mbar_wait(bar_acc_full(buf), (n >> 1) & 1, abort_flag, g.status, wait_code(KCODE, 4));
+      ok = KIND == GRAD ? named_barrier_all(1 + part, 128, ok && alive) : (bool)__all_sync(0xffffffffu, ok);
       if (!ok) break;
       tc_fence_after_sync();
-      auto release = [&]() {                               // the accumulator is in registers
-        tc_fence_before_sync();
-        __syncwarp();
-        if (lane == 0) mbar_arrive_cluster(map_rank(bar_acc_empty(buf), 0));
-      };
       float* part_row = nullptr;
-      if (item.part) part_row = g.parts + (((size_t)(i - g.full) * 2 + rank) * 128 + row) * 256 + half * kHalfN;
+      if (item.part) part_row = g.parts + (((size_t)(i - g.full) * 2 + rank) * 128 + row) * 256 + part * kColumns;
 
 #pragma unroll 1
-      for (int c = 0; c < kChunks; ++c) {
-        const int col = col0 + 64 * c;
-        const bool in = col < r.cols;                      // uniform
-        if (!item.part) {
-          // the buffers: the stores before have read them, and the inputs are there
-          if (inputs) {
-            const bool there = mbar_wait(bar_in_full(half), asked & 1, abort_flag, g.status, wait_code(KCODE, 6));
-            alive = named_barrier_all(3 + half, 128, there) && alive;
-            ++asked;
-          } else {
-            if (leader) bulk_wait_group_read_all();
-            named_barrier_sync(3 + half, 128);
-          }
+      for (int c = 0; c < kColumns; c += 32) {
+        uint32_t low[KIND == PLAIN ? 1 : 8], hs[KIND == GATED ? 16 : 1];
+        if constexpr (KIND == GRAD) {
+          alive = mbar_wait(bar_in, fetched & 1, abort_flag, g.status, wait_code(KCODE, 6)) && alive;
+          ++fetched;
+#pragma unroll
+          for (int e = 0; e < 2; ++e) load_shared16(in_low + sw32(row, e), &low[4 * e]);
+        } else if (c == 0 || keep) {                       // the staging: what left it last has been read
+          if (lane == 0) bulk_wait_group_read_all();
         }
 #pragma unroll
-        for (int s = 0; s < 64; s += 32) {
-          uint32_t v[32], v2[32];
-          tmem_ld32(acc + 64 * c + s, v);
-          if constexpr (kGate) tmem_ld32(acc + 128 + s, v2);
-          tmem_ld_wait32(v);
-          if constexpr (kGate) tmem_ld_wait32(v2);
-          if (c + 1 == kChunks && s == 32) release();
-          if (!in) continue;
-          if (item.part) {
-            float4* at = reinterpret_cast<float4*>(part_row + 64 * c + s);
+        for (int q = 0; q < 2; ++q) {
+          __syncwarp();
+          uint32_t v[16], v2[kGate ? 16 : 1];
+          tmem_ld16(acc + c + 16 * q, v);
+          if constexpr (kGate) tmem_ld16(acc + 128 + c + 16 * q, v2);
+          tmem_ld_wait(v);
+          if constexpr (kGate) tmem_ld_wait(v2);
+          if (c + 32 == kColumns && q == 1) {              // the accumulator is in registers
+            tc_fence_before_sync();
+            __syncwarp();
+            if (lane == 0) mbar_arrive_cluster_local(map_rank(bar_acc_empty(buf), 0));
+          }
+          const int col = col0 + c + 16 * q, left = r.cols - col;
+          if (left <= 0) continue;                         // uniform
+          if (KIND == PLAIN && item.part) {
+            float4* to = reinterpret_cast<float4*>(part_row + c + 16 * q);
 #pragma unroll
-            for (int q = 0; q < 8; ++q)
-              __stcg(at + q, make_float4(__uint_as_float(v[4 * q]), __uint_as_float(v[4 * q + 1]), __uint_as_float(v[4 * q + 2]), __uint_as_float(v[4 * q + 3])));
+            for (int e = 0; e < 4; ++e)
+              __stcg(to + e, make_float4(__uint_as_float(v[4 * e]), __uint_as_float(v[4 * e + 1]), __uint_as_float(v[4 * e + 2]), __uint_as_float(v[4 * e + 3])));
             continue;
           }
+          float2 f[8];
 #pragma unroll
-          for (int q = 0; q < 32; q += 16) {
-            float f[16];
+          for (int e = 0; e < 8; ++e) f[e] = make_float2(__uint_as_float(v[2 * e]), __uint_as_float(v[2 * e + 1]));
+          uint32_t w[8];
+          if constexpr (kGate) {
+            float2 u[8];
 #pragma unroll
-            for (int e = 0; e < 16; ++e) f[e] = __uint_as_float(v[q + e]);
-            if constexpr (kGate) {
-              float u[16];
+            for (int e = 0; e < 8; ++e) u[e] = make_float2(__uint_as_float(v2[2 * e]), __uint_as_float(v2[2 * e + 1]));
+            if (keep) {
+              uint32_t wu[8];
 #pragma unroll
-              for (int e = 0; e < 16; ++e) u[e] = __uint_as_float(v2[q + e]);
-              if constexpr (KIND == KEPT) {
-                keep16<T>(buf1, row, s + q, f);
-                keep16<T>(buf2, row, s + q, u);
+              for (int e = 0; e < 8; e += 2) {
+                const uint32_t cz[4] = {Kept<T>::code(f[e].x), Kept<T>::code(f[e].y), Kept<T>::code(f[e + 1].x), Kept<T>::code(f[e + 1].y)};
+                const uint32_t cu[4] = {Kept<T>::code(u[e].x), Kept<T>::code(u[e].y), Kept<T>::code(u[e + 1].x), Kept<T>::code(u[e + 1].y)};
+                w[e] = kept_high(cz[0], cz[1]);
+                w[e + 1] = kept_high(cz[2], cz[3]);
+                wu[e] = kept_high(cu[0], cu[1]);
+                wu[e + 1] = kept_high(cu[2], cu[3]);
+                low[4 * q + (e >> 1)] = kept_low(cz, cu);
               }
-              with_activation(g.act, [&](auto act) {
-#pragma unroll
-                for (int e = 0; e < 16; ++e) {
-                  float a, d1, d2;
-                  activate<decltype(act)::value, false, 0>(f[e], a, d1, d2);
-                  f[e] = a * u[e];
-                }
-              });
-              put16<T>(buf0, row, s + q, f);
-            } else if constexpr (KIND == GRAD) {
-              uint32_t wz[8], wu[8];
-              load_op16(buf0, row, s + q, wz);
-              load_op16(buf1, row, s + q, wu);
-              float z[16], u[16];
-              unpack16<T>(wz, z);
-              unpack16<T>(wu, u);
-              with_activation(g.act, [&](auto act) {
-#pragma unroll
-                for (int e = 0; e < 16; ++e) {
-                  float a, d1, d2;
-                  activate<decltype(act)::value, false, 1>(z[e], a, d1, d2);
-                  z[e] = f[e] * d1 * u[e];
-                  u[e] = f[e] * a;
-                }
-              });
-              put16<T>(buf0, row, s + q, z);
-              put16<T>(buf1, row, s + q, u);
-            } else {
-              if (g.bias != nullptr) {
-                float b[16];
-                bias16<T>(g.bias, col + s + q, r.cols, b);
-#pragma unroll
-                for (int e = 0; e < 16; ++e) f[e] += b[e];
-              }
-              if constexpr (KIND == KEEP) keep16<T>(buf1, row, s + q, f);
-              if (g.act != ACT_NONE)
-                with_activation(g.act, [&](auto act) {
-#pragma unroll
-                  for (int e = 0; e < 16; ++e) {
-                    float d1, d2;
-                    activate<decltype(act)::value, false, 0>(f[e], f[e], d1, d2);
-                  }
-                });
-              if (inputs) {
-                uint32_t w[8];
-                float x[16];
-                load_op16(buf0, row, s + q, w);
-                unpack16<T>(w, x);
-#pragma unroll
-                for (int e = 0; e < 16; ++e) f[e] += x[e];
-              }
-              put16<T>(buf0, row, s + q, f);
+              stage16(staging, false, lane, 16 * q, w);
+              stage16(staging + 2048, false, lane, 16 * q, wu);
             }
+            with_activation(g.act, [&](auto act) {
+#pragma unroll
+              for (int e = 0; e < 8; ++e) {
+                float2 a, d;
+                activate2<decltype(act)::value, false>(f[e], a, d);
+                f[e] = __fmul2_rn(a, u[e]);
+              }
+            });
+#pragma unroll
+            for (int e = 0; e < 8; ++e) hs[8 * q + e] = Pack<T>::pack(f[e].x, f[e].y);
+          } else if constexpr (KIND == GRAD) {
+            uint32_t wu[8];
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+              load_shared16(in_z + sw64(row, 2 * q + h), &w[4 * h]);
+              load_shared16(in_u + sw64(row, 2 * q + h), &wu[4 * h]);
+            }
+            with_activation(g.act, [&](auto act) {
+#pragma unroll
+              for (int e = 0; e < 8; ++e) {
+                const uint32_t hz = w[e], hu = wu[e], nz = kept_z(low[4 * q + (e >> 1)]), nu = kept_u(low[4 * q + (e >> 1)]);
+                const float2 z = (e & 1) ? make_float2(Kept<T>::value(kept_code<2>(hz, nz)), Kept<T>::value(kept_code<3>(hz, nz)))
+                                         : make_float2(Kept<T>::value(kept_code<0>(hz, nz)), Kept<T>::value(kept_code<1>(hz, nz)));
+                const float2 u = (e & 1) ? make_float2(Kept<T>::value(kept_code<2>(hu, nu)), Kept<T>::value(kept_code<3>(hu, nu)))
+                                         : make_float2(Kept<T>::value(kept_code<0>(hu, nu)), Kept<T>::value(kept_code<1>(hu, nu)));
+                float2 a, d;
+                activate2<decltype(act)::value, true>(z, a, d);
+                a = __fmul2_rn(f[e], a);
+                f[e] = __fmul2_rn(__fmul2_rn(f[e], d), u);
+                w[e] = Pack<T>::pack(f[e].x, f[e].y);
+                wu[e] = Pack<T>::pack(a.x, a.y);
+              }
+            });
+            stage16(in_z, false, row, 16 * q, w);
+            stage16(in_u, false, row, 16 * q, wu);
+          } else {
+            if (g.bias != nullptr) {
+              uint32_t b[8];
+              bias16<T>(g.bias, col, left, b);
+#pragma unroll
+              for (int e = 0; e < 8; ++e) f[e] = __fadd2_rn(f[e], Pack<T>::unpack(b[e]));
+            }
+            if (keep) {
+#pragma unroll
+              for (int e = 0; e < 8; ++e) w[e] = pack_finite<T>(f[e].x, f[e].y);
+              stage16(staging + 2048, false, lane, 16 * q, w);
+            }
+            if (g.act != ACT_NONE)
+              with_activation(g.act, [&](auto act) {
+#pragma unroll
+                for (int e = 0; e < 8; ++e) {
+                  float2 d;
+                  activate2<decltype(act)::value, false>(f[e], f[e], d);
+                }
+              });
+            if (residual) {
+#pragma unroll
+              for (int e = 0; e < 8; ++e) f[e] = __fadd2_rn(f[e], Pack<T>::unpack(next[q][e]));
+              if (c + 32 < kColumns) ask(c + 32, q);
+            }
+#pragma unroll
+            for (int e = 0; e < 8; ++e) w[e] = Pack<T>::pack(f[e].x, f[e].y);
+            stage16(staging, !keep, lane, (keep ? 0 : c) + 16 * q, w);
           }
         }
-        if (item.part) continue;
-        fence_proxy_async_smem();
-        named_barrier_sync(3 + half, 128);
-        if (leader) {
-          if (in) {
-            tma_store_2d(&maps.out[p], buf0, col, r0);
-            if constexpr (KIND == KEEP) tma_store_2d(&maps.side[1], buf1, col, r0);
-            if constexpr (KIND == KEPT) {
-              tma_store_2d(&maps.side[0], buf1, col, r0);
-              tma_store_2d(&maps.side[1], buf2, col, r0);
+        if constexpr (KIND == GRAD) {
+          fence_proxy_async_smem();
+          alive = named_barrier_all(1 + part, 128, alive);
+          if (leader) {
+            if (col0 + c < r.cols) {                       // rows of the whole part: quarter 0's first one
+              tma_store_2d(&maps.out[0], in_z, col0 + c, r0);
+              tma_store_2d(&maps.out[1], in_u, col0 + c, r0);
+              bulk_commit_group();
+              bulk_wait_group_read_all();
             }
-            if constexpr (KIND == GRAD) tma_store_2d(&maps.out2, buf1, col, r0);
-            bulk_commit_group();
+            if (c + 32 < kColumns) fetch(i, c + 32);
+            else fetch(i + pairs, 0);
           }
-          if (inputs) {
-            bulk_wait_group_read_all();
-            if (c + 1 < kChunks) ask(i, c + 1);
-            else ask(i + pairs, 0);
+          continue;
+        }
+        if (item.part || r0 >= r.rows) continue;           // uniform
+        if constexpr (kGate) {
+          const int col = col0 + c;
+          if (keep) {
+            leave([&] {
+              tma_store_2d(&maps.side[0], staging, col, r0);
+              tma_store_2d(&maps.side[1], staging + 2048, col, r0);
+            }, col < r.cols);
+            if (lane == 0) bulk_wait_group_read_all();
+            __syncwarp();
+#pragma unroll
+            for (int h = 0; h < 2; ++h) store_shared16(staging + 2048 + sw32(lane, h), low[4 * h], low[4 * h + 1], low[4 * h + 2], low[4 * h + 3]);
           }
+#pragma unroll
+          for (int h = 0; h < 4; ++h) store_shared16(staging + sw64(lane, h), hs[4 * h], hs[4 * h + 1], hs[4 * h + 2], hs[4 * h + 3]);
+          leave([&] {
+            tma_store_2d(&maps.out[0], staging, col, r0);
+            if (keep) tma_store_2d(&maps.side[2], staging + 2048, col, r0);
+          }, col < r.cols);
+        } else if (keep) {
+          leave([&] {
+            tma_store_2d(&maps.out[0], staging, col0 + c, r0);
+            tma_store_2d(&maps.side[0], staging + 2048, col0 + c, r0);
+          }, col0 + c < r.cols);
+        } else if (c + 32 == kColumns) {
+          leave([&] { tma_store_2d(&maps.out[p], staging, col0, r0); }, col0 < r.cols);
         }
       }
     }
-    if (leader) {
-      if (!ok || !alive) {
-        const long long t0 = clock64();
-        while (clock64() - t0 < 2000000LL) { }
-      }
-      bulk_wait_group_read_all();
+    if (lane == 0) bulk_wait_group_read_all();
+    if (!alive) {      // inputs that are still on their way: a bounded chance to land before the CTA exits
+      const long long t0 = clock64();
+      while (clock64() - t0 < 2000000LL) { }
     }
   }
   tc_fence_before_sync();
@@ -476,46 +530,52 @@ join_kernel(const __grid_constant__ ProductArgs g) {
       const float4 x = from_l2(reinterpret_cast<const float4*>(g.parts + (((size_t)(q * g.rest + tile) * 2 + rank) * 128 + row) * 256 + c));
       v[0] += x.x; v[1] += x.y; v[2] += x.z; v[3] += x.w;
     }
-    // rows start at 16 bytes and col is a multiple of 4
-    const int width = min(4, res.cols - col);
-    auto pack = [](const float (&f)[4]) { return make_uint2(Pack<T>::pack(f[0], f[1]), Pack<T>::pack(f[2], f[3])); };
-    auto put = [&](void* base, long long ld, const float (&f)[4]) {
-      T* at = static_cast<T*>(base) + r * ld + col;
-      if (width == 4) *reinterpret_cast<uint2*>(at) = pack(f);
+    const int width = min(4, res.cols - col);      // col is a multiple of 4
+    auto put = [&](const Rows& to, uint32_t w0, uint32_t w1) {
+      uint16_t* p = static_cast<uint16_t*>(to.p) + r * to.ld + col;
+      if (width == 4 && to.wide > 0) *reinterpret_cast<uint2*>(p) = make_uint2(w0, w1);
       else
-        for (int e = 0; e < width; ++e) at[e] = Elem<T>::from_float(f[e]);
+        for (int e = 0; e < width; ++e) p[e] = (uint16_t)((e < 2 ? w0 : w1) >> (16 * (e & 1)));
     };
     if (g.bias != nullptr)
       for (int e = 0; e < width; ++e) v[e] += Elem<T>::to_float(static_cast<const T*>(g.bias)[col + e]);
-    if (g.z != nullptr) {
-      float k[4];
-#pragma unroll
-      for (int e = 0; e < 4; ++e) k[e] = within<T>(v[e]);
-      put(g.z, g.ld_z, k);
-    }
+    if (g.kept.p != nullptr) put(g.kept, pack_finite<T>(v[0], v[1]), pack_finite<T>(v[2], v[3]));
     with_activation(g.act, [&](auto act) {
 #pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        float d1, d2;
-        activate<decltype(act)::value, false, 0>(v[e], v[e], d1, d2);
+      for (int e = 0; e < 4; e += 2) {
+        float2 a, d;
+        activate2<decltype(act)::value, false>(make_float2(v[e], v[e + 1]), a, d);
+        v[e] = a.x; v[e + 1] = a.y;
       }
     });
-    if (g.residual != nullptr)
-      for (int e = 0; e < width; ++e) v[e] += Elem<T>::to_float(static_cast<const T*>(g.residual)[r * g.ld_residual + col + e]);
-    put(res.out, res.ldo, v);
+    if (g.residual.p != nullptr)
+      for (int e = 0; e < width; ++e) v[e] += Elem<T>::to_float(static_cast<const T*>(g.residual.p)[r * g.residual.ld + col + e]);
+    put(res.out, Pack<T>::pack(v[0], v[1]), Pack<T>::pack(v[2], v[3]));
   }
 }
 
 // ---- host ---------------------------------------------------------------------------------------
-static int kind_of(const attn_products_t& c) {
-  if (c.kind == ATTN_PRODUCT_GATED) return c.kept[0] != nullptr ? KEPT : GATED;
-  if (c.kind == ATTN_PRODUCT_GATED_GRAD) return GRAD;
-  return c.kept[0] != nullptr ? KEEP : PLAIN;
+static Rows rows_of(const void* p, int64_t ld) {
+  const uintptr_t a = reinterpret_cast<uintptr_t>(p) | (uintptr_t)(ld * 2);
+  return {const_cast<void*>(p), ld, a % 32 == 0 ? 2 : a % 16 == 0 ? 1 : 0};
+}
+
+// a matrix of `size` bytes an element, boxes of 32 columns
+static bool encode_plane(CUtensorMap* map, const void* p, int size, long long rows, long long cols, long long ld, int box_rows) {
+  const EncodeTiledFn fn = encode_fn();
+  if (fn == nullptr) return false;
+  cuuint64_t dims[2] = {(cuuint64_t)cols, (cuuint64_t)rows};
+  cuuint64_t strides[1] = {(cuuint64_t)(ld * size)};
+  cuuint32_t box[2] = {32, (cuuint32_t)box_rows};
+  cuuint32_t estr[2] = {1, 1};
+  return fn(map, size == 1 ? CU_TENSOR_MAP_DATA_TYPE_UINT8 : CU_TENSOR_MAP_DATA_TYPE_UINT16, 2, const_cast<void*>(p), dims, strides, box, estr,
+            CU_TENSOR_MAP_INTERLEAVE_NONE, size == 1 ? CU_TENSOR_MAP_SWIZZLE_32B : CU_TENSOR_MAP_SWIZZLE_64B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+            CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
 // Results, tiles and shares of a call; results without rows, columns or k have no tiles
 static long long plan(const attn_products_t& c, ProductArgs& g) {
-  const int kind = kind_of(c), tile_n = kind == GATED || kind == KEPT ? kHalfN : kTileN;
+  const int tile_n = c.kind == ATTN_PRODUCT_GATED ? kHalfN : kTileN;
   long long tiles = 0;
   bool equal = true;
   int factors = 0;
@@ -531,8 +591,7 @@ static long long plan(const attn_products_t& c, ProductArgs& g) {
     r.first_factor = factors;
     r.factor_blocks = blocks_of(p.k);
     r.blocks = r.factor_blocks * p.pairs;
-    r.out = p.out;
-    r.ldo = p.ldo;
+    r.out = rows_of(p.out, p.ldo);
     factors += p.pairs;
     tiles += (long long)r.m_tiles * r.n_tiles;
     if (tiles > 0x3fffffffLL) return -1;
@@ -541,7 +600,7 @@ static long long plan(const attn_products_t& c, ProductArgs& g) {
     ++g.results;
   }
   SharePlan s{(int)tiles, 0, 1, 0};
-  if (tiles > 0 && equal && (kind == PLAIN || kind == KEEP)) s = plan_shares((int)tiles, g.result[0].blocks);
+  if (tiles > 0 && equal && c.kind == ATTN_PRODUCT_PLAIN) s = plan_shares((int)tiles, g.result[0].blocks);
   g.full = s.full; g.rest = s.rest; g.splits = s.splits; g.split_blocks = s.split_blocks;
   return tiles;
 }
@@ -556,8 +615,8 @@ template <typename T, int FORM, int KIND>
 static cudaError_t launch(const Maps& maps, const ProductArgs& g, cudaStream_t stream, int* launches) {
   static std::atomic<unsigned long long> smem_set;
   const int items = g.full + g.rest * g.splits, pairs = items < kSms / 2 ? items : kSms / 2;
-  cudaError_t e = set_smem_once(product_kernel<T, FORM, KIND>, smem_bytes<KIND>(), smem_set);
-  if (e == cudaSuccess) e = launch_pdl_cluster(product_kernel<T, FORM, KIND>, (unsigned)pairs * 2, kThreads, smem_bytes<KIND>(), 2, stream, maps, g);
+  cudaError_t e = set_smem_once(product_kernel<T, FORM, KIND>, kSmemOf<KIND>, smem_set);
+  if (e == cudaSuccess) e = launch_pdl_cluster(product_kernel<T, FORM, KIND>, (unsigned)pairs * 2, kThreads, kSmemOf<KIND>, 2, stream, maps, g);
   ++*launches;
   if (g.splits > 1 && e == cudaSuccess) {
     e = launch_pdl(join_kernel<T>, (unsigned)g.rest * 32, 256u, 0, stream, g);
@@ -567,46 +626,43 @@ static cudaError_t launch(const Maps& maps, const ProductArgs& g, cudaStream_t s
 }
 
 template <typename T>
-static cudaError_t launch_type(int form, int kind, const Maps& maps, const ProductArgs& g, cudaStream_t stream, int* launches) {
-  if (kind == GATED) return launch<T, ATTN_FORM_NT, GATED>(maps, g, stream, launches);
-  if (kind == KEPT) return launch<T, ATTN_FORM_NT, KEPT>(maps, g, stream, launches);
-  if (kind == GRAD) return launch<T, ATTN_FORM_NN, GRAD>(maps, g, stream, launches);
-  if (kind == KEEP) return launch<T, ATTN_FORM_NT, KEEP>(maps, g, stream, launches);
-  if (form == ATTN_FORM_NT) return launch<T, ATTN_FORM_NT, PLAIN>(maps, g, stream, launches);
-  if (form == ATTN_FORM_NN) return launch<T, ATTN_FORM_NN, PLAIN>(maps, g, stream, launches);
+static cudaError_t launch_type(const attn_products_t& c, const Maps& maps, const ProductArgs& g, cudaStream_t stream, int* launches) {
+  if (c.kind == ATTN_PRODUCT_GATED) return launch<T, ATTN_FORM_NT, GATED>(maps, g, stream, launches);
+  if (c.kind == ATTN_PRODUCT_GATED_GRAD) return launch<T, ATTN_FORM_NN, GRAD>(maps, g, stream, launches);
+  if (c.form == ATTN_FORM_NT) return launch<T, ATTN_FORM_NT, PLAIN>(maps, g, stream, launches);
+  if (c.form == ATTN_FORM_NN) return launch<T, ATTN_FORM_NN, PLAIN>(maps, g, stream, launches);
   return launch<T, ATTN_FORM_TN, PLAIN>(maps, g, stream, launches);
 }
 
 cudaError_t tc_products(const attn_products_t& c, float* parts, unsigned int* status, cudaStream_t stream, int* launches, const char** why) {
   Maps maps;
   ProductArgs g = {};
-  const int kind = kind_of(c);
   const bool bf = c.dtype == ATTN_BF16;
   if (plan(c, g) < 0) return cudaErrorInvalidValue;
   if (g.results == 0) return cudaSuccess;
   bool ok = true;
   int factor = 0, result = 0;
+  const bool keep = c.kept[0] != nullptr, of64 = c.kind == ATTN_PRODUCT_PLAIN && !keep;      // how results are staged
+  const int box_rows = c.kind == ATTN_PRODUCT_GATED_GRAD ? 128 : 32;
   for (int i = 0; i < c.count; ++i) {
     const attn_product_t& p = c.product[i];
     if (p.rows == 0 || p.cols == 0 || p.k == 0) continue;
+    ok = ok && (of64 ? encode(&maps.out[result], p.out, bf, p.rows, p.cols, p.ldo, 32) : encode_plane(&maps.out[result], p.out, 2, p.rows, p.cols, p.ldo, box_rows));
+    ++result;
     for (int q = 0; q < p.pairs; ++q, ++factor) {
       const attn_factors_t& f = p.pair[q];
       ok = ok && (c.form == ATTN_FORM_TN ? encode(&maps.a[factor], f.a, bf, p.k, p.rows, f.lda, 64) : encode(&maps.a[factor], f.a, bf, p.rows, p.k, f.lda, 128));
       ok = ok && (c.form == ATTN_FORM_NT ? encode(&maps.b[factor], f.b, bf, p.cols, p.k, f.ldb, 128) : encode(&maps.b[factor], f.b, bf, p.k, p.cols, f.ldb, 64));
     }
-    ok = ok && encode(&maps.out[result++], p.out, bf, p.rows, p.cols, p.ldo, 128);
   }
   const attn_product_t& p = c.product[0];
-  auto side = [&](CUtensorMap* map, const void* at, int64_t ld) { ok = ok && encode(map, at, bf, p.rows, p.cols, ld, 128); };
-  if (kind == PLAIN || kind == KEEP) {
-    if (c.residual != nullptr) side(&maps.side[0], c.residual, c.ld_residual);
-    if (kind == KEEP) side(&maps.side[1], c.kept[0], c.ld_kept[0]);
-  } else {
-    if (kind != GRAD) ok = ok && encode(&maps.b[1], c.b2, bf, p.cols, p.k, c.ldb2, 128);
-    if (kind != GATED)
-      for (int q = 0; q < 2; ++q) side(&maps.side[q], c.kept[q], c.ld_kept[q]);
-    if (kind == GRAD) side(&maps.out2, c.out2, c.ldo2);
+  if (c.kind == ATTN_PRODUCT_GATED) ok = ok && encode(&maps.b[1], c.b2, bf, p.cols, p.k, c.ldb2, 128);
+  if (keep) {
+    const int planes = c.kind == ATTN_PRODUCT_PLAIN ? 1 : 2;
+    for (int q = 0; q < planes; ++q) ok = ok && encode_plane(&maps.side[q], c.kept[q], 2, p.rows, p.cols, c.ld_kept[q], box_rows);
+    if (planes == 2) ok = ok && encode_plane(&maps.side[2], c.kept_low, 1, p.rows, p.cols, c.ld_low, box_rows);
   }
+  if (c.kind == ATTN_PRODUCT_GATED_GRAD) ok = ok && encode_plane(&maps.out[1], c.out2, 2, p.rows, p.cols, c.ldo2, box_rows);
   if (!ok) {
     *why = "cuTensorMapEncodeTiled refused a tensor";
     return cudaErrorInvalidValue;
@@ -614,12 +670,10 @@ cudaError_t tc_products(const attn_products_t& c, float* parts, unsigned int* st
   g.act = c.activation;
   g.parts = parts;
   g.bias = c.bias;
-  g.residual = c.residual;
-  g.ld_residual = c.ld_residual;
-  g.z = kind == KEEP ? c.kept[0] : nullptr;
-  g.ld_z = c.ld_kept[0];
+  g.residual = rows_of(c.residual, c.ld_residual);
+  g.kept = rows_of(c.kept[0], c.ld_kept[0]);
   g.status = status;
-  return bf ? launch_type<__nv_bfloat16>(c.form, kind, maps, g, stream, launches) : launch_type<__half>(c.form, kind, maps, g, stream, launches);
+  return bf ? launch_type<__nv_bfloat16>(c, maps, g, stream, launches) : launch_type<__half>(c, maps, g, stream, launches);
 }
 
 }  // namespace layer

@@ -278,6 +278,10 @@ __device__ __forceinline__ uint32_t map_rank(uint32_t addr, uint32_t rank) {
 __device__ __forceinline__ void mbar_arrive_cluster(uint32_t mapped) {
   asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(mapped) : "memory");
 }
+// The same without waiting for this thread's own writes to global memory to be seen by the cluster: for what the barrier hands on is read from tensor memory.
+__device__ __forceinline__ void mbar_arrive_cluster_local(uint32_t mapped) {
+  asm volatile("mbarrier.arrive.release.cta.shared::cluster.b64 _, [%0];" ::"r"(mapped) : "memory");
+}
 // 2-D tiled load into this CTA's shared memory, completing on a barrier of either CTA of the pair (mapped address)
 __device__ __forceinline__ void tma_load_2d_pair(uint32_t smem_dst, const CUtensorMap* map, int x, int y, uint32_t mapped_bar) {
   asm volatile(

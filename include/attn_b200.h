@@ -277,8 +277,10 @@ int attn_b200_linear_ce_backward(const attn_lce_shape_t* shape, const void* x, c
  *                        out = activation(z) u
  *   ATTN_PRODUCT_GATED_GRAD   NN, one result, without bias: given kept = (z, u), out = sum activation'(z) u, out2 = sum activation(z)
  * Rows are `ld` elements apart, columns dense.  f16 and bf16 on the tensor cores: bases 16-byte aligned, strides multiples of 8;
- * f32 on the CUDA cores, in any alignment of an element.  Values that are kept are cut to the type's finite range.  Only columns
- * of a result are written, never what lies between them and the next row.  Inputs must not overlap outputs. */
+ * f32 on the CUDA cores.  A residual and a bias may have any alignment of an element.  Only columns of a result are written, never what lies between them
+ * and the next row.  z of a plain product is kept in the type, within its finite range; z and u
+ * of a gated one in 20 bits of f16 and bf16: 16 of each in kept, and 4 of both in a plane of bytes, kept_low, whose rows are a multiple of 32
+ * apart from a 32-byte aligned base.  Their encoding is the kernels' own.  Inputs must not overlap outputs. */
 enum { ATTN_FORM_NT = 0, ATTN_FORM_NN = 1, ATTN_FORM_TN = 2 };
 enum { ATTN_PRODUCT_PLAIN = 0, ATTN_PRODUCT_GATED = 1, ATTN_PRODUCT_GATED_GRAD = 2 };
 enum { ATTN_ACT_NONE = 0, ATTN_ACT_SILU = 1, ATTN_ACT_GELU = 2, ATTN_ACT_GELU_TANH = 3 };
@@ -301,6 +303,7 @@ typedef struct attn_products {
   const void* residual; int64_t ld_residual;
   const void* b2; int64_t ldb2;
   void* kept[2]; int64_t ld_kept[2];
+  void* kept_low; int64_t ld_low;
   void* out2; int64_t ldo2;
 } attn_products_t;
 
@@ -313,7 +316,7 @@ int attn_b200_products(const attn_products_t* call, void* scratch, void* stream)
  *   SECOND         in g, z, t        out t activation'(z), s = g activation''(z) t, dz;  sum: of s.  t is the tangent of z
  *   GATED_SECOND   in gh, z, u, zt, ut, gh2 (or null)   out, with h = a(z) u, zt and ut the tangents of z and u, gh the gradient of h and gh2 a
  *                  part of the gradient of h's tangent's factor:  ht = a' zt u + a ut,  gh a' u,  gh a,  gh (a'' zt u + a' ut) + gh2 a' u,
- *                  gh a' zt + gh2 a
+ *                  gh a' zt + gh2 a.  z and u as a gated product keeps them
  * sum: [m] of the type, or null; scratch is used with it. */
 enum { ATTN_ELEMENTS_FIRST = 0, ATTN_ELEMENTS_SECOND = 1, ATTN_ELEMENTS_GATED_SECOND = 2 };
 typedef struct attn_elements {
@@ -321,6 +324,7 @@ typedef struct attn_elements {
   int32_t dtype, activation, pass;
   int32_t reserved;
   const void* in[6]; int64_t ld_in[6];
+  const void* kept_low; int64_t ld_low;
   void* out[5]; int64_t ld_out[5];
   void* sum;
 } attn_elements_t;
@@ -360,8 +364,8 @@ int attn_b200_last_launch_count(void);
  * code here and returns.  Code = (kernel id + 1) << 8 | wait id, kernel ids:
  * 4 / 5 / 6 double-backward scalar + g_dO / g_Q / g_K + g_V kernel, 18 / 19
  * backward row / column kernel, 20 forward, 21 forward of packed batches by pairs of tiles,
- * 32 to 35 the linear cross entropy's products (scores, gradient of the logits, dx, dW), 40 to 44 a layer's
- * products (plain, with z kept, gated, with both kept, gated gradient), 0x6f the
+ * 32 to 35 the linear cross entropy's products (scores, gradient of the logits, dx, dW), 40 to 42 a layer's
+ * products (plain, gated, gated gradient), 0x6f the
  * primitive self-test (codes 0x7001..0x7003); wait id 15 = the launch gave the kernel less shared memory
  * than its layout needs. */
 int attn_b200_device_status(uint32_t* code);
