@@ -28,7 +28,7 @@ NVCC_FLAGS = ["-gencode", "arch=compute_100a,code=sm_100a", "-lineinfo", "-O3", 
               "-Xcompiler", "-fPIC", "-I" + INCLUDE, "-I" + CSRC]
 CU_SOURCES = ["attn_capi.cu", "attn_prep.cu", "attn_simt.cu", "attn_tc.cu", "attn_tc_fb.cu", "attn_tc_fwd.cu", "attn_tc_hvp_row.cu", "attn_tc_hvp_col.cu",
               "packed_capi.cu", "packed_plan.cu", "packed_rope.cu", "packed_fwd.cu", "lce_capi.cu", "lce_tc.cu", "lce_rows.cu", "lce_simt.cu",
-              "layer_capi.cu", "layer_elem.cu", "layer_norm_forward.cu", "layer_norm_first.cu", "layer_norm_second.cu", "product_tc.cu", "product_simt.cu"]
+              "layer_capi.cu", "layer_elem.cu", "layer_norm_forward.cu", "layer_norm_first.cu", "layer_norm_second.cu", "product_few.cu", "product_tc.cu", "product_simt.cu"]
 EXT_SOURCES = ["attention_ext.cpp", "packed_ext.cpp", "loss_ext.cpp", "layers_ext.cpp"]
 HEADERS = ["activation.cuh", "attn_common.cuh", "attn_launch.h", "capi_common.h", "packed_geometry.cuh", "packed_launch.h", "packed_order.h", "layer_launch.h", "layer_norm.cuh", "lce_launch.h", "product_common.cuh", "simt_product.cuh", "simt_split.h", "tc_primitives.cuh", "tc_common.cuh", os.path.join(INCLUDE, "attn_b200.h")]
 

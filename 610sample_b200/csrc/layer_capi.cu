@@ -95,7 +95,7 @@ int check_products(const attn_products_t* c, bool pointers) {
   return rc;
 }
 
-size_t parts_bytes(const attn_products_t& c) { return c.dtype == ATTN_F32 ? simt_parts_bytes(c) : tc_parts_bytes(c); }
+size_t parts_bytes(const attn_products_t& c) { return c.dtype == ATTN_F32 ? simt_parts_bytes(c) : few_rows(c) ? 0 : tc_parts_bytes(c); }
 
 int inputs_of(int pass, int act) { return pass == ATTN_ELEMENTS_FIRST ? (act == ATTN_ACT_NONE ? 1 : 2) : pass == ATTN_ELEMENTS_SECOND ? 3 : 5; }
 int outputs_of(int pass, int act) { return pass == ATTN_ELEMENTS_FIRST ? (act == ATTN_ACT_NONE ? 0 : 1) : pass == ATTN_ELEMENTS_SECOND ? 3 : 5; }
@@ -173,7 +173,9 @@ int attn_b200_products(const attn_products_t* call, void* scratch, void* stream)
   }
   if (e == cudaSuccess) {
     float* const parts = static_cast<float*>(scratch);
-    e = call->dtype == ATTN_F32 ? simt_products(*call, parts, cs, &launches) : tc_products(*call, parts, status, cs, &launches, &why);
+    e = call->dtype == ATTN_F32 ? simt_products(*call, parts, cs, &launches)
+        : few_rows(*call)       ? few_products(*call, cs, &launches)
+                                : tc_products(*call, parts, status, cs, &launches, &why);
   }
   return capi::done(e, "products launch failed", why, launches);
 }

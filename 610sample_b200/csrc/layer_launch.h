@@ -14,6 +14,9 @@ constexpr int kMaxPairs = ATTN_PRODUCT_PAIRS, kMaxProducts = ATTN_PRODUCT_COUNT,
 // matrix products on the tensor cores (product_tc.cu): f16 / bf16.  parts: tc_parts_bytes
 size_t tc_parts_bytes(const attn_products_t& c);
 cudaError_t tc_products(const attn_products_t& c, float* parts, unsigned int* status, cudaStream_t stream, int* launches, const char** why);
+// few rows against a weight (product_few.cu): f16 / bf16, what few_rows says
+bool few_rows(const attn_products_t& c);
+cudaError_t few_products(const attn_products_t& c, cudaStream_t stream, int* launches);
 // on the CUDA cores (product_simt.cu): float32
 size_t simt_parts_bytes(const attn_products_t& c);
 cudaError_t simt_products(const attn_products_t& c, float* parts, cudaStream_t stream, int* launches);
