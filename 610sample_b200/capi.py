@@ -30,7 +30,9 @@ EXPORTS = (
     "attn_b200_packed_backward_scratch_bytes",
     "attn_b200_linear_ce_forward_scratch_bytes", "attn_b200_linear_ce_forward", "attn_b200_linear_ce_backward_scratch_bytes",
     "attn_b200_linear_ce_backward", "attn_b200_packed_qk_norm_rope", "attn_b200_packed_qk_norm_rope_backward_scratch_bytes",
-    "attn_b200_packed_qk_norm_rope_backward",
+    "attn_b200_packed_qk_norm_rope_backward", "attn_b200_products_scratch_bytes", "attn_b200_products", "attn_b200_elements_scratch_bytes",
+    "attn_b200_elements", "attn_b200_layer_norm", "attn_b200_layer_norm_backward_scratch_bytes", "attn_b200_layer_norm_backward",
+    "attn_b200_layer_norm_second_backward",
 )
 
 
@@ -52,6 +54,31 @@ class RopeShape(C.Structure):
     _fields_ = [(n, C.c_int32) for n in ("n_tok", "q_heads", "k_heads", "D", "dtype", "table_rows", "axes", "positions64")] + [
         ("section", C.c_int32 * 4), ("weight_float", C.c_int32 * 2), ("eps", C.c_float), ("reserved", C.c_int32), ("axis_stride", C.c_int64),
         ("row_stride", C.c_int64 * 2), ("head_stride", C.c_int64 * 2), ("g_row_stride", C.c_int64 * 2), ("g_head_stride", C.c_int64 * 2)]
+
+
+class Factors(C.Structure):
+    _fields_ = [("a", C.c_void_p), ("b", C.c_void_p), ("lda", C.c_int64), ("ldb", C.c_int64)]
+
+
+class Product(C.Structure):
+    _fields_ = [(n, C.c_int32) for n in ("rows", "cols", "k", "pairs")] + [("pair", Factors * 4), ("out", C.c_void_p), ("ldo", C.c_int64)]
+
+
+class Products(C.Structure):
+    _fields_ = [(n, C.c_int32) for n in ("dtype", "form", "kind", "activation", "count", "reserved")] + [
+        ("product", Product * 3), ("bias", C.c_void_p), ("residual", C.c_void_p), ("ld_residual", C.c_int64), ("b2", C.c_void_p), ("ldb2", C.c_int64),
+        ("kept", C.c_void_p * 2), ("ld_kept", C.c_int64 * 2), ("kept_low", C.c_void_p), ("ld_low", C.c_int64), ("out2", C.c_void_p), ("ldo2", C.c_int64)]
+
+
+class Elements(C.Structure):
+    _fields_ = [(n, C.c_int32) for n in ("n", "m", "dtype", "activation", "pass_", "reserved")] + [
+        ("input", C.c_void_p * 6), ("ld_input", C.c_int64 * 6), ("kept_low", C.c_void_p), ("ld_low", C.c_int64), ("out", C.c_void_p * 5),
+        ("ld_out", C.c_int64 * 5), ("sum", C.c_void_p)]
+
+
+class NormShape(C.Structure):
+    _fields_ = [(n, C.c_int32) for n in ("n", "d", "dtype", "param_float")] + [("eps", C.c_float), ("reserved", C.c_int32)] + [
+        (n, C.c_int64) for n in ("ldx", "ldg", "ldu")]
 
 
 _lib = None
@@ -99,6 +126,17 @@ def lib() -> C.CDLL:
         L.attn_b200_packed_qk_norm_rope_backward.argtypes = [C.POINTER(RopeShape)] + [vp] * 14
         L.attn_b200_packed_qk_norm_rope_backward_scratch_bytes.argtypes = [C.POINTER(RopeShape)]
         L.attn_b200_packed_qk_norm_rope_backward_scratch_bytes.restype = C.c_size_t
+        L.attn_b200_products_scratch_bytes.argtypes = [C.POINTER(Products)]
+        L.attn_b200_products_scratch_bytes.restype = C.c_size_t
+        L.attn_b200_products.argtypes = [C.POINTER(Products), vp, vp]
+        L.attn_b200_elements_scratch_bytes.argtypes = [C.POINTER(Elements)]
+        L.attn_b200_elements_scratch_bytes.restype = C.c_size_t
+        L.attn_b200_elements.argtypes = [C.POINTER(Elements), vp, vp]
+        L.attn_b200_layer_norm.argtypes = [C.POINTER(NormShape)] + [vp] * 7
+        L.attn_b200_layer_norm_backward_scratch_bytes.argtypes = [C.POINTER(NormShape)]
+        L.attn_b200_layer_norm_backward_scratch_bytes.restype = C.c_size_t
+        L.attn_b200_layer_norm_backward.argtypes = [C.POINTER(NormShape)] + [vp] * 10
+        L.attn_b200_layer_norm_second_backward.argtypes = [C.POINTER(NormShape)] + [vp] * 13
         for name in EXPORTS:
             getattr(L, name)
         _lib = L

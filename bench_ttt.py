@@ -2,6 +2,7 @@
 """End-to-end test-time-training (TTT) step benchmark: the caller of the attention path.
 
     python bench_ttt.py [--gpus N] [--steps K] [--warmup W] [--impl ours|reference] [--small] [--loss logits|linear]
+                        [--layers torch|fused] [--mlp gelu|gated]
 
 Workload: a random-init 12-layer pre-norm decoder, d_model 768,
 12 heads (D = 64), GELU MLP 3072, vocabulary 32000, sequence 2048, batch 8 per GPU, bf16,
@@ -17,7 +18,9 @@ The pattern (functional forward with a parameter dict, `autograd.grad(..., creat
 not the reference's SwiGLU/RoPE model.  Attention goes through `flash_attention_v7`
 (`--impl ours`) or through the reference's math attention (`--impl reference`, on the CPU,
 on a reduced sample that is stated in the output).  `--loss linear` takes the loss through
-`linear_cross_entropy`, which does not keep the logits; the default keeps them, as the reference does.
+`linear_cross_entropy`, which does not keep the logits; the default keeps them, as the reference does.  `--layers fused`
+takes layer norms, projections and MLPs through `layers` (norms, products with activation and residual, gated blocks); the
+default uses PyTorch's.  `--mlp gated` puts SwiGLU blocks of the same width in place of the GELU MLPs.
 
 Prints one JSON line: metric `ttt_tokens_per_s`.
 """
@@ -61,43 +64,63 @@ def init_params(cfg, device, dtype, seed=0):
         fast[p + "qkv"] = w(3 * d, d); fast[p + "proj"] = w(d, d)
         fast[p + "ln2.w"] = ones(d); fast[p + "ln2.b"] = zeros(d)
         fast[p + "fc1"] = w(f, d); fast[p + "fc2"] = w(d, f)
+        if cfg.get("mlp") == "gated":
+            fast[p + "gate"] = w(f, d)
     return slow, fast
 
 
-def forward_loss(cfg, slow, fast, ids, targets, attention, linear_loss=None):
-    """Mean cross entropy of the decoder with the given fast weights."""
-    import torch
+def layer_functions(kind):
+    """(layer_norm(x, w, b), linear(x, w, residual or None), mlp(x, fc1, fc2, residual), gated(x, gate, fc1, fc2, residual))"""
     import torch.nn.functional as F
+    if kind == "fused":
+        if os.path.join(ROOT, "610sample_b200") not in sys.path:
+            sys.path.insert(0, os.path.join(ROOT, "610sample_b200"))
+        import layers
+        return (layers.layer_norm, lambda x, w, r=None: layers.linear(x, w, residual=r),
+                lambda x, a, b, r: layers.linear(layers.linear(x, a, activation="gelu"), b, residual=r),
+                lambda x, g, a, b, r: layers.gated_feed_forward(x, g, a, b, residual=r))
+    return (lambda x, w, b: F.layer_norm(x, (x.shape[-1],), w, b), lambda x, w, r=None: F.linear(x, w) if r is None else r + F.linear(x, w),
+            lambda x, a, b, r: r + F.linear(F.gelu(F.linear(x, a)), b),
+            lambda x, g, a, b, r: r + F.linear(F.silu(F.linear(x, g)) * F.linear(x, a), b))
+
+
+def forward_loss(cfg, slow, fast, ids, targets, attention, linear_loss=None, functions=None):
+    """Mean cross entropy of the decoder with the given fast weights."""
+    import torch.nn.functional as F
+    layer_norm, linear, mlp, gated = functions or layer_functions("torch")
     B, N = ids.shape
     d, H = cfg["d_model"], cfg["heads"]
     hd = d // H
     x = slow["embed"][ids]                                              # [B, N, d]
     for i in range(cfg["layers"]):
         p = f"blk{i}."
-        h = F.layer_norm(x, (d,), fast[p + "ln1.w"], fast[p + "ln1.b"])
+        h = layer_norm(x, fast[p + "ln1.w"], fast[p + "ln1.b"])
         # one GEMM for the three projections, then three 25 MB copies into the attention layout
         # (about 10 us each at this size, under 1 % of the step; per-head GEMMs that write
         # [B, H, N, hd] directly have N = 64 outputs and cost more than the copies they save)
-        qkv = F.linear(h, fast[p + "qkv"]).view(B, N, 3, H, hd).permute(2, 0, 3, 1, 4)   # [3, B, H, N, hd]
+        qkv = linear(h, fast[p + "qkv"]).view(B, N, 3, H, hd).permute(2, 0, 3, 1, 4)   # [3, B, H, N, hd]
         o = attention(qkv[0].contiguous(), qkv[1].contiguous(), qkv[2].contiguous())     # [B, H, N, hd]
-        x = x + F.linear(o.transpose(1, 2).reshape(B, N, d), fast[p + "proj"])
-        h = F.layer_norm(x, (d,), fast[p + "ln2.w"], fast[p + "ln2.b"])
-        x = x + F.linear(F.gelu(F.linear(h, fast[p + "fc1"])), fast[p + "fc2"])
-    x = F.layer_norm(x, (d,), slow["ln_f.w"], slow["ln_f.b"])
+        x = linear(o.transpose(1, 2).reshape(B, N, d), fast[p + "proj"], x)
+        h = layer_norm(x, fast[p + "ln2.w"], fast[p + "ln2.b"])
+        if cfg.get("mlp") == "gated":
+            x = gated(h, fast[p + "gate"], fast[p + "fc1"], fast[p + "fc2"], x)
+        else:
+            x = mlp(h, fast[p + "fc1"], fast[p + "fc2"], x)
+    x = layer_norm(x, slow["ln_f.w"], slow["ln_f.b"])
     if linear_loss is not None:
         return linear_loss(x, slow["head"], targets)
     logits = F.linear(x, slow["head"])
     return F.cross_entropy(logits.float().view(B * N, -1), targets.reshape(B * N))
 
 
-def ttt_step(cfg, slow, fast, ids, targets, attention, linear_loss=None):
+def ttt_step(cfg, slow, fast, ids, targets, attention, linear_loss=None, functions=None):
     """One meta step; returns the outer loss (call .backward() on it)."""
     import torch
     names = list(fast.keys())
-    inner = forward_loss(cfg, slow, fast, ids, targets, attention, linear_loss)
+    inner = forward_loss(cfg, slow, fast, ids, targets, attention, linear_loss, functions)
     grads = torch.autograd.grad(inner, [fast[n] for n in names], create_graph=True)
     updated = {n: fast[n] - INNER_LR * g for n, g in zip(names, grads)}
-    return forward_loss(cfg, slow, updated, ids, targets, attention, linear_loss)
+    return forward_loss(cfg, slow, updated, ids, targets, attention, linear_loss, functions)
 
 
 def make_batch(cfg, device, seed):
@@ -168,9 +191,10 @@ def measure(args, init_process_group=True):
     cfg = dict(SMALL if args.small else FULL)
     reference = args.impl == "reference"
     linear = getattr(args, "loss", "logits") == "linear"
-    linear_loss = sample = None
-    if linear and reference:
-        raise SystemExit("--loss linear needs the kernels: it goes with --impl ours")
+    layer_kind, cfg["mlp"] = getattr(args, "layers", "torch"), getattr(args, "mlp", "gelu")
+    linear_loss = sample = functions = None
+    if (linear or layer_kind == "fused") and reference:
+        raise SystemExit("--loss linear and --layers fused need the kernels: they go with --impl ours")
     if reference:
         # CPU arm: the reference's math attention; a reduced sample of the workload, stated below
         if rank != 0:
@@ -194,6 +218,7 @@ def measure(args, init_process_group=True):
         sys.path.insert(0, os.path.join(ROOT, "610sample_b200"))
         import attention_cuda
         from attention import FlashAttentionV7, flash_attention_v7
+        functions = layer_functions(layer_kind)
         if linear:
             from loss import linear_cross_entropy as linear_loss
         timer = AttentionTimer(attention_cuda)
@@ -210,7 +235,7 @@ def measure(args, init_process_group=True):
     def step():
         for p in params:
             p.grad = None
-        loss = ttt_step(cfg, slow, fast, ids, targets, attention, linear_loss)
+        loss = ttt_step(cfg, slow, fast, ids, targets, attention, linear_loss, functions)
         loss.backward()
         if world > 1:
             flat = torch.cat([p.grad.reshape(-1) for p in params])
@@ -262,7 +287,8 @@ def measure(args, init_process_group=True):
             "impl": args.impl,
             "config": {"workload": "ttt_step_12L_d768_h12_seq2048_b8" if not args.small else "ttt_step_small",
                        **{k: cfg[k] for k in ("layers", "d_model", "heads", "d_ff", "vocab", "seq", "batch")},
-                       "inner_lr": INNER_LR, "sample": sample, **({"loss": "linear"} if linear else {})},
+                       "inner_lr": INNER_LR, "sample": sample, **({"loss": "linear"} if linear else {}),
+                       **({"layers": layer_kind} if layer_kind != "torch" else {}), **({"mlp": cfg["mlp"]} if cfg["mlp"] != "gelu" else {})},
             "outer_loss": float(loss.detach()), "peak_memory_mb": peak_mb,
         }
         if attn_ms is not None:
@@ -291,6 +317,8 @@ def main():
     ap.add_argument("--impl", default="ours", choices=["ours", "reference"])
     ap.add_argument("--small", action="store_true", help="2-layer toy configuration (tests)")
     ap.add_argument("--loss", default="logits", choices=["logits", "linear"], help="cross entropy of kept logits, or linear_cross_entropy")
+    ap.add_argument("--layers", default="torch", choices=["torch", "fused"], help="norms, projections and MLPs: PyTorch's, or this framework's")
+    ap.add_argument("--mlp", default="gelu", choices=["gelu", "gated"], help="GELU MLPs, or gated (SwiGLU) blocks of the same width")
     run(ap.parse_args())
 
 
