@@ -277,8 +277,9 @@ int attn_b200_linear_ce_backward(const attn_lce_shape_t* shape, const void* x, c
  *                        out = activation(z) u
  *   ATTN_PRODUCT_GATED_GRAD   NN, one result, without bias: given kept = (z, u), out = sum activation'(z) u, out2 = sum activation(z)
  * Rows are `ld` elements apart, columns dense.  f16 and bf16 on the tensor cores: bases 16-byte aligned, strides multiples of 8;
- * f32 on the CUDA cores.  A residual and a bias may have any alignment of an element.  Only columns of a result are written, never what lies between them
- * and the next row.  z of a plain product is kept in the type, within its finite range; z and u
+ * f32 on the CUDA cores.  A residual and a bias may have any alignment of an element.  Rows of results and of what is kept are written up to the next
+ * multiple of 8 columns in half types (the last row's memory has to reach there too), never behind it.  z of a plain product is kept in the type, within its finite
+ * range; z and u
  * of a gated one in 20 bits of f16 and bf16: 16 of each in kept, and 4 of both in a plane of bytes, kept_low, whose rows are a multiple of 32
  * apart from a 32-byte aligned base.  Their encoding is the kernels' own.  Inputs must not overlap outputs. */
 enum { ATTN_FORM_NT = 0, ATTN_FORM_NN = 1, ATTN_FORM_TN = 2 };
