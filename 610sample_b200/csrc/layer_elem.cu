@@ -109,6 +109,7 @@ __global__ void __launch_bounds__(256)
 elementwise_kernel(const __grid_constant__ ElementArgs a) {
   constexpr bool kPrecise = sizeof(T) == 4;
   typedef Columns<T, WIDE> C;
+  typedef Columns<typename ArgumentOf<T>::type, WIDE> Z;      // z of a plain product
   __shared__ float sums[8][kElemCols];
   tc::pdl_wait();
   tc::pdl_trigger();
@@ -123,12 +124,13 @@ elementwise_kernel(const __grid_constant__ ElementArgs a) {
   if constexpr (PASS == PASS_FIRST) {
     constexpr int kRows = sizeof(T) == 2 ? 4 : 2;      // of a thread, on their way at once
     for (int r0 = (int)first + group; r0 < end; r0 += 8 * kRows) {
-      typename C::Raw rg[kRows], rz[ACT != ACT_NONE ? kRows : 1];
+      typename C::Raw rg[kRows];
+      typename Z::Raw rz[ACT != ACT_NONE ? kRows : 1];
 #pragma unroll
       for (int i = 0; i < kRows; ++i) {
         const int r = min(r0 + 8 * i, end - 1);
         rg[i] = C::fetch(a.in[0], a.ld_in[0], r, c0, a.m);
-        if constexpr (ACT != ACT_NONE) rz[i] = C::fetch(a.in[1], a.ld_in[1], r, c0, a.m);
+        if constexpr (ACT != ACT_NONE) rz[i] = Z::fetch(a.in[1], a.ld_in[1], r, c0, a.m);
       }
 #pragma unroll
       for (int i = 0; i < kRows; ++i) {
@@ -138,7 +140,7 @@ elementwise_kernel(const __grid_constant__ ElementArgs a) {
         C::values(rg[i], g);
         if constexpr (ACT != ACT_NONE) {
           float z[8];
-          C::values(rz[i], z);
+          Z::values(rz[i], z);
 #pragma unroll
           for (int e = 0; e < 8; e += 2) {
             if constexpr (kPrecise) {
@@ -167,7 +169,7 @@ elementwise_kernel(const __grid_constant__ ElementArgs a) {
     load(0, r, g);
     if constexpr (PASS == PASS_SECOND) {
       float t[8], gg[8], s[8];
-      load(1, r, z);
+      Z::load(a.in[1], a.ld_in[1], r, c0, a.m, z);
       load(2, r, t);
 #pragma unroll
       for (int e = 0; e < 8; ++e) {

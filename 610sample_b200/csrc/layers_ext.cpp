@@ -14,9 +14,9 @@ struct Matrix {
   const void* data() const { return t.data_ptr(); }
 };
 
-torch::Tensor padded(int64_t rows, int64_t cols, const torch::Tensor& like) {
-  const int64_t pitch = like.scalar_type() == at::kFloat ? cols : (cols + 7) / 8 * 8;
-  torch::Tensor t = fresh({rows, pitch}, like.scalar_type(), like);
+torch::Tensor padded(int64_t rows, int64_t cols, const torch::Tensor& like, at::ScalarType type) {
+  const int64_t pitch = type == at::kFloat ? cols : (cols + 7) / 8 * 8;
+  torch::Tensor t = fresh({rows, pitch}, type, like);
   return pitch == cols ? t : t.narrow(1, 0, cols);
 }
 
@@ -29,15 +29,15 @@ Matrix matrix(const torch::Tensor& t_in, bool any_rows = false) {
   const int64_t ld = rows > 1 ? t.stride(0) : (cols + 7) / 8 * 8;      // one row: any distance
   const bool dense_rows = (cols <= 1 || t.stride(1) == 1) && ld >= cols;
   if (t.numel() > 0 && dense_rows && (any_rows || !half || (ld % 8 == 0 && reinterpret_cast<uintptr_t>(t.data_ptr()) % 16 == 0))) return {t, ld};
-  torch::Tensor copy = any_rows ? fresh({rows, cols}, t.scalar_type(), t) : padded(rows, cols, t);
+  torch::Tensor copy = any_rows ? fresh({rows, cols}, t.scalar_type(), t) : padded(rows, cols, t, t.scalar_type());
   copy.copy_(t);
   return {copy, rows > 1 ? copy.stride(0) : (cols + 7) / 8 * 8};
 }
 
-Matrix result(int64_t rows, int64_t cols, const torch::Tensor& like) {
-  torch::Tensor t = padded(rows, cols, like);
-  return {t, like.scalar_type() == at::kFloat ? cols : (cols + 7) / 8 * 8};
+Matrix result(int64_t rows, int64_t cols, const torch::Tensor& like, at::ScalarType type) {
+  return {padded(rows, cols, like, type), type == at::kFloat ? cols : (cols + 7) / 8 * 8};
 }
+Matrix result(int64_t rows, int64_t cols, const torch::Tensor& like) { return result(rows, cols, like, like.scalar_type()); }
 // a result as the caller gets it
 torch::Tensor handed(const Matrix& m, at::IntArrayRef sizes) {
   const torch::Tensor t = m.t.is_contiguous() ? m.t : m.t.contiguous();
@@ -192,7 +192,7 @@ variable_list linear_forward(const torch::Tensor& x_in, const torch::Tensor& w_i
   const Matrix x = matrix(x_in), w = matrix(w_in), y = result(n, m, x_in);
   Matrix r, z;
   if (r_in.defined()) r = matrix(r_in);
-  if (keep) z = result(n, m, x_in);
+  if (keep) z = result(n, m, x_in, x_in.scalar_type() == at::kFloat ? at::kFloat : at::kHalf);
   const torch::Tensor b = b_in.defined() ? b_in.contiguous() : b_in;
   Products(x_in, ATTN_FORM_NT, ATTN_PRODUCT_PLAIN, activation).add(y, n, m, k, {{&x, &w}}).bias(b).residual(r).kept(0, z).run("linear");
   return {handed(y, with_columns(x_in, m)), z.t};

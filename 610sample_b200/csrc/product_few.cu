@@ -133,7 +133,7 @@ product_few_kernel(const __grid_constant__ FewArgs g) {
         static_cast<uint16_t*>(g.kept[1])[r * g.ld_kept[1] + j] = (uint16_t)(cu >> 16);
         static_cast<uint8_t*>(g.low)[r * g.ld_low + j] = (uint8_t)((cz >> 12 & 0xfu) | (cu >> 8 & 0xf0u));
       } else {
-        static_cast<uint16_t*>(g.kept[0])[r * g.ld_kept[0] + j] = (uint16_t)pack_finite<T>(z, z);
+        static_cast<uint16_t*>(g.kept[0])[r * g.ld_kept[0] + j] = (uint16_t)pack_argument(z, z);
       }
     }
     float y = z;

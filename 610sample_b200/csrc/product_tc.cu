@@ -430,7 +430,7 @@ product_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Produc
             }
             if (keep) {
 #pragma unroll
-              for (int e = 0; e < 8; ++e) w[e] = pack_finite<T>(f[e].x, f[e].y);
+              for (int e = 0; e < 8; ++e) w[e] = pack_argument(f[e].x, f[e].y);
               stage16(staging + 2048, false, lane, 16 * q, w);
             }
             if (g.act != ACT_NONE)
@@ -539,7 +539,7 @@ join_kernel(const __grid_constant__ ProductArgs g) {
     };
     if (g.bias != nullptr)
       for (int e = 0; e < width; ++e) v[e] += Elem<T>::to_float(static_cast<const T*>(g.bias)[col + e]);
-    if (g.kept.p != nullptr) put(g.kept, pack_finite<T>(v[0], v[1]), pack_finite<T>(v[2], v[3]));
+    if (g.kept.p != nullptr) put(g.kept, pack_argument(v[0], v[1]), pack_argument(v[2], v[3]));
     with_activation(g.act, [&](auto act) {
 #pragma unroll
       for (int e = 0; e < 4; e += 2) {

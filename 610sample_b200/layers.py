@@ -37,7 +37,7 @@ def linear(x, weight, bias=None, activation=None, residual=None):
     """activation(x weight^T + bias) + residual.  x: (..., k); weight: (m, k); bias: (m,); residual: (..., m); of one type.
 
     activation: None, "silu", "gelu" (with the normal distribution) or "gelu_tanh".  Sums are float32, and the result is rounded once.
-    With an activation the backward keeps its argument, rounded to the type of x.  Half types run on the tensor cores: slices whose rows start
+    With an activation the backward keeps its argument, of half types in fp16 within its range.  Half types run on the tensor cores: slices whose rows start
     at multiples of 16 bytes are read in place, others (odd widths, transposed weights) are copied first.  float32 runs on the
     CUDA cores, without TF32."""
     return _attention_cuda.linear(x, weight, bias, residual, _activation(activation))
@@ -48,5 +48,6 @@ def gated_feed_forward(x, w_gate, w_up, w_down, activation="silu", residual=None
     residual: (..., m); of one type.
 
     Both projections, the activation and the product are one kernel, the second projection with the residual another.  The inner
-    values are rounded to the type of x before the second projection; the backward keeps them and both projections."""
+    values are rounded to the type of x before the second projection; the backward keeps them and both projections, of half types
+with four bits more than 16 each (in fp16 projections beyond 65504 are kept as that)."""
     return _attention_cuda.gated_feed_forward(x, w_gate, w_up, w_down, residual, _activation(activation))

@@ -278,8 +278,8 @@ int attn_b200_linear_ce_backward(const attn_lce_shape_t* shape, const void* x, c
  *   ATTN_PRODUCT_GATED_GRAD   NN, one result, without bias: given kept = (z, u), out = sum activation'(z) u, out2 = sum activation(z)
  * Rows are `ld` elements apart, columns dense.  f16 and bf16 on the tensor cores: bases 16-byte aligned, strides multiples of 8;
  * f32 on the CUDA cores.  A residual and a bias may have any alignment of an element.  Rows of results and of what is kept are written up to the next
- * multiple of 8 columns in half types (the last row's memory has to reach there too), never behind it.  z of a plain product is kept in the type, within its finite
- * range; z and u
+ * multiple of 8 columns in half types (the last row's memory has to reach there too), never behind it.  z of a plain product is kept in f16 of half types, within its
+ * finite range; z and u
  * of a gated one in 20 bits of f16 and bf16: 16 of each in kept, and 4 of both in a plane of bytes, kept_low, whose rows are a multiple of 32
  * apart from a 32-byte aligned base.  Their encoding is the kernels' own.  Inputs must not overlap outputs. */
 enum { ATTN_FORM_NT = 0, ATTN_FORM_NN = 1, ATTN_FORM_TN = 2 };
@@ -317,7 +317,7 @@ int attn_b200_products(const attn_products_t* call, void* scratch, void* stream)
  *   SECOND         in g, z, t        out t activation'(z), s = g activation''(z) t, dz;  sum: of s.  t is the tangent of z
  *   GATED_SECOND   in gh, z, u, zt, ut, gh2 (or null)   out, with h = a(z) u, zt and ut the tangents of z and u, gh the gradient of h and gh2 a
  *                  part of the gradient of h's tangent's factor:  ht = a' zt u + a ut,  gh a' u,  gh a,  gh (a'' zt u + a' ut) + gh2 a' u,
- *                  gh a' zt + gh2 a.  z and u as a gated product keeps them
+ *                  gh a' zt + gh2 a.  z, and z and u, as plain and gated products keep them
  * sum: [m] of the type, or null; scratch is used with it. */
 enum { ATTN_ELEMENTS_FIRST = 0, ATTN_ELEMENTS_SECOND = 1, ATTN_ELEMENTS_GATED_SECOND = 2 };
 typedef struct attn_elements {

@@ -234,8 +234,8 @@ def linear_reference(x, w, b, r, g, kind, dtype):
     ea = ez * 1.2 + own
     y = a if r is None else a + r
     ey = ea + 2 * F32 * y.abs()
-    # z is kept rounded; |a''| <= 1.25 for all of them
-    kept = ez if dtype == torch.float32 else rounded(z, ez, dtype)
+    # z is kept in f16; |a''| <= 1.25 for all of them
+    kept = ez if dtype == torch.float32 else rounded(z, ez, torch.float16)
     ed = own + (kept * 1.25 if kind else 0.0)
     dz = g * d1
     edz = rounded(dz, g.abs() * ed + 4 * F32 * dz.abs(), dtype) if kind else zero(dz)
