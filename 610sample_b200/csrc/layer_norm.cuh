@@ -7,7 +7,8 @@
 //            m(q) and m(q xh) follow from the means of c, u, g uw and their products with xh, so one round of sums over the row does
 //
 // Every pass reads its rows once: a row stays in the registers of a group of 32 to 1024 threads, so that the variance is that of the centred row.  Bound by memory.  Sums over the rows stay in registers while a group goes from row to row, its next row on the way; a
-// kernel behind adds what the CTAs have, in order.
+// kernel behind adds what the CTAs have, in order.  16384 x 768 bf16 (ncu, cold): forward 15 us (50 MB), dx with dw and db 20 (75 MB) and 7; 8195 x 4096 f16: 34 (3.9 TB/s), 45
+// (4.5) and 8.  Above 8192 columns the backward's registers spill.
 #pragma once
 
 #include "attn_common.cuh"

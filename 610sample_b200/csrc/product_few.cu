@@ -4,6 +4,9 @@
 // A CTA has 16 rows of the weight (of Wg and of Wu in a gated product), its warps share k in blocks of 32.  A thread reads 16 bytes of two rows of
 // the weight and of one row of `a` straight into the fragments of two m16n8k16 products, whose order of k does not matter as long as both operands have
 // the same.  Four blocks of a warp are on their way at once.  The warps' sums meet in shared memory, in order.
+//
+// One row, bf16, in a graph of many calls on weights from HBM: 768 -> 2304 2.6 us, 2048 -> 5504 6.7, 5504 -> 2048 7.3 (9.7 with eight warps), 4096 -> 14336 26.5 (4.4 TB/s; the copy
+// rate takes 17.9): latency of loads.  Eight blocks on their way were 7.7 at 2048 -> 5504, with fewer CTAs an SM.
 #include "activation.cuh"
 #include "layer_launch.h"
 #include "tc_common.cuh"
