@@ -123,7 +123,7 @@ elementwise_kernel(const __grid_constant__ ElementArgs a) {
   auto load = [&](int i, int r, float (&f)[8]) { C::load(a.in[i], a.ld_in[i], r, c0, a.m, f); };
   auto store = [&](int i, int r, const float (&f)[8]) { C::store(a.out[i], a.ld_out[i], r, c0, a.m, f); };
   if constexpr (PASS == PASS_FIRST) {
-    constexpr int kRows = sizeof(T) == 2 ? 4 : 2;      // of a thread, on their way at once
+    constexpr int kRows = (sizeof(T) == 2 ? 4 : 2) * (ACT == ACT_NONE ? 2 : 1);      // of a thread, on their way at once
     for (int r0 = (int)first + group; r0 < end; r0 += 8 * kRows) {
       typename C::Raw rg[kRows];
       typename Z::Raw rz[ACT != ACT_NONE ? kRows : 1];
