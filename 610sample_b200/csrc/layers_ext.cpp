@@ -34,6 +34,10 @@ Matrix matrix(const torch::Tensor& t_in, bool any_rows = false) {
   return {copy, rows > 1 ? copy.stride(0) : (cols + 7) / 8 * 8};
 }
 
+// The copy that `matrix` made of a tensor, for the backward to read again; nothing where it made none
+torch::Tensor copied(const Matrix& m, const torch::Tensor& from) { return m.t.is_alias_of(from) ? torch::Tensor() : m.t; }
+const torch::Tensor& either(const torch::Tensor& copy, const torch::Tensor& from) { return copy.defined() ? copy : from; }
+
 Matrix result(int64_t rows, int64_t cols, const torch::Tensor& like, at::ScalarType type) {
   return {padded(rows, cols, like, type), type == at::kFloat ? cols : (cols + 7) / 8 * 8};
 }
@@ -183,7 +187,7 @@ void check_linear(const torch::Tensor& x, const torch::Tensor& w, const torch::T
   TORCH_CHECK(!r.defined() || r.sizes() == at::IntArrayRef(with_columns(x, w.size(0))), "residual must have the shape of the result");
 }
 
-// {y, z}; z, what the activation is applied to, where it is to be kept
+// {y, z, copies of x and w}; z, what the activation is applied to, where it is to be kept
 variable_list linear_forward(const torch::Tensor& x_in, const torch::Tensor& w_in, const torch::Tensor& b_in, const torch::Tensor& r_in,
                              int64_t activation, bool keep) {
   c10::cuda::CUDAGuard guard(x_in.device());
@@ -195,12 +199,12 @@ variable_list linear_forward(const torch::Tensor& x_in, const torch::Tensor& w_i
   if (keep) z = result(n, m, x_in, x_in.scalar_type() == at::kFloat ? at::kFloat : at::kHalf);
   const torch::Tensor b = b_in.defined() ? b_in.contiguous() : b_in;
   Products(x_in, ATTN_FORM_NT, ATTN_PRODUCT_PLAIN, activation).add(y, n, m, k, {{&x, &w}}).bias(b).residual(r).kept(0, z).run("linear");
-  return {handed(y, with_columns(x_in, m)), z.t};
+  return {handed(y, with_columns(x_in, m)), z.t, copied(x, x_in), copied(w, w_in)};
 }
 
-// {dx, dw, db}, undefined where not wanted
+// {dx, dw, db}, undefined where not wanted.  x_copy, w_copy: the forward's, where it made any
 variable_list linear_backward(const torch::Tensor& g_in, const torch::Tensor& x_in, const torch::Tensor& w_in, const torch::Tensor& z_in,
-                              int64_t activation, bool want_x, bool want_w, bool want_b) {
+                              int64_t activation, bool want_x, bool want_w, bool want_b, const torch::Tensor& x_copy = {}, const torch::Tensor& w_copy = {}) {
   variable_list out(3);
   if (!want_x && !want_w && !want_b) return out;
   c10::cuda::CUDAGuard guard(x_in.device());
@@ -216,12 +220,12 @@ variable_list linear_backward(const torch::Tensor& g_in, const torch::Tensor& x_
     Elements(x_in, n, m, ATTN_ELEMENTS_FIRST, activation).in(0, g).run(out[2], "linear backward");
   }
   if (want_x) {
-    const Matrix w = matrix(w_in), dx = result(n, k, x_in);
+    const Matrix w = matrix(either(w_copy, w_in)), dx = result(n, k, x_in);
     Products(x_in, ATTN_FORM_NN).add(dx, n, k, m, {{&dz, &w}}).run("linear backward");
     out[0] = handed(dx, x_in.sizes());
   }
   if (want_w) {
-    const Matrix x = matrix(x_in), dw = result(m, k, x_in);
+    const Matrix x = matrix(either(x_copy, x_in)), dw = result(m, k, x_in);
     Products(x_in, ATTN_FORM_TN).add(dw, m, k, n, {{&dz, &x}}).run("linear backward");
     out[1] = handed(dw, w_in.sizes());
   }
@@ -307,7 +311,7 @@ struct Linear : public torch::autograd::Function<Linear> {
     ctx->set_materialize_grads(false);
     ctx->saved_data["activation"] = activation;
     ctx->saved_data["residual"] = r.defined();
-    ctx->save_for_backward({x, w, b, out[1]});
+    ctx->save_for_backward({x, w, b, out[1], out[2], out[3]});
     return out[0];
   }
 
@@ -320,7 +324,7 @@ struct Linear : public torch::autograd::Function<Linear> {
     variable_list r = at::GradMode::is_enabled()
                           ? LinearBackward::apply(g[0], s[0], s[1], maybe(s[2]), maybe(s[3]), activation)
                           : linear_backward(g[0], s[0], s[1], s[3], activation, ctx->needs_input_grad(0), ctx->needs_input_grad(1),
-                                            s[2].defined() && ctx->needs_input_grad(2));
+                                            s[2].defined() && ctx->needs_input_grad(2), s[4], s[5]);
     for (size_t i = 0; i < r.size(); ++i) out[i] = std::move(r[i]);
     if (ctx->saved_data["residual"].toBool()) out[3] = g[0];
     return out;
@@ -349,7 +353,7 @@ void check_gated(const torch::Tensor& x, const torch::Tensor& wg, const torch::T
   TORCH_CHECK(!r.defined() || r.sizes() == at::IntArrayRef(with_columns(x, wd.size(0))), "residual must have the shape of the result");
 }
 
-// {y, z, u, their lower bits, h}; z = x wg^T and u = x wu^T where they are to be kept, h = a(z) u
+// {y, z, u, their lower bits, h, copies of x, wg, wu, wd}; z = x wg^T and u = x wu^T where they are to be kept, h = a(z) u
 variable_list gated_forward(const torch::Tensor& x_in, const torch::Tensor& wg_in, const torch::Tensor& wu_in, const torch::Tensor& wd_in,
                             const torch::Tensor& r_in, int64_t activation, bool keep) {
   c10::cuda::CUDAGuard guard(x_in.device());
@@ -366,22 +370,22 @@ variable_list gated_forward(const torch::Tensor& x_in, const torch::Tensor& wg_i
   inner.c.ldb2 = wu.ld;
   inner.run("gated_feed_forward");
   Products(x_in, ATTN_FORM_NT).add(y, n, m, f, {{&h, &wd}}).residual(r).run("gated_feed_forward");
-  return {handed(y, with_columns(x_in, m)), kept.z.t, kept.u.t, kept.low, h.t};
+  return {handed(y, with_columns(x_in, m)), kept.z.t, kept.u.t, kept.low, h.t, copied(x, x_in), copied(wg, wg_in), copied(wu, wu_in), copied(wd, wd_in)};
 }
 
-// {dx, dwg, dwu, dwd}, undefined where not wanted.  The gradient of h exists in the product's epilogue only, where it becomes those of z and u.
+// {dx, dwg, dwu, dwd}, undefined where not wanted; copies: the forward's of x, wg, wu, wd, or none.  The gradient of h exists in the product's epilogue only, where it becomes those of z and u.
 variable_list gated_backward(const torch::Tensor& g_in, const torch::Tensor& x_in, const torch::Tensor& wg_in, const torch::Tensor& wu_in,
                              const torch::Tensor& wd_in, const KeptPlanes& kept, const torch::Tensor& h_in,
-                             int64_t activation, bool want_x, bool want_g, bool want_u, bool want_d) {
+                             int64_t activation, bool want_x, bool want_g, bool want_u, bool want_d, const variable_list& copies = variable_list(4)) {
   variable_list out(4);
   if (!want_x && !want_g && !want_u && !want_d) return out;
   c10::cuda::CUDAGuard guard(x_in.device());
   begin_call(x_in);
   const int64_t d = columns_of(x_in), n = x_in.numel() / d, f = wg_in.size(0), m = wd_in.size(0);
-  const Matrix g = matrix(g_in), x = matrix(x_in);
+  const Matrix g = matrix(g_in), x = matrix(either(copies[0], x_in));
   Matrix dz, du;
   if (want_x || want_g || want_u) {
-    const Matrix wd = matrix(wd_in);
+    const Matrix wd = matrix(either(copies[3], wd_in));
     dz = result(n, f, x_in);
     du = result(n, f, x_in);
     Products inner(x_in, ATTN_FORM_NN, ATTN_PRODUCT_GATED_GRAD, activation);
@@ -391,7 +395,7 @@ variable_list gated_backward(const torch::Tensor& g_in, const torch::Tensor& x_i
     inner.run("gated_feed_forward backward");
   }
   if (want_x) {
-    const Matrix wg = matrix(wg_in), wu = matrix(wu_in), dx = result(n, d, x_in);
+    const Matrix wg = matrix(either(copies[1], wg_in)), wu = matrix(either(copies[2], wu_in)), dx = result(n, d, x_in);
     Products(x_in, ATTN_FORM_NN).add(dx, n, d, f, {{&dz, &wg}, {&du, &wu}}).run("gated_feed_forward backward");
     out[0] = handed(dx, x_in.sizes());
   }
@@ -476,7 +480,7 @@ struct Gated : public torch::autograd::Function<Gated> {
     ctx->set_materialize_grads(false);
     ctx->saved_data["activation"] = activation;
     ctx->saved_data["residual"] = r.defined();
-    ctx->save_for_backward({x, wg, wu, wd, out[1], out[2], out[3], out[4]});
+    ctx->save_for_backward({x, wg, wu, wd, out[1], out[2], out[3], out[4], out[5], out[6], out[7], out[8]});
     return out[0];
   }
 
@@ -489,7 +493,7 @@ struct Gated : public torch::autograd::Function<Gated> {
     variable_list r = at::GradMode::is_enabled()
                           ? GatedBackward::apply(g[0], s[0], s[1], s[2], s[3], s[4], s[5], maybe(s[6]), s[7], activation)
                           : gated_backward(g[0], s[0], s[1], s[2], s[3], kept_planes(s[4], s[5], s[6]), s[7], activation, ctx->needs_input_grad(0), ctx->needs_input_grad(1),
-                                           ctx->needs_input_grad(2), ctx->needs_input_grad(3));
+                                           ctx->needs_input_grad(2), ctx->needs_input_grad(3), {s[8], s[9], s[10], s[11]});
     for (int i = 0; i < 4; ++i) out[i] = std::move(r[i]);
     if (ctx->saved_data["residual"].toBool()) out[4] = g[0];
     return out;
