@@ -31,7 +31,7 @@ EXPORTS = (
     "attn_b200_linear_ce_forward_scratch_bytes", "attn_b200_linear_ce_forward", "attn_b200_linear_ce_backward_scratch_bytes",
     "attn_b200_linear_ce_backward", "attn_b200_packed_qk_norm_rope", "attn_b200_packed_qk_norm_rope_backward_scratch_bytes",
     "attn_b200_packed_qk_norm_rope_backward", "attn_b200_products_scratch_bytes", "attn_b200_products", "attn_b200_elements_scratch_bytes",
-    "attn_b200_elements", "attn_b200_layer_norm", "attn_b200_layer_norm_backward_scratch_bytes", "attn_b200_layer_norm_backward",
+    "attn_b200_elements", "attn_b200_copy_rows", "attn_b200_layer_norm", "attn_b200_layer_norm_backward_scratch_bytes", "attn_b200_layer_norm_backward",
     "attn_b200_layer_norm_second_backward",
 )
 
@@ -132,6 +132,7 @@ def lib() -> C.CDLL:
         L.attn_b200_elements_scratch_bytes.argtypes = [C.POINTER(Elements)]
         L.attn_b200_elements_scratch_bytes.restype = C.c_size_t
         L.attn_b200_elements.argtypes = [C.POINTER(Elements), vp, vp]
+        L.attn_b200_copy_rows.argtypes = [vp, C.c_int64, vp, C.c_int64] + [C.c_int32] * 3 + [vp]
         L.attn_b200_layer_norm.argtypes = [C.POINTER(NormShape)] + [vp] * 7
         L.attn_b200_layer_norm_backward_scratch_bytes.argtypes = [C.POINTER(NormShape)]
         L.attn_b200_layer_norm_backward_scratch_bytes.restype = C.c_size_t

@@ -216,6 +216,22 @@ int attn_b200_elements(const attn_elements_t* e, void* scratch, void* stream) {
   return capi::done(err, "elements launch failed", nullptr, launches);
 }
 
+int attn_b200_copy_rows(const void* src, int64_t lds, void* dst, int64_t ldd, int32_t rows, int32_t cols, int32_t dtype, void* stream) {
+  if (!known_type(dtype)) return fail(ATTN_EUNSUPPORTED, "dtype %d: expected ATTN_F16, ATTN_BF16 or ATTN_F32", dtype);
+  if (rows < 0 || cols < 0 || rows > kMostRows || cols > kMostRows) return fail(ATTN_EINVAL, "rows and cols must be in [0, 2^30] (got %d, %d)", rows, cols);
+  int rc = ATTN_OK;
+  if (rows > 0 && cols > 0) {
+    rc = check_rows("src", src, lds, cols, dtype);
+    if (rc == ATTN_OK) rc = check_rows("dst", dst, ldd, cols, dtype);
+  }
+  if (rc != ATTN_OK) return rc;
+  unsigned int* status = nullptr;
+  rc = capi::begin(&status);
+  if (rc != ATTN_OK) return rc;
+  if (rows == 0 || cols == 0) return capi::done(cudaSuccess, "", nullptr, 0);
+  return capi::done(launch_copy_rows(src, lds, dst, ldd, rows, cols, size_of(dtype), static_cast<cudaStream_t>(stream)), "copy launch failed", nullptr, 1);
+}
+
 int attn_b200_layer_norm(const attn_norm_shape_t* s, const void* x, const void* w, const void* b, void* y, float* mean, float* rstd, void* stream) {
   int rc = check_norm(s);
   if (rc != ATTN_OK) return rc;

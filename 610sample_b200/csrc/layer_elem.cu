@@ -259,6 +259,34 @@ cudaError_t launch_sum_rows(const float* partial, int rows, int kinds, int d, in
 }
 
 
+// Rows into rows of another pitch, for widths that the tensor cores' loads do not take as they are: one element of `sizeof(U)` bytes at a time, neighbouring
+// threads on neighbouring elements.  The ten copies of a gated block's pass of odd widths took
+// the host 80 us as tensor operations, about 55 so.  I: unsigned where all elements have one.
+template <typename U, typename I>
+__global__ void __launch_bounds__(256)
+copy_rows_kernel(const U* src, long long lds, U* dst, long long ldd, I total, I cols) {
+  tc::pdl_wait();
+  tc::pdl_trigger();
+  const I step = (I)gridDim.x * 256;
+#pragma unroll 4
+  for (I i = (I)blockIdx.x * 256 + threadIdx.x; i < total; i += step) {
+    const I r = i / cols, c = i - r * cols;
+    dst[(long long)r * ldd + c] = src[(long long)r * lds + c];
+  }
+}
+
+template <typename U>
+static cudaError_t copy_rows(const void* src, long long lds, void* dst, long long ldd, int rows, int cols, cudaStream_t stream) {
+  const unsigned long long total = (unsigned long long)rows * cols, want = (total + 1023) / 1024;
+  const unsigned ctas = (unsigned)(want < 16 * kSms ? want : 16 * kSms);
+  if (total < (1ull << 31))      // a step beyond the last element stays below 2^32
+    return tc::launch_pdl(copy_rows_kernel<U, unsigned>, ctas, 256u, 0, stream, (const U*)src, lds, (U*)dst, ldd, (unsigned)total, (unsigned)cols);
+  return tc::launch_pdl(copy_rows_kernel<U, unsigned long long>, ctas, 256u, 0, stream, (const U*)src, lds, (U*)dst, ldd, total, (unsigned long long)cols);
+}
+cudaError_t launch_copy_rows(const void* src, long long lds, void* dst, long long ldd, int rows, int cols, int size, cudaStream_t stream) {
+  return size == 2 ? copy_rows<uint16_t>(src, lds, dst, ldd, rows, cols, stream) : copy_rows<uint32_t>(src, lds, dst, ldd, rows, cols, stream);
+}
+
 // ---- host ---------------------------------------------------------------------------------------
 // Runs of rows: six CTAs an SM, 64 rows each at least
 int element_chunks(int n, int m) {

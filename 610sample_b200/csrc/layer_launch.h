@@ -37,6 +37,8 @@ struct ElementArgs {
 };
 int element_chunks(int n, int m);
 cudaError_t launch_elementwise(ElementArgs a, int pass, int act, int dtype, cudaStream_t stream);
+// dst[r][c] = src[r][c], elements of 2 or 4 bytes
+cudaError_t launch_copy_rows(const void* src, long long lds, void* dst, long long ldd, int rows, int cols, int size, cudaStream_t stream);
 // out_k[c] = sum over the rows of partial [rows][kinds][d], in order; one or two kinds
 cudaError_t launch_sum_rows(const float* partial, int rows, int kinds, int d, int dtype, void* out0, void* out1, cudaStream_t stream);
 

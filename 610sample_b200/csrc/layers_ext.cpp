@@ -22,6 +22,13 @@ torch::Tensor padded(int64_t rows, int64_t cols, const torch::Tensor& like, at::
 
 int64_t columns_of(const torch::Tensor& t) { return t.size(t.dim() - 1); }
 
+// a matrix whose columns are dense, into another one
+void copy_rows(const torch::Tensor& from, int64_t from_ld, const torch::Tensor& to, int64_t to_ld) {
+  check_rc(attn_b200_copy_rows(from.data_ptr(), from_ld, to.data_ptr(), to_ld, (int32_t)from.size(0), (int32_t)from.size(1), dtype_code(from),
+                               at::cuda::getCurrentCUDAStream().stream()),
+           "copy");
+}
+
 Matrix matrix(const torch::Tensor& t_in, bool any_rows = false) {
   const int64_t cols = columns_of(t_in), rows = cols > 0 ? t_in.numel() / cols : 0;
   torch::Tensor t = t_in.dim() == 2 ? t_in : t_in.reshape({rows, cols});
@@ -30,8 +37,10 @@ Matrix matrix(const torch::Tensor& t_in, bool any_rows = false) {
   const bool dense_rows = (cols <= 1 || t.stride(1) == 1) && ld >= cols;
   if (t.numel() > 0 && dense_rows && (any_rows || !half || (ld % 8 == 0 && reinterpret_cast<uintptr_t>(t.data_ptr()) % 16 == 0))) return {t, ld};
   torch::Tensor copy = any_rows ? fresh({rows, cols}, t.scalar_type(), t) : padded(rows, cols, t, t.scalar_type());
-  copy.copy_(t);
-  return {copy, rows > 1 ? copy.stride(0) : (cols + 7) / 8 * 8};
+  const int64_t pitch = any_rows || !half ? cols : (cols + 7) / 8 * 8;
+  if (dense_rows && t.numel() > 0) copy_rows(t, ld, copy, pitch);
+  else copy.copy_(t);
+  return {copy, rows > 1 ? pitch : (cols + 7) / 8 * 8};
 }
 
 // The copy that `matrix` made of a tensor, for the backward to read again; nothing where it made none
@@ -44,8 +53,10 @@ Matrix result(int64_t rows, int64_t cols, const torch::Tensor& like, at::ScalarT
 Matrix result(int64_t rows, int64_t cols, const torch::Tensor& like) { return result(rows, cols, like, like.scalar_type()); }
 // a result as the caller gets it
 torch::Tensor handed(const Matrix& m, at::IntArrayRef sizes) {
-  const torch::Tensor t = m.t.is_contiguous() ? m.t : m.t.contiguous();
-  return t.sizes() == sizes ? t : t.view(sizes);
+  if (m.t.is_contiguous()) return m.t.sizes() == sizes ? m.t : m.t.view(sizes);
+  const torch::Tensor t = fresh(sizes, m.t.scalar_type(), m.t);
+  copy_rows(m.t, m.ld, t, m.t.size(1));
+  return t;
 }
 
 // What a gated product keeps (attn_products_t): of half types z and u in rows of whole sectors, and a plane of bytes

@@ -332,6 +332,9 @@ typedef struct attn_elements {
 size_t attn_b200_elements_scratch_bytes(const attn_elements_t* e);
 int attn_b200_elements(const attn_elements_t* e, void* scratch, void* stream);
 
+/* Rows of cols elements, lds apart, into rows ldd apart: what products of half types need of widths that are no multiple of 8. */
+int attn_b200_copy_rows(const void* src, int64_t lds, void* dst, int64_t ldd, int32_t rows, int32_t cols, int32_t dtype, void* stream);
+
 /* ---- Layer norm ---------------------------------------------------------------------------------------
  * y = (x - mean) / sqrt(variance + eps) w + b over rows of d, d up to 32768; x: [n, d], rows ldx apart (and the gradient's ldg, a tangent's
  * ldu), results dense; w, b: [d], of the type of x or (param_float) float32, either null for none.  Arithmetic in fp32, rounded once. */

@@ -131,6 +131,9 @@ def test_refused_elements_and_norms(capi):
     elements("aligned", input=4097)
     elements("kept_low", pass_=2)
     assert L.attn_b200_elements(None, None, None) == -1
+    for args, code in (((4096, 8, 4096, 16, 4, 9, 1), -1), ((4096, 16, 4096, 8, 4, 9, 1), -1), ((None, 16, 4096, 16, 4, 9, 1), -1), ((4097, 16, 4096, 16, 4, 9, 1), -1),
+                       ((4096, 16, 4096, 16, -1, 9, 1), -1), ((4096, 16, 4096, 16, 4, 9, 7), -2)):
+        assert L.attn_b200_copy_rows(*args, None) == code
 
     def shape(**over):
         d = dict(n=8, d=64, dtype=capi.ATTN_BF16, param_float=0, eps=1e-5, ld=64)
