@@ -131,11 +131,14 @@ __device__ __forceinline__ void activate2(float2 z, float2& a, float2& d) {
 // What a gated product keeps of a half-precision call, 20 bits a value: 16 in a plane of the type's size, and 4 of either value in a plane of bytes.  A
 // product of two values that were rounded to the type, rounded again, would have gradients 3.0e-3 (bf16) from 64 bits in the 2-norm, where rounding the
 // gradients' own factors and results makes 2.4e-3; 4 more bits cost 1 byte beside 4.  bf16: sign, 8 bits of exponent, 11 of mantissa; f16, cut to its
-// range: 5 and 14.  They are cut off, and read as the middle of what they stand for.
+// range: 5 and 14.  Codes are the nearest ones and are read as they stand, so that 0 stays 0: what gradients have as a factor vanishes with it.
 template <typename T> struct Kept;
 template <> struct Kept<__nv_bfloat16> {
-  static __device__ __forceinline__ uint32_t code(float v) { return __float_as_uint(v); }      // in the upper 20 bits
-  static __device__ __forceinline__ float value(uint32_t code) { return __uint_as_float(code); }
+  static __device__ __forceinline__ uint32_t code(float v) {      // in the upper 20 bits
+    const uint32_t b = __float_as_uint(v);
+    return (b & 0x80000000u) | min((b & 0x7fffffffu) + 0x800u, 0x7fc00000u);      // NaN would carry into the sign
+  }
+  static __device__ __forceinline__ float value(uint32_t code) { return __uint_as_float(code & 0xfffff000u); }
 };
 template <> struct Kept<__half> {
   // the exponent moved to where 5 bits hold it: what is below goes to denormals, as in f16
@@ -144,10 +147,10 @@ template <> struct Kept<__half> {
     asm("min.NaN.f32 %0, %0, %1;" : "+f"(x) : "f"(65504.f * 0x1p-112f));
     asm("max.NaN.f32 %0, %0, %1;" : "+f"(x) : "f"(-65504.f * 0x1p-112f));
     const uint32_t b = __float_as_uint(x);
-    return (b & 0x80000000u) | (b << 3 & 0x7fffffffu);      // NaN beyond the largest exponent of a number
+    return (b & 0x80000000u) | min((b & 0x7fffffffu) + 0x100u, 0x0fffffffu) << 3;      // NaN beyond the largest exponent of a number
   }
   static __device__ __forceinline__ float value(uint32_t code) {
-    const float v = __uint_as_float((code & 0x80000000u) | (code & 0x7fffffffu) >> 3) * 0x1p112f;
+    const float v = __uint_as_float((code & 0x80000000u) | (code & 0x7ffff000u) >> 3) * 0x1p112f;
     return fabsf(v) >= 65536.f ? NAN : v;
   }
 };
@@ -159,11 +162,11 @@ __device__ __forceinline__ uint32_t kept_nibbles(const uint32_t (&c)[4]) {      
 __device__ __forceinline__ uint32_t kept_low(const uint32_t (&z)[4], const uint32_t (&u)[4]) {
   return (kept_nibbles(z) >> 4 & 0x0f0f0f0fu) | (kept_nibbles(u) & 0xf0f0f0f0u);
 }
-// the codes of value E of four from the halves' pair that holds it and the nibbles' word, 0xf0 or 0x0f of `low` in its place with the middle bit
-__device__ __forceinline__ uint32_t kept_z(uint32_t low) { return (low << 4 & 0xf0f0f0f0u) | 0x08080808u; }
-__device__ __forceinline__ uint32_t kept_u(uint32_t low) { return (low & 0xf0f0f0f0u) | 0x08080808u; }
+// the codes of value E of four from the halves' pair that holds it and the nibbles' word, 0xf0 or 0x0f of `low` in its place
+__device__ __forceinline__ uint32_t kept_z(uint32_t low) { return low << 4 & 0xf0f0f0f0u; }
+__device__ __forceinline__ uint32_t kept_u(uint32_t low) { return low & 0xf0f0f0f0u; }
 template <int E> __device__ __forceinline__ uint32_t kept_code(uint32_t high, uint32_t nibbles) {
-  constexpr uint32_t kHalf = (E & 1) ? 0x3200u : 0x1000u;      // the half's two bytes on top, the nibble's byte below; what is below that counts 2^-16
+  constexpr uint32_t kHalf = (E & 1) ? 0x3200u : 0x1000u;      // the half's two bytes on top, the nibble's byte below; what is below that is not read
   return __byte_perm(high, nibbles, kHalf | (4u + E) << 4 | (4u + E));
 }
 
