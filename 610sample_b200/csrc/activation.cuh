@@ -130,8 +130,9 @@ __device__ __forceinline__ void activate2(float2 z, float2& a, float2& d) {
 
 // What a gated product keeps of a half-precision call, 20 bits a value: 16 in a plane of the type's size, and 4 of either value in a plane of bytes.  A
 // product of two values that were rounded to the type, rounded again, would have gradients 3.0e-3 (bf16) from 64 bits in the 2-norm, where rounding the
-// gradients' own factors and results makes 2.4e-3; 4 more bits cost 1 byte beside 4.  bf16: sign, 8 bits of exponent, 11 of mantissa; f16, cut to its
-// range: 5 and 14.  Codes are the nearest ones and are read as they stand, so that 0 stays 0: what gradients have as a factor vanishes with it.
+// gradients' own factors and results makes 2.4e-3; 4 more bits cost 1 byte beside 4.  bf16: sign, 8 bits of exponent, 11 of mantissa; f16: 6 and
+// 13, since a(z) u may be in its range where z or u is not.  Codes are the nearest ones and are read as they stand, so that 0 stays 0: what gradients have
+// as a factor vanishes with it.
 template <typename T> struct Kept;
 template <> struct Kept<__nv_bfloat16> {
   static __device__ __forceinline__ uint32_t code(float v) {      // in the upper 20 bits
@@ -141,17 +142,14 @@ template <> struct Kept<__nv_bfloat16> {
   static __device__ __forceinline__ float value(uint32_t code) { return __uint_as_float(code & 0xfffff000u); }
 };
 template <> struct Kept<__half> {
-  // the exponent moved to where 5 bits hold it: what is below goes to denormals, as in f16
+  // the exponent moved to where 6 bits hold it: normal numbers from 2^-15, below them 2^-28 apart; from 2^46 on NaN
   static __device__ __forceinline__ uint32_t code(float v) {
-    float x = v * 0x1p-112f;
-    asm("min.NaN.f32 %0, %0, %1;" : "+f"(x) : "f"(65504.f * 0x1p-112f));
-    asm("max.NaN.f32 %0, %0, %1;" : "+f"(x) : "f"(-65504.f * 0x1p-112f));
-    const uint32_t b = __float_as_uint(x);
-    return (b & 0x80000000u) | min((b & 0x7fffffffu) + 0x100u, 0x0fffffffu) << 3;      // NaN beyond the largest exponent of a number
+    const uint32_t b = __float_as_uint(v * 0x1p-111f);
+    return (b & 0x80000000u) | min((b & 0x7fffffffu) + 0x200u, 0x1f800000u) << 2;
   }
   static __device__ __forceinline__ float value(uint32_t code) {
-    const float v = __uint_as_float((code & 0x80000000u) | (code & 0x7ffff000u) >> 3) * 0x1p112f;
-    return fabsf(v) >= 65536.f ? NAN : v;
+    const float v = __uint_as_float((code & 0x80000000u) | (code & 0x7ffff000u) >> 2) * 0x1p111f;
+    return fabsf(v) >= 0x1p46f ? NAN : v;      // the codes that are f16's NaN and infinities
   }
 };
 // The planes' words of four values of either: the upper halves in pairs, and a word of bytes, bits of z low and of u high

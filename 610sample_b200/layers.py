@@ -49,5 +49,5 @@ def gated_feed_forward(x, w_gate, w_up, w_down, activation="silu", residual=None
 
     Both projections, the activation and the product are one kernel, the second projection with the residual another.  The inner
     values are rounded to the type of x before the second projection; the backward keeps them and both projections, of half types
-with four bits more than 16 each (in fp16 projections beyond 65504 are kept as that)."""
+with four bits more than 16 each: fp16 with 13 bits of mantissa up to 2^46, beyond which gradients are NaN."""
     return _attention_cuda.gated_feed_forward(x, w_gate, w_up, w_down, residual, _activation(activation))

@@ -39,3 +39,104 @@ def test_zeros_stay_zeros(layers, dtype, kind, n):
     t = [v.detach().requires_grad_(True) for v in (x, wg, none, wd)]
     grad_x, = torch.autograd.grad(call(*t), t[0], g, create_graph=True)
     assert not bool(torch.autograd.grad(grad_x, t[1], torch.ones_like(x))[0].any())
+
+
+def gated_bounds(x, wg, wu, wd, g, kind, dtype):
+    """(y, gx, gg, gu, gd) in 64 bits, each with what roundings may make of it.  z and u are kept with 11 bits of mantissa (bf16) and 13 (f16), to the nearest; below
+    2^-15 f16's are 2^-28 apart."""
+    x, wg, wu, wd, g = (t.double() for t in (x, wg, wu, wd, g))
+    zero = torch.zeros_like
+    z, ez = mm(x, zero(x), wg.T, zero(wg.T), x.shape[1])
+    u, eu = mm(x, zero(x), wu.T, zero(wu.T), x.shape[1])
+    a, d1, _ = curve(z, kind)
+    own = curve_error(z, dtype)
+    own_slope = curve_error(z, dtype) - 4 * F32 * z.abs() + 4 * F32
+    change = torch.where(z.abs() > 60, 0.0, 1.25)      # |a''| <= 1.25, and far out the slope does not change
+    h = a * u
+    eh = rounded(h, (ez * 1.2 + own) * (u.abs() + eu) + a.abs() * eu + 4 * F32 * h.abs(), dtype)
+    y, ey = mm(h, eh, wd.T, zero(wd.T), wd.shape[1])
+    step, tiny = {torch.bfloat16: (2.0 ** -12, 0.0), torch.float16: (2.0 ** -14, 2.0 ** -29), torch.float32: (0.0, 0.0)}[dtype]
+    kz, ku = ez + step * (z.abs() + ez) + tiny, eu + step * (u.abs() + eu) + tiny
+    ea, ed = kz * 1.2 + own, kz * change + own_slope
+    gh, egh = mm(g, zero(g), wd, zero(wd), wd.shape[0])
+    dz, du = gh * d1 * u, gh * a
+    edz = rounded(dz, egh * (d1 * u).abs() + (gh.abs() + egh) * (ed * (u.abs() + ku) + d1.abs() * ku) + 6 * F32 * dz.abs(), dtype)
+    edu = rounded(du, egh * a.abs() + (gh.abs() + egh) * ea + 4 * F32 * du.abs(), dtype)
+    x1, e1 = mm(dz, edz, wg, zero(wg), 2 * wg.shape[0])
+    x2, e2 = mm(du, edu, wu, zero(wu), 2 * wg.shape[0])
+    results = [(y, ey), (x1 + x2, e1 + e2), mm(dz.T, edz.T, x, zero(x), x.shape[0]), mm(du.T, edu.T, x, zero(x), x.shape[0]), mm(g.T, zero(g.T), h, eh, x.shape[0])]
+    return [(v, rounded(v, e, dtype)) for v, e in results]
+
+
+def far_inputs(n, dtype, d=24, f=48, seed=0):
+    """A block whose rows' first element, about 4, goes into u alone for half of the inner columns (u about 1e5 or -1e5 beside z about -2), and into z alone
+    for the others (z about 1e5 or -1e5 beside a small u), so that h stays below 65504"""
+    x, wg, wu, wd, g = inputs([((n, d), 0.4), ((f, d), 0.05), ((f, d), 0.03), ((d, f), 2.0 ** -7), ((n, d), 2.0 ** -5)], dtype, seed)
+    v = torch.Generator().manual_seed(seed + 1)
+    x[:, 0] = (3.8 + 0.4 * torch.rand(n, generator=v)).to(dtype).cuda()
+    x[:, 1] = 1
+    far = torch.where(torch.rand(f, generator=v) < 0.5, -25000.0, 25000.0).to(dtype).cuda()
+    half = f // 2
+    wu[:half, 0], wg[:half, 0], wg[:half, 1] = far[:half], 0, -2
+    wg[half:, 0], wu[half:, 0] = far[half:], 0
+    return x, wg, wu, wd, g
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("kind", CURVES)
+@pytest.mark.parametrize("n", [5, 20, 150])
+def test_projections_beyond_65504(layers, dtype, kind, n):
+    x, wg, wu, wd, g = far_inputs(n, dtype)
+    call = lambda *t: layers.gated_feed_forward(*t, kind)
+    want = gated_bounds(x, wg, wu, wd, g, kind, dtype)
+    z, u = x.double() @ wg.double().T, x.double() @ wu.double().T
+    assert float(z.abs().max()) > 7e4 and float(u.abs().max()) > 7e4 and float((curve(z, kind)[0] * u).abs().max()) < 65504
+    for name, a, (v, e) in zip(("y", "gx", "gg", "gu", "gd"), passes(call, [x, wg, wu, wd], g), want):
+        near(a, v, e, name)
+    # second derivatives: the halves of the weights' gradients by themselves, which have different sizes
+    tangents = inputs([((n, 24), 0.4), ((48, 24), 0.03), ((48, 24), 0.03), ((24, 48), 2.0 ** -7)], dtype, 3)
+    define = lambda x, a, b, c: (define_act(x @ a.T, kind) * (x @ b.T)) @ c.T
+    got, ref = second(call, [x, wg, wu, wd], g, tangents, define)
+    for a, b in zip(got, ref):
+        for p, q in ((a[:24], b[:24]), (a[24:], b[24:])) if b.shape[0] == 48 else ((a, b),):
+            close([p], [q], dtype)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("n", [5, 150])
+def test_projections_beyond_what_is_kept(layers, n):
+    # f16, u = 20000 x 60000^2 > 2^46 beside z = -40: h = -0.012, and gradients that say that they are lost
+    x, wu = (torch.full(s, 60000.0, device="cuda", dtype=torch.float16) for s in ((n, 20000), (8, 20000)))
+    wg = torch.zeros_like(wu)
+    wg[:, 0] = -40 / 60000
+    wd, g = torch.eye(8, device="cuda", dtype=torch.float16), torch.ones(n, 8, device="cuda", dtype=torch.float16)
+    y, _, gg, _, _ = passes(lambda *t: layers.gated_feed_forward(*t), [x, wg, wu, wd], g)
+    z = -60000.0 * -float(wg[0, 0])
+    want = z / (1 + math.exp(-z)) * 20000 * 60000.0 ** 2
+    assert bool(((y.double() - want).abs() <= 1e-3 * abs(want)).all()) and bool(gg.isnan().all())
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", HALF)
+@pytest.mark.parametrize("kind", CURVES)
+@pytest.mark.parametrize("n", [401, 21])
+def test_far_arguments_and_slopes(layers, dtype, kind, n):
+    # one input times one weight: z over a wide range, u = 2^-15 z, results and all gradients
+    top = 32000 if dtype == torch.float16 else 1e15
+    z = torch.logspace(-4, math.log10(top), n // 2)
+    x = torch.cat([-z, torch.zeros(1), z]).to(dtype).cuda()[:, None]
+    w, v = torch.ones(8, 1, device="cuda", dtype=dtype), torch.full((8, 1), 2.0 ** -15, device="cuda", dtype=dtype)
+    eye, g = torch.eye(8, device="cuda", dtype=dtype), torch.full((n, 8), 2.0 ** -3, device="cuda", dtype=dtype)
+    want = gated_bounds(x, w, v, eye, g, kind, dtype)
+    got = passes(lambda *t: layers.gated_feed_forward(*t, kind), [x, w, v, eye], g)
+    for name, a, (t, e) in zip(("y", "gx", "gg", "gu", "gd"), got, want):
+        if name in ("y", "gx") or dtype == torch.bfloat16:      # sums of squares leave the range of f16
+            near(a, t, e, name)
+    # a linear layer: eight equal terms make the slope, which is 0 or 1 far out
+    gx = passes(lambda x, w: layers.linear(x, w, activation=kind), [x, w], g)[1]
+    zz = x.double()
+    slope = torch.where(zz.abs() > 60, (zz > 0).double(), curve(zz, kind)[1])
+    kept = rounded(zz.clamp(-60, 60), 0 * zz, torch.float16)
+    error = torch.where(zz.abs() > 60, 0.0, curve_error(zz, dtype) + 1.25 * kept)
+    near(gx, slope, rounded(slope, rounded(slope, error + 12 * F32, dtype), dtype), "slope")
