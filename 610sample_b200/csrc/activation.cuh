@@ -87,8 +87,13 @@ __device__ __forceinline__ void activate(float z, float& a, float& d1, float& d2
 }
 
 // The fast form of two elements at a time, in packed arithmetic: the products' epilogues compute it for every element of a tile, in the time that the
-// tensor cores take for the next one.  a(z), for any z; with GRAD its derivative too, for finite z.
+// tensor cores take for the next one.  a(z), for any z; with GRAD its derivative too, for finite z and NaN.
 __device__ __forceinline__ float2 both(float v) { return make_float2(v, v); }
+__device__ __forceinline__ float bounded(float v, float most) {      // NaN stays
+  asm("min.NaN.f32 %0, %0, %1;" : "+f"(v) : "f"(most));
+  asm("max.NaN.f32 %0, %0, %1;" : "+f"(v) : "f"(-most));
+  return v;
+}
 template <int ACT, bool GRAD>
 __device__ __forceinline__ void activate2(float2 z, float2& a, float2& d) {
   if constexpr (ACT == ACT_NONE) {
@@ -114,7 +119,7 @@ __device__ __forceinline__ void activate2(float2 z, float2& a, float2& d) {
     constexpr float kRoot = 1.5957691216057308f, kCube = 0.044715f;      // sqrt(8 / pi)
     float2 c = z, u = z;
     if constexpr (ACT == ACT_GELU_TANH) {
-      if constexpr (GRAD) c = make_float2(fminf(fmaxf(z.x, -30.f), 30.f), fminf(fmaxf(z.y, -30.f), 30.f));
+      if constexpr (GRAD) c = make_float2(bounded(z.x, 30.f), bounded(z.y, 30.f));
       u = __fmul2_rn(c, __ffma2_rn(__fmul2_rn(c, c), both(kRoot * kCube), both(kRoot)));
     }
     const float2 q = __fmul2_rn(u, both(-kLog2e)), e = __fadd2_rn(make_float2(tc::ex2(q.x), tc::ex2(q.y)), both(1.f));

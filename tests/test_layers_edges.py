@@ -140,3 +140,36 @@ def test_far_arguments_and_slopes(layers, dtype, kind, n):
     kept = rounded(zz.clamp(-60, 60), 0 * zz, torch.float16)
     error = torch.where(zz.abs() > 60, 0.0, curve_error(zz, dtype) + 1.25 * kept)
     near(gx, slope, rounded(slope, rounded(slope, error + 12 * F32, dtype), dtype), "slope")
+
+
+# ---- NaN ----------------------------------------------------------------------------------------------
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("kind", CURVES)
+@pytest.mark.parametrize("n", [5, 20, 150])
+def test_nan_in_a_weight_reaches_its_gradients(layers, dtype, kind, n):
+    # a row of a weight: the inner column that it makes is NaN, with its gradients, and the other columns' gradients are as they were
+    x, wg, wu, wd, r, g = gated_inputs(n, 64, 96, 64, dtype)
+    w, b, gf = inputs([((96, 64), 0.2), ((96,), 0.3), ((n, 96), 1.0)], dtype, 4)
+    others = torch.arange(96, device="cuda") != 40
+    spoil = lambda t: torch.where(others[:, None], t, torch.full_like(t, float("nan")))
+
+    def look(grad, clean, lost):
+        assert torch.equal(grad[others], clean[others])
+        assert bool(grad[40].isnan().all()) if lost else torch.equal(grad[40], clean[40])
+
+    call = lambda x, w, b: layers.linear(x, w, b, kind)
+    clean, soiled = passes(call, [x, w, b], gf), passes(call, [x, spoil(w), b], gf)
+    look(soiled[0].T, clean[0].T, True)
+    assert bool(soiled[1].isnan().all())
+    look(soiled[2], clean[2], True)
+    look(soiled[3], clean[3], True)
+    call = lambda *t: layers.gated_feed_forward(*t, kind)
+    clean = passes(call, [x, wg, wu, wd], g)
+    for weights, gate_lost, up_lost in (([spoil(wg), wu], True, True), ([wg, spoil(wu)], True, False)):
+        soiled = passes(call, [x, *weights, wd], g)
+        assert bool(soiled[0].isnan().all()) and bool(soiled[1].isnan().all())
+        look(soiled[2], clean[2], gate_lost)
+        look(soiled[3], clean[3], up_lost)
+        look(soiled[4].T, clean[4].T, True)
