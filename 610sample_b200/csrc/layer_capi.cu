@@ -293,7 +293,7 @@ int attn_b200_layer_norm_backward(const attn_norm_shape_t* s, const void* x, con
                                   void* dx, void* dw, void* db, void* scratch, void* stream) {
   const int rc = check_norm_backward(s, x, g, mean, rstd, dw != nullptr || db != nullptr, scratch);
   if (rc != ATTN_OK) return rc;
-  if (dx == nullptr && dw == nullptr && db == nullptr) return fail(ATTN_EINVAL, "no gradient is asked for");
+  if (s->n > 0 && dx == nullptr && dw == nullptr && db == nullptr) return fail(ATTN_EINVAL, "no gradient is asked for");
   NormArgs a = norm_args(s, x, w);
   a.g = g;
   a.gx = dx;
@@ -306,7 +306,7 @@ int attn_b200_layer_norm_second_backward(const attn_norm_shape_t* s, const void*
   int rc = check_norm_backward(s, x, g, mean, rstd, gw != nullptr, scratch);
   if (rc == ATTN_OK && u != nullptr && s->n > 0) rc = check_rows("u", u, s->ldu, s->d, s->dtype);
   if (rc != ATTN_OK) return rc;
-  if (gg == nullptr && gx == nullptr && gw == nullptr) return fail(ATTN_EINVAL, "no gradient is asked for");
+  if (s->n > 0 && gg == nullptr && gx == nullptr && gw == nullptr) return fail(ATTN_EINVAL, "no gradient is asked for");
   NormArgs a = norm_args(s, x, w);
   a.g = g;
   a.u = u; a.uw = uw; a.ub = ub;

@@ -15,6 +15,19 @@ from test_layers import (ACTIVATIONS, F32, HALF, PKG_DIR, SECOND, TYPES, capi, c
 CURVES = [a for a in ACTIVATIONS if a is not None]
 
 
+# ---- no rows ---------------------------------------------------------------------------------------------
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", TYPES)
+def test_norm_of_no_rows_without_parameters(layers, dtype):
+    # gradients without elements have no address; both orders
+    x, g = (torch.zeros(2, 0, 16, device="cuda", dtype=dtype, requires_grad=True) for _ in range(2))
+    first, = torch.autograd.grad(layers.layer_norm(x), x, g, create_graph=True)
+    assert first.shape == x.shape
+    for t in torch.autograd.grad(first, [x, g], torch.zeros_like(x)):
+        assert t.shape == x.shape
+
+
 # ---- gated blocks: zeros, and projections beyond 65504 -----------------------------------------------------
 
 @pytest.mark.gpu
