@@ -51,9 +51,13 @@ Matrix result(int64_t rows, int64_t cols, const torch::Tensor& like, at::ScalarT
   return {padded(rows, cols, like, type), type == at::kFloat ? cols : (cols + 7) / 8 * 8};
 }
 Matrix result(int64_t rows, int64_t cols, const torch::Tensor& like) { return result(rows, cols, like, like.scalar_type()); }
-// a result as the caller gets it
+// A result as the caller gets it: of its own, not a view that autograd knows of, which could not be changed in place behind a custom function
 torch::Tensor handed(const Matrix& m, at::IntArrayRef sizes) {
-  if (m.t.is_contiguous()) return m.t.sizes() == sizes ? m.t : m.t.view(sizes);
+  if (m.t.is_contiguous()) {
+    if (m.t.sizes() == sizes && !m.t.is_view()) return m.t;
+    at::AutoDispatchBelowADInplaceOrView untracked;
+    return m.t.view(sizes);
+  }
   const torch::Tensor t = fresh(sizes, m.t.scalar_type(), m.t);
   copy_rows(m.t, m.ld, t, m.t.size(1));
   return t;

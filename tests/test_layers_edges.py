@@ -28,6 +28,37 @@ def test_norm_of_no_rows_without_parameters(layers, dtype):
         assert t.shape == x.shape
 
 
+# ---- results belong to the caller -----------------------------------------------------------------------
+
+def calls(layers, dtype, lead, k, m):
+    """(operator, leaves, cotangent) of rows with these leading axes"""
+    n = math.prod(lead)
+    x, w, b, r, g = inputs([((n, k), 1.0), ((m, k), 0.2), ((m,), 0.5), ((n, m), 1.0), ((n, m), 1.0)], dtype)
+    wg, wu, wd = inputs([((m, k), 0.2), ((m, k), 0.2), ((k, m), 0.2)], dtype, 1)
+    at = lambda t: t.reshape(*lead, t.shape[-1])
+    x, r, g, gx = at(x), at(r), at(g), at(inputs([((n, k), 1.0)], dtype, 2)[0])
+    return [(lambda x, w: layers.linear(x, w), [x, w], g), (lambda x, w, b, r: layers.linear(x, w, b, "gelu", r), [x, w, b, r], g),
+            (lambda x, a, b, c: layers.gated_feed_forward(x, a, b, c), [x, wg, wu, wd], gx), (lambda x: layers.layer_norm(x), [x], gx)]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("lead", [(), (1,), (5,), (2, 3), (1, 1), (4, 50), (0,), (2, 0)])
+@pytest.mark.parametrize("k, m", [(16, 24), (24, 21), (13, 16)])
+def test_results_may_be_changed_in_place(layers, dtype, lead, k, m):
+    # as those of PyTorch's own operators: y, then 2 (y + 1), whose gradients are those of twice the cotangent
+    for call, leaves, g in calls(layers, dtype, lead, k, m):
+        want = passes(call, leaves, 2 * g)
+        t = [v.detach().requires_grad_(True) for v in leaves]
+        y = call(*t)
+        assert torch.equal(y, want[0]) and not y._is_view()
+        y += 1
+        y.mul_(2)
+        assert torch.equal(y, (want[0] + 1) * 2)
+        for a, b in zip(torch.autograd.grad(y, t, g), want[1:]):
+            assert torch.equal(a, b)
+
+
 # ---- gated blocks: zeros, and projections beyond 65504 -----------------------------------------------------
 
 @pytest.mark.gpu
