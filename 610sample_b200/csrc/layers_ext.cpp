@@ -264,7 +264,8 @@ variable_list linear_second(const torch::Tensor& u_in, const torch::Tensor& uw_i
     t = result(n, m, x_in);
     Products(x_in, ATTN_FORM_NT).add(t, n, m, k, {{&u, &w}, {&x, &uw}}).bias(ub).run("linear second backward");
   } else {
-    t = matrix(ub.unsqueeze(0).expand({n, m}));
+    t = result(n, m, x_in);      // in memory of its own: without an activation it is a gradient
+    t.t.copy_(ub.unsqueeze(0).expand({n, m}));
   }
   variable_list out(4);      // g, x, w, b
   Matrix dz = g, s;

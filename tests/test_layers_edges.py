@@ -59,6 +59,18 @@ def test_results_may_be_changed_in_place(layers, dtype, lead, k, m):
             assert torch.equal(a, b)
 
 
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", TYPES)
+def test_gradients_are_not_their_cotangents(layers, dtype):
+    # one row: the bias' cotangent is a gradient of the row's, in memory of its own
+    x, w, b, g = inputs([((1, 16), 1.0), ((24, 16), 0.2), ((24,), 0.5), ((1, 24), 1.0)], dtype)
+    t = [v.detach().requires_grad_(True) for v in (x, w, b, g)]
+    grad_b = torch.autograd.grad(layers.linear(*t[:3]), t[2], t[3], create_graph=True)[0]
+    u, = inputs([((24,), 1.0)], dtype, 1)
+    got, = torch.autograd.grad(grad_b, t[3], u)
+    assert torch.equal(got[0], u) and got.data_ptr() != u.data_ptr()
+
+
 # ---- gated blocks: zeros, and projections beyond 65504 -----------------------------------------------------
 
 @pytest.mark.gpu
