@@ -291,6 +291,7 @@ cudaError_t launch_copy_rows(const void* src, long long lds, void* dst, long lon
 // Runs of rows: six CTAs an SM, 64 rows each at least
 int element_chunks(int n, int m) {
   const long long tiles = ((long long)m + kElemCols - 1) / kElemCols;
+  if (tiles == 0) return 1;
   long long chunks = (6 * kSms + tiles - 1) / tiles;
   if (chunks > (n + 63) / 64) chunks = (n + 63) / 64;
   return chunks < 1 ? 1 : (int)chunks;

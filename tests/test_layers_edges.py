@@ -15,6 +15,31 @@ from test_layers import (ACTIVATIONS, F32, HALF, PKG_DIR, SECOND, TYPES, capi, c
 CURVES = [a for a in ACTIVATIONS if a is not None]
 
 
+# ---- CPU ------------------------------------------------------------------------------------------
+
+def test_scratch_of_calls_without_rows_or_columns(capi):
+    L = capi.lib()
+    for dtype in (capi.ATTN_F16, capi.ATTN_BF16, capi.ATTN_F32):
+        for n, m in ((0, 0), (0, 16), (16, 0)):
+            for pass_ in range(3):
+                e = capi.Elements()
+                e.n, e.m, e.dtype, e.activation, e.pass_ = n, m, dtype, 1, pass_
+                least = L.attn_b200_elements_scratch_bytes(ctypes.byref(e))
+                assert least == (4 * m if n == 0 else 0)
+            for form in range(3):
+                for rows, cols, k in ((n, m, 64), (n, m, 0), (64, n, m), (n, 64, m)):
+                    if k == 0 and rows and cols:
+                        continue
+                    c = capi.Products()
+                    c.dtype, c.form, c.count = dtype, form, 1
+                    p = c.product[0]
+                    p.rows, p.cols, p.k, p.pairs = rows, cols, k, 1
+                    if rows == 0 or cols == 0:
+                        assert L.attn_b200_products_scratch_bytes(ctypes.byref(c)) == 0
+        s = capi.NormShape(0, 64, dtype, 0, 1e-5, 0, 64, 64, 64)
+        assert L.attn_b200_layer_norm_backward_scratch_bytes(ctypes.byref(s)) == 0
+
+
 # ---- no rows ---------------------------------------------------------------------------------------------
 
 @pytest.mark.gpu
