@@ -254,3 +254,144 @@ def test_nan_in_a_weight_reaches_its_gradients(layers, dtype, kind, n):
         look(soiled[2], clean[2], gate_lost)
         look(soiled[3], clean[3], up_lost)
         look(soiled[4].T, clean[4].T, True)
+
+
+# ---- second derivatives as they are called ---------------------------------------------------------------
+
+def second_steps(layers, dtype, n=150, d=72, f=104, seed=0):
+    """(tensors, a function that gives all second derivatives of the three operators)"""
+    x, wg, wu, wd, r, g = gated_inputs(n, d, f, d, dtype, seed)
+    w, b, gf = inputs([((f, d), 0.2), ((f,), 0.3), ((n, f), 1.0)], dtype, seed + 40)
+    nw, nb = inputs([((d,), 0.3), ((d,), 0.3)], dtype, seed + 41)
+    u = gated_inputs(n, d, f, d, dtype, seed + 42)
+    uw, ub, uf = inputs([((f, d), 0.2), ((f,), 0.3), ((d,), 0.3)], dtype, seed + 43)
+    tensors = [x, wg, wu, wd, g, w, b, gf, nw, nb, *u[:4], uw, ub, uf]
+
+    def step(x, wg, wu, wd, g, w, b, gf, nw, nb, ux, ug, uu, ud, uw, ub, uf):
+        out = []
+        for call, leaves, up, along in ((lambda *t: layers.gated_feed_forward(*t), [x, wg, wu, wd], g, [ux, ug, uu, ud]),
+                                        (lambda *t: layers.linear(*t, "gelu"), [x, w, b], gf, [ux, uw, ub]), (lambda *t: layers.linear(*t), [x, w, b], gf, [ux, uw, ub]),
+                                        (lambda *t: layers.layer_norm(*t), [x, nw, nb], g, [ux, uf, uf])):
+            t = [v.detach().requires_grad_(True) for v in leaves + [up]]
+            first = torch.autograd.grad(call(*t[:-1]), t[:-1], t[-1], create_graph=True)
+            out += [v for v in torch.autograd.grad(first, t, along, allow_unused=True) if v is not None]
+        return out
+
+    return tensors, step
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("n", [3, 150])
+def test_captured_second_derivatives(layers, dtype, n):
+    tensors, step = second_steps(layers, dtype, n)
+    step(*tensors)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = step(*tensors)
+    for seed in (1, 2):
+        for t, s in zip(tensors, second_steps(layers, dtype, n, seed=seed)[0]):
+            t.copy_(s)
+        graph.replay()
+        torch.cuda.synchronize()
+        for a, b in zip(out, step(*tensors)):
+            assert torch.equal(a, b)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("n", [6, 150])
+def test_second_derivatives_of_views(layers, dtype, n):
+    # cotangents and inputs that are slices of wider rows (where 16 bytes divide their starts, the norm reads them as it reads dense ones), transposed, expanded
+    tensors, step = second_steps(layers, dtype, n)
+    plain = step(*tensors)
+
+    def inside(t):
+        wide = torch.full((t.shape[0], t.shape[1] + 16), float("nan"), device="cuda", dtype=dtype)
+        wide[:, 8:8 + t.shape[1]] = t
+        return wide[:, 8:8 + t.shape[1]]
+
+    for view in (inside, lambda t: t.T.contiguous().T):
+        for a, b in zip(step(*[view(t) if t.dim() == 2 else t for t in tensors]), plain):
+            assert torch.equal(a, b)
+    spread = lambda t: t[:1].expand(t.shape) if t.dim() == 2 else t[:1].expand(t.shape)
+    along = range(10, len(tensors))
+    for a, b in zip(step(*[spread(t) if i in along else t for i, t in enumerate(tensors)]), step(*[spread(t).contiguous() if i in along else t for i, t in enumerate(tensors)])):
+        assert torch.equal(a, b)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", HALF)
+def test_second_derivatives_of_many_tiles(layers, dtype):
+    # several rounds of tiles, and sums over the rows that are shared out
+    n, k, m = 2500, 520, 2600
+    leaves = inputs([((n, k), 1.0), ((m, k), 1.5 / math.sqrt(k)), ((m,), 0.5)], dtype)
+    g, = inputs([((n, m), 1.0)], dtype, 5)
+    tangents = inputs([((n, k), 1.0), ((m, k), 1 / math.sqrt(k)), ((m,), 1.0)], dtype, 6)
+    close(*second(lambda x, w, b: layers.linear(x, w, b, "silu"), leaves, g, tangents, lambda x, w, b: define_act(x @ w.T + b, "silu")), dtype)
+    x, wg, wu, wd, r, g = gated_inputs(n, k, 1304, k, dtype)
+    tangents = gated_inputs(n, k, 1304, k, dtype, 9)[:4]
+    close(*second(lambda *t: layers.gated_feed_forward(*t, "gelu"), [x, wg, wu, wd], g, tangents, lambda x, a, b, c: (define_act(x @ a.T, "gelu") * (x @ b.T)) @ c.T), dtype)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("d, f", [(64, 96), (61, 99)])
+def test_saved_tensors_that_move(layers, dtype, d, f):
+    # what is kept goes to the host and comes back, with other strides
+    x, wg, wu, wd, r, g = gated_inputs(150, d, f, d, dtype)
+    w, gf = inputs([((f, d), 0.2), ((150, f), 1.0)], dtype, 4)
+    for call, leaves, up in ((lambda *t: layers.gated_feed_forward(*t), [x, wg, wu, wd], g), (lambda *t: layers.linear(*t, None, "gelu"), [x, w], gf),
+                             (lambda t: layers.layer_norm(t), [x], g)):
+        want = passes(call, leaves, up)
+        with torch.autograd.graph.save_on_cpu():
+            got = passes(call, leaves, up)
+        for a, b in zip(got, want):
+            assert torch.equal(a, b)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("k, m", [(64, 96), (61, 99)])
+def test_inputs_changed_before_the_backward_are_noticed(layers, dtype, k, m):
+    for call, leaves, up in calls(layers, dtype, (9,), k, m):
+        for i in range(min(2, len(leaves))):
+            t = [v.detach().clone().requires_grad_(True) for v in leaves]
+            y = call(*t)
+            with torch.no_grad():
+                t[i].mul_(2)
+            with pytest.raises(RuntimeError, match="inplace"):
+                torch.autograd.grad(y, t, up)
+
+
+# ---- the benchmark's step ----------------------------------------------------------------------------------
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("mlp", ["gelu", "gated"])
+def test_meta_step_by_relative_size(layers, mlp):
+    # every parameter's gradient in the 2-norm.  float32: sums of up to 256 products are off by 256 f of their sizes at most, in about 60 products one behind the other: 1e-3.
+    # bf16: the operators round less often than PyTorch's chain of separate operations, so they are no further from float32 than twice what that chain is
+    root = os.path.dirname(PKG_DIR)
+    if root not in sys.path:
+        sys.path.insert(0, root)
+    bt = importlib.import_module("bench_ttt")
+    attention = importlib.import_module("attention").flash_attention_v7
+    cfg = dict(bt.SMALL, mlp=mlp)
+    dev = torch.device("cuda")
+
+    def gradients(kind, dtype):
+        slow, fast = bt.init_params(cfg, dev, torch.bfloat16, seed=1)
+        slow, fast = ({n: p.detach().to(dtype).requires_grad_(True) for n, p in group.items()} for group in (slow, fast))
+        ids, targets = bt.make_batch(cfg, dev, seed=2)
+        bt.ttt_step(cfg, slow, fast, ids, targets, lambda q, k, v: attention(q, k, v, cfg["seq"], 0), None, bt.layer_functions(kind)).backward()
+        return {n: p.grad.double() for n, p in {**slow, **fast}.items()}
+
+    want = gradients("torch", torch.float32)
+    away = lambda got: {n: float((got[n] - want[n]).norm() / want[n].norm()) for n in want}
+    assert all(float(v.norm()) > 0 for v in want.values())
+    for n, e in away(gradients("fused", torch.float32)).items():
+        assert e <= 1e-3, (n, e)
+    chain = away(gradients("torch", torch.bfloat16))
+    for n, e in away(gradients("fused", torch.bfloat16)).items():
+        assert e <= 2 * chain[n], (n, e, chain[n])
