@@ -288,7 +288,7 @@ def measure(args, init_process_group=True):
             "config": {"workload": "ttt_step_12L_d768_h12_seq2048_b8" if not args.small else "ttt_step_small",
                        **{k: cfg[k] for k in ("layers", "d_model", "heads", "d_ff", "vocab", "seq", "batch")},
                        "inner_lr": INNER_LR, "sample": sample, **({"loss": "linear"} if linear else {}),
-                       **({"layers": layer_kind} if layer_kind != "torch" else {}), **({"mlp": cfg["mlp"]} if cfg["mlp"] != "gelu" else {})},
+                       **({"layer_operators": layer_kind} if layer_kind != "torch" else {}), **({"mlp": cfg["mlp"]} if cfg["mlp"] != "gelu" else {})},
             "outer_loss": float(loss.detach()), "peak_memory_mb": peak_mb,
         }
         if attn_ms is not None:

@@ -2,8 +2,10 @@
 NaN in weights, second derivatives that are captured, of many tiles and of views, the benchmark's meta-step by relative size."""
 import ctypes
 import importlib
+import json
 import math
 import os
+import subprocess
 import sys
 
 import pytest
@@ -395,3 +397,14 @@ def test_meta_step_by_relative_size(layers, mlp):
     chain = away(gradients("torch", torch.bfloat16))
     for n, e in away(gradients("fused", torch.bfloat16)).items():
         assert e <= 2 * chain[n], (n, e, chain[n])
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("mlp", ["gelu", "gated"])
+def test_the_benchmark_says_what_it_ran(mlp):
+    root = os.path.dirname(PKG_DIR)
+    run = subprocess.run([sys.executable, os.path.join(root, "bench_ttt.py"), "--small", "--steps", "1", "--warmup", "1", "--layers", "fused", "--mlp", mlp],
+                         capture_output=True, text=True, timeout=300, cwd=root)
+    assert run.returncode == 0, run.stderr[-2000:]
+    config = json.loads(run.stdout.strip().splitlines()[-1])["config"]
+    assert config["layers"] == 2 and config["layer_operators"] == "fused" and config.get("mlp", "gelu") == mlp
