@@ -5,8 +5,9 @@
 // the weight and of one row of `a` straight into the fragments of two m16n8k16 products, whose order of k does not matter as long as both operands have
 // the same.  Four blocks of a warp are on their way at once.  The warps' sums meet in shared memory, in order.
 //
-// One row, bf16, in a graph of many calls on weights from HBM: 768 -> 2304 2.6 us, 2048 -> 5504 6.7, 5504 -> 2048 7.3 (9.7 with eight warps), 4096 -> 14336 26.5 (4.4 TB/s; the copy
-// rate takes 17.9): latency of loads.  Eight blocks on their way were 7.7 at 2048 -> 5504, with fewer CTAs an SM.
+// One row, bf16, in a graph of many calls on weights from HBM: 768 -> 2304 2.6 us, 2048 -> 5504 6.6, 5504 -> 2048 7.2 (9.7 with eight warps), 4096 -> 14336 25.6 (4.6 TB/s; the copy
+// rate takes 17.9).  Short of it by how CTAs fill the SMs: 5504 -> 2048 is 128 CTAs for 148 SMs, a gated 2048 -> 5504 (13 us) 344 CTAs of 114 registers, two to an SM, 1.16
+// waves.  Eight blocks on their way were 7.7 at 2048 -> 5504, with fewer CTAs an SM.
 #include "activation.cuh"
 #include "layer_launch.h"
 #include "tc_common.cuh"
@@ -151,12 +152,23 @@ product_few_kernel(const __grid_constant__ FewArgs g) {
   }
 }
 
-// Up to eight rows always; up to 32 against weights of up to 12 million elements.  Both forms timed, us (rows x k -> columns, bf16): 16 x 4096 -> 14336 here 34.6, in
-// tiles 30.5 (the rows are read by every CTA), 32 rows 43.6 and 30.5; 32 x 2048 -> 5504 14.8 and 15.3; 32 x 768 -> 2304 3.8 and 8.9; 32 x 5504 -> 2048 13.6 and 19.6.
+// Up to 16 rows always; up to 32 against a weight of up to 20 million elements, or two of a gated product of 12 million together.  The rows are read by every CTA,
+// so more of them cost more here, and nothing in tiles, where the number of tiles decides.  Both forms timed in graphs, us here / in tiles (k -> columns, bf16, weights from HBM):
+//                            1 row          16 rows        17 rows        32 rows
+//   plain   768 ->  2304    2.6 /  8.4     2.9 /  8.6     3.5 /  8.6     3.9 /  8.6
+//          2048 ->  5504    6.6 / 15.9    11.2 / 14.9    12.5 / 14.9    14.3 / 15.0      11.3 million
+//          4096 ->  4096   10.2 / 21.2    12.6 / 19.9    14.6 / 19.9    16.5 / 20.0      16.8
+//          4096 ->  6144   11.8 / 25.6    19.5 / 22.4    21.7 / 22.2    24.8 / 22.4      25.2
+//          4096 -> 14336   25.6 / 40.3    30.7 / 29.0    52.2 / 29.0    53.9 / 29.4      58.7
+//   gated  2048 ->  2048    5.6 / 14.5     6.8 / 14.4     8.5 / 14.3     8.8 / 14.4       8.4, both weights
+//          2048 ->  2752    7.3 / 15.6     8.6 / 14.6    14.9 / 14.6    15.5 / 14.6      11.3
+//          2048 ->  5504   13.0 / 23.0    16.1 / 19.6    22.4 / 19.3    23.1 / 16.1      22.5
+//          4096 -> 14336   43.1 / 68.1    49.7 / 52.2    88.1 / 52.2    90.1 / 52.7     117
 bool few_rows(const attn_products_t& c) {
   const attn_product_t& p = c.product[0];
+  const long long most = c.kind == ATTN_PRODUCT_GATED ? 6000000 : 20000000;      // elements of a weight
   return c.form == ATTN_FORM_NT && c.kind != ATTN_PRODUCT_GATED_GRAD && c.count == 1 && p.pairs == 1 && p.rows > 0 && p.cols > 0 && p.k > 0 &&
-         (p.rows <= 8 || (p.rows <= 32 && (long long)p.cols * p.k <= 12000000));
+         (p.rows <= 16 || (p.rows <= 32 && (long long)p.cols * p.k <= most));
 }
 
 template <typename T, int FEW, int WARPS>

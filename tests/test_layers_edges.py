@@ -42,6 +42,19 @@ def test_scratch_of_calls_without_rows_or_columns(capi):
         assert L.attn_b200_layer_norm_backward_scratch_bytes(ctypes.byref(s)) == 0
 
 
+def test_which_calls_are_of_few_rows(capi):
+    # tiles of a long sum are shared out and need scratch, few rows do not
+    def scratch(rows, k, cols):
+        c = capi.Products()
+        c.dtype, c.form, c.count = capi.ATTN_BF16, 0, 1
+        p = c.product[0]
+        p.rows, p.cols, p.k, p.pairs = rows, cols, k, 1
+        return capi.lib().attn_b200_products_scratch_bytes(ctypes.byref(c))
+
+    assert scratch(16, 4096, 6144) == 0 and scratch(17, 4096, 6144) > 0
+    assert scratch(32, 8192, 2048) == 0 and scratch(33, 8192, 2048) > 0
+
+
 # ---- no rows ---------------------------------------------------------------------------------------------
 
 @pytest.mark.gpu
