@@ -6,8 +6,9 @@
 //                  ht = a' zt u + a ut,  ez = gh a' u,  eu = gh a,  dz = gh (a'' zt u + a' ut) + gh2 a' u,  du = gh a' zt + gh2 a
 //
 // A CTA of 256 threads has 256 columns, eight to a thread (neighbouring threads' in sequence with 16-byte accesses, or one by one where widths or
-// addresses do not allow that), and a run of rows, eight at a time; the first pass has four rows of a thread on their way (two: 45 us).  Bound by memory: the first pass with gelu and
-// the bias' gradient, 16384 x 2048 bf16, 201 MB, 37 us (5.4 TB/s) and 6 for the sums over the runs.
+// addresses do not allow that), and a run of rows, eight at a time.  In the first pass a thread has several rows on their way: with an activation four of half types (two:
+// 45 us) and two of float32, without one twice as many; the others have two.  16384 x 2048 bf16 (ncu, cold): the first pass with gelu and the bias' gradient, 201 MB, 36 to 38 us
+// (5.4 TB/s) and 6 for the sums over the runs; the second, 403 MB, 72; of a gated block, 772 MB, 150.
 #include "activation.cuh"
 #include "layer_launch.h"
 
@@ -288,7 +289,8 @@ cudaError_t launch_copy_rows(const void* src, long long lds, void* dst, long lon
 }
 
 // ---- host ---------------------------------------------------------------------------------------
-// Runs of rows: six CTAs an SM, 64 rows each at least
+// Runs of rows: as many as make six CTAs an SM, 64 rows each at least.  The first pass in half types has 54 registers (without an activation) or 64 (gelu), and four
+// CTAs run on an SM: 888 of them (16384 x 2048) are 1.5 waves
 int element_chunks(int n, int m) {
   const long long tiles = ((long long)m + kElemCols - 1) / kElemCols;
   if (tiles == 0) return 1;

@@ -6,9 +6,13 @@
 //            to x: r (q - m(q) - xh m(q xh)) - r^2 xh (m(c u) - m(c) m(u) - m(c xh) m(u xh)),  q = g uw - r (c m(u xh) + u m(c xh))
 //            m(q) and m(q xh) follow from the means of c, u, g uw and their products with xh, so one round of sums over the row does
 //
-// Every pass reads its rows once: a row stays in the registers of a group of 32 to 1024 threads, so that the variance is that of the centred row.  Bound by memory.  Sums over the rows stay in registers while a group goes from row to row, its next row on the way; a
-// kernel behind adds what the CTAs have, in order.  16384 x 768 bf16 (ncu, cold): forward 15 us (50 MB), dx with dw and db 20 (75 MB) and 7; 8195 x 4096 f16: 34 (3.9 TB/s), 45
-// (4.5) and 8.  Above 8192 columns the backward's registers spill.
+// Every pass reads its rows once: a row stays in the registers of a group of 32 to 1024 threads, so that the variance is that of the centred row.  Sums over the rows
+// stay in registers while a group goes from row to row, its next row on the way; a kernel behind adds what the CTAs have, in order.
+//
+// 16384 x 768 bf16 (ncu, cold): forward 15 to 17 us (50 MB: 8 us at the copy rate), dx with dw and db 20 to 23 (75 MB) and 7 to 9, second 72 (126 MB) and 8; 8195 x 4096 f16:
+// 32 to 35, 45 to 48 and 8 to 10, 145 (336 MB) and 8.  The forward issues in 64 % of its cycles: a row's warps load and unpack w and b for every row, and the arithmetic is
+// scalar.  The backward passes wait, for loads and the sums over a row, with two CTAs an SM or one.  The kernel behind has 48 CTAs at 768 columns, whose threads add ten
+// of 296 rows each.  Above 8192 columns the backward's registers spill.
 #pragma once
 
 #include "attn_common.cuh"

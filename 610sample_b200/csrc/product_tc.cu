@@ -23,10 +23,10 @@
 // of 256 blocks of k) fill the 74 pairs once.  Where the last round of tiles stays short of them, its tiles are shared out along k and a small kernel behind adds
 // the parts in order and does the epilogue (PLAIN and KEEP).
 //
-// 16384 rows, 768 wide, 2048 inner, bf16, each by itself (ncu, cold): PLAIN with gelu and z kept 54 to 59 us, without either 44; NN 43, of two pairs 72; TN 43 and 7 to join,
-// three results 94 (1 640 TFLOP/s, tensor pipe 77 % active); GATED 72, with z and u kept 86 to 92 (178 MB written); GRAD 73 (201 MB read, 94 written: 4.1 TB/s).  At the peak
-// rate the operands come in at 64 bytes a clock and go out at 64, all that an SM's shared memory carries: with 12 blocks of k to a tile, what the epilogue stages there is
-// the difference between these and the 31 and 63 us of the tensor cores.  With 64 blocks (16384 x 4096 -> 2048) 177 us, 1 556 TFLOP/s.
+// 16384 rows, 768 wide, 2048 inner, bf16, each by itself (ncu, cold, over boards): PLAIN with gelu and z kept 53 to 60 us, without either 44; NN 42 to 47, of two pairs 72 to 80;
+// TN 41 to 46 and 7 to join, three results 93 to 107 (1 450 to 1 640 TFLOP/s, tensor pipe 77 to 84 % active); GATED 72, with z and u kept 86 to 94 (178 MB written); GRAD 72 to 79 (201 MB
+// read, 94 written).  At the peak rate the operands come in at 64 bytes a clock and go out at 64, all that an SM's shared memory carries: with 12 blocks of k to a tile, what the
+// epilogue stages there is the difference between these and the 31 and 63 us of the tensor cores.  With 64 blocks (16384 x 4096 -> 2048) 177 us, 1 556 TFLOP/s.
 #include "activation.cuh"
 #include "layer_launch.h"
 #include "product_common.cuh"

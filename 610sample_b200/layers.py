@@ -7,9 +7,11 @@ feed-forward blocks.
     x = gated_feed_forward(h, w_gate, w_up, w_down, residual=x)
 
 All are differentiable to second order, as `flash_attention_v7`, with kernels for both backward passes; a third derivative is
-refused.  fp16, bf16 or fp32 CUDA tensors; leading axes are rows.  The reference's model has these steps as separate eager
-operations (e2e/ttt_pytorch/model.py).  There is no fallback: importing this module fails if the
-compiled extension `attention_cuda` is missing.
+refused.  fp16, bf16 or fp32 CUDA tensors; leading axes are rows.  The reference's model has linear layers and gated blocks as
+separate eager operations (e2e/ttt_pytorch/model.py); its norms are RMS norms, where `layer_norm` is what a pre-norm decoder with
+layer norm needs.  Autocast changes nothing here: no tensor is cast, so half-precision rows beside float32 weights are refused, and
+float32 rows are computed in float32.  There is no fallback: importing this module fails if the compiled extension
+`attention_cuda` is missing.
 """
 try:  # used as part of the package
     from . import attention_cuda as _attention_cuda
@@ -49,5 +51,5 @@ def gated_feed_forward(x, w_gate, w_up, w_down, activation="silu", residual=None
 
     Both projections, the activation and the product are one kernel, the second projection with the residual another.  The inner
     values are rounded to the type of x before the second projection; the backward keeps them and both projections, of half types
-with four bits more than 16 each: fp16 with 13 bits of mantissa up to 2^46, beyond which gradients are NaN."""
+    with four bits more than 16 each: fp16 with 13 bits of mantissa up to 2^46, beyond which gradients are NaN."""
     return _attention_cuda.gated_feed_forward(x, w_gate, w_up, w_down, residual, _activation(activation))
