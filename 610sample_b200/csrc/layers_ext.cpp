@@ -32,6 +32,7 @@ void copy_rows(const torch::Tensor& from, int64_t from_ld, const torch::Tensor& 
 Matrix matrix(const torch::Tensor& t_in, bool any_rows = false) {
   const int64_t cols = columns_of(t_in), rows = cols > 0 ? t_in.numel() / cols : 0;
   torch::Tensor t = t_in.dim() == 2 ? t_in : t_in.reshape({rows, cols});
+  if (t.is_neg()) t = t.resolve_neg();      // a negation that has not been carried out yet (the imaginary part of a conjugate)
   const bool half = t.scalar_type() != at::kFloat;
   const int64_t ld = rows > 1 ? t.stride(0) : (cols + 7) / 8 * 8;      // one row: any distance
   const bool dense_rows = (cols <= 1 || t.stride(1) == 1) && ld >= cols;
@@ -42,6 +43,9 @@ Matrix matrix(const torch::Tensor& t_in, bool any_rows = false) {
   else copy.copy_(t);
   return {copy, rows > 1 ? pitch : (cols + 7) / 8 * 8};
 }
+
+// a vector as the kernels take it
+torch::Tensor packed(const torch::Tensor& t) { return t.defined() ? t.resolve_neg().contiguous() : t; }
 
 // The copy that `matrix` made of a tensor, for the backward to read again; nothing where it made none
 torch::Tensor copied(const Matrix& m, const torch::Tensor& from) { return m.t.is_alias_of(from) ? torch::Tensor() : m.t; }
@@ -212,7 +216,7 @@ variable_list linear_forward(const torch::Tensor& x_in, const torch::Tensor& w_i
   Matrix r, z;
   if (r_in.defined()) r = matrix(r_in);
   if (keep) z = result(n, m, x_in, x_in.scalar_type() == at::kFloat ? at::kFloat : at::kHalf);
-  const torch::Tensor b = b_in.defined() ? b_in.contiguous() : b_in;
+  const torch::Tensor b = packed(b_in);
   Products(x_in, ATTN_FORM_NT, ATTN_PRODUCT_PLAIN, activation).add(y, n, m, k, {{&x, &w}}).bias(b).residual(r).kept(0, z).run("linear");
   return {handed(y, with_columns(x_in, m)), z.t, copied(x, x_in), copied(w, w_in)};
 }
@@ -259,7 +263,7 @@ variable_list linear_second(const torch::Tensor& u_in, const torch::Tensor& uw_i
   Matrix u, uw, t;
   if (u_in.defined()) u = matrix(u_in);
   if (uw_in.defined()) uw = matrix(uw_in);
-  const torch::Tensor ub = ub_in.defined() ? ub_in.contiguous() : ub_in;
+  const torch::Tensor ub = packed(ub_in);
   if (u_in.defined() || uw_in.defined()) {
     t = result(n, m, x_in);
     Products(x_in, ATTN_FORM_NT).add(t, n, m, k, {{&u, &w}, {&x, &uw}}).bias(ub).run("linear second backward");
@@ -558,7 +562,6 @@ attn_norm_shape_t norm_shape(const torch::Tensor& x, const Matrix& m, at::Scalar
 }
 const void* pointer(const torch::Tensor& t) { return t.defined() ? t.data_ptr() : nullptr; }
 void* target(const torch::Tensor& t) { return t.defined() ? t.data_ptr() : nullptr; }
-torch::Tensor packed(const torch::Tensor& t) { return t.defined() ? t.contiguous() : t; }
 
 // {y, mean, rstd}; the last two where they are to be kept
 variable_list norm_forward(const torch::Tensor& x_in, const torch::Tensor& w_in, const torch::Tensor& b_in, double eps, bool keep) {

@@ -111,6 +111,22 @@ def test_gradients_are_not_their_cotangents(layers, dtype):
     assert torch.equal(got[0], u) and got.data_ptr() != u.data_ptr()
 
 
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", TYPES)
+def test_negations_that_have_not_been_carried_out(layers, dtype):
+    # views with the negative bit, as the imaginary part of a conjugate is: the results of the negated tensors
+    views = [lambda t: torch._neg_view(t)] + [lambda t: torch.complex(torch.zeros_like(t), t).conj().imag] * (dtype == torch.float32)
+    for k, m in ((16, 24), (13, 1)):
+        for call, leaves, g in calls(layers, dtype, (9,), k, m):
+            for view in views:
+                want = passes(call, [-t for t in leaves], -g)
+                t = [v.detach().requires_grad_(True) for v in leaves]
+                y = call(*[view(v) for v in t])
+                assert torch.equal(y, want[0])
+                for a, b in zip(torch.autograd.grad(y, t, view(g)), want[1:]):
+                    assert torch.equal(a, -b)
+
+
 # ---- gated blocks: zeros, and projections beyond 65504 -----------------------------------------------------
 
 @pytest.mark.gpu
