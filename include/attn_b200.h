@@ -280,8 +280,8 @@ int attn_b200_linear_ce_backward(const attn_lce_shape_t* shape, const void* x, c
  * f32 on the CUDA cores.  A residual and a bias may have any alignment of an element.  Rows of results and of what is kept are written up to the next
  * multiple of 8 columns in half types (the last row's memory has to reach there too), never behind it.  z of a plain product is kept in f16 of half types, within its
  * finite range; z and u
- * of a gated one in 20 bits of f16 and bf16: 16 of each in kept, and 4 of both in a plane of bytes, kept_low, whose rows are a multiple of 32
- * apart from a 32-byte aligned base.  Their encoding is the kernels' own.  Inputs must not overlap outputs. */
+ * of a gated one, of half types, in 20 bits a value: 16 of each in kept, and 4 of both in a plane of bytes, kept_low, whose rows are a multiple of 32
+ * apart from a 32-byte aligned base.  Their encoding is the kernels' own (f16: up to 2^46, and NaN beyond).  Inputs must not overlap outputs. */
 enum { ATTN_FORM_NT = 0, ATTN_FORM_NN = 1, ATTN_FORM_TN = 2 };
 enum { ATTN_PRODUCT_PLAIN = 0, ATTN_PRODUCT_GATED = 1, ATTN_PRODUCT_GATED_GRAD = 2 };
 enum { ATTN_ACT_NONE = 0, ATTN_ACT_SILU = 1, ATTN_ACT_GELU = 2, ATTN_ACT_GELU_TANH = 3 };

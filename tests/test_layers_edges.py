@@ -127,6 +127,20 @@ def test_negations_that_have_not_been_carried_out(layers, dtype):
                     assert torch.equal(a, -b)
 
 
+@pytest.mark.gpu
+def test_autocast_casts_nothing(layers):
+    x, wg, wu, wd, r, g = gated_inputs(9, 32, 48, 32, torch.float32)
+    nw = torch.ones(32, device="cuda")
+    for call, leaves in ((lambda *t: layers.gated_feed_forward(*t), [x, wg, wu, wd]), (lambda *t: layers.linear(*t), [x, wd[:, :32].contiguous()]), (lambda *t: layers.layer_norm(*t), [x, nw])):
+        want = passes(call, leaves, g)
+        with torch.autocast("cuda", torch.bfloat16):
+            for a, b in zip(passes(call, leaves, g), want):
+                assert a.dtype == torch.float32 and torch.equal(a, b)
+            if leaves[1].dim() == 2:
+                with pytest.raises(RuntimeError, match="dtype of x"):
+                    call(x.bfloat16(), *leaves[1:])
+
+
 # ---- gated blocks: zeros, and projections beyond 65504 -----------------------------------------------------
 
 @pytest.mark.gpu
